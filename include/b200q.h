@@ -357,6 +357,53 @@ b200q_status b200q_plan_create(b200q_ctx *ctx, const b200q_job *jobs, int32_t n_
 b200q_status b200q_plan_run(b200q_ctx *ctx, b200q_plan *plan, void *stream);
 void b200q_plan_destroy(b200q_plan *plan);
 
+/* -- expert layers ------------------------------------------------------------------------------- */
+
+/* The expert part of a mixture-of-experts layer for few tokens (ggml MUL_MAT_ID with quantized src0, three products and the
+ * activation function between them): row m with choices e = ids[m][j] and weights w = weights[m][j], j < top_k, gets
+ *     y[m] = sum_j w * (D_e h + down_bias_e),   h = act(G_e x[m] + gate_bias_e, U_e x[m] + up_bias_e).
+ * The reference runs it inside context.decode(batch) (icn-engine/src/lib.rs:2264) for models with expert tensors.  A
+ * layer keeps its weights re-laid-out on the device, and a workspace for max_rows rows: calls allocate nothing, so they
+ * may be captured from the first one on; two calls of one layer must not overlap (same stream, or an event between
+ * them; that holds for the replays of graphs that captured them, too). */
+typedef struct b200q_moe b200q_moe;
+
+enum {
+    B200Q_MOE_SWIGLU = 0,          /* act(a, b) = a / (1 + exp(-a)) * b */
+    B200Q_MOE_SWIGLU_CLAMPED = 1   /* a' = min(a, limit), b' = max(-limit, min(b, limit)): a' / (1 + exp(-alpha a')) * (b' + 1) */
+};
+enum {
+    B200Q_MOE_ACCUMULATE = 1       /* flag of b200q_moe_run: the result is added to what y holds (residual connection) */
+};
+
+typedef struct b200q_moe_config {
+    int32_t n_experts;             /* 1..1024 */
+    int32_t top_k;                 /* choices of a row: 1..16, at most n_experts */
+    int64_t n_embd, n_ff;          /* widths of x and y, and of h; multiples of their tensors' blocks */
+    int64_t max_rows;              /* 1..512: rows of a call at most (longer prompts: in pieces) */
+    int32_t gate_up_type, down_type;
+    const void *gate, *up;         /* GGUF blocks [expert][n_ff rows][n_embd], as a GGUF file's 3-D expert tensors hold them */
+    const void *down;              /* [expert][n_embd rows][n_ff].  All pointers here: host memory, or device memory whose contents */
+    size_t gate_bytes, up_bytes, down_bytes;      /* are complete; copied before b200q_moe_create returns */
+    const float *gate_bias, *up_bias;      /* [expert][n_ff] or NULL */
+    const float *down_bias;                /* [expert][n_embd] or NULL */
+    int32_t activation;            /* B200Q_MOE_* */
+    float alpha, limit;            /* of the clamped gate */
+    int32_t reserved;              /* 0 */
+} b200q_moe_config;
+
+b200q_status b200q_moe_create(b200q_ctx *ctx, const b200q_moe_config *config, b200q_moe **out);
+
+/* x[M][n_embd] F32 or BF16, ids and weights [M][top_k] in device memory, y[M][n_embd] F32 or BF16; M <= max_rows, M == 0 is a
+ * no-op.  A choice outside 0..n_experts-1 (-1 for padding) contributes nothing; the same expert twice in a row counts twice.
+ * Activations enter as fixed point, 256 elements to a scale: 16 bits where y is BF16, 31 bits where it is F32; sums are
+ * integers and fp32.  A piece of 256 elements that holds an infinity or a NaN makes that row's result NaN, no other row's.
+ * Results do not depend on the other rows of the call but through the order of sums over K. */
+b200q_status b200q_moe_run(b200q_ctx *ctx, b200q_moe *moe, const void *x_dev, int32_t x_dtype, int64_t M, int64_t ldx,
+                           const int32_t *ids_dev, int64_t ld_ids, const float *weights_dev, int64_t ld_weights,
+                           void *y_dev, int32_t y_dtype, int64_t ldy, int32_t flags, void *stream);
+void b200q_moe_destroy(b200q_moe *moe);     /* may follow b200q_ctx_destroy, like b200q_weight_destroy */
+
 /* -- tensor parallel exchange ------------------------------------------------------------------ */
 
 /* 128-byte NCCL unique id for rank 0 to broadcast out of band. */

@@ -7,6 +7,8 @@ PyTorch or other fallback for the products it computes.
 from . import _binding
 from ._binding import (  # noqa: F401
     B200QError,
+    MOE_SWIGLU,
+    MOE_SWIGLU_CLAMPED,
     ROUTE_GEMM,
     ROUTE_GEMV,
     ROUTE_NONE,
@@ -22,6 +24,7 @@ from ._binding import (  # noqa: F401
     TYPE_Q6_K,
     TYPE_Q8_0,
 )
+from .rows import MoeLayer  # noqa: F401
 from .projection import (  # noqa: F401
     Backend,
     GgufFile,

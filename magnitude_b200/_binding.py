@@ -36,6 +36,36 @@ JOB_SUM_RANKS = 2
 JOB_SWIGLU = 4
 JOB_ACCUMULATE = 8
 
+MOE_SWIGLU, MOE_SWIGLU_CLAMPED = 0, 1
+MOE_ACCUMULATE = 1
+
+
+class MoeConfig(ctypes.Structure):
+    """struct b200q_moe_config of include/b200q.h."""
+
+    _fields_ = [
+        ("n_experts", c_int32),
+        ("top_k", c_int32),
+        ("n_embd", c_int64),
+        ("n_ff", c_int64),
+        ("max_rows", c_int64),
+        ("gate_up_type", c_int32),
+        ("down_type", c_int32),
+        ("gate", c_void_p),
+        ("up", c_void_p),
+        ("down", c_void_p),
+        ("gate_bytes", c_size_t),
+        ("up_bytes", c_size_t),
+        ("down_bytes", c_size_t),
+        ("gate_bias", c_void_p),
+        ("up_bias", c_void_p),
+        ("down_bias", c_void_p),
+        ("activation", c_int32),
+        ("alpha", ctypes.c_float),
+        ("limit", ctypes.c_float),
+        ("reserved", c_int32),
+    ]
+
 
 class Job(ctypes.Structure):
     """struct b200q_job of include/b200q.h."""
@@ -109,6 +139,13 @@ SIGNATURES = {
     "b200q_plan_create": (c_int32, [c_void_p, POINTER(Job), c_int32, c_int64, POINTER(c_void_p)]),
     "b200q_plan_run": (c_int32, [c_void_p, c_void_p, c_void_p]),
     "b200q_plan_destroy": (None, [c_void_p]),
+    "b200q_moe_create": (c_int32, [c_void_p, POINTER(MoeConfig), POINTER(c_void_p)]),
+    "b200q_moe_run": (
+        c_int32,
+        [c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int32, c_int64, c_int32,
+         c_void_p],
+    ),
+    "b200q_moe_destroy": (None, [c_void_p]),
     "b200q_tp_unique_id": (c_int32, [c_void_p]),
     "b200q_tp_init": (c_int32, [c_void_p, c_int32, c_int32, c_void_p]),
     "b200q_allreduce": (c_int32, [c_void_p, c_void_p, c_int64, c_int32, c_void_p]),

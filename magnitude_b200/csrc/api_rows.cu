@@ -1,0 +1,189 @@
+// C-ABI layer of the products whose weights every row picks for itself: expert layers.
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+#include <new>
+
+#include "context.h"
+#include "moe_types.h"
+
+using namespace b200q;
+
+struct b200q_moe {
+    b200q_ctx *ctx = nullptr;
+    int device = 0;                   // the context's device, kept here: the layer may outlive the context
+    MoeShapeInfo shape{};
+    int gate_up_type = 0, down_type = 0;
+    int activation = 0;
+    float alpha = 0.f, limit = 0.f;
+    uint8_t *gate_up = nullptr, *down = nullptr;
+    float *gate_bias = nullptr, *up_bias = nullptr, *down_bias = nullptr;
+    uint8_t *ws = nullptr;
+    MoeBuffers buf{};
+};
+
+namespace {
+
+// is `p` memory that kernels of the current device can read at full rate?
+bool on_device(const void *p, int device) {
+    cudaPointerAttributes a;
+    if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    return a.type == cudaMemoryTypeDevice && a.device == device;
+}
+
+constexpr size_t kStageBytes = size_t(128) << 20;
+
+// GGUF rows of all experts into records at dst, a few experts at a time where the rows are not in this device's memory
+cudaError_t upload_experts(int qt, const void *src0, const void *src1, uint8_t *dst, int64_t experts, int64_t rows, int64_t K, int device) {
+    const size_t each = (size_t)(rows * (K / gguf_block_elems(qt)) * gguf_block_bytes(qt));
+    const size_t each_out = moe_matrix_bytes(qt, 1, rows, K, src1 != nullptr);
+    if (on_device(src0, device) && (!src1 || on_device(src1, device)))
+        return moe_repack(qt, (const uint8_t *)src0, (const uint8_t *)src1, dst, experts, rows, K, nullptr);
+    const int64_t step = std::max<int64_t>(1, std::min<int64_t>(experts, (int64_t)(kStageBytes / each)));
+    uint8_t *stage = nullptr;
+    const size_t half = (step * each + 255) / 256 * 256;
+    cudaError_t e = cudaMalloc(reinterpret_cast<void **>(&stage), (src1 ? 2 : 1) * half);
+    for (int64_t i = 0; e == cudaSuccess && i < experts; i += step) {
+        const int64_t n = std::min(step, experts - i);
+        e = cudaMemcpy(stage, (const uint8_t *)src0 + i * each, n * each, cudaMemcpyDefault);
+        if (e == cudaSuccess && src1) e = cudaMemcpy(stage + half, (const uint8_t *)src1 + i * each, n * each, cudaMemcpyDefault);
+        if (e == cudaSuccess) e = moe_repack(qt, stage, src1 ? stage + half : nullptr, dst + i * each_out, n, rows, K, nullptr);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);      // the stage is free again
+    }
+    if (stage) cudaFree(stage);
+    return e;
+}
+
+cudaError_t upload_floats(const float *src, int64_t n, float **out) {
+    if (!src) return cudaSuccess;
+    cudaError_t e = cudaMalloc(reinterpret_cast<void **>(out), n * sizeof(float));
+    if (e == cudaSuccess) e = cudaMemcpy(*out, src, n * sizeof(float), cudaMemcpyDefault);
+    return e;
+}
+
+}  // namespace
+
+extern "C" {
+
+b200q_status b200q_moe_create(b200q_ctx *ctx, const b200q_moe_config *c, b200q_moe **out) {
+    b200q_status s = check_ctx(ctx);
+    if (s != B200Q_OK) return s;
+    if (!out) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null out pointer");
+    *out = nullptr;
+    if (!c) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null expert layer description");
+    if (c->reserved != 0) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "expert layer: reserved is not 0");
+    if (!known_type(c->gate_up_type) || !known_type(c->down_type))
+        return fail(ctx, B200Q_ERR_INVALID_CONFIG, "unsupported ggml type id %d", known_type(c->gate_up_type) ? c->down_type : c->gate_up_type);
+    if (c->n_experts < 1 || c->n_experts > kMoeMaxExperts || c->top_k < 1 || c->top_k > kMoeMaxTopK || c->top_k > c->n_experts)
+        return fail(ctx, B200Q_ERR_INVALID_CONFIG, "expert layer: 1..%d experts and 1..%d choices (at most the experts); got %d and %d", kMoeMaxExperts,
+                    kMoeMaxTopK, c->n_experts, c->top_k);
+    if (c->max_rows < 1 || c->max_rows > kMoeMaxRows) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "expert layer: max_rows must be 1..%d", kMoeMaxRows);
+    if (c->n_embd < 1 || c->n_ff < 1 || c->n_embd > (1 << 20) || c->n_ff > (1 << 20))
+        return fail(ctx, B200Q_ERR_INVALID_CONFIG, "expert layer: widths must be 1..%d", 1 << 20);
+    if (c->n_embd % gguf_block_elems(c->gate_up_type))
+        return fail(ctx, B200Q_ERR_INVALID_CONFIG, "n_embd=%lld is not a multiple of the %d-weight block", (long long)c->n_embd, gguf_block_elems(c->gate_up_type));
+    if (c->n_ff % gguf_block_elems(c->down_type))
+        return fail(ctx, B200Q_ERR_INVALID_CONFIG, "n_ff=%lld is not a multiple of the %d-weight block", (long long)c->n_ff, gguf_block_elems(c->down_type));
+    if (!c->gate || !c->up || !c->down) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null weight pointer");
+    const int64_t elems = (int64_t)c->n_experts * c->n_embd * c->n_ff;
+    const int64_t gu = b200q_tensor_storage_bytes(c->gate_up_type, elems), dn = b200q_tensor_storage_bytes(c->down_type, elems);
+    if ((int64_t)c->gate_bytes != gu || (int64_t)c->up_bytes != gu || (int64_t)c->down_bytes != dn)
+        return fail(ctx, B200Q_ERR_INVALID_CONFIG, "byte counts %zu, %zu, %zu do not match the experts (%lld, %lld, %lld expected)", c->gate_bytes, c->up_bytes,
+                    c->down_bytes, (long long)gu, (long long)gu, (long long)dn);
+    if (c->activation != B200Q_MOE_SWIGLU && c->activation != B200Q_MOE_SWIGLU_CLAMPED)
+        return fail(ctx, B200Q_ERR_INVALID_CONFIG, "unknown activation function %d", c->activation);
+    if (c->activation == B200Q_MOE_SWIGLU_CLAMPED && !(isfinite(c->alpha) && c->limit > 0.f))
+        return fail(ctx, B200Q_ERR_INVALID_CONFIG, "the clamped gate takes a finite alpha and a limit above 0");
+
+    b200q_moe *m = new (std::nothrow) b200q_moe();
+    if (!m) return fail(ctx, B200Q_ERR_OVERLOADED, "out of host memory");
+    m->ctx = ctx;
+    m->device = ctx->device;
+    m->shape = MoeShapeInfo{c->n_experts, c->top_k, c->n_embd, c->n_ff, c->max_rows, ctx->sm_count};
+    m->gate_up_type = c->gate_up_type;
+    m->down_type = c->down_type;
+    m->activation = c->activation;
+    m->alpha = c->alpha;
+    m->limit = c->limit;
+    const size_t gu_bytes = moe_matrix_bytes(c->gate_up_type, c->n_experts, c->n_ff, c->n_embd, true);
+    const size_t d_bytes = moe_matrix_bytes(c->down_type, c->n_experts, c->n_embd, c->n_ff, false);
+    const size_t ws_bytes = moe_workspace(m->shape, nullptr, nullptr);
+    cudaError_t e = cudaMalloc(reinterpret_cast<void **>(&m->gate_up), gu_bytes);
+    if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void **>(&m->down), d_bytes);
+    if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void **>(&m->ws), ws_bytes);
+    if (e == cudaSuccess) e = cudaMemset(m->ws, 0, ws_bytes);
+    if (e == cudaSuccess) e = upload_floats(c->gate_bias, c->n_experts * c->n_ff, &m->gate_bias);
+    if (e == cudaSuccess) e = upload_floats(c->up_bias, c->n_experts * c->n_ff, &m->up_bias);
+    if (e == cudaSuccess) e = upload_floats(c->down_bias, c->n_experts * c->n_embd, &m->down_bias);
+    if (e == cudaSuccess) e = upload_experts(c->gate_up_type, c->gate, c->up, m->gate_up, c->n_experts, c->n_ff, c->n_embd, ctx->device);
+    if (e == cudaSuccess) e = upload_experts(c->down_type, c->down, nullptr, m->down, c->n_experts, c->n_embd, c->n_ff, ctx->device);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);      // in place before a call on any stream reads it
+    if (e != cudaSuccess) {
+        b200q_moe_destroy(m);
+        return cuda_fail(ctx, e, "expert layer upload");
+    }
+    moe_workspace(m->shape, &m->buf, m->ws);
+    *out = m;
+    return B200Q_OK;
+}
+
+void b200q_moe_destroy(b200q_moe *m) {
+    if (!m) return;
+    cudaSetDevice(m->device);         // not through m->ctx: the context may be gone already
+    for (void *p : {(void *)m->gate_up, (void *)m->down, (void *)m->gate_bias, (void *)m->up_bias, (void *)m->down_bias, (void *)m->ws})
+        if (p) cudaFree(p);
+    delete m;
+}
+
+b200q_status b200q_moe_run(b200q_ctx *ctx, b200q_moe *moe, const void *x_dev, int32_t x_dtype, int64_t M, int64_t ldx, const int32_t *ids_dev, int64_t ld_ids,
+                           const float *weights_dev, int64_t ld_weights, void *y_dev, int32_t y_dtype, int64_t ldy, int32_t flags, void *stream) {
+    b200q_status s = check_ctx(ctx);
+    if (s != B200Q_OK) return s;
+    if (!moe) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null expert layer");
+    if (moe->ctx != ctx) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "expert layer belongs to another context");
+    if (!act_type(x_dtype) || !act_type(y_dtype)) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "activation/output dtype must be F32 (0) or BF16 (30)");
+    if (flags & ~B200Q_MOE_ACCUMULATE) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "unknown flags %d", flags);
+    if (M < 0) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "M < 0");
+    if (M > moe->shape.max_rows)
+        return fail(ctx, B200Q_ERR_INVALID_CONFIG, "M=%lld is above the layer's max_rows=%lld", (long long)M, (long long)moe->shape.max_rows);
+    if (M == 0) return B200Q_OK;
+    if (!x_dev || !y_dev || !ids_dev || !weights_dev) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null activation, choice or output pointer");
+    if (ldx < moe->shape.n_embd || ldy < moe->shape.n_embd || ld_ids < moe->shape.top_k || ld_weights < moe->shape.top_k)
+        return fail(ctx, B200Q_ERR_INVALID_CONFIG, "leading dimension smaller than the row");
+    MoeRun r{};
+    r.shape = moe->shape;
+    r.buf = moe->buf;
+    r.gate_up_type = moe->gate_up_type;
+    r.down_type = moe->down_type;
+    r.gate_up = moe->gate_up;
+    r.down = moe->down;
+    r.gate_bias = moe->gate_bias;
+    r.up_bias = moe->up_bias;
+    r.down_bias = moe->down_bias;
+    r.activation = moe->activation;
+    r.alpha = moe->alpha;
+    r.limit = moe->limit;
+    r.x = x_dev;
+    r.ldx = ldx;
+    r.x_is_bf16 = x_dtype == B200Q_TYPE_BF16;
+    r.m = (int)M;
+    r.ids = ids_dev;
+    r.ld_ids = ld_ids;
+    r.weights = weights_dev;
+    r.ld_weights = ld_weights;
+    r.y = y_dev;
+    r.ldy = ldy;
+    r.y_is_bf16 = y_dtype == B200Q_TYPE_BF16;
+    r.accumulate = (flags & B200Q_MOE_ACCUMULATE) != 0;
+    int launches = 0;
+    cudaError_t e = moe_run(r, (cudaStream_t)stream, &launches);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "expert layer launch");
+    ctx->last_launches = launches;
+    return B200Q_OK;
+}
+
+}  // extern "C"

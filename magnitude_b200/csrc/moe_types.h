@@ -1,0 +1,145 @@
+// What the host side of the expert layer (moe.cu) and its kernels (moe_kernel.cuh) share.
+#pragma once
+
+#include "common.cuh"
+
+namespace b200q {
+
+// ---------------------------------------------------------------------------------------------
+// Weights of experts
+//
+// An expert's matrix is cut into tiles of 16 rows x 256 weights ("records"); the records of a tile of rows follow each
+// other, then the next tile's, then the next expert's.  A warp multiplies one record at a time, so a record is one
+// contiguous piece of memory, and inside it the weights lie in the order in which the lanes of a warp take them as the A
+// operand of mma.m16n8k32: lane 4 g + t owns, of rows g and g + 8 and of every block of 32 weights, weights 4 t .. 4 t + 3 and
+// 16 + 4 t .. 16 + 4 t + 3.  The 16-byte vectors of the 32 lanes lie side by side, so both the copy into shared memory and the
+// reads from it are whole 512-byte lines.  Gate and up of the gated product share tiles: rows 0 .. 7 of a tile are
+// eight gate rows, rows 8 .. 15 the same eight up rows, and one lane holds both sums of an output.
+//   vectors [v][lane][16 bytes], per lane [row g: word 0, word 1][row g + 8: word 0, word 1], word w = weights 16 w + 4 t ..
+//   Q4_K    4 x: bytes hold block 2 v (low nibbles) and 2 v + 1 (high); then the rows' 16-byte headers [d dmin scales]
+//   Q5_K    as Q4_K; then 1 x of fifth bits (bit b of a byte: block b); then the headers
+//   Q4_0    4 x as Q4_K; then the rows' eight fp16 d
+//   Q8_0    8 x: block v; then the rows' eight fp16 d
+//   MXFP4   4 x: per row block 2 v, block 2 v + 1: eight codes each (low half word 0, high half word 1); the rows' 8 scale bytes
+//   Q6_K    6 x: a lane's row has four triples of words, triple i made of blocks 2 i, 2 i + 1 (words 0, 1 of the first, word 0 of the
+//           second): a byte's upper six bits are 4 (level - 32) as a signed byte, the lower two bits of the three hold those six
+//           bits of the fourth word's byte.  Vectors 3 (i / 2) + n hold words 2 n, 2 n + 1 of the six of triples i, i + 1;
+//           then the rows' 16 int8 scales, then their d
+// The byte count is GGUF's (blocks of 32 weights: K padded to 256, rows to 16 with zeros).
+// ---------------------------------------------------------------------------------------------
+constexpr int kMoeWarps = 8, kMoeThreads = 32 * kMoeWarps;
+__host__ __device__ constexpr int moe_rec_bytes(int qt) { return 16 * (qt == QT_Q4_K || qt == QT_Q4_0 ? 144 : qt == QT_Q5_K ? 176 : qt == QT_Q6_K ? 210 : qt == QT_Q8_0 ? 272 : 136); }
+// stages of a warp's ring
+__host__ __device__ constexpr int moe_depth(int qt) { return moe_rec_bytes(qt) <= 2304 ? 4 : moe_rec_bytes(qt) <= 2816 ? 3 : 2; }
+
+// ---------------------------------------------------------------------------------------------
+// Activations
+//
+// A row enters as signed bytes: 256 elements share a scale, an element is P bytes ("planes", P = 2: 16 bits, P = 4: 31 bits), and
+// the planes are the columns of the B operand: a column tile of eight holds 8 / P rows.  The image of 256 elements is
+//   [pair of blocks 4][plane P][t 4][block of the pair 2][word 2] x 4 bytes: lane 4 c + t reads column c's 16 bytes per pair
+//   [plane P] 16 bytes: the sums over the blocks of 32 as 64 a + b: [blocks 0 .. 3, 4 .. 7][a, b] x 4 bytes
+//   [P / 2] fp32: what one unit of the plane pair is worth; padding to 16 bytes
+// ---------------------------------------------------------------------------------------------
+__host__ __device__ constexpr int moe_image_bytes(int planes) { return planes * (256 + 16) + 16; }
+
+constexpr int kMoeMaxRows = 512, kMoeMaxTopK = 16, kMoeMaxSlots = kMoeMaxRows * kMoeMaxTopK, kMoeMaxExperts = 1024;
+
+// rows of one expert that are multiplied together
+struct MoeGroup {
+    int expert, first, n, reserved;      // slots sorted[first .. first + n)
+};
+
+struct MoeLists {
+    int *ngroups;
+    MoeGroup *groups;
+    int *sorted;                         // slots (row * top_k + choice) by expert
+};
+
+struct MoeGateUp {
+    const uint8_t *w;
+    long long expert_bytes;
+    int tiles, nrec, split;              // split: warps that share a tile's records
+    MoeLists lists;
+    const uint8_t *img;                  // images of the rows
+    unsigned img_stride;                 // bytes of a row's image
+    int top_k;
+    float *h;                            // [slot][ff]
+    int ff;
+    int activation;
+    float alpha, limit;
+    const float *gate_bias, *up_bias;    // [expert][ff] or null
+};
+
+struct MoeDown {
+    const uint8_t *w;
+    long long expert_bytes;
+    int tiles, nrec, split;
+    MoeLists lists;
+    const uint8_t *img;                  // images of the slots' h
+    unsigned img_stride;
+    int top_k, experts;
+    const int *ids;
+    long long ld_ids;
+    const float *weights;
+    long long ld_weights;
+    const float *bias;                   // [expert][n] or null
+    float *z;                            // [tile of a block][split][slot][16], or null: in shared memory
+    void *y;
+    long long ldy;
+    int y_is_bf16, accumulate;
+    int n, m;                            // output width, rows
+};
+
+struct MoeConfig {                       // what picks a kernel
+    int planes, column_tiles;
+};
+
+// ---- moe.cu: what the C ABI layer calls ----------------------------------------------------------
+struct MoeShapeInfo {
+    int64_t n_experts, top_k, n_embd, n_ff, max_rows;
+    int sm_count;
+};
+struct MoeBuffers {
+    MoeLists lists;
+    float *h;
+    uint8_t *x_img, *h_img;
+    float *z;
+};
+struct MoeRun {
+    MoeShapeInfo shape;
+    MoeBuffers buf;
+    int gate_up_type, down_type;
+    const uint8_t *gate_up, *down;
+    const float *gate_bias, *up_bias, *down_bias;
+    int activation;
+    float alpha, limit;
+    const void *x;
+    long long ldx;
+    int x_is_bf16, m;
+    const int *ids;
+    long long ld_ids;
+    const float *weights;
+    long long ld_weights;
+    void *y;
+    long long ldy;
+    int y_is_bf16, accumulate;
+};
+size_t moe_matrix_bytes(int qt, int64_t experts, int64_t rows, int64_t K, bool paired);
+// GGUF rows [expert][row] in device memory -> records; src1: the up matrix that shares tiles with src0, or null
+cudaError_t moe_repack(int qt, const uint8_t *src0, const uint8_t *src1, uint8_t *dst, int64_t experts, int64_t rows, int64_t K, cudaStream_t st);
+// bytes of a layer's workspace, and its parts from `base` on
+size_t moe_workspace(const MoeShapeInfo &s, MoeBuffers *out, uint8_t *base);
+cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches);
+
+#define MOE_DECLARE(NAME)                                                                                     \
+    cudaError_t moe_gate_up_##NAME(const MoeGateUp &p, const MoeConfig &c, int grid, cudaStream_t st);          \
+    cudaError_t moe_down_##NAME(const MoeDown &p, const MoeConfig &c, int grid, size_t z_bytes, cudaStream_t st);
+MOE_DECLARE(q4_k)
+MOE_DECLARE(q5_k)
+MOE_DECLARE(q6_k)
+MOE_DECLARE(q8_0)
+MOE_DECLARE(q4_0)
+MOE_DECLARE(mxfp4)
+
+}  // namespace b200q

@@ -15,6 +15,7 @@ from typing import Sequence
 import numpy as np
 
 from . import _binding as B
+from .rows import MoeLayer, invalid, matrix
 
 _TORCH_DTYPE = {}
 
@@ -284,6 +285,33 @@ class Backend:
         out = c_void_p()
         self._check(B.lib().b200q_plan_create(self._h, arr, n, m or 1, byref(out)))
         return Plan(self, out.value, keep)
+
+    # -- products whose weights every row picks for itself ------------------------------------
+    def moe(self, gate, up, down, *, gate_up_type: int, down_type: int, top_k: int, n_embd: int, n_ff: int, max_rows: int,
+            activation: int = B.MOE_SWIGLU, alpha: float = 0.0, limit: float = 0.0, gate_bias=None, up_bias=None,
+            down_bias=None) -> MoeLayer:
+        """The experts of a layer (b200q_moe_create).  gate, up: packed uint8 [experts, n_ff, row bytes] of one type, down: [experts,
+        n_embd, row bytes], NumPy arrays or tensors on the host or the GPU; biases: float32 [experts, width] or None."""
+        return MoeLayer(self, gate, up, down, gate_up_type=gate_up_type, down_type=down_type, top_k=top_k, n_embd=n_embd, n_ff=n_ff,
+                        max_rows=max_rows, activation=activation, alpha=alpha, limit=limit, gate_bias=gate_bias, up_bias=up_bias,
+                        down_bias=down_bias)
+
+    def run_moe(self, layer: MoeLayer, x, ids, weights, out=None, out_dtype=None, accumulate: bool = False, stream=None):
+        """out[m] = the weighted sum of the experts ids[m] of x[m] (b200q_moe_run); with accumulate it is added to out.  x [M, n_embd] bf16
+        or fp32, ids int32 and weights float32 [M, top_k], all on this GPU; ids outside 0..experts-1 count for nothing."""
+        torch = _torch()
+        if accumulate and out is None:
+            raise invalid("accumulate needs an output to add to")
+        xp, xd, ldx = matrix(x, "x", self.device, layer.n_embd, _TORCH_DTYPE)
+        m = x.shape[0]
+        ip, _, ldi = matrix(ids, "ids", self.device, layer.top_k, {torch.int32: 0}, m)
+        wp, _, ldw = matrix(weights, "weights", self.device, layer.top_k, {torch.float32: 0}, m)
+        if out is None:
+            out = torch.empty((m, layer.n_embd), dtype=out_dtype or torch.float32, device=x.device)
+        yp, yd, ldy = matrix(out, "out", self.device, layer.n_embd, _TORCH_DTYPE, m)
+        self._check(B.lib().b200q_moe_run(self._h, layer._h, xp, xd, m, ldx, ip, ldi, wp, ldw, yp, yd, ldy,
+                                          B.MOE_ACCUMULATE if accumulate else 0, self._stream_ptr(stream)))
+        return out
 
     # -- host-buffer path (the reference's own boundary: host in, host out) ------------------
     def project_host(self, w: ProjectionWeight, x: np.ndarray, x_dtype: int = B.TYPE_F32, out: np.ndarray | None = None,

@@ -1,0 +1,107 @@
+"""Products whose weights every row picks for itself: expert layers (b200q_moe_*).
+
+A `Backend` makes the handles; they keep their weights and workspaces on its GPU until they are closed.  As everywhere
+in this package PyTorch only holds device memory and streams.
+"""
+from __future__ import annotations
+
+import ctypes
+from ctypes import byref, c_void_p
+
+import numpy as np
+
+from . import _binding as B
+
+
+def invalid(text: str) -> "B.B200QError":
+    return B.B200QError(B.ERR_INVALID_CONFIG, text)
+
+
+class Source:
+    """Contiguous memory that a create or load call copies from: a NumPy array or a torch tensor, on the host or a GPU."""
+
+    def __init__(self, data, what: str, dtype: str):
+        if isinstance(data, np.ndarray):
+            if data.dtype.name != dtype:
+                raise invalid(f"{what} is {data.dtype}, not {dtype}")
+            self.keep = np.ascontiguousarray(data)
+            self.ptr, self.bytes, self.shape = self.keep.ctypes.data, self.keep.nbytes, self.keep.shape
+            return
+        if str(getattr(data, "dtype", "")) != "torch." + dtype:
+            raise invalid(f"{what} is {getattr(data, 'dtype', type(data).__name__)}, not {dtype}")
+        self.keep = data.detach().contiguous()
+        if data.is_cuda:             # the copy runs on a stream of its own: what fills the tensor has to be done
+            import torch
+
+            torch.cuda.current_stream(data.device).synchronize()
+        self.ptr, self.bytes, self.shape = self.keep.data_ptr(), self.keep.numel() * self.keep.element_size(), tuple(self.keep.shape)
+
+
+def matrix(t, what: str, device: int, columns: int, dtypes: dict, rows: int | None = None):
+    """(pointer, dtype id, leading dimension) of a CUDA tensor [rows, columns] whose rows are contiguous."""
+    if not t.is_cuda or t.device.index != device:
+        raise invalid(f"{what} is on {t.device}, not on cuda:{device}")
+    d = dtypes.get(t.dtype)
+    if d is None:
+        raise invalid(f"{what} is {t.dtype}, not one of {', '.join(map(str, dtypes))}")
+    if t.dim() != 2 or t.shape[1] != columns or (rows is not None and t.shape[0] != rows):
+        raise invalid(f"{what} has shape {tuple(t.shape)}, not ({'rows' if rows is None else rows}, {columns})")
+    m = t.shape[0]
+    if columns > 1 and t.stride(1) != 1:
+        raise invalid(f"the rows of {what} are not contiguous")
+    ld = t.stride(0) if m > 1 else columns
+    if ld < columns:
+        raise invalid(f"the rows of {what} overlap")
+    return t.data_ptr(), d, ld
+
+
+class Handle:
+    """An object of the library that a Backend owns."""
+
+    _destroy = ""
+
+    def __init__(self, backend, handle: int):
+        self.backend = backend
+        self._h = c_void_p(handle)
+        backend._children.add(self)
+
+    def close(self) -> None:
+        if self._h:
+            getattr(B.lib(), self._destroy)(self._h)
+            self._h = c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class MoeLayer(Handle):
+    """The experts of one layer, resident on the GPU (b200q_moe_create); `Backend.run_moe` runs them."""
+
+    _destroy = "b200q_moe_destroy"
+
+    def __init__(self, backend, gate, up, down, *, gate_up_type: int, down_type: int, top_k: int, n_embd: int, n_ff: int, max_rows: int,
+                 activation: int, alpha: float, limit: float, gate_bias, up_bias, down_bias):
+        parts = {n: Source(v, n, "uint8") for n, v in (("gate", gate), ("up", up), ("down", down))}
+        per = B.lib().b200q_tensor_storage_bytes(gate_up_type, n_embd * n_ff)
+        if per <= 0 or parts["gate"].bytes % per:
+            raise invalid(f"gate: {parts['gate'].bytes} bytes are no whole number of experts of {n_ff} x {n_embd} weights of type {gate_up_type}")
+        c = B.MoeConfig()
+        c.n_experts, c.top_k, c.n_embd, c.n_ff, c.max_rows = parts["gate"].bytes // per, top_k, n_embd, n_ff, max_rows
+        c.gate_up_type, c.down_type = gate_up_type, down_type
+        for n, s in parts.items():
+            setattr(c, n, s.ptr)
+            setattr(c, n + "_bytes", s.bytes)
+        for n, v, width in (("gate_bias", gate_bias, n_ff), ("up_bias", up_bias, n_ff), ("down_bias", down_bias, n_embd)):
+            if v is not None:
+                s = parts[n] = Source(v, n, "float32")
+                if s.bytes != 4 * c.n_experts * width:
+                    raise invalid(f"{n} has shape {s.shape}, not ({c.n_experts}, {width})")
+                setattr(c, n, s.ptr)
+        c.activation, c.alpha, c.limit = activation, alpha, limit
+        out = c_void_p()
+        backend._check(B.lib().b200q_moe_create(backend._h, byref(c), byref(out)))
+        super().__init__(backend, out.value)
+        self.n_experts, self.top_k, self.n_embd, self.n_ff, self.max_rows = c.n_experts, top_k, n_embd, n_ff, max_rows
