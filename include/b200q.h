@@ -61,6 +61,7 @@ enum {
 /* ggml tensor type ids, the values GGUF files carry (gguf.rs:126 reads them as u32). */
 enum {
     B200Q_TYPE_F32 = 0,
+    B200Q_TYPE_F16 = 1,     /* low-rank adapters */
     B200Q_TYPE_Q4_0 = 2,
     B200Q_TYPE_Q8_0 = 8,
     B200Q_TYPE_Q4_K = 12,
@@ -403,6 +404,63 @@ b200q_status b200q_moe_run(b200q_ctx *ctx, b200q_moe *moe, const void *x_dev, in
                            const int32_t *ids_dev, int64_t ld_ids, const float *weights_dev, int64_t ld_weights,
                            void *y_dev, int32_t y_dtype, int64_t ldy, int32_t flags, void *stream);
 void b200q_moe_destroy(b200q_moe *moe);     /* may follow b200q_ctx_destroy, like b200q_weight_destroy */
+
+/* The router in front of it: logits l = W x[m] + logit_bias, the top_k experts of every row and their weights, in the form
+ * b200q_moe_run takes.  Sums are held in 64 bits, so that the choice depends neither on the batch nor on the order of a sum;
+ * of equal ones the lower index is chosen first.  A NaN among the logits counts as the lowest number, infinities as the largest.
+ * Two calls of one router must not overlap (it has a workspace for max_rows rows; calls allocate nothing). */
+typedef struct b200q_router b200q_router;
+
+enum {
+    B200Q_SCORING_SOFTMAX = 0,     /* weights softmax(l) over all experts; the largest l are chosen */
+    B200Q_SCORING_SIGMOID = 1      /* weights s = 1 / (1 + exp(-l)); the largest s + select_bias are chosen */
+};
+
+typedef struct b200q_router_config {
+    int32_t n_experts;             /* 1..1024 */
+    int32_t top_k;                 /* 1..32, at most n_experts */
+    int64_t n_embd;
+    int64_t max_rows;              /* 1..1048576 */
+    int32_t w_dtype;               /* F32 or BF16 */
+    int32_t scoring;               /* B200Q_SCORING_* */
+    int32_t normalise;             /* non-zero: the chosen weights are divided by their sum */
+    float scale;                   /* factor of the weights, after that */
+    const void *w;                 /* [n_experts][n_embd]; this and the biases: host memory, or device memory whose contents are complete */
+    const float *logit_bias;       /* [n_experts] or NULL */
+    const float *select_bias;      /* [n_experts] or NULL; sigmoid scores only */
+    int32_t reserved;              /* 0 */
+} b200q_router_config;
+
+b200q_status b200q_router_create(b200q_ctx *ctx, const b200q_router_config *config, b200q_router **out);
+/* x[M][n_embd] F32 or BF16 -> ids, weights [M][top_k], in falling order of what they were chosen by; M <= max_rows, M == 0 is a no-op */
+b200q_status b200q_router_run(b200q_ctx *ctx, b200q_router *router, const void *x_dev, int32_t x_dtype, int64_t M, int64_t ldx,
+                              int32_t *ids_dev, int64_t ld_ids, float *weights_dev, int64_t ld_weights, void *stream);
+void b200q_router_destroy(b200q_router *router);
+
+/* -- low-rank adapters ---------------------------------------------------------------------------- */
+
+/* Adapters of many requests at once beside one shared projection (the LoRA adapters that llama.cpp applies to a whole
+ * batch, here one per row): y[m] += scale_a * B_a (A_a x[m]) with a = slots[m], added to what b200q_matmul or a plan left in
+ * y.  A set has numbered slots, which may be empty; adapters are loaded and replaced while the set lives. */
+typedef struct b200q_adapters b200q_adapters;
+
+/* N x K: the projection's shape.  dtype F16 or BF16 is what adapters are kept and multiplied in; ranks up to max_rank <= 256,
+ * 1..65536 slots.  Device memory for all slots is taken here: about max_adapters * max_rank * (N + K) * 2 bytes. */
+b200q_status b200q_adapters_create(b200q_ctx *ctx, int64_t N, int64_t K, int32_t dtype, int32_t max_adapters, int32_t max_rank,
+                                   b200q_adapters **out);
+/* A[rank][K], B[N][rank] (a GGUF adapter's lora_a and lora_b) in host memory, or in device memory whose contents are complete;
+ * rank 0 empties the slot.  Copied before the call returns; no call that uses the slot may be in flight. */
+b200q_status b200q_adapters_load(b200q_ctx *ctx, b200q_adapters *set, int32_t slot, int32_t rank, float scale, const void *A,
+                                 const void *B);
+/* One activation and 1..4 sets of one dtype and K (the adapters of Q, K and V, or of gate and up), one launch: y_i[M][N_i] of the rows whose
+ * slot holds an adapter are added to, other rows (slot -1, beyond the set, or empty) are not touched.  slots_dev [M] in
+ * device memory is read by the launch.  Sums are fp32 over exact products (fp32 activations and, for fp32 outputs, A x enter
+ * with 24 bits, for bf16 outputs A x with 16); a bf16 result is rounded once.  Calls of any sets may overlap that add to
+ * different outputs; a row that holds an infinity or a NaN spoils no other. */
+b200q_status b200q_adapters_apply(b200q_ctx *ctx, const b200q_adapters *const *sets, int32_t n_sets, const void *x_dev,
+                                  int32_t x_dtype, int64_t M, int64_t ldx, const int32_t *slots_dev, void *const *y_dev,
+                                  int32_t y_dtype, const int64_t *ldy, void *stream);
+void b200q_adapters_destroy(b200q_adapters *set);
 
 /* -- tensor parallel exchange ------------------------------------------------------------------ */
 

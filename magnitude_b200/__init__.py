@@ -13,9 +13,12 @@ from ._binding import (  # noqa: F401
     ROUTE_GEMV,
     ROUTE_NONE,
     ROUTE_SKINNY,
+    SCORING_SIGMOID,
+    SCORING_SOFTMAX,
     SPLIT_COLUMN,
     SPLIT_ROW,
     TYPE_BF16,
+    TYPE_F16,
     TYPE_F32,
     TYPE_MXFP4,
     TYPE_Q4_0,
@@ -24,7 +27,7 @@ from ._binding import (  # noqa: F401
     TYPE_Q6_K,
     TYPE_Q8_0,
 )
-from .rows import MoeLayer  # noqa: F401
+from .rows import AdapterSet, MoeLayer, Router  # noqa: F401
 from .projection import (  # noqa: F401
     Backend,
     GgufFile,

@@ -25,7 +25,7 @@ STATUS_NAMES = {
     7: "Timeout",
 }
 
-TYPE_F32, TYPE_Q4_0, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q5_K, TYPE_Q6_K, TYPE_BF16, TYPE_MXFP4 = 0, 2, 8, 12, 13, 14, 30, 39
+TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q5_K, TYPE_Q6_K, TYPE_BF16, TYPE_MXFP4 = 0, 1, 2, 8, 12, 13, 14, 30, 39
 SPLIT_COLUMN, SPLIT_ROW = 0, 1
 ROUTE_NONE, ROUTE_GEMV, ROUTE_SKINNY, ROUTE_GEMM = 0, 1, 2, 3
 
@@ -38,6 +38,26 @@ JOB_ACCUMULATE = 8
 
 MOE_SWIGLU, MOE_SWIGLU_CLAMPED = 0, 1
 MOE_ACCUMULATE = 1
+SCORING_SOFTMAX, SCORING_SIGMOID = 0, 1
+
+
+class RouterConfig(ctypes.Structure):
+    """struct b200q_router_config of include/b200q.h."""
+
+    _fields_ = [
+        ("n_experts", c_int32),
+        ("top_k", c_int32),
+        ("n_embd", c_int64),
+        ("max_rows", c_int64),
+        ("w_dtype", c_int32),
+        ("scoring", c_int32),
+        ("normalise", c_int32),
+        ("scale", ctypes.c_float),
+        ("w", c_void_p),
+        ("logit_bias", c_void_p),
+        ("select_bias", c_void_p),
+        ("reserved", c_int32),
+    ]
 
 
 class MoeConfig(ctypes.Structure):
@@ -146,6 +166,16 @@ SIGNATURES = {
          c_void_p],
     ),
     "b200q_moe_destroy": (None, [c_void_p]),
+    "b200q_router_create": (c_int32, [c_void_p, POINTER(RouterConfig), POINTER(c_void_p)]),
+    "b200q_router_run": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    "b200q_router_destroy": (None, [c_void_p]),
+    "b200q_adapters_create": (c_int32, [c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, POINTER(c_void_p)]),
+    "b200q_adapters_load": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, ctypes.c_float, c_void_p, c_void_p]),
+    "b200q_adapters_apply": (
+        c_int32,
+        [c_void_p, POINTER(c_void_p), c_int32, c_void_p, c_int32, c_int64, c_int64, c_void_p, POINTER(c_void_p), c_int32, POINTER(c_int64), c_void_p],
+    ),
+    "b200q_adapters_destroy": (None, [c_void_p]),
     "b200q_tp_unique_id": (c_int32, [c_void_p]),
     "b200q_tp_init": (c_int32, [c_void_p, c_int32, c_int32, c_void_p]),
     "b200q_allreduce": (c_int32, [c_void_p, c_void_p, c_int64, c_int32, c_void_p]),

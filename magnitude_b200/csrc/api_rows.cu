@@ -1,12 +1,14 @@
-// C-ABI layer of the products whose weights every row picks for itself: expert layers.
+// C-ABI layer of the products whose weights every row picks for itself: expert layers with their routers, low-rank adapters.
 #include <math.h>
 #include <string.h>
 
 #include <algorithm>
 #include <new>
 
+#include "adapters.h"
 #include "context.h"
 #include "moe_types.h"
+#include "router.h"
 
 using namespace b200q;
 
@@ -21,6 +23,27 @@ struct b200q_moe {
     float *gate_bias = nullptr, *up_bias = nullptr, *down_bias = nullptr;
     uint8_t *ws = nullptr;
     MoeBuffers buf{};
+};
+
+struct b200q_router {
+    b200q_ctx *ctx = nullptr;
+    int device = 0;
+    RouterRun run{};                  // what does not change from call to call
+    int64_t max_rows = 0;
+    void *w = nullptr;
+    float *logit_bias = nullptr, *select_bias = nullptr;
+    double *logits = nullptr;
+};
+
+struct b200q_adapters {
+    b200q_ctx *ctx = nullptr;
+    int device = 0;
+    int64_t N = 0, K = 0;
+    int dtype = 0, slots = 0, max_rank = 0;
+    int64_t a_stride = 0, b_stride = 0;
+    uint8_t *a = nullptr, *b = nullptr;
+    int *rank = nullptr;
+    float *scale = nullptr;
 };
 
 namespace {
@@ -183,6 +206,217 @@ b200q_status b200q_moe_run(b200q_ctx *ctx, b200q_moe *moe, const void *x_dev, in
     cudaError_t e = moe_run(r, (cudaStream_t)stream, &launches);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "expert layer launch");
     ctx->last_launches = launches;
+    return B200Q_OK;
+}
+
+// -- routers ------------------------------------------------------------------------------------
+
+b200q_status b200q_router_create(b200q_ctx *ctx, const b200q_router_config *c, b200q_router **out) {
+    b200q_status s = check_ctx(ctx);
+    if (s != B200Q_OK) return s;
+    if (!out) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null out pointer");
+    *out = nullptr;
+    if (!c) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null router description");
+    if (c->reserved != 0) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "router: reserved is not 0");
+    if (!act_type(c->w_dtype)) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "router weights must be F32 (0) or BF16 (30)");
+    if (c->n_experts < 1 || c->n_experts > kRouterMaxExperts || c->top_k < 1 || c->top_k > kRouterMaxTopK || c->top_k > c->n_experts)
+        return fail(ctx, B200Q_ERR_INVALID_CONFIG, "router: 1..%d experts and 1..%d choices (at most the experts); got %d and %d", kRouterMaxExperts,
+                    kRouterMaxTopK, c->n_experts, c->top_k);
+    if (c->n_embd < 1 || c->n_embd > (1 << 20)) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "router: n_embd must be 1..%d", 1 << 20);
+    if (c->max_rows < 1 || c->max_rows > (1 << 20)) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "router: max_rows must be 1..%d", 1 << 20);
+    if (c->scoring != B200Q_SCORING_SOFTMAX && c->scoring != B200Q_SCORING_SIGMOID) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "unknown scoring %d", c->scoring);
+    if (c->scoring == B200Q_SCORING_SOFTMAX && c->select_bias)
+        return fail(ctx, B200Q_ERR_INVALID_CONFIG, "a bias of the choice goes with sigmoid scores; softmax takes logit_bias");
+    if (!isfinite(c->scale)) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "router: scale is not finite");
+    if (!c->w) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null weight pointer");
+    b200q_router *r = new (std::nothrow) b200q_router();
+    if (!r) return fail(ctx, B200Q_ERR_OVERLOADED, "out of host memory");
+    r->ctx = ctx;
+    r->device = ctx->device;
+    r->max_rows = c->max_rows;
+    const size_t elt = act_size(c->w_dtype), row = (size_t)c->n_embd * elt;
+    const int64_t ld = (c->n_embd + 31) / 32 * 32;
+    cudaError_t e = cudaMalloc(&r->w, c->n_experts * ld * elt);
+    if (e == cudaSuccess) e = cudaMemset(r->w, 0, c->n_experts * ld * elt);
+    if (e == cudaSuccess) e = cudaMemcpy2D(r->w, ld * elt, c->w, row, row, c->n_experts, cudaMemcpyDefault);
+    if (e == cudaSuccess) e = upload_floats(c->logit_bias, c->n_experts, &r->logit_bias);
+    if (e == cudaSuccess) e = upload_floats(c->select_bias, c->n_experts, &r->select_bias);
+    if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void **>(&r->logits), (size_t)c->max_rows * c->n_experts * sizeof(double));
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);      // in place before a call on any stream reads it
+    if (e != cudaSuccess) {
+        b200q_router_destroy(r);
+        return cuda_fail(ctx, e, "router upload");
+    }
+    r->run.w = r->w;
+    r->run.w_ld = ld;
+    r->run.w_is_bf16 = c->w_dtype == B200Q_TYPE_BF16;
+    r->run.logit_bias = r->logit_bias;
+    r->run.select_bias = r->select_bias;
+    r->run.experts = c->n_experts;
+    r->run.top_k = c->top_k;
+    r->run.K = (int)c->n_embd;
+    r->run.sigmoid = c->scoring == B200Q_SCORING_SIGMOID;
+    r->run.normalise = c->normalise != 0;
+    r->run.scale = c->scale;
+    r->run.logits = r->logits;
+    *out = r;
+    return B200Q_OK;
+}
+
+void b200q_router_destroy(b200q_router *r) {
+    if (!r) return;
+    cudaSetDevice(r->device);         // not through r->ctx: the context may be gone already
+    for (void *p : {r->w, (void *)r->logit_bias, (void *)r->select_bias, (void *)r->logits})
+        if (p) cudaFree(p);
+    delete r;
+}
+
+b200q_status b200q_router_run(b200q_ctx *ctx, b200q_router *router, const void *x_dev, int32_t x_dtype, int64_t M, int64_t ldx, int32_t *ids_dev, int64_t ld_ids,
+                              float *weights_dev, int64_t ld_weights, void *stream) {
+    b200q_status s = check_ctx(ctx);
+    if (s != B200Q_OK) return s;
+    if (!router) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null router");
+    if (router->ctx != ctx) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "router belongs to another context");
+    if (!act_type(x_dtype)) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "activation dtype must be F32 (0) or BF16 (30)");
+    if (M < 0) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "M < 0");
+    if (M > router->max_rows) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "M=%lld is above the router's max_rows=%lld", (long long)M, (long long)router->max_rows);
+    if (M == 0) return B200Q_OK;
+    if (!x_dev || !ids_dev || !weights_dev) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null activation or output pointer");
+    RouterRun r = router->run;
+    if (ldx < r.K || ld_ids < r.top_k || ld_weights < r.top_k) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "leading dimension smaller than the row");
+    r.x = x_dev;
+    r.ldx = ldx;
+    r.x_is_bf16 = x_dtype == B200Q_TYPE_BF16;
+    r.x_vec = (reinterpret_cast<uintptr_t>(x_dev) & 15) == 0 && (ldx * act_size(x_dtype)) % 16 == 0;
+    r.m = (int)M;
+    r.ids = ids_dev;
+    r.ld_ids = ld_ids;
+    r.weights = weights_dev;
+    r.ld_weights = ld_weights;
+    cudaError_t e = router_run(r, ctx->sm_count, (cudaStream_t)stream);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "router launch");
+    return B200Q_OK;
+}
+
+// -- low-rank adapters ----------------------------------------------------------------------------
+
+b200q_status b200q_adapters_create(b200q_ctx *ctx, int64_t N, int64_t K, int32_t dtype, int32_t max_adapters, int32_t max_rank, b200q_adapters **out) {
+    b200q_status s = check_ctx(ctx);
+    if (s != B200Q_OK) return s;
+    if (!out) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null out pointer");
+    *out = nullptr;
+    if (dtype != B200Q_TYPE_F16 && dtype != B200Q_TYPE_BF16) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "adapter dtype must be F16 (1) or BF16 (30)");
+    if (N < 1 || K < 1 || N > (1 << 24) || K > (1 << 24)) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "adapters: N and K must be 1..%d", 1 << 24);
+    if (max_adapters < 1 || max_adapters > 65536) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "adapters: max_adapters must be 1..65536");
+    if (max_rank < 1 || max_rank > kAdapterMaxRank) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "adapters: max_rank must be 1..%d", kAdapterMaxRank);
+    b200q_adapters *a = new (std::nothrow) b200q_adapters();
+    if (!a) return fail(ctx, B200Q_ERR_OVERLOADED, "out of host memory");
+    a->ctx = ctx;
+    a->device = ctx->device;
+    a->N = N;
+    a->K = K;
+    a->dtype = dtype;
+    a->slots = max_adapters;
+    a->max_rank = max_rank;
+    a->a_stride = adapter_a_bytes(max_rank, K);
+    a->b_stride = adapter_b_bytes(max_rank, N);
+    cudaError_t e = cudaMalloc(reinterpret_cast<void **>(&a->a), a->a_stride * max_adapters);
+    if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void **>(&a->b), a->b_stride * max_adapters);
+    if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void **>(&a->rank), max_adapters * sizeof(int));
+    if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void **>(&a->scale), max_adapters * sizeof(float));
+    if (e == cudaSuccess) e = cudaMemset(a->rank, 0, max_adapters * sizeof(int));
+    if (e == cudaSuccess) e = cudaMemset(a->scale, 0, max_adapters * sizeof(float));
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
+    if (e != cudaSuccess) {
+        b200q_adapters_destroy(a);
+        return cuda_fail(ctx, e, "adapter set");
+    }
+    *out = a;
+    return B200Q_OK;
+}
+
+void b200q_adapters_destroy(b200q_adapters *a) {
+    if (!a) return;
+    cudaSetDevice(a->device);         // not through a->ctx: the context may be gone already
+    for (void *p : {(void *)a->a, (void *)a->b, (void *)a->rank, (void *)a->scale})
+        if (p) cudaFree(p);
+    delete a;
+}
+
+b200q_status b200q_adapters_load(b200q_ctx *ctx, b200q_adapters *set, int32_t slot, int32_t rank, float scale, const void *A, const void *B) {
+    b200q_status s = check_ctx(ctx);
+    if (s != B200Q_OK) return s;
+    if (!set) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null adapter set");
+    if (set->ctx != ctx) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "adapter set belongs to another context");
+    if (slot < 0 || slot >= set->slots) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "slot %d is outside 0..%d", slot, set->slots - 1);
+    if (rank < 0 || rank > set->max_rank) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "rank %d is outside 0..%d", rank, set->max_rank);
+    if (rank > 0 && (!A || !B)) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null adapter pointer");
+    // the slot is empty until its weights are in place
+    const int none = 0;
+    CU_TRY(ctx, cudaMemcpy(set->rank + slot, &none, sizeof(int), cudaMemcpyHostToDevice));
+    if (rank > 0) {
+        const size_t a_bytes = (size_t)rank * set->K * 2, b_bytes = (size_t)rank * set->N * 2, at = (a_bytes + 255) / 256 * 256;
+        uint8_t *stage = nullptr;
+        cudaError_t e = cudaMalloc(reinterpret_cast<void **>(&stage), at + b_bytes);
+        if (e == cudaSuccess) e = cudaMemcpy(stage, A, a_bytes, cudaMemcpyDefault);
+        if (e == cudaSuccess) e = cudaMemcpy(stage + at, B, b_bytes, cudaMemcpyDefault);
+        if (e == cudaSuccess)
+            e = adapter_pack(stage, stage + at, set->a + slot * set->a_stride, set->b + slot * set->b_stride, rank, (int)set->K, (int)set->N, nullptr);
+        if (e == cudaSuccess) e = cudaMemcpy(set->scale + slot, &scale, sizeof(float), cudaMemcpyHostToDevice);
+        if (e == cudaSuccess) e = cudaMemcpy(set->rank + slot, &rank, sizeof(int), cudaMemcpyHostToDevice);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
+        if (stage) cudaFree(stage);
+        if (e != cudaSuccess) return cuda_fail(ctx, e, "adapter upload");
+    }
+    return B200Q_OK;
+}
+
+b200q_status b200q_adapters_apply(b200q_ctx *ctx, const b200q_adapters *const *sets, int32_t n_sets, const void *x_dev, int32_t x_dtype, int64_t M, int64_t ldx,
+                                  const int32_t *slots_dev, void *const *y_dev, int32_t y_dtype, const int64_t *ldy, void *stream) {
+    b200q_status s = check_ctx(ctx);
+    if (s != B200Q_OK) return s;
+    if (!sets || !y_dev || !ldy || n_sets < 1 || n_sets > kAdapterMaxSets) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "adapters_apply takes 1..%d sets", kAdapterMaxSets);
+    if (!act_type(x_dtype) || !act_type(y_dtype)) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "activation/output dtype must be F32 (0) or BF16 (30)");
+    if (M < 0 || M > (1 << 24)) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "M must be 0..%d", 1 << 24);
+    for (int i = 0; i < n_sets; ++i) {
+        if (!sets[i]) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null adapter set");
+        if (sets[i]->ctx != ctx) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "adapter set belongs to another context");
+        if (sets[i]->K != sets[0]->K || sets[i]->dtype != sets[0]->dtype) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "adapter sets of one call must share dtype and K");
+    }
+    if (M == 0) return B200Q_OK;
+    if (!x_dev || !slots_dev) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null activation or slot pointer");
+    if (ldx < sets[0]->K) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "leading dimension smaller than the row");
+    AdaptersParams p{};
+    p.sets = n_sets;
+    p.x = x_dev;
+    p.ldx = ldx;
+    p.x_vec = (reinterpret_cast<uintptr_t>(x_dev) & 15) == 0 && (ldx * act_size(x_dtype)) % 16 == 0;
+    p.K = (int)sets[0]->K;
+    p.kchunks = (p.K + 31) / 32;
+    p.rows = slots_dev;
+    p.m = (int)M;
+    for (int i = 0; i < n_sets; ++i) {
+        if (!y_dev[i]) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null output pointer");
+        if (ldy[i] < sets[i]->N) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "leading dimension smaller than the row");
+        for (int j = 0; j < i; ++j)
+            if (y_dev[j] == y_dev[i]) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "sets %d and %d of one call add to the same output", j, i);
+        AdapterSet &d = p.set[i];
+        d.a = sets[i]->a;
+        d.b = sets[i]->b;
+        d.a_stride = sets[i]->a_stride;
+        d.b_stride = sets[i]->b_stride;
+        d.rank = sets[i]->rank;
+        d.scale = sets[i]->scale;
+        d.slots = sets[i]->slots;
+        d.n = (int)sets[i]->N;
+        d.nchunks = (d.n + 31) / 32;
+        d.y = y_dev[i];
+        d.ldy = ldy[i];
+        d.y_vec = (reinterpret_cast<uintptr_t>(y_dev[i]) & 15) == 0 && (ldy[i] * act_size(y_dtype)) % 16 == 0;
+        p.rank_pad = std::max(p.rank_pad, (sets[i]->max_rank + 15) / 16 * 16);
+    }
+    cudaError_t e = adapters_run(p, sets[0]->dtype == B200Q_TYPE_F16, x_dtype == B200Q_TYPE_F32, y_dtype == B200Q_TYPE_F32, (cudaStream_t)stream);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "adapter launch");
     return B200Q_OK;
 }
 

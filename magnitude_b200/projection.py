@@ -15,7 +15,7 @@ from typing import Sequence
 import numpy as np
 
 from . import _binding as B
-from .rows import MoeLayer, invalid, matrix
+from .rows import AdapterSet, MoeLayer, Router, invalid, matrix
 
 _TORCH_DTYPE = {}
 
@@ -312,6 +312,50 @@ class Backend:
         self._check(B.lib().b200q_moe_run(self._h, layer._h, xp, xd, m, ldx, ip, ldi, wp, ldw, yp, yd, ldy,
                                           B.MOE_ACCUMULATE if accumulate else 0, self._stream_ptr(stream)))
         return out
+
+    def router(self, weight, top_k: int, *, scoring: int = B.SCORING_SOFTMAX, normalise: bool = True, scale: float = 1.0, logit_bias=None,
+               select_bias=None, max_rows: int = 512) -> Router:
+        """The router of an expert layer (b200q_router_create).  weight: float32 or bfloat16 [experts, n_embd]; biases float32 [experts]."""
+        return Router(self, weight, top_k, scoring=scoring, normalise=normalise, scale=scale, logit_bias=logit_bias, select_bias=select_bias,
+                      max_rows=max_rows)
+
+    def route(self, router: Router, x, ids=None, weights=None, stream=None):
+        """Every row's experts (int32) and their weights (float32), both [M, top_k] (b200q_router_run); x [M, n_embd] bf16 or fp32."""
+        torch = _torch()
+        xp, xd, ldx = matrix(x, "x", self.device, router.n_embd, _TORCH_DTYPE)
+        m = x.shape[0]
+        if ids is None:
+            ids = torch.empty((m, router.top_k), dtype=torch.int32, device=x.device)
+        if weights is None:
+            weights = torch.empty((m, router.top_k), dtype=torch.float32, device=x.device)
+        ip, _, ldi = matrix(ids, "ids", self.device, router.top_k, {torch.int32: 0}, m)
+        wp, _, ldw = matrix(weights, "weights", self.device, router.top_k, {torch.float32: 0}, m)
+        self._check(B.lib().b200q_router_run(self._h, router._h, xp, xd, m, ldx, ip, ldi, wp, ldw, self._stream_ptr(stream)))
+        return ids, weights
+
+    def adapters(self, n: int, k: int, dtype, max_adapters: int, max_rank: int) -> AdapterSet:
+        """Slots for the low-rank adapters of an n x k projection (b200q_adapters_create); dtype torch.float16 or torch.bfloat16."""
+        return AdapterSet(self, n, k, dtype, max_adapters, max_rank)
+
+    def apply_adapters(self, sets: Sequence[AdapterSet], x, slots, outs, stream=None):
+        """outs[i][m] += the adapter in slot slots[m] of sets[i] applied to x[m] (b200q_adapters_apply): beside `project` and
+        `project_multi`, whose results outs hold.  slots: int32 [M] on this GPU, -1 for rows without an adapter."""
+        torch = _torch()
+        if not 1 <= len(sets) <= 4 or len(sets) != len(outs):
+            raise invalid("apply_adapters takes 1..4 sets and as many outputs")
+        xp, xd, ldx = matrix(x, "x", self.device, sets[0].k, _TORCH_DTYPE)
+        m = x.shape[0]
+        if slots.dim() != 1 or slots.dtype != torch.int32 or slots.shape[0] != m or not slots.is_cuda or slots.device.index != self.device or (
+                m > 1 and slots.stride(0) != 1):
+            raise invalid(f"slots is {slots.dtype} {tuple(slots.shape)} on {slots.device}, not contiguous int32 ({m},) on cuda:{self.device}")
+        n = len(sets)
+        parts = [matrix(o, "an output", self.device, s.n, _TORCH_DTYPE, m) for s, o in zip(sets, outs)]
+        if any(p[1] != parts[0][1] for p in parts):
+            raise invalid("the outputs of one call are of one dtype")
+        self._check(B.lib().b200q_adapters_apply(
+            self._h, (c_void_p * n)(*[s._h for s in sets]), n, xp, xd, m, ldx, slots.data_ptr(), (c_void_p * n)(*[p[0] for p in parts]),
+            parts[0][1], (c_int64 * n)(*[p[2] for p in parts]), self._stream_ptr(stream)))
+        return outs
 
     # -- host-buffer path (the reference's own boundary: host in, host out) ------------------
     def project_host(self, w: ProjectionWeight, x: np.ndarray, x_dtype: int = B.TYPE_F32, out: np.ndarray | None = None,

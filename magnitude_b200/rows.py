@@ -1,4 +1,5 @@
-"""Products whose weights every row picks for itself: expert layers (b200q_moe_*).
+"""Products whose weights every row picks for itself: expert layers (b200q_moe_*) with their routers (b200q_router_*), and low-rank
+adapters (b200q_adapters_*).
 
 A `Backend` makes the handles; they keep their weights and workspaces on its GPU until they are closed.  As everywhere
 in this package PyTorch only holds device memory and streams.
@@ -105,3 +106,58 @@ class MoeLayer(Handle):
         backend._check(B.lib().b200q_moe_create(backend._h, byref(c), byref(out)))
         super().__init__(backend, out.value)
         self.n_experts, self.top_k, self.n_embd, self.n_ff, self.max_rows = c.n_experts, top_k, n_embd, n_ff, max_rows
+
+
+class Router(Handle):
+    """The router of an expert layer (b200q_router_create); `Backend.route` runs it."""
+
+    _destroy = "b200q_router_destroy"
+
+    def __init__(self, backend, weight, top_k: int, *, scoring: int, normalise: bool, scale: float, logit_bias, select_bias, max_rows: int):
+        bf16 = str(getattr(weight, "dtype", "")) == "torch.bfloat16"
+        w = Source(weight, "weight", "bfloat16" if bf16 else "float32")
+        if len(w.shape) != 2:
+            raise invalid(f"weight has shape {w.shape}, not (experts, n_embd)")
+        c = B.RouterConfig()
+        c.n_experts, c.n_embd = w.shape
+        c.top_k, c.max_rows, c.w_dtype, c.scoring = top_k, max_rows, B.TYPE_BF16 if bf16 else B.TYPE_F32, scoring
+        c.normalise, c.scale, c.w = bool(normalise), scale, w.ptr
+        keep = []
+        for n, v in (("logit_bias", logit_bias), ("select_bias", select_bias)):
+            if v is not None:
+                s = Source(v, n, "float32")
+                if s.bytes != 4 * c.n_experts:
+                    raise invalid(f"{n} has shape {s.shape}, not ({c.n_experts},)")
+                keep.append(s)
+                setattr(c, n, s.ptr)
+        out = c_void_p()
+        backend._check(B.lib().b200q_router_create(backend._h, byref(c), byref(out)))
+        super().__init__(backend, out.value)
+        self.n_experts, self.n_embd, self.top_k, self.max_rows = c.n_experts, c.n_embd, top_k, max_rows
+
+
+class AdapterSet(Handle):
+    """Numbered slots for the low-rank adapters of one projection (b200q_adapters_create); `Backend.apply_adapters` applies them."""
+
+    _destroy = "b200q_adapters_destroy"
+
+    def __init__(self, backend, n: int, k: int, dtype, max_adapters: int, max_rank: int):
+        name = str(dtype).replace("torch.", "")
+        kinds = {"float16": B.TYPE_F16, "bfloat16": B.TYPE_BF16}
+        if name not in kinds:
+            raise invalid(f"adapter dtype {dtype} is not float16 or bfloat16")
+        out = c_void_p()
+        backend._check(B.lib().b200q_adapters_create(backend._h, n, k, kinds[name], max_adapters, max_rank, byref(out)))
+        super().__init__(backend, out.value)
+        self.n, self.k, self.dtype, self.max_adapters, self.max_rank = n, k, name, max_adapters, max_rank
+
+    def load(self, slot: int, a, b, scale: float = 1.0) -> None:
+        """Puts an adapter into a slot: a [rank, k] and b [n, rank] of the set's dtype, on the host or the GPU."""
+        pa, pb = Source(a, "a", self.dtype), Source(b, "b", self.dtype)
+        rank = pa.shape[0] if len(pa.shape) == 2 else -1
+        if pa.shape != (rank, self.k) or pb.shape != (self.n, rank):
+            raise invalid(f"a has shape {pa.shape} and b {pb.shape}, not (rank, {self.k}) and ({self.n}, rank)")
+        self.backend._check(B.lib().b200q_adapters_load(self.backend._h, self._h, slot, rank, scale, pa.ptr, pb.ptr))
+
+    def unload(self, slot: int) -> None:
+        self.backend._check(B.lib().b200q_adapters_load(self.backend._h, self._h, slot, 0, 0.0, None, None))

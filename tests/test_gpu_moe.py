@@ -4,8 +4,8 @@ Tolerances, relative to the row's root mean square r of y (or to |y| where that 
 enter as 16-bit fixed point per 256 elements: a step is largest / 32512, an error at most half of it and, being spread evenly,
 step / sqrt(12) on average; for normal data (largest about 4 sigma) that is 3.6e-5 sigma on x and as much on h, whose error passes
 through the gate's slope (at most 1.1) once.  Summed over independent terms the relative error of a result is of that size, and
-the largest of some ten thousand results lies below 6 of it: 3 * 6 * 3.6e-5 = 6.5e-4, plus half a bf16 step, 2^-9 of the
-value: 2.6e-3 together, 4e-3 with some room for h's longer tails (largest about 10 sigma).  With fp32 results the 31-bit form is exact to
+the largest of some ten thousand results lies below 6 of it: 3 * 6 * 3.6e-5 = 6.5e-4, plus half a bf16 step, 2^-8 = 3.9e-3 of the
+value; h has longer tails than x (largest about 10 sigma instead of 4), so 1e-3 is taken for the first: 4.9e-3 together.  With fp32 results the 31-bit form is exact to
 2^-30 of the largest and fp32 sums of n terms err by about sqrt(n) 2^-24 r: with n of some thousand 4e-6, and 2e-5 is taken; expf
 errs by 2 ulp, less."""
 import numpy as np
@@ -72,7 +72,7 @@ def _check(got, want, bf16):
     got = got.float().cpu().numpy().astype(np.float64)
     rms = np.sqrt(np.mean(want ** 2, axis=1, keepdims=True))
     err = np.abs(got - want) / np.maximum(np.maximum(np.abs(want), rms), 1e-30)
-    assert err.max() <= (4e-3 if bf16 else 2e-5), f"worst relative error {err.max():.2e}"
+    assert err.max() <= (4.9e-3 if bf16 else 2e-5), f"worst relative error {err.max():.2e}"
 
 
 @pytest.mark.parametrize("qt", TYPES)
