@@ -304,9 +304,45 @@ template <int P> __global__ void __launch_bounds__(256) moe_image_kernel(const _
         moe_make_image<P>(p, task, threadIdx.x & 31);
 }
 
-template <typename Kernel, typename Params> cudaError_t launch(Kernel kern, const Params &p, int grid, cudaStream_t st) {
+// y[m] = sum over the row's choices, in their order
+struct MoeCombine {
+    const float *z;
+    long long ld_z;
+    const int *ids;
+    long long ld_ids;
+    const float *weights;
+    long long ld_weights;
+    const float *bias;                   // [expert][n] or null
+    void *y;
+    long long ldy;
+    int y_is_bf16, accumulate, n, m, top_k, experts;
+};
+__global__ void __launch_bounds__(256) moe_combine_kernel(const __grid_constant__ MoeCombine p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int n = blockIdx.x * 256 + threadIdx.x, m = blockIdx.y;
+    if (n >= p.n) return;
+    float sum = 0.f;
+    for (int j = 0; j < p.top_k; ++j) {
+        const int e = p.ids[m * p.ld_ids + j];
+        if ((unsigned)e >= (unsigned)p.experts) continue;
+        float v = p.z[(long long)(m * p.top_k + j) * p.ld_z + n];
+        if (p.bias) v += p.bias[(long long)e * p.n + n];
+        sum = fmaf(p.weights[m * p.ld_weights + j], v, sum);
+    }
+    const long long at = m * p.ldy + n;
+    if (p.y_is_bf16) {
+        __nv_bfloat16 *y = reinterpret_cast<__nv_bfloat16 *>(p.y) + at;
+        *y = __float2bfloat16_rn(p.accumulate ? __bfloat162float(*y) + sum : sum);
+    } else {
+        float *y = reinterpret_cast<float *>(p.y) + at;
+        *y = p.accumulate ? *y + sum : sum;
+    }
+}
+
+template <typename Kernel, typename Params> cudaError_t launch(Kernel kern, const Params &p, dim3 grid, cudaStream_t st) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)grid);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -330,19 +366,16 @@ cudaError_t gate_up_launch(int qt, const MoeGateUp &p, const MoeConfig &c, int g
     default: return moe_gate_up_mxfp4(p, c, grid, st);
     }
 }
-cudaError_t down_launch(int qt, const MoeDown &p, const MoeConfig &c, int grid, size_t z, cudaStream_t st) {
+cudaError_t down_launch(int qt, const MoeDown &p, const MoeConfig &c, int grid, cudaStream_t st) {
     switch (qt) {
-    case QT_Q4_K: return moe_down_q4_k(p, c, grid, z, st);
-    case QT_Q5_K: return moe_down_q5_k(p, c, grid, z, st);
-    case QT_Q6_K: return moe_down_q6_k(p, c, grid, z, st);
-    case QT_Q8_0: return moe_down_q8_0(p, c, grid, z, st);
-    case QT_Q4_0: return moe_down_q4_0(p, c, grid, z, st);
-    default: return moe_down_mxfp4(p, c, grid, z, st);
+    case QT_Q4_K: return moe_down_q4_k(p, c, grid, st);
+    case QT_Q5_K: return moe_down_q5_k(p, c, grid, st);
+    case QT_Q6_K: return moe_down_q6_k(p, c, grid, st);
+    case QT_Q8_0: return moe_down_q8_0(p, c, grid, st);
+    case QT_Q4_0: return moe_down_q4_0(p, c, grid, st);
+    default: return moe_down_mxfp4(p, c, grid, st);
     }
 }
-
-// partial sums of a block's outputs that still fit beside the rings of two blocks an SM
-constexpr size_t kMoeZShared = 16384;
 
 }  // namespace
 
@@ -385,8 +418,7 @@ size_t moe_workspace(const MoeShapeInfo &s, MoeBuffers *out, uint8_t *base) {
     b.h = reinterpret_cast<float *>(take(sizeof(float) * (size_t)(slots * s.n_ff)));
     b.x_img = take((size_t)s.max_rows * ceil_div(s.n_embd, SB) * moe_image_bytes(4));
     b.h_img = take((size_t)slots * ceil_div(s.n_ff, SB) * moe_image_bytes(4));
-    // partial sums that do not fit into shared memory: every block's
-    b.z = reinterpret_cast<float *>(take((size_t)2 * s.sm_count * slots * 16 * sizeof(float)));
+    b.z = reinterpret_cast<float *>(take((size_t)slots * ceil_div(s.n_embd, 16) * 16 * sizeof(float)));
     if (out) *out = b;
     return at;
 }
@@ -415,22 +447,33 @@ cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches) {
     pr.m = r.m;
     pr.top_k = (int)s.top_k;
     pr.experts = (int)s.n_experts;
-    pr.group = c.column_tiles * 8 / c.planes;
+    pr.group = moe_group_rows(c.planes, c.column_tiles);
     pr.lists = r.buf.lists;
     const int prep_grid = 1 + (int)std::min<long long>(ceil_div((long long)r.m * x_rec, 8), 4 * s.sm_count);
     cudaError_t e = c.planes == 2 ? launch(moe_prep_kernel<2>, pr, prep_grid, st) : launch(moe_prep_kernel<4>, pr, prep_grid, st);
     if (e != cudaSuccess) return e;
 
     const int used = (int)std::min<long long>(slots, s.n_experts);      // experts that may have been chosen
+    // Records of a tile are shared by as many warps as it takes to give every warp of the chip work
+    auto product = [&](const uint8_t *w, int qt, int tiles, int nrec, const uint8_t *img, unsigned stride, int per_row) {
+        MoeProduct p{};
+        p.w = w;
+        p.tiles = tiles;
+        p.nrec = nrec;
+        p.expert_bytes = (long long)tiles * nrec * moe_rec_bytes(qt);
+        p.lists = r.buf.lists;
+        p.img = img;
+        p.img_stride = stride;
+        p.slots_per_row = per_row;
+        p.split = 1;
+        while (p.split < moe_max_split(qt, c.planes, c.column_tiles) && 2 * p.split <= nrec && (long long)used * tiles * p.split < 2ll * kMoeWarps * s.sm_count) p.split *= 2;
+        return p;
+    };
+    auto grid_of = [&](const MoeProduct &p) {
+        return (int)std::min<long long>(2 * s.sm_count, (long long)slots * ceil_div(p.tiles, kMoeWarps / p.split));
+    };
     MoeGateUp gu{};
-    gu.w = r.gate_up;
-    gu.tiles = (int)ceil_div(s.n_ff, 8);
-    gu.nrec = x_rec;
-    gu.expert_bytes = (long long)gu.tiles * gu.nrec * moe_rec_bytes(r.gate_up_type);
-    gu.lists = r.buf.lists;
-    gu.img = r.buf.x_img;
-    gu.img_stride = pr.rows.img_stride;
-    gu.top_k = (int)s.top_k;
+    gu.product = product(r.gate_up, r.gate_up_type, (int)ceil_div(s.n_ff, 8), x_rec, r.buf.x_img, pr.rows.img_stride, (int)s.top_k);
     gu.h = r.buf.h;
     gu.ff = (int)s.n_ff;
     gu.activation = r.activation;
@@ -438,10 +481,7 @@ cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches) {
     gu.limit = r.limit;
     gu.gate_bias = r.gate_bias;
     gu.up_bias = r.up_bias;
-    gu.split = 1;
-    while (gu.split < kMoeWarps && 2 * gu.split <= gu.nrec && (long long)used * gu.tiles * gu.split < 8ll * 2 * kMoeWarps * s.sm_count) gu.split *= 2;
-    const int gu_grid = (int)std::min<long long>(2 * s.sm_count, ceil_div((long long)slots * gu.tiles * gu.split, kMoeWarps));
-    if ((e = gate_up_launch(r.gate_up_type, gu, c, gu_grid, st)) != cudaSuccess) return e;
+    if ((e = gate_up_launch(r.gate_up_type, gu, c, grid_of(gu.product), st)) != cudaSuccess) return e;
 
     MoeRows hr{};
     hr.x = r.buf.h;
@@ -461,37 +501,29 @@ cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches) {
     if (e != cudaSuccess) return e;
 
     MoeDown d{};
-    d.w = r.down;
-    d.tiles = (int)ceil_div(s.n_embd, 16);
-    d.nrec = h_rec;
-    d.expert_bytes = (long long)d.tiles * d.nrec * moe_rec_bytes(r.down_type);
-    d.lists = r.buf.lists;
-    d.img = r.buf.h_img;
-    d.img_stride = hr.img_stride;
-    d.top_k = (int)s.top_k;
-    d.experts = (int)s.n_experts;
-    d.ids = r.ids;
-    d.ld_ids = r.ld_ids;
-    d.weights = r.weights;
-    d.ld_weights = r.ld_weights;
-    d.bias = r.down_bias;
-    d.y = r.y;
-    d.ldy = r.ldy;
-    d.y_is_bf16 = r.y_is_bf16;
-    d.accumulate = r.accumulate;
-    d.n = (int)s.n_embd;
-    d.m = r.m;
-    d.split = 1;
-    while (d.split < kMoeWarps && 2 * d.split <= d.nrec && used * d.split < kMoeWarps) d.split *= 2;
-    size_t z = (size_t)d.split * slots * 16 * sizeof(float);
-    if (z > kMoeZShared) {
-        d.z = r.buf.z;
-        d.split = 1;                       // the workspace's parts hold one sum per slot
-        z = 0;
-    }
-    const int d_grid = std::min(2 * s.sm_count, d.tiles);
-    if ((e = down_launch(r.down_type, d, c, d_grid, z, st)) != cudaSuccess) return e;
-    *launches = 4;
+    d.product = product(r.down, r.down_type, (int)ceil_div(s.n_embd, 16), h_rec, r.buf.h_img, hr.img_stride, 1);
+    d.z = r.buf.z;
+    d.ld_z = ceil_div(s.n_embd, 16) * 16;
+    if ((e = down_launch(r.down_type, d, c, grid_of(d.product), st)) != cudaSuccess) return e;
+
+    MoeCombine cb{};
+    cb.z = d.z;
+    cb.ld_z = d.ld_z;
+    cb.ids = r.ids;
+    cb.ld_ids = r.ld_ids;
+    cb.weights = r.weights;
+    cb.ld_weights = r.ld_weights;
+    cb.bias = r.down_bias;
+    cb.y = r.y;
+    cb.ldy = r.ldy;
+    cb.y_is_bf16 = r.y_is_bf16;
+    cb.accumulate = r.accumulate;
+    cb.n = (int)s.n_embd;
+    cb.m = r.m;
+    cb.top_k = (int)s.top_k;
+    cb.experts = (int)s.n_experts;
+    if ((e = launch(moe_combine_kernel, cb, dim3((unsigned)ceil_div(s.n_embd, 256), (unsigned)r.m), st)) != cudaSuccess) return e;
+    *launches = 5;
     return cudaSuccess;
 }
 

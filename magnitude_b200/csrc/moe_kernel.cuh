@@ -6,7 +6,8 @@
 // 16); its integer sums are multiplied by the block's integer scale and added up as integers over the record (Q4_K, Q5_K,
 // Q6_K), or scaled in fp32 (types with an fp16 or power-of-two scale per block), so nothing is multiplied per weight.  The
 // minima of Q4_K and Q5_K are two more MMAs with the sums of the activations' blocks.
-// Warps work alone: each copies its records into a ring of its own with cp.async and waits for nobody.
+// A block takes one group and the records of eight tile rows a step (its warps one each), through a ring of stages that hold the
+// weights and the group's activations; the warps share the activations.
 #pragma once
 
 #include "kernels.h"
@@ -42,29 +43,30 @@ template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile(
 __device__ __forceinline__ int byte_u(uint32_t w, int i) { return (w >> (8 * i)) & 0xFF; }
 __device__ __forceinline__ int byte_s(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
 
-// where a lane finds its column of a column tile: offsets from the images' base
+// where a lane finds its column of a column tile in the group's images: byte offsets
 template <int NT> struct MoeColumns {
-    uint32_t b[NT];          // the bytes of column g (lane >> 2), its t's share
-    uint32_t s[NT];          // the scale of columns 2 t, 2 t + 1
+    int b[NT];               // the bytes of column g (lane >> 2), its t's share
+    int s[NT];               // the scale of columns 2 t, 2 t + 1
     int live;                // column tiles that hold rows
 };
 
+__device__ __forceinline__ uint4 moe_lds(const uint8_t *p) { return *reinterpret_cast<const uint4 *>(p); }
 // the lane's B words of block pair j: x, y of block 2 j, z, w of block 2 j + 1
-template <int P> __device__ __forceinline__ uint4 moe_b(const uint8_t *img, int j) { return *reinterpret_cast<const uint4 *>(img + j * (64 * P)); }
+template <int P> __device__ __forceinline__ uint4 moe_b(const uint8_t *img, int j) { return moe_lds(img + j * (64 * P)); }
 
 // One record: acc[nt][0], [1] += rows g, g + 8 against the column tile's columns 2 t, 2 t + 1 (one plane pair).
-// rec: shared address of the record; img: images' base + offset of the record's image
+// rec: the record, img: the group's images of this record, both in shared memory
 template <int QT, int P, int NT> struct MoeRecord;
 
 // Q4_K, Q5_K
 template <int QT, int P, int NT> struct MoeRecordK {
-    static __device__ __forceinline__ void run(uint32_t rec, int lane, const uint8_t *img, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
+    static __device__ __forceinline__ void run(const uint8_t *rec, int lane, const uint8_t *img, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
         const int g = lane >> 2, t = lane & 3;
         constexpr int kHead = QT == QT_Q5_K ? 2560 : 2048;
         uint4 hd[2], f;
-        hd[0] = lds128(rec + kHead + 16 * g);
-        hd[1] = lds128(rec + kHead + 16 * g + 128);
-        if (QT == QT_Q5_K) f = lds128(rec + 2048 + 16 * lane);
+        hd[0] = moe_lds(rec + kHead + 16 * g);
+        hd[1] = moe_lds(rec + kHead + 16 * g + 128);
+        if (QT == QT_Q5_K) f = moe_lds(rec + 2048 + 16 * lane);
         uint32_t sc[2][2], am[2];            // scales of blocks 0 .. 3, 4 .. 7; minima of blocks 4 t .. as an A word (t < 2)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -80,7 +82,7 @@ template <int QT, int P, int NT> struct MoeRecordK {
             for (int x = 0; x < 4; ++x) even[nt][x] = odd[nt][x] = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint4 q = lds128(rec + 512 * j + 16 * lane);
+            const uint4 q = moe_lds(rec + 512 * j + 16 * lane);
             uint32_t lo[4], hi[4];           // [row g: words 0, 1][row g + 8: words 0, 1]
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -139,10 +141,10 @@ template <int P, int NT> struct MoeRecord<QT_Q4_K, P, NT> : MoeRecordK<QT_Q4_K, 
 template <int P, int NT> struct MoeRecord<QT_Q5_K, P, NT> : MoeRecordK<QT_Q5_K, P, NT> {};
 
 template <int P, int NT> struct MoeRecord<QT_Q6_K, P, NT> {
-    static __device__ __forceinline__ void run(uint32_t rec, int lane, const uint8_t *img, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
+    static __device__ __forceinline__ void run(const uint8_t *rec, int lane, const uint8_t *img, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
         const int g = lane >> 2;
-        const uint4 s0 = lds128(rec + 3072 + 16 * g), s1 = lds128(rec + 3072 + 16 * g + 128);
-        const float d[2] = {half_bits_to_float(lds16(rec + 3328 + 2 * g)) * 0.25f, half_bits_to_float(lds16(rec + 3328 + 2 * g + 16)) * 0.25f};
+        const uint4 s0 = moe_lds(rec + 3072 + 16 * g), s1 = moe_lds(rec + 3072 + 16 * g + 128);
+        const float d[2] = {half_bits_to_float(*reinterpret_cast<const uint16_t *>(rec + 3328 + 2 * g)) * 0.25f, half_bits_to_float(*reinterpret_cast<const uint16_t *>(rec + 3328 + 2 * g + 16)) * 0.25f};
         int sum[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -154,7 +156,7 @@ template <int P, int NT> struct MoeRecord<QT_Q6_K, P, NT> {
             uint32_t w[2][6];
 #pragma unroll
             for (int n = 0; n < 3; ++n) {
-                const uint4 v = lds128(rec + 512 * (3 * h + n) + 16 * lane);
+                const uint4 v = moe_lds(rec + 512 * (3 * h + n) + 16 * lane);
                 w[0][2 * n] = v.x, w[0][2 * n + 1] = v.y, w[1][2 * n] = v.z, w[1][2 * n + 1] = v.w;
             }
 #pragma unroll
@@ -195,15 +197,15 @@ template <int P, int NT> struct MoeRecord<QT_Q6_K, P, NT> {
 
 // types with one scale per 32 weights
 template <int QT, int P, int NT> struct MoeRecordBlock {
-    static __device__ __forceinline__ void run(uint32_t rec, int lane, const uint8_t *img, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
+    static __device__ __forceinline__ void run(const uint8_t *rec, int lane, const uint8_t *img, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
         const int g = lane >> 2;
         uint4 hd[2];                                  // eight fp16 d (MXFP4: eight scale bytes)
         if (QT == QT_MXFP4) {
-            const uint2 e0 = lds64(rec + 2048 + 8 * g), e1 = lds64(rec + 2048 + 8 * g + 64);
+            const uint2 e0 = *reinterpret_cast<const uint2 *>(rec + 2048 + 8 * g), e1 = *reinterpret_cast<const uint2 *>(rec + 2048 + 8 * g + 64);
             hd[0] = make_uint4(e0.x, e0.y, 0, 0), hd[1] = make_uint4(e1.x, e1.y, 0, 0);
         } else {
             constexpr int kHead = QT == QT_Q8_0 ? 4096 : 2048;
-            hd[0] = lds128(rec + kHead + 16 * g), hd[1] = lds128(rec + kHead + 16 * g + 128);
+            hd[0] = moe_lds(rec + kHead + 16 * g), hd[1] = moe_lds(rec + kHead + 16 * g + 128);
         }
         float e[NT][2];
 #pragma unroll
@@ -214,11 +216,11 @@ template <int QT, int P, int NT> struct MoeRecordBlock {
             if (QT == QT_Q8_0) {
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
-                    const uint4 v = lds128(rec + 512 * (2 * j + b) + 16 * lane);
+                    const uint4 v = moe_lds(rec + 512 * (2 * j + b) + 16 * lane);
                     a[b][0] = v.x, a[b][1] = v.y, a[b][2] = v.z, a[b][3] = v.w;
                 }
             } else {
-                const uint4 v = lds128(rec + 512 * j + 16 * lane);
+                const uint4 v = moe_lds(rec + 512 * j + 16 * lane);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t q = word_of(v, i);
@@ -268,44 +270,19 @@ template <int P, int NT> struct MoeRecord<QT_Q8_0, P, NT> : MoeRecordBlock<QT_Q8
 template <int P, int NT> struct MoeRecord<QT_Q4_0, P, NT> : MoeRecordBlock<QT_Q4_0, P, NT> {};
 template <int P, int NT> struct MoeRecord<QT_MXFP4, P, NT> : MoeRecordBlock<QT_MXFP4, P, NT> {};
 
-// The lane's columns of a group: rows beyond the group's last repeat it (their sums are not stored)
-template <int P, int NT> __device__ __forceinline__ MoeColumns<NT> moe_columns(const MoeLists &l, const MoeGroup &grp, int lane, unsigned stride, int top_k) {
+// The lane's columns of a group of n rows: rows beyond the last repeat it (their sums are not stored)
+template <int P, int NT> __device__ __forceinline__ MoeColumns<NT> moe_columns(int n, int lane) {
+    constexpr int IMG = moe_image_bytes(P);
     const int g = lane >> 2, t = lane & 3;
     MoeColumns<NT> c;
-    c.live = (grp.n * P + 7) / 8;
+    c.live = (n * P + 7) / 8;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int in_b = min(nt * (8 / P) + g / P, grp.n - 1), in_s = min(nt * (8 / P) + 2 * t / P, grp.n - 1);
-        c.b[nt] = (unsigned)(l.sorted[grp.first + in_b] / top_k) * stride + (g % P) * 64 + t * 16;
-        c.s[nt] = (unsigned)(l.sorted[grp.first + in_s] / top_k) * stride + P * 272 + 4 * ((2 * t % P) / 2);
+        c.b[nt] = min(nt * (8 / P) + g / P, n - 1) * IMG + (g % P) * 64 + t * 16;
+        c.s[nt] = min(nt * (8 / P) + 2 * t / P, n - 1) * IMG + P * 272 + 4 * ((2 * t % P) / 2);
     }
     return c;
 }
-
-template <int QT> struct MoeRing {
-    static constexpr int REC = moe_rec_bytes(QT), D = moe_depth(QT), kBytes = REC * D;
-    uint32_t at;             // the warp's ring
-    int put = 0, get = 0;
-    __device__ __forceinline__ void fetch(const uint8_t *src, int lane) {      // src null: nothing left, the group stays empty
-        if (src) {
-            const uint32_t dst = at + put * REC;
-#pragma unroll
-            for (int i = 0; i < (REC / 16 + 31) / 32; ++i)
-                if ((REC / 16) % 32 == 0 || i * 32 + lane < REC / 16) cp_async_16(dst + 16 * (i * 32 + lane), src + 16 * (i * 32 + lane));
-        }
-        cp_async_commit();
-        if (++put == D) put = 0;
-    }
-    __device__ __forceinline__ uint32_t wait() {
-        cp_async_wait<D - 1>();
-        __syncwarp();
-        return at + get * REC;
-    }
-    __device__ __forceinline__ void done() {
-        __syncwarp();
-        if (++get == D) get = 0;
-    }
-};
 
 // both plane pairs of a row (P = 4) are added up; every lane of a pair has the sum
 template <int P, int NT> __device__ __forceinline__ void moe_join_planes(float (&acc)[NT][2]) {
@@ -317,62 +294,105 @@ template <int P, int NT> __device__ __forceinline__ void moe_join_planes(float (
     }
 }
 
-// ---- gate, up and the activation function --------------------------------------------------------
-template <int QT, int P, int NT>
-__global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __grid_constant__ MoeGateUp p) {
-    constexpr int REC = moe_rec_bytes(QT), D = moe_depth(QT);
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float part[kMoeWarps][NT][2][32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    pdl_launch_dependents();
-    pdl_wait();
-    const int ws = warp % p.split, teams = gridDim.x * (kMoeWarps / p.split), team = blockIdx.x * (kMoeWarps / p.split) + warp / p.split;
-    const int units = *p.lists.ngroups * p.tiles;
-    MoeRing<QT> ring;
-    ring.at = smem_u32(smem) + warp * MoeRing<QT>::kBytes;
-    int fu = team, fr = ws;                  // what is fetched next
+// A product's part of one block: units (group, run of tiles) in turn, every unit's records a step at a time.  With `split` warps a tile
+// (few tiles in all), a step takes as many records of 8 / split tiles, and the warps' sums are added up in order.
+//   finish(unit's group, tile, acc): one warp per tile, its lanes hold the sums of rows g, g + 8 and columns 2 t, 2 t + 1
+template <int QT, int P, int NT, typename Finish>
+__device__ __forceinline__ void moe_product(const MoeProduct &p, uint8_t *smem, float (*part)[NT][2][32], Finish finish) {
+    constexpr int REC = moe_rec_bytes(QT), D = moe_depth(QT, P, NT), IMG = moe_image_bytes(P), kGroup = moe_group_rows(P, NT);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int split = p.split, per = kMoeWarps / split, ws = warp % split, wt = warp / split;     // the warp's record of a step and tile of a unit
+    const int runs = (p.tiles + per - 1) / per, units = *p.lists.ngroups * runs, steps = (p.nrec + split - 1) / split;
+    const int stage_bytes = moe_stage_bytes(QT, P, NT, split);
+
+    // what is copied next
+    int fu = blockIdx.x, fs = 0, put = 0;
+    const uint8_t *w_src = nullptr;          // the warp's record
+    uint32_t b_src[kMoeChunks];              // the thread's pieces of the images: offsets of the next step's
+    int b_rec[kMoeChunks], b_dst[kMoeChunks];
     auto fetch = [&] {
-        const uint8_t *src = nullptr;
         if (fu < units) {
-            const int grp = fu / p.tiles;
-            src = p.w + p.lists.groups[grp].expert * p.expert_bytes + ((long long)(fu - grp * p.tiles) * p.nrec + fr) * REC;
-            fr += p.split;
-            if (fr >= p.nrec) fr = ws, fu += teams;
+            if (fs == 0) {
+                const int gi = fu / runs, tile = (fu - gi * runs) * per + wt;
+                const MoeGroup grp = p.lists.groups[gi];
+                w_src = tile < p.tiles ? p.w + grp.expert * p.expert_bytes + ((long long)tile * p.nrec + ws) * REC : nullptr;
+#pragma unroll
+                for (int i = 0; i < kMoeChunks; ++i) {
+                    const int piece = i * kMoeThreads + tid, row = piece / (IMG / 16), at = piece - row * (IMG / 16);     // row = (record of the step, row of the group)
+                    const int s = row / grp.n, m = row - s * grp.n;
+                    b_rec[i] = s < split ? s : 0x40000000;
+                    b_dst[i] = (s * kGroup + m) * IMG + at * 16;
+                    b_src[i] = s < split ? (uint32_t)(p.lists.sorted[grp.first + m] / p.slots_per_row) * p.img_stride + s * IMG + at * 16 : 0u;
+                }
+            }
+            uint8_t *stage = smem + put * stage_bytes;
+            if (w_src && fs * split + ws < p.nrec) {
+                const uint32_t dst = smem_u32(stage + warp * REC) + 16 * lane;
+#pragma unroll
+                for (int i = 0; i < (REC / 16 + 31) / 32; ++i)
+                    if ((REC / 16) % 32 == 0 || i * 32 + lane < REC / 16) cp_async_16(dst + 512 * i, w_src + 512 * i + 16 * lane);
+            }
+            if (w_src) w_src += split * REC;
+            const uint32_t img = smem_u32(stage + kMoeWarps * REC);
+#pragma unroll
+            for (int i = 0; i < kMoeChunks; ++i) {
+                if (b_rec[i] < p.nrec) cp_async_16(img + b_dst[i], p.img + b_src[i]);
+                b_rec[i] += split;
+                b_src[i] += split * IMG;
+            }
+            if (++fs == steps) fs = 0, fu += gridDim.x;
         }
-        ring.fetch(src, lane);
+        cp_async_commit();
+        if (++put == D) put = 0;
     };
 #pragma unroll
-    for (int i = 0; i < D; ++i) fetch();
-    for (int u = team; u < units; u += teams) {
-        const int gi = u / p.tiles, tile = u - gi * p.tiles;
+    for (int i = 0; i < D - 1; ++i) fetch();
+    int get = 0;
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+        const int gi = u / runs, tile = (u - gi * runs) * per + wt;
         const MoeGroup grp = p.lists.groups[gi];
-        const MoeColumns<NT> col = moe_columns<P, NT>(p.lists, grp, lane, p.img_stride, p.top_k);
+        const MoeColumns<NT> col = moe_columns<P, NT>(grp.n, lane);
         float acc[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = 0.f;
-        for (int r = ws; r < p.nrec; r += p.split) {
-            const uint32_t rec = ring.wait();
-            MoeRecord<QT, P, NT>::run(rec, lane, p.img + (size_t)r * moe_image_bytes(P), col, acc);
-            ring.done();
+        for (int s = 0; s < steps; ++s) {
+            cp_async_wait<D - 2>();
+            __syncthreads();                 // the stage is here, and the one before it has been read
             fetch();
+            const uint8_t *stage = smem + get * stage_bytes;
+            if (tile < p.tiles && s * split + ws < p.nrec)
+                MoeRecord<QT, P, NT>::run(stage + warp * REC, lane, stage + kMoeWarps * REC + ws * kGroup * IMG, col, acc);
+            if (++get == D) get = 0;
         }
         moe_join_planes<P, NT>(acc);
-        if (p.split > 1) {                   // the team's warps in order
+        if (split > 1) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) part[warp][nt][i][lane] = acc[nt][i];
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / p.split), "r"(32 * p.split) : "memory");
+            __syncthreads();                 // (the next unit's are written after at least one more)
             if (ws == 0) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
-                        for (int s = 1; s < p.split; ++s) acc[nt][i] += part[warp + s][nt][i][lane];
+                        for (int k = 1; k < split; ++k) acc[nt][i] += part[warp + k][nt][i][lane];
             }
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / p.split), "r"(32 * p.split) : "memory");
-            if (ws != 0) continue;
         }
+        if (ws == 0 && tile < p.tiles) finish(grp, tile, acc);
+    }
+    cp_async_wait<0>();
+}
+
+// ---- gate, up and the activation function --------------------------------------------------------
+template <int QT, int P, int NT>
+__global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __grid_constant__ MoeGateUp p) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float part[kMoeWarps][NT][2][32];
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    pdl_launch_dependents();
+    pdl_wait();
+    moe_product<QT, P, NT>(p.product, smem, part, [&](const MoeGroup &grp, int tile, const float (&acc)[NT][2]) {
         const int f = tile * 8 + g;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -390,88 +410,29 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __gri
             } else {
                 h = a / (1.f + expf(-a)) * b;
             }
-            p.h[(long long)p.lists.sorted[grp.first + r] * p.ff + f] = h;
+            p.h[(long long)p.product.lists.sorted[grp.first + r] * p.ff + f] = h;
         }
-    }
-    cp_async_wait<0>();
+    });
 }
 
-// ---- down and the weighted sum --------------------------------------------------------------------
-// A block owns 16 output columns: its warps take (group, part of K) in turn and leave every slot's sums in z; then the rows' outputs
-// are added up in the order of their choices.
+// ---- down ------------------------------------------------------------------------------------------
 template <int QT, int P, int NT>
 __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(const __grid_constant__ MoeDown p) {
-    constexpr int REC = moe_rec_bytes(QT), D = moe_depth(QT);
     extern __shared__ __align__(128) uint8_t smem[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    __shared__ float part[kMoeWarps][NT][2][32];
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     pdl_launch_dependents();
     pdl_wait();
-    const int items = *p.lists.ngroups * p.split, slots = p.m * p.top_k;
-    float *z = p.z ? p.z + (size_t)blockIdx.x * p.split * slots * 16 : reinterpret_cast<float *>(smem + kMoeWarps * MoeRing<QT>::kBytes);
-    MoeRing<QT> ring;
-    ring.at = smem_u32(smem) + warp * MoeRing<QT>::kBytes;
-    int ft = blockIdx.x, fi = warp, fr = warp % p.split;
-    auto fetch = [&] {
-        const uint8_t *src = nullptr;
-        if (fi >= items) fi = warp, fr = warp % p.split, ft += gridDim.x;
-        if (ft < p.tiles && fi < items) {
-            src = p.w + p.lists.groups[fi / p.split].expert * p.expert_bytes + ((long long)ft * p.nrec + fr) * REC;
-            fr += p.split;
-            if (fr >= p.nrec) fi += kMoeWarps, fr = fi % p.split;
-        }
-        ring.fetch(src, lane);
-    };
+    moe_product<QT, P, NT>(p.product, smem, part, [&](const MoeGroup &grp, int tile, const float (&acc)[NT][2]) {
 #pragma unroll
-    for (int i = 0; i < D; ++i) fetch();
-    for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
-        for (int it = warp; it < items; it += kMoeWarps) {
-            const int ws = it % p.split;
-            const MoeGroup grp = p.lists.groups[it / p.split];
-            const MoeColumns<NT> col = moe_columns<P, NT>(p.lists, grp, lane, p.img_stride, 1);
-            float acc[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = 0.f;
-            for (int r = ws; r < p.nrec; r += p.split) {
-                const uint32_t rec = ring.wait();
-                MoeRecord<QT, P, NT>::run(rec, lane, p.img + (size_t)r * moe_image_bytes(P), col, acc);
-                ring.done();
-                fetch();
-            }
-            moe_join_planes<P, NT>(acc);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const int r = nt * (8 / P) + 2 * t / P;
-                if (r >= grp.n || (2 * t) % P) continue;
-                float *dst = z + ((size_t)ws * slots + p.lists.sorted[grp.first + r]) * 16 + g;
-                dst[0] = acc[nt][0];
-                dst[8] = acc[nt][1];
-            }
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = nt * (8 / P) + 2 * t / P;
+            if (r >= grp.n || (2 * t) % P) continue;
+            float *z = p.z + (long long)p.product.lists.sorted[grp.first + r] * p.ld_z + tile * 16 + g;
+            z[0] = acc[nt][0];
+            z[8] = acc[nt][1];
         }
-        __syncthreads();
-        for (int i = threadIdx.x; i < p.m * 16; i += kMoeThreads) {
-            const int m = i >> 4, n = tile * 16 + (i & 15);
-            if (n >= p.n) continue;
-            float sum = 0.f;
-            for (int j = 0; j < p.top_k; ++j) {
-                const int e = p.ids[m * p.ld_ids + j];
-                if ((unsigned)e >= (unsigned)p.experts) continue;
-                float v = 0.f;
-                for (int s = 0; s < p.split; ++s) v += z[((size_t)s * slots + m * p.top_k + j) * 16 + (i & 15)];
-                if (p.bias) v += p.bias[(long long)e * p.n + n];
-                sum = fmaf(p.weights[m * p.ld_weights + j], v, sum);
-            }
-            const long long at = m * p.ldy + n;
-            if (p.y_is_bf16) {
-                __nv_bfloat16 *y = reinterpret_cast<__nv_bfloat16 *>(p.y) + at;
-                *y = __float2bfloat16_rn(p.accumulate ? __bfloat162float(*y) + sum : sum);
-            } else {
-                float *y = reinterpret_cast<float *>(p.y) + at;
-                *y = p.accumulate ? *y + sum : sum;
-            }
-        }
-        __syncthreads();
-    }
-    cp_async_wait<0>();
+    });
 }
 
 template <typename Kernel, typename Params> cudaError_t moe_launch(Kernel kern, const Params &p, int grid, size_t smem, cudaStream_t st) {
@@ -497,15 +458,20 @@ template <typename Kernel, typename Params> cudaError_t moe_launch(Kernel kern, 
 // one source file per weight type (they compile side by side)
 #define MOE_INSTANTIATE(NAME, QT)                                                                                                     \
     namespace b200q {                                                                                                                 \
+    namespace {                                                                                                                       \
+    size_t moe_smem(const MoeProduct &p, const MoeConfig &c) {                                                                          \
+        return (size_t)moe_depth(QT, c.planes, c.column_tiles) * moe_stage_bytes(QT, c.planes, c.column_tiles, p.split);                   \
+    }                                                                                                                                 \
+    }                                                                                                                                 \
     cudaError_t moe_gate_up_##NAME(const MoeGateUp &p, const MoeConfig &c, int grid, cudaStream_t st) {                                 \
-        constexpr size_t smem = kMoeWarps * MoeRing<QT>::kBytes;                                                                        \
+        const size_t smem = moe_smem(p.product, c);                                                                                     \
         if (c.planes == 2) return c.column_tiles == 1 ? moe_launch(moe_gate_up_kernel<QT, 2, 1>, p, grid, smem, st)                     \
                                                       : moe_launch(moe_gate_up_kernel<QT, 2, 4>, p, grid, smem, st);                    \
         return c.column_tiles == 1 ? moe_launch(moe_gate_up_kernel<QT, 4, 1>, p, grid, smem, st)                                        \
                                    : moe_launch(moe_gate_up_kernel<QT, 4, 4>, p, grid, smem, st);                                       \
     }                                                                                                                                 \
-    cudaError_t moe_down_##NAME(const MoeDown &p, const MoeConfig &c, int grid, size_t z_bytes, cudaStream_t st) {                      \
-        const size_t smem = kMoeWarps * MoeRing<QT>::kBytes + z_bytes;                                                                  \
+    cudaError_t moe_down_##NAME(const MoeDown &p, const MoeConfig &c, int grid, cudaStream_t st) {                                      \
+        const size_t smem = moe_smem(p.product, c);                                                                                     \
         if (c.planes == 2) return c.column_tiles == 1 ? moe_launch(moe_down_kernel<QT, 2, 1>, p, grid, smem, st)                        \
                                                       : moe_launch(moe_down_kernel<QT, 2, 4>, p, grid, smem, st);                       \
         return c.column_tiles == 1 ? moe_launch(moe_down_kernel<QT, 4, 1>, p, grid, smem, st)                                           \

@@ -29,9 +29,6 @@ namespace b200q {
 // ---------------------------------------------------------------------------------------------
 constexpr int kMoeWarps = 8, kMoeThreads = 32 * kMoeWarps;
 __host__ __device__ constexpr int moe_rec_bytes(int qt) { return 16 * (qt == QT_Q4_K || qt == QT_Q4_0 ? 144 : qt == QT_Q5_K ? 176 : qt == QT_Q6_K ? 210 : qt == QT_Q8_0 ? 272 : 136); }
-// stages of a warp's ring
-__host__ __device__ constexpr int moe_depth(int qt) { return moe_rec_bytes(qt) <= 2304 ? 4 : moe_rec_bytes(qt) <= 2816 ? 3 : 2; }
-
 // ---------------------------------------------------------------------------------------------
 // Activations
 //
@@ -42,6 +39,28 @@ __host__ __device__ constexpr int moe_depth(int qt) { return moe_rec_bytes(qt) <
 //   [P / 2] fp32: what one unit of the plane pair is worth; padding to 16 bytes
 // ---------------------------------------------------------------------------------------------
 __host__ __device__ constexpr int moe_image_bytes(int planes) { return planes * (256 + 16) + 16; }
+
+// A block's ring: a stage holds eight records and the images of a group's rows, once per record of a tile in it.  As many stages (2 to
+// 4) as leave room for two blocks an SM (half of 228 KB each, less 1 KB that a block costs by itself) beside the warps' sums.
+constexpr int kMoeSmem = 115712, kMoeMaxDepth = 4;
+// 16-byte pieces of a step's images that a thread copies, at most
+constexpr int kMoeChunks = 4;
+__host__ __device__ constexpr int moe_group_rows(int planes, int column_tiles) { return column_tiles * 8 / planes; }
+__host__ __device__ constexpr int moe_part_bytes(int column_tiles) { return kMoeWarps * column_tiles * 256; }
+__host__ __device__ constexpr int moe_stage_bytes(int qt, int planes, int column_tiles, int split) {
+    return kMoeWarps * moe_rec_bytes(qt) + split * moe_group_rows(planes, column_tiles) * moe_image_bytes(planes);
+}
+__host__ __device__ constexpr int moe_depth(int qt, int planes, int column_tiles) {
+    const int d = (kMoeSmem - moe_part_bytes(column_tiles)) / moe_stage_bytes(qt, planes, column_tiles, 1);
+    return d < 2 ? 2 : d > kMoeMaxDepth ? kMoeMaxDepth : d;
+}
+__host__ __device__ constexpr int moe_max_split(int qt, int planes, int column_tiles) {
+    int s = kMoeWarps;
+    while (s > 1 && (s * moe_group_rows(planes, column_tiles) * (moe_image_bytes(planes) / 16) > kMoeChunks * kMoeThreads ||
+                     moe_depth(qt, planes, column_tiles) * moe_stage_bytes(qt, planes, column_tiles, s) > kMoeSmem - moe_part_bytes(column_tiles)))
+        s /= 2;
+    return s;
+}
 
 constexpr int kMoeMaxRows = 512, kMoeMaxTopK = 16, kMoeMaxSlots = kMoeMaxRows * kMoeMaxTopK, kMoeMaxExperts = 1024;
 
@@ -56,14 +75,18 @@ struct MoeLists {
     int *sorted;                         // slots (row * top_k + choice) by expert
 };
 
-struct MoeGateUp {
+struct MoeProduct {
     const uint8_t *w;
     long long expert_bytes;
     int tiles, nrec, split;              // split: warps that share a tile's records
     MoeLists lists;
-    const uint8_t *img;                  // images of the rows
+    const uint8_t *img;                  // images
     unsigned img_stride;                 // bytes of a row's image
-    int top_k;
+    int slots_per_row;                   // slot / slots_per_row = row of the images
+};
+
+struct MoeGateUp {
+    MoeProduct product;
     float *h;                            // [slot][ff]
     int ff;
     int activation;
@@ -72,23 +95,9 @@ struct MoeGateUp {
 };
 
 struct MoeDown {
-    const uint8_t *w;
-    long long expert_bytes;
-    int tiles, nrec, split;
-    MoeLists lists;
-    const uint8_t *img;                  // images of the slots' h
-    unsigned img_stride;
-    int top_k, experts;
-    const int *ids;
-    long long ld_ids;
-    const float *weights;
-    long long ld_weights;
-    const float *bias;                   // [expert][n] or null
-    float *z;                            // [tile of a block][split][slot][16], or null: in shared memory
-    void *y;
-    long long ldy;
-    int y_is_bf16, accumulate;
-    int n, m;                            // output width, rows
+    MoeProduct product;
+    float *z;                            // [slot][ld_z]
+    long long ld_z;
 };
 
 struct MoeConfig {                       // what picks a kernel
@@ -134,7 +143,7 @@ cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches);
 
 #define MOE_DECLARE(NAME)                                                                                     \
     cudaError_t moe_gate_up_##NAME(const MoeGateUp &p, const MoeConfig &c, int grid, cudaStream_t st);          \
-    cudaError_t moe_down_##NAME(const MoeDown &p, const MoeConfig &c, int grid, size_t z_bytes, cudaStream_t st);
+    cudaError_t moe_down_##NAME(const MoeDown &p, const MoeConfig &c, int grid, cudaStream_t st);
 MOE_DECLARE(q4_k)
 MOE_DECLARE(q5_k)
 MOE_DECLARE(q6_k)
