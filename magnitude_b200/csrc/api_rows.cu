@@ -179,6 +179,7 @@ b200q_status b200q_moe_run(b200q_ctx *ctx, b200q_moe *moe, const void *x_dev, in
         return fail(ctx, B200Q_ERR_INVALID_CONFIG, "leading dimension smaller than the row");
     MoeRun r{};
     r.shape = moe->shape;
+    r.status = ctx->status_dev;
     r.buf = moe->buf;
     r.gate_up_type = moe->gate_up_type;
     r.down_type = moe->down_type;

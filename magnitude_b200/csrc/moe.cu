@@ -239,47 +239,48 @@ struct MoePrep {
 // consecutive experts and read all ids.
 __device__ void moe_make_lists(const MoePrep &p) {
     __shared__ int ids[kMoeMaxSlots];
-    __shared__ int2 sums[8];
+    __shared__ int sums[8];
     const int slots = p.m * p.top_k, tid = threadIdx.x, lane = tid & 31;
     for (int s = tid; s < slots; s += 256) ids[s] = p.ids[s / p.top_k * p.ld_ids + s % p.top_k];
     __syncthreads();
     const int per = (p.experts + 255) / 256, e0 = tid * per;
     int count[kMoeMaxExperts / 256];
-    int2 mine = make_int2(0, 0);         // slots, groups
+    int mine = 0;                        // groups
 #pragma unroll
     for (int i = 0; i < kMoeMaxExperts / 256; ++i) {
         count[i] = 0;
         if (i < per && e0 + i < p.experts) {
             for (int s = 0; s < slots; ++s) count[i] += ids[s] == e0 + i;
-            mine.x += count[i];
-            mine.y += (count[i] + p.group - 1) / p.group;
+            mine += (count[i] + p.group - 1) / p.group;
         }
     }
-    int2 run = mine;
+    int run = mine;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
-        const int x = __shfl_up_sync(0xFFFFFFFFu, run.x, d), y = __shfl_up_sync(0xFFFFFFFFu, run.y, d);
-        if (lane >= d) run.x += x, run.y += y;
+        const int y = __shfl_up_sync(0xFFFFFFFFu, run, d);
+        if (lane >= d) run += y;
     }
     if (lane == 31) sums[tid >> 5] = run;
     __syncthreads();
-    int2 at = make_int2(run.x - mine.x, run.y - mine.y);
-    for (int w = 0; w < (tid >> 5); ++w) at.x += sums[w].x, at.y += sums[w].y;
-    if (tid == 255) *p.lists.ngroups = at.y + mine.y;
+    int at = run - mine;
+    for (int w = 0; w < (tid >> 5); ++w) at += sums[w];
+    if (tid == 255) *p.lists.ngroups = at + mine;
 #pragma unroll
     for (int i = 0; i < kMoeMaxExperts / 256; ++i) {
         if (i >= per || count[i] == 0) continue;
-        const int first = at.x;
+        int n = 0;
         for (int s = 0; s < slots; ++s)
-            if (ids[s] == e0 + i) p.lists.sorted[at.x++] = s;
-        for (int done = 0; done < count[i]; done += p.group) {
-            MoeGroup g;
-            g.expert = e0 + i;
-            g.first = first + done;
-            g.n = min(p.group, count[i] - done);
-            g.reserved = 0;
-            p.lists.groups[at.y++] = g;
-        }
+            if (ids[s] == e0 + i) {
+                MoeGroup &g = p.lists.groups[at];
+                g.slot[n++] = s;
+                --count[i];
+                if (n == p.group || count[i] == 0) {
+                    g.expert = e0 + i;
+                    g.n = n;
+                    n = 0;
+                    ++at;
+                }
+            }
     }
 }
 
@@ -414,7 +415,6 @@ size_t moe_workspace(const MoeShapeInfo &s, MoeBuffers *out, uint8_t *base) {
     MoeBuffers b{};
     b.lists.ngroups = reinterpret_cast<int *>(take(sizeof(int)));
     b.lists.groups = reinterpret_cast<MoeGroup *>(take(sizeof(MoeGroup) * (size_t)slots));
-    b.lists.sorted = reinterpret_cast<int *>(take(sizeof(int) * (size_t)slots));
     b.h = reinterpret_cast<float *>(take(sizeof(float) * (size_t)(slots * s.n_ff)));
     b.x_img = take((size_t)s.max_rows * ceil_div(s.n_embd, SB) * moe_image_bytes(4));
     b.h_img = take((size_t)slots * ceil_div(s.n_ff, SB) * moe_image_bytes(4));
@@ -465,6 +465,7 @@ cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches) {
         p.img = img;
         p.img_stride = stride;
         p.slots_per_row = per_row;
+        p.status = r.status;
         p.split = 1;
         while (p.split < moe_max_split(qt, c.planes, c.column_tiles) && 2 * p.split <= nrec && (long long)used * tiles * p.split < 2ll * kMoeWarps * s.sm_count) p.split *= 2;
         return p;
@@ -524,6 +525,13 @@ cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches) {
     cb.experts = (int)s.n_experts;
     if ((e = launch(moe_combine_kernel, cb, dim3((unsigned)ceil_div(s.n_embd, 256), (unsigned)r.m), st)) != cudaSuccess) return e;
     *launches = 5;
+    return cudaSuccess;
+}
+
+cudaError_t moe_set_wait_limit_ns(unsigned long long ns) {
+    cudaError_t e;
+    for (auto set : {moe_wait_limit_q4_k, moe_wait_limit_q5_k, moe_wait_limit_q6_k, moe_wait_limit_q8_0, moe_wait_limit_q4_0, moe_wait_limit_mxfp4})
+        if ((e = set(ns)) != cudaSuccess) return e;
     return cudaSuccess;
 }
 

@@ -6,8 +6,8 @@
 // 16); its integer sums are multiplied by the block's integer scale and added up as integers over the record (Q4_K, Q5_K,
 // Q6_K), or scaled in fp32 (types with an fp16 or power-of-two scale per block), so nothing is multiplied per weight.  The
 // minima of Q4_K and Q5_K are two more MMAs with the sums of the activations' blocks.
-// A block takes one group and the records of eight tile rows a step (its warps one each), through a ring of stages that hold the
-// weights and the group's activations; the warps share the activations.
+// A block takes one group and the records of eight tile rows a step: a producer warp copies the weights and the group's activations
+// into a ring of stages, eight warps multiply, one record each, and share the activations.
 #pragma once
 
 #include "kernels.h"
@@ -16,54 +16,83 @@
 namespace b200q {
 namespace {
 
-// D = A (16 x 32 bytes) * B (32 x 8 signed bytes)
-template <bool SIGNED> __device__ __forceinline__ void moe_mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+// D += A (16 x 32 bytes) * B (32 x 8 signed bytes); first: D = A * B
+template <bool SIGNED> __device__ __forceinline__ void moe_mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, bool first) {
+    const int c0 = first ? 0 : d[0], c1 = first ? 0 : d[1], c2 = first ? 0 : d[2], c3 = first ? 0 : d[3];
     if (SIGNED)
-        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
             : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
     else
-        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
             : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
 }
-// D = A (16 x 16 signed bytes) * B (16 x 8)
-__device__ __forceinline__ void moe_mma16(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-    asm("mma.sync.aligned.m16n8k16.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%7, %7, %7, %7};"
+// D += A (16 x 16 signed bytes) * B (16 x 8)
+__device__ __forceinline__ void moe_mma16(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0, bool first) {
+    const int c0 = first ? 0 : d[0], c1 = first ? 0 : d[1], c2 = first ? 0 : d[2], c3 = first ? 0 : d[3];
+    asm("mma.sync.aligned.m16n8k16.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%7, %8, %9, %10};"
         : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-        : "r"(a0), "r"(a1), "r"(b0), "r"(0));
+        : "r"(a0), "r"(a1), "r"(b0), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
 }
 
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ int byte_u(uint32_t w, int i) { return __byte_perm(w, 0u, 0x4440 | i); }
+// (the upper bit of a selector's digit repeats the byte's sign; __byte_perm leaves it out)
+__device__ __forceinline__ int byte_s(uint32_t w, int i) {
+    int v;
+    asm("prmt.b32 %0, %1, 0, %2;" : "=r"(v) : "r"(w), "r"(0x1111 * i | 0x8880));
+    return v;
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-__device__ __forceinline__ int byte_u(uint32_t w, int i) { return (w >> (8 * i)) & 0xFF; }
-__device__ __forceinline__ int byte_s(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
+// How a warp's columns are used.  NL column tiles hold 8 / P rows each.  A group of few rows needs only half or a quarter
+// of one tile: then the columns also tell F blocks apart (column = class F, row, plane; class f holds blocks f, f + F, .. and zeros for the
+// others), F MMAs add up into the same sums, and a lane has 1 / F of the scaling to do.
+template <int NL_, int F_> struct MoeMode {
+    static constexpr int NL = NL_, F = F_;
+};
 
-// where a lane finds its column of a column tile in the group's images: byte offsets
+// where a lane finds its column in the group's images: byte offsets
 template <int NT> struct MoeColumns {
     int b[NT];               // the bytes of column g (lane >> 2), its t's share
     int s[NT];               // the scale of columns 2 t, 2 t + 1
-    int live;                // column tiles that hold rows
+    int classes, class_b, class_s;      // F; the class of column g, of columns 2 t, 2 t + 1
+    int row;                 // the row of columns 2 t, 2 t + 1 of the first tile; -1: the lane has nothing to store
 };
 
 __device__ __forceinline__ uint4 moe_lds(const uint8_t *p) { return *reinterpret_cast<const uint4 *>(p); }
 // the lane's B words of block pair j: x, y of block 2 j, z, w of block 2 j + 1
 template <int P> __device__ __forceinline__ uint4 moe_b(const uint8_t *img, int j) { return moe_lds(img + j * (64 * P)); }
+template <int P> __device__ __forceinline__ uint2 moe_b_block(const uint8_t *img, int b) { return *reinterpret_cast<const uint2 *>(img + (b >> 1) * (64 * P) + 8 * (b & 1)); }
 
-// One record: acc[nt][0], [1] += rows g, g + 8 against the column tile's columns 2 t, 2 t + 1 (one plane pair).
-// rec: the record, img: the group's images of this record, both in shared memory
-template <int QT, int P, int NT> struct MoeRecord;
+// One record: acc[nt][0], [1] += rows g, g + 8 against columns 2 t, 2 t + 1 (one plane pair) of column tile nt.
+// rec: the record, img: the group's images of this record, zero: as many zeros, all in shared memory
+template <int QT, int P> struct MoeRecord;
 
 // Q4_K, Q5_K
-template <int QT, int P, int NT> struct MoeRecordK {
-    static __device__ __forceinline__ void run(const uint8_t *rec, int lane, const uint8_t *img, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
+template <int QT, int P> struct MoeRecordK {
+    // A words of blocks 2 j (low nibbles) and 2 j + 1: [row g: words 0, 1][row g + 8: words 0, 1]
+    static __device__ __forceinline__ void words(const uint8_t *rec, int lane, int j, const uint4 &f, uint32_t (&lo)[4], uint32_t (&hi)[4]) {
+        const uint4 q = moe_lds(rec + 512 * j + 16 * lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t v = word_of(q, i);
+            if (QT == QT_Q4_K) {
+                lo[i] = v & 0x0F0F0F0Fu;
+                hi[i] = v & 0xF0F0F0F0u;         // 16 x level
+            } else {
+                const uint32_t b = word_of(f, i);
+                const uint32_t b0 = 2 * j < 4 ? b << (4 - 2 * j) : b >> (2 * j - 4), b1 = 2 * j + 1 < 4 ? b << (3 - 2 * j) : b >> (2 * j - 3);
+                lo[i] = (v & 0x0F0F0F0Fu) | (b0 & 0x10101010u);
+                hi[i] = ((v >> 4) & 0x0F0F0F0Fu) | (b1 & 0x10101010u);
+            }
+        }
+    }
+    template <typename Mode, int NT>
+    static __device__ __forceinline__ void run(const uint8_t *rec, int lane, const uint8_t *img, const uint8_t *zero, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
+        constexpr int NL = Mode::NL, F = Mode::F;
         const int g = lane >> 2, t = lane & 3;
         constexpr int kHead = QT == QT_Q5_K ? 2560 : 2048;
-        uint4 hd[2], f;
+        uint4 hd[2], f = make_uint4(0, 0, 0, 0);
         hd[0] = moe_lds(rec + kHead + 16 * g);
         hd[1] = moe_lds(rec + kHead + 16 * g + 128);
         if (QT == QT_Q5_K) f = moe_lds(rec + 2048 + 16 * lane);
@@ -75,79 +104,98 @@ template <int QT, int P, int NT> struct MoeRecordK {
             const uint32_t m1 = ((hd[i].w >> 4) & 0x0F0F0F0Fu) | ((hd[i].z >> 2) & 0x30303030u);
             am[i] = t == 0 ? hd[i].z & 0x3F3F3F3Fu : t == 1 ? m1 : 0u;
         }
-        int even[NT][4], odd[NT][4];         // Q4_K: high nibbles enter as 16 x level and are added up apart
+        int sum[NL][4];
+        float scale = 1.f;
+        if (F == 1) {
+            int odd[NL][4];                  // Q4_K: high nibbles are added up apart
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+            for (int j = 0; j < 4; ++j) {
+                uint32_t lo[4], hi[4];
+                words(rec, lane, j, f, lo, hi);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) even[nt][x] = odd[nt][x] = 0;
+                for (int nt = 0; nt < NL; ++nt) {
+                    const uint4 b = moe_b<P>(img + col.b[nt], j);
+                    int c[4];
+                    moe_mma<false>(c, lo[0], lo[2], lo[1], lo[3], b.x, b.y, true);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint4 q = moe_lds(rec + 512 * j + 16 * lane);
-            uint32_t lo[4], hi[4];           // [row g: words 0, 1][row g + 8: words 0, 1]
+                    for (int x = 0; x < 4; ++x) sum[nt][x] = (j ? sum[nt][x] : 0) + c[x] * byte_u(sc[x >> 1][j >> 1], 2 * (j & 1));
+                    moe_mma<false>(c, hi[0], hi[2], hi[1], hi[3], b.z, b.w, true);
+                    int(&o)[4] = QT == QT_Q4_K ? odd[nt] : sum[nt];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t v = word_of(q, i);
-                if (QT == QT_Q4_K) {
-                    lo[i] = v & 0x0F0F0F0Fu;
-                    hi[i] = v & 0xF0F0F0F0u;
-                } else {
-                    const uint32_t b = word_of(f, i);
-                    const uint32_t b0 = 2 * j < 4 ? b << (4 - 2 * j) : b >> (2 * j - 4), b1 = 2 * j + 1 < 4 ? b << (3 - 2 * j) : b >> (2 * j - 3);
-                    lo[i] = (v & 0x0F0F0F0Fu) | (b0 & 0x10101010u);
-                    hi[i] = ((v >> 4) & 0x0F0F0F0Fu) | (b1 & 0x10101010u);
+                    for (int x = 0; x < 4; ++x) o[x] = (j || QT != QT_Q4_K ? o[x] : 0) + c[x] * byte_u(sc[x >> 1][j >> 1], 2 * (j & 1) + 1);
                 }
             }
+            if (QT == QT_Q4_K) {
+                scale = 0.0625f;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                if (nt > 0 && nt >= col.live) break;
-                const uint4 b = moe_b<P>(img + col.b[nt], j);
-                int c[4];
-                moe_mma<false>(c, lo[0], lo[2], lo[1], lo[3], b.x, b.y);
+                for (int nt = 0; nt < NL; ++nt)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) even[nt][x] += c[x] * byte_u(sc[x >> 1][j >> 1], 2 * (j & 1));
-                moe_mma<false>(c, hi[0], hi[2], hi[1], hi[3], b.z, b.w);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) odd[nt][x] += c[x] * byte_u(sc[x >> 1][j >> 1], 2 * (j & 1) + 1);
+                    for (int x = 0; x < 4; ++x) sum[nt][x] = 16 * sum[nt][x] + odd[nt][x];
             }
+        } else {
+            const uint8_t *bp[F];
+#pragma unroll
+            for (int r = 0; r < F; ++r) bp[r] = r == col.class_b ? img + col.b[0] : zero;
+            int c[8 / F][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t lo[4], hi[4];
+                words(rec, lane, j, f, lo, hi);
+                const uint2 b0 = moe_b_block<P>(bp[2 * j % F], 2 * j), b1 = moe_b_block<P>(bp[(2 * j + 1) % F], 2 * j + 1);
+                moe_mma<false>(c[2 * j / F], lo[0], lo[2], lo[1], lo[3], b0.x, b0.y, 2 * j % F == 0);
+                moe_mma<false>(c[2 * j / F], hi[0], hi[2], hi[1], hi[3], b1.x, b1.y, false);
+            }
+            // the lane's blocks: F q + class
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sum[0][x] = 0;
+#pragma unroll
+            for (int q = 0; q < 8 / F; ++q)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) sum[0][x] += c[q][x] * byte_u(sc[x >> 1][q * F / 4], q * F % 4 + col.class_s);
+            if (QT == QT_Q4_K && (col.class_s & 1)) scale = 0.0625f;
         }
-        const float scale = QT == QT_Q4_K ? 0.0625f : 1.f;
         float d[2], dmin[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             d[i] = half_bits_to_float(hd[i].x) * scale;
-            dmin[i] = half_bits_to_float(hd[i].x >> 16);
+            dmin[i] = F == 1 || col.class_s == 0 ? half_bits_to_float(hd[i].x >> 16) : 0.f;
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            if (nt > 0 && nt >= col.live) break;
-            // block sums 64 a + b: lanes t < 2 bring a and b of blocks 4 t .. 4 t + 3, the others' A words are zero
-            const uint2 bs = *reinterpret_cast<const uint2 *>(img + col.b[nt] + 256 * P - 48 * (g % P) - 16 * t + 8 * (t & 1));
+        for (int nt = 0; nt < NL; ++nt) {
+            // block sums 64 a + b: lanes t < 2 bring a and b of blocks 4 t .. 4 t + 3, the others' A words are zero.  (class F's bytes begin
+            // where the image does, so the plane follows from the offset)
+            const int plane = F == 1 ? g % P : g % (8 / F) % P;
+            const uint2 bs = *reinterpret_cast<const uint2 *>(img + col.b[nt] + 256 * P - 48 * plane - 16 * t + 8 * (t & 1));
             int ma[4], mb[4];
-            moe_mma<false>(ma, am[0], am[1], 0u, 0u, bs.x, 0u);
-            moe_mma<false>(mb, am[0], am[1], 0u, 0u, bs.y, 0u);
+            moe_mma<false>(ma, am[0], am[1], 0u, 0u, bs.x, 0u, true);
+            moe_mma<false>(mb, am[0], am[1], 0u, 0u, bs.y, 0u, true);
             const float s = *reinterpret_cast<const float *>(img + col.s[nt]);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int v0 = QT == QT_Q4_K ? 16 * even[nt][2 * i] + odd[nt][2 * i] : even[nt][2 * i] + odd[nt][2 * i];
-                const int v1 = QT == QT_Q4_K ? 16 * even[nt][2 * i + 1] + odd[nt][2 * i + 1] : even[nt][2 * i + 1] + odd[nt][2 * i + 1];
-                const float v = fmaf(256.f, (float)v0, (float)v1);
+                const float v = fmaf(256.f, (float)sum[nt][2 * i], (float)sum[nt][2 * i + 1]);
                 const float m = fmaf(256.f, (float)(64 * ma[2 * i] + mb[2 * i]), (float)(64 * ma[2 * i + 1] + mb[2 * i + 1]));
                 acc[nt][i] = fmaf(s, fmaf(d[i], v, -dmin[i] * m), acc[nt][i]);
             }
         }
     }
 };
-template <int P, int NT> struct MoeRecord<QT_Q4_K, P, NT> : MoeRecordK<QT_Q4_K, P, NT> {};
-template <int P, int NT> struct MoeRecord<QT_Q5_K, P, NT> : MoeRecordK<QT_Q5_K, P, NT> {};
+template <int P> struct MoeRecord<QT_Q4_K, P> : MoeRecordK<QT_Q4_K, P> {};
+template <int P> struct MoeRecord<QT_Q5_K, P> : MoeRecordK<QT_Q5_K, P> {};
 
-template <int P, int NT> struct MoeRecord<QT_Q6_K, P, NT> {
-    static __device__ __forceinline__ void run(const uint8_t *rec, int lane, const uint8_t *img, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
+template <int P> struct MoeRecord<QT_Q6_K, P> {
+    template <typename Mode, int NT>
+    static __device__ __forceinline__ void run(const uint8_t *rec, int lane, const uint8_t *img, const uint8_t *zero, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
+        constexpr int NL = Mode::NL, F = Mode::F;
         const int g = lane >> 2;
         const uint4 s0 = moe_lds(rec + 3072 + 16 * g), s1 = moe_lds(rec + 3072 + 16 * g + 128);
-        const float d[2] = {half_bits_to_float(*reinterpret_cast<const uint16_t *>(rec + 3328 + 2 * g)) * 0.25f, half_bits_to_float(*reinterpret_cast<const uint16_t *>(rec + 3328 + 2 * g + 16)) * 0.25f};
-        int sum[NT][4];
+        const float d[2] = {half_bits_to_float(*reinterpret_cast<const uint16_t *>(rec + 3328 + 2 * g)) * 0.25f,
+                            half_bits_to_float(*reinterpret_cast<const uint16_t *>(rec + 3328 + 2 * g + 16)) * 0.25f};
+        const uint8_t *bp[F];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int r = 0; r < F; ++r) bp[r] = F == 1 || r == col.class_b ? img + col.b[0] : zero;
+        int sum[NL][4];
+#pragma unroll
+        for (int nt = 0; nt < NL; ++nt)
 #pragma unroll
             for (int x = 0; x < 4; ++x) sum[nt][x] = 0;
 #pragma unroll
@@ -171,23 +219,32 @@ template <int P, int NT> struct MoeRecord<QT_Q6_K, P, NT> {
                     a[r][2] = z & 0xFCFCFCFCu;
                     a[r][3] = ((x << 6) & 0xC0C0C0C0u) | ((y << 4) & 0x30303030u) | ((z << 2) & 0x0C0C0C0Cu);
                 }
+                if (F == 1) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    if (nt > 0 && nt >= col.live) break;
-                    const uint4 b = moe_b<P>(img + col.b[nt], j);
+                    for (int nt = 0; nt < NL; ++nt) {
+                        const uint4 b = moe_b<P>(img + col.b[nt], j);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        int c[4];
-                        moe_mma16(c, a[0][e], a[1][e], word_of(b, e));
+                        for (int e = 0; e < 4; ++e) {
+                            int c[4];
+                            moe_mma16(c, a[0][e], a[1][e], word_of(b, e), true);
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) sum[nt][x] += c[x] * byte_s(word_of(x < 2 ? s0 : s1, j), e);
+                            for (int x = 0; x < 4; ++x) sum[nt][x] += c[x] * byte_s(word_of(x < 2 ? s0 : s1, j), e);
+                        }
                     }
+                } else {
+                    int c[4 / F][4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        moe_mma16(c[e / F], a[0][e], a[1][e], *reinterpret_cast<const uint32_t *>(bp[e % F] + j * (64 * P) + 4 * e), e % F == 0);
+#pragma unroll
+                    for (int q = 0; q < 4 / F; ++q)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) sum[0][x] += c[q][x] * byte_s(word_of(x < 2 ? s0 : s1, j), q * F + col.class_s);
                 }
             }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            if (nt > 0 && nt >= col.live) break;
+        for (int nt = 0; nt < NL; ++nt) {
             const float s = *reinterpret_cast<const float *>(img + col.s[nt]);
 #pragma unroll
             for (int i = 0; i < 2; ++i) acc[nt][i] = fmaf(s, d[i] * fmaf(256.f, (float)sum[nt][2 * i], (float)sum[nt][2 * i + 1]), acc[nt][i]);
@@ -196,8 +253,15 @@ template <int P, int NT> struct MoeRecord<QT_Q6_K, P, NT> {
 };
 
 // types with one scale per 32 weights
-template <int QT, int P, int NT> struct MoeRecordBlock {
-    static __device__ __forceinline__ void run(const uint8_t *rec, int lane, const uint8_t *img, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
+template <int QT, int P> struct MoeRecordBlock {
+    // scale of block k of a row from its header
+    static __device__ __forceinline__ float scale_of(const uint4 &hd, int k) {
+        if (QT == QT_MXFP4) return __uint_as_float(e8m0_half_bits(byte_u(k < 4 ? hd.x : hd.y, k & 3)));
+        return half_bits_to_float((k < 4 ? (k < 2 ? hd.x : hd.y) : (k < 6 ? hd.z : hd.w)) >> (16 * (k & 1)));
+    }
+    template <typename Mode, int NT>
+    static __device__ __forceinline__ void run(const uint8_t *rec, int lane, const uint8_t *img, const uint8_t *zero, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
+        constexpr int NL = Mode::NL, F = Mode::F;
         const int g = lane >> 2;
         uint4 hd[2];                                  // eight fp16 d (MXFP4: eight scale bytes)
         if (QT == QT_MXFP4) {
@@ -207,9 +271,13 @@ template <int QT, int P, int NT> struct MoeRecordBlock {
             constexpr int kHead = QT == QT_Q8_0 ? 4096 : 2048;
             hd[0] = moe_lds(rec + kHead + 16 * g), hd[1] = moe_lds(rec + kHead + 16 * g + 128);
         }
-        float e[NT][2];
+        const uint8_t *bp[F];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) e[nt][0] = e[nt][1] = 0.f;
+        for (int r = 0; r < F; ++r) bp[r] = F == 1 || r == col.class_b ? img + col.b[0] : zero;
+        float e[NL][2];
+#pragma unroll
+        for (int nt = 0; nt < NL; ++nt) e[nt][0] = e[nt][1] = 0.f;
+        int cf[F == 1 ? 1 : 8 / F][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             uint32_t a[2][4];                         // blocks 2 j, 2 j + 1: [row g: words 0, 1][row g + 8: words 0, 1]
@@ -234,170 +302,234 @@ template <int QT, int P, int NT> struct MoeRecordBlock {
                     }
                 }
             }
-            float d[2][2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const int k = 2 * j + b;
-                    if (QT == QT_MXFP4) d[r][b] = __uint_as_float(e8m0_half_bits(byte_u(k < 4 ? hd[r].x : hd[r].y, k & 3)));
-                    else d[r][b] = half_bits_to_float(word_of(hd[r], j) >> (16 * b));
-                }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                if (nt > 0 && nt >= col.live) break;
-                const uint4 b = moe_b<P>(img + col.b[nt], j);
+            if (F == 1) {
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    int c[4];
-                    moe_mma<true>(c, a[k][0], a[k][2], a[k][1], a[k][3], k ? b.z : b.x, k ? b.w : b.y);
-                    e[nt][0] = fmaf(d[0][k], (float)(256 * c[0] + c[1]), e[nt][0]);
-                    e[nt][1] = fmaf(d[1][k], (float)(256 * c[2] + c[3]), e[nt][1]);
+                    const float d0 = scale_of(hd[0], 2 * j + k), d1 = scale_of(hd[1], 2 * j + k);
+#pragma unroll
+                    for (int nt = 0; nt < NL; ++nt) {
+                        const uint2 b = moe_b_block<P>(img + col.b[nt], 2 * j + k);
+                        int c[4];
+                        moe_mma<true>(c, a[k][0], a[k][2], a[k][1], a[k][3], b.x, b.y, true);
+                        e[nt][0] = fmaf(d0, (float)(256 * c[0] + c[1]), e[nt][0]);
+                        e[nt][1] = fmaf(d1, (float)(256 * c[2] + c[3]), e[nt][1]);
+                    }
                 }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int b = 2 * j + k;
+                    const uint2 v = moe_b_block<P>(bp[b % F], b);
+                    moe_mma<true>(cf[b / F], a[k][0], a[k][2], a[k][1], a[k][3], v.x, v.y, b % F == 0);
+                }
+            }
+        }
+        if (F > 1) {
+#pragma unroll
+            for (int q = 0; q < 8 / F; ++q) {
+                const int b = q * F + col.class_s;
+                e[0][0] = fmaf(scale_of(hd[0], b), (float)(256 * cf[q][0] + cf[q][1]), e[0][0]);
+                e[0][1] = fmaf(scale_of(hd[1], b), (float)(256 * cf[q][2] + cf[q][3]), e[0][1]);
             }
         }
         constexpr float scale = QT == QT_Q8_0 ? 1.f : QT == QT_Q4_0 ? 0.0625f : 0.5f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            if (nt > 0 && nt >= col.live) break;
+        for (int nt = 0; nt < NL; ++nt) {
             const float s = *reinterpret_cast<const float *>(img + col.s[nt]) * scale;
             acc[nt][0] = fmaf(s, e[nt][0], acc[nt][0]);
             acc[nt][1] = fmaf(s, e[nt][1], acc[nt][1]);
         }
     }
 };
-template <int P, int NT> struct MoeRecord<QT_Q8_0, P, NT> : MoeRecordBlock<QT_Q8_0, P, NT> {};
-template <int P, int NT> struct MoeRecord<QT_Q4_0, P, NT> : MoeRecordBlock<QT_Q4_0, P, NT> {};
-template <int P, int NT> struct MoeRecord<QT_MXFP4, P, NT> : MoeRecordBlock<QT_MXFP4, P, NT> {};
+template <int P> struct MoeRecord<QT_Q8_0, P> : MoeRecordBlock<QT_Q8_0, P> {};
+template <int P> struct MoeRecord<QT_Q4_0, P> : MoeRecordBlock<QT_Q4_0, P> {};
+template <int P> struct MoeRecord<QT_MXFP4, P> : MoeRecordBlock<QT_MXFP4, P> {};
 
-// The lane's columns of a group of n rows: rows beyond the last repeat it (their sums are not stored)
+// The lane's columns of a group of n rows: columns beyond the last row repeat it (their sums are not stored)
 template <int P, int NT> __device__ __forceinline__ MoeColumns<NT> moe_columns(int n, int lane) {
     constexpr int IMG = moe_image_bytes(P);
     const int g = lane >> 2, t = lane & 3;
     MoeColumns<NT> c;
-    c.live = (n * P + 7) / 8;
+    const int width = P == 2 && n * P <= 2 ? 2 : n * P <= 4 ? 4 : 8;      // columns of a class
+    c.classes = 8 / width;
+    c.class_b = g / width;
+    c.class_s = 2 * t / width;
+    const int gc = g % width, tc = 2 * t % width;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        c.b[nt] = min(nt * (8 / P) + g / P, n - 1) * IMG + (g % P) * 64 + t * 16;
-        c.s[nt] = min(nt * (8 / P) + 2 * t / P, n - 1) * IMG + P * 272 + 4 * ((2 * t % P) / 2);
+        c.b[nt] = min(nt * (8 / P) + gc / P, n - 1) * IMG + (gc % P) * 64 + t * 16;
+        c.s[nt] = min(nt * (8 / P) + tc / P, n - 1) * IMG + P * 272 + 4 * (tc % P / 2);
     }
+    c.row = c.class_s == 0 && tc % P == 0 ? tc / P : -1;
     return c;
 }
 
-// both plane pairs of a row (P = 4) are added up; every lane of a pair has the sum
-template <int P, int NT> __device__ __forceinline__ void moe_join_planes(float (&acc)[NT][2]) {
-    if (P == 4) {
+// adds up a row's lanes: its plane pairs (P = 4) and classes
+template <int P, int NT> __device__ __forceinline__ void moe_join(const MoeColumns<NT> &col, float (&acc)[NT][2]) {
+    if (P == 4 || col.classes == 4) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 2; ++i) acc[nt][i] += __shfl_xor_sync(0xFFFFFFFFu, acc[nt][i], 1);
     }
+    if (col.classes >= 2) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) acc[0][i] += __shfl_xor_sync(0xFFFFFFFFu, acc[0][i], 2);
+    }
+}
+
+struct MoeHead {
+    uint64_t full[kMoeMaxDepth];     // the producer's arrival and its copies' bytes
+    uint64_t empty[kMoeMaxDepth];    // the eight warps
+    MoeGroup group[kMoeMaxDepth];    // the stage's
+    int fail;                        // some wait ran out: every role leaves its work
+};
+
+// one bounded wait of a role; on expiry (or when another role already gave up) the role leaves
+__device__ __forceinline__ bool moe_wait(uint32_t bar, uint32_t parity, volatile int *fail, int *status) {
+    if (mbar_try_wait_hint(bar, parity, 32)) return true;
+    if (*fail) return false;
+    if (mbar_wait_bounded_fast(bar, parity)) return true;
+    atomicMax(status, DEV_ERR_PIPE_TIMEOUT);
+    *fail = 1;
+    return false;
 }
 
 // A product's part of one block: units (group, run of tiles) in turn, every unit's records a step at a time.  With `split` warps a tile
 // (few tiles in all), a step takes as many records of 8 / split tiles, and the warps' sums are added up in order.
-//   finish(unit's group, tile, acc): one warp per tile, its lanes hold the sums of rows g, g + 8 and columns 2 t, 2 t + 1
-template <int QT, int P, int NT, typename Finish>
-__device__ __forceinline__ void moe_product(const MoeProduct &p, uint8_t *smem, float (*part)[NT][2][32], Finish finish) {
+//   finish(unit's group, tile, slots, acc): one warp per tile; the lane holds the sums of rows g, g + 8 of slots[nt] (-1: of none)
+template <int QT, int P, int NT, typename Finish> __device__ __forceinline__ void moe_product(const MoeProduct &p, uint8_t *smem, Finish finish) {
     constexpr int REC = moe_rec_bytes(QT), D = moe_depth(QT, P, NT), IMG = moe_image_bytes(P), kGroup = moe_group_rows(P, NT);
+    __shared__ MoeHead head;
+    __shared__ __align__(16) uint8_t zero[256 * P];
+    __shared__ float part[NT == 1 ? 2 : 1][NT == 1 ? kMoeWarps : 1][2][32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int split = p.split, per = kMoeWarps / split, ws = warp % split, wt = warp / split;     // the warp's record of a step and tile of a unit
+    const int split = NT == 1 ? p.split : 1, per = kMoeWarps / split;
     const int runs = (p.tiles + per - 1) / per, units = *p.lists.ngroups * runs, steps = (p.nrec + split - 1) / split;
     const int stage_bytes = moe_stage_bytes(QT, P, NT, split);
-
-    // what is copied next
-    int fu = blockIdx.x, fs = 0, put = 0;
-    const uint8_t *w_src = nullptr;          // the warp's record
-    uint32_t b_src[kMoeChunks];              // the thread's pieces of the images: offsets of the next step's
-    int b_rec[kMoeChunks], b_dst[kMoeChunks];
-    auto fetch = [&] {
-        if (fu < units) {
-            if (fs == 0) {
-                const int gi = fu / runs, tile = (fu - gi * runs) * per + wt;
-                const MoeGroup grp = p.lists.groups[gi];
-                w_src = tile < p.tiles ? p.w + grp.expert * p.expert_bytes + ((long long)tile * p.nrec + ws) * REC : nullptr;
-#pragma unroll
-                for (int i = 0; i < kMoeChunks; ++i) {
-                    const int piece = i * kMoeThreads + tid, row = piece / (IMG / 16), at = piece - row * (IMG / 16);     // row = (record of the step, row of the group)
-                    const int s = row / grp.n, m = row - s * grp.n;
-                    b_rec[i] = s < split ? s : 0x40000000;
-                    b_dst[i] = (s * kGroup + m) * IMG + at * 16;
-                    b_src[i] = s < split ? (uint32_t)(p.lists.sorted[grp.first + m] / p.slots_per_row) * p.img_stride + s * IMG + at * 16 : 0u;
-                }
-            }
-            uint8_t *stage = smem + put * stage_bytes;
-            if (w_src && fs * split + ws < p.nrec) {
-                const uint32_t dst = smem_u32(stage + warp * REC) + 16 * lane;
-#pragma unroll
-                for (int i = 0; i < (REC / 16 + 31) / 32; ++i)
-                    if ((REC / 16) % 32 == 0 || i * 32 + lane < REC / 16) cp_async_16(dst + 512 * i, w_src + 512 * i + 16 * lane);
-            }
-            if (w_src) w_src += split * REC;
-            const uint32_t img = smem_u32(stage + kMoeWarps * REC);
-#pragma unroll
-            for (int i = 0; i < kMoeChunks; ++i) {
-                if (b_rec[i] < p.nrec) cp_async_16(img + b_dst[i], p.img + b_src[i]);
-                b_rec[i] += split;
-                b_src[i] += split * IMG;
-            }
-            if (++fs == steps) fs = 0, fu += gridDim.x;
+    volatile int *fail = &head.fail;
+    if (tid == 0) {
+        for (int i = 0; i < D; ++i) {
+            mbar_init(smem_u32(&head.full[i]), 1);
+            mbar_init(smem_u32(&head.empty[i]), kMoeWarps);
         }
-        cp_async_commit();
-        if (++put == D) put = 0;
-    };
-#pragma unroll
-    for (int i = 0; i < D - 1; ++i) fetch();
-    int get = 0;
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
-        const int gi = u / runs, tile = (u - gi * runs) * per + wt;
-        const MoeGroup grp = p.lists.groups[gi];
-        const MoeColumns<NT> col = moe_columns<P, NT>(grp.n, lane);
-        float acc[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = 0.f;
-        for (int s = 0; s < steps; ++s) {
-            cp_async_wait<D - 2>();
-            __syncthreads();                 // the stage is here, and the one before it has been read
-            fetch();
-            const uint8_t *stage = smem + get * stage_bytes;
-            if (tile < p.tiles && s * split + ws < p.nrec)
-                MoeRecord<QT, P, NT>::run(stage + warp * REC, lane, stage + kMoeWarps * REC + ws * kGroup * IMG, col, acc);
-            if (++get == D) get = 0;
-        }
-        moe_join_planes<P, NT>(acc);
-        if (split > 1) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) part[warp][nt][i][lane] = acc[nt][i];
-            __syncthreads();                 // (the next unit's are written after at least one more)
-            if (ws == 0) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        for (int k = 1; k < split; ++k) acc[nt][i] += part[warp + k][nt][i][lane];
-            }
-        }
-        if (ws == 0 && tile < p.tiles) finish(grp, tile, acc);
+        head.fail = 0;
+        mbar_fence_init();
+        fence_proxy_async();
     }
-    cp_async_wait<0>();
+    for (int i = tid; i < 64 * P; i += kMoeThreads) reinterpret_cast<uint32_t *>(zero)[i] = 0u;
+    __syncthreads();
+
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    if (warp == kMoeWarps) {
+        // ===== producer ==================================================================================
+        bool full_ring = false;
+        for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+            const int gi = u / runs, tile0 = (u - gi * runs) * per, tiles = min(per, p.tiles - tile0);
+            const int word = lane < (int)(sizeof(MoeGroup) / 4) ? reinterpret_cast<const int *>(p.lists.groups + gi)[lane] : 0;
+            const int expert = __shfl_sync(0xFFFFFFFFu, word, 0), n = __shfl_sync(0xFFFFFFFFu, word, 1);
+            const uint8_t *w = p.w + expert * p.expert_bytes + (long long)tile0 * p.nrec * REC;
+            const int slot = __shfl_sync(0xFFFFFFFFu, word, 2 + lane % 16);          // of row lane % 16
+            const uint8_t *img = p.img + (size_t)(lane % 16 < n ? slot / p.slots_per_row : 0) * p.img_stride;
+            for (int s = 0; s < steps; ++s) {
+                if (full_ring) {
+                    ok = __all_sync(0xFFFFFFFFu, moe_wait(smem_u32(&head.empty[stage]), phase ^ 1, fail, p.status));
+                    if (!ok) break;
+                }
+                const int recs = min(split, p.nrec - s * split);
+                const uint32_t bar = smem_u32(&head.full[stage]), dst = smem_u32(smem + stage * stage_bytes);
+                if (lane < (int)(sizeof(MoeGroup) / 4)) reinterpret_cast<int *>(&head.group[stage])[lane] = word;
+                fence_proxy_async();         // the readers' last accesses precede the copies
+                __syncwarp();
+                if (lane == 0) mbar_expect_tx(bar, recs * (tiles * REC + n * IMG));
+                __syncwarp();
+                if (lane < kMoeWarps) {      // warp lane's record
+                    const int t = lane / split, r = lane % split;
+                    if (t < tiles && r < recs) bulk_g2s(dst + lane * REC, w + ((long long)t * p.nrec + s * split + r) * REC, REC, bar);
+                }
+                if (lane % 16 < n)           // row lane % 16 of the group, every other record
+                    for (int r = lane / 16; r < recs; r += 2)
+                        bulk_g2s(dst + kMoeWarps * REC + (r * kGroup + lane % 16) * IMG, img + (size_t)(s * split + r) * IMG, IMG, bar);
+                if (++stage == D) stage = 0, phase ^= 1, full_ring = true;
+            }
+        }
+    } else {
+        // ===== products ===================================================================================
+        const int ws = warp % split, wt = warp / split;     // the warp's record of a step and tile of a unit
+        int turn = 0;
+        for (int u = blockIdx.x; u < units; u += gridDim.x) {
+            const int gi = u / runs, tile = (u - gi * runs) * per + wt;
+            MoeGroup grp;
+            float acc[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = 0.f;
+            // after a failure the products are left out, but the warps still meet
+            ok = ok && __all_sync(0xFFFFFFFFu, moe_wait(smem_u32(&head.full[stage]), phase, fail, p.status));
+            grp.expert = ok ? head.group[stage].expert : 0;
+            grp.n = ok ? head.group[stage].n : 0;
+            const int n = __shfl_sync(0xFFFFFFFFu, grp.n, 0);
+            const MoeColumns<NT> col = moe_columns<P, NT>(max(n, 1), lane);
+            int slot[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int r = nt * (8 / P) + col.row;
+                slot[nt] = ok && col.row >= 0 && r < n ? head.group[stage].slot[r] : -1;
+            }
+            auto work = [&](auto mode) {
+                for (int s = 0; s < steps; ++s) {
+                    if (s > 0) ok = ok && __all_sync(0xFFFFFFFFu, moe_wait(smem_u32(&head.full[stage]), phase, fail, p.status));
+                    if (!ok) break;
+                    const uint8_t *at = smem + stage * stage_bytes;
+                    if (tile < p.tiles && s * split + ws < p.nrec)
+                        MoeRecord<QT, P>::template run<decltype(mode)>(at + warp * REC, lane, at + kMoeWarps * REC + ws * kGroup * IMG, zero, col, acc);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&head.empty[stage]));
+                    if (++stage == D) stage = 0, phase ^= 1;
+                }
+            };
+            const int used = n * P;              // columns
+            if (P == 2 && used <= 2) work(MoeMode<1, 4>{});
+            else if (used <= 4) work(MoeMode<1, 2>{});
+            else if (used <= 8 || NT == 1) work(MoeMode<1, 1>{});
+            else if (used <= 16) work(MoeMode<NT == 1 ? 1 : 2, 1>{});
+            else work(MoeMode<NT, 1>{});
+            moe_join<P, NT>(col, acc);
+            if (NT == 1 && split > 1) {
+                part[turn][warp][0][lane] = acc[0][0];
+                part[turn][warp][1][lane] = acc[0][1];
+                // a tile's warps meet.  (The next unit's sums go to the other half; that half's readers have met here since.)
+                asm volatile("bar.sync %0, %1;" ::"r"(1 + wt), "r"(32 * split) : "memory");
+                if (ws == 0)
+                    for (int k = 1; k < split; ++k) acc[0][0] += part[turn][warp + k][0][lane], acc[0][1] += part[turn][warp + k][1][lane];
+                turn ^= 1;
+            }
+            if (ok && ws == 0 && tile < p.tiles) finish(grp, tile, slot, acc);
+        }
+    }
+    // After a failure copies may still be on their way: they get time to land (far above a copy's latency) before the block's
+    // shared memory is released.
+    __syncthreads();
+    if (*fail) {
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 100000) {
+        }
+    }
 }
 
 // ---- gate, up and the activation function --------------------------------------------------------
 template <int QT, int P, int NT>
 __global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __grid_constant__ MoeGateUp p) {
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float part[kMoeWarps][NT][2][32];
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int lane = threadIdx.x & 31, g = lane >> 2;
     pdl_launch_dependents();
     pdl_wait();
-    moe_product<QT, P, NT>(p.product, smem, part, [&](const MoeGroup &grp, int tile, const float (&acc)[NT][2]) {
+    moe_product<QT, P, NT>(p.product, smem, [&](const MoeGroup &grp, int tile, const int (&slot)[NT], const float (&acc)[NT][2]) {
         const int f = tile * 8 + g;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int r = nt * (8 / P) + 2 * t / P;
-            if (f >= p.ff || r >= grp.n || (2 * t) % P) continue;
+            if (f >= p.ff || slot[nt] < 0) continue;
             float a = acc[nt][0], b = acc[nt][1];
             if (p.gate_bias) a += p.gate_bias[(long long)grp.expert * p.ff + f];
             if (p.up_bias) b += p.up_bias[(long long)grp.expert * p.ff + f];
@@ -410,7 +542,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __gri
             } else {
                 h = a / (1.f + expf(-a)) * b;
             }
-            p.h[(long long)p.product.lists.sorted[grp.first + r] * p.ff + f] = h;
+            p.h[(long long)slot[nt] * p.ff + f] = h;
         }
     });
 }
@@ -419,16 +551,14 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __gri
 template <int QT, int P, int NT>
 __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(const __grid_constant__ MoeDown p) {
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float part[kMoeWarps][NT][2][32];
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int lane = threadIdx.x & 31, g = lane >> 2;
     pdl_launch_dependents();
     pdl_wait();
-    moe_product<QT, P, NT>(p.product, smem, part, [&](const MoeGroup &grp, int tile, const float (&acc)[NT][2]) {
+    moe_product<QT, P, NT>(p.product, smem, [&](const MoeGroup &grp, int tile, const int (&slot)[NT], const float (&acc)[NT][2]) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int r = nt * (8 / P) + 2 * t / P;
-            if (r >= grp.n || (2 * t) % P) continue;
-            float *z = p.z + (long long)p.product.lists.sorted[grp.first + r] * p.ld_z + tile * 16 + g;
+            if (slot[nt] < 0) continue;
+            float *z = p.z + (long long)slot[nt] * p.ld_z + tile * 16 + g;
             z[0] = acc[nt][0];
             z[8] = acc[nt][1];
         }
@@ -477,4 +607,5 @@ template <typename Kernel, typename Params> cudaError_t moe_launch(Kernel kern, 
         return c.column_tiles == 1 ? moe_launch(moe_down_kernel<QT, 4, 1>, p, grid, smem, st)                                           \
                                    : moe_launch(moe_down_kernel<QT, 4, 4>, p, grid, smem, st);                                          \
     }                                                                                                                                 \
+    cudaError_t moe_wait_limit_##NAME(unsigned long long ns) { return cudaMemcpyToSymbol(s_wait_limit_ns, &ns, sizeof(ns)); }            \
     }

@@ -27,7 +27,7 @@ namespace b200q {
 //           then the rows' 16 int8 scales, then their d
 // The byte count is GGUF's (blocks of 32 weights: K padded to 256, rows to 16 with zeros).
 // ---------------------------------------------------------------------------------------------
-constexpr int kMoeWarps = 8, kMoeThreads = 32 * kMoeWarps;
+constexpr int kMoeWarps = 8, kMoeThreads = 32 * (kMoeWarps + 1);      // warps that multiply; with the producer
 __host__ __device__ constexpr int moe_rec_bytes(int qt) { return 16 * (qt == QT_Q4_K || qt == QT_Q4_0 ? 144 : qt == QT_Q5_K ? 176 : qt == QT_Q6_K ? 210 : qt == QT_Q8_0 ? 272 : 136); }
 // ---------------------------------------------------------------------------------------------
 // Activations
@@ -41,38 +41,35 @@ __host__ __device__ constexpr int moe_rec_bytes(int qt) { return 16 * (qt == QT_
 __host__ __device__ constexpr int moe_image_bytes(int planes) { return planes * (256 + 16) + 16; }
 
 // A block's ring: a stage holds eight records and the images of a group's rows, once per record of a tile in it.  As many stages (2 to
-// 4) as leave room for two blocks an SM (half of 228 KB each, less 1 KB that a block costs by itself) beside the warps' sums.
-constexpr int kMoeSmem = 115712, kMoeMaxDepth = 4;
-// 16-byte pieces of a step's images that a thread copies, at most
-constexpr int kMoeChunks = 4;
+// 4) as leave room for two blocks an SM: half of 228 KB each, less 1 KB that a block costs by itself and 6 KB of its own.
+constexpr int kMoeSmem = 109568, kMoeMaxDepth = 4;
 __host__ __device__ constexpr int moe_group_rows(int planes, int column_tiles) { return column_tiles * 8 / planes; }
-__host__ __device__ constexpr int moe_part_bytes(int column_tiles) { return kMoeWarps * column_tiles * 256; }
 __host__ __device__ constexpr int moe_stage_bytes(int qt, int planes, int column_tiles, int split) {
     return kMoeWarps * moe_rec_bytes(qt) + split * moe_group_rows(planes, column_tiles) * moe_image_bytes(planes);
 }
 __host__ __device__ constexpr int moe_depth(int qt, int planes, int column_tiles) {
-    const int d = (kMoeSmem - moe_part_bytes(column_tiles)) / moe_stage_bytes(qt, planes, column_tiles, 1);
+    const int d = kMoeSmem / moe_stage_bytes(qt, planes, column_tiles, 1);
     return d < 2 ? 2 : d > kMoeMaxDepth ? kMoeMaxDepth : d;
 }
+// warps that may share a tile's records: with one column tile only, and while the stages fit
 __host__ __device__ constexpr int moe_max_split(int qt, int planes, int column_tiles) {
-    int s = kMoeWarps;
-    while (s > 1 && (s * moe_group_rows(planes, column_tiles) * (moe_image_bytes(planes) / 16) > kMoeChunks * kMoeThreads ||
-                     moe_depth(qt, planes, column_tiles) * moe_stage_bytes(qt, planes, column_tiles, s) > kMoeSmem - moe_part_bytes(column_tiles)))
-        s /= 2;
+    int s = column_tiles == 1 ? kMoeWarps : 1;
+    while (s > 1 && moe_depth(qt, planes, column_tiles) * moe_stage_bytes(qt, planes, column_tiles, s) > kMoeSmem) s /= 2;
     return s;
 }
 
 constexpr int kMoeMaxRows = 512, kMoeMaxTopK = 16, kMoeMaxSlots = kMoeMaxRows * kMoeMaxTopK, kMoeMaxExperts = 1024;
 
 // rows of one expert that are multiplied together
+constexpr int kMoeGroupRows = 16;
 struct MoeGroup {
-    int expert, first, n, reserved;      // slots sorted[first .. first + n)
+    int expert, n;
+    int slot[kMoeGroupRows];             // row * top_k + choice
 };
 
 struct MoeLists {
     int *ngroups;
     MoeGroup *groups;
-    int *sorted;                         // slots (row * top_k + choice) by expert
 };
 
 struct MoeProduct {
@@ -83,6 +80,7 @@ struct MoeProduct {
     const uint8_t *img;                  // images
     unsigned img_stride;                 // bytes of a row's image
     int slots_per_row;                   // slot / slots_per_row = row of the images
+    int *status;
 };
 
 struct MoeGateUp {
@@ -117,6 +115,7 @@ struct MoeBuffers {
 };
 struct MoeRun {
     MoeShapeInfo shape;
+    int *status;
     MoeBuffers buf;
     int gate_up_type, down_type;
     const uint8_t *gate_up, *down;
@@ -143,7 +142,8 @@ cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches);
 
 #define MOE_DECLARE(NAME)                                                                                     \
     cudaError_t moe_gate_up_##NAME(const MoeGateUp &p, const MoeConfig &c, int grid, cudaStream_t st);          \
-    cudaError_t moe_down_##NAME(const MoeDown &p, const MoeConfig &c, int grid, cudaStream_t st);
+    cudaError_t moe_down_##NAME(const MoeDown &p, const MoeConfig &c, int grid, cudaStream_t st);               \
+    cudaError_t moe_wait_limit_##NAME(unsigned long long ns);
 MOE_DECLARE(q4_k)
 MOE_DECLARE(q5_k)
 MOE_DECLARE(q6_k)
