@@ -185,24 +185,15 @@ b200q_status b200q_moe_run(b200q_ctx *ctx, b200q_moe *moe, const void *x_dev, in
     r.down_type = moe->down_type;
     r.gate_up = moe->gate_up;
     r.down = moe->down;
-    r.gate_bias = moe->gate_bias;
-    r.up_bias = moe->up_bias;
-    r.down_bias = moe->down_bias;
-    r.activation = moe->activation;
-    r.alpha = moe->alpha;
-    r.limit = moe->limit;
-    r.x = x_dev;
-    r.ldx = ldx;
-    r.x_is_bf16 = x_dtype == B200Q_TYPE_BF16;
-    r.m = (int)M;
-    r.ids = ids_dev;
-    r.ld_ids = ld_ids;
-    r.weights = weights_dev;
-    r.ld_weights = ld_weights;
-    r.y = y_dev;
-    r.ldy = ldy;
-    r.y_is_bf16 = y_dtype == B200Q_TYPE_BF16;
-    r.accumulate = (flags & B200Q_MOE_ACCUMULATE) != 0;
+    r.act = MoeActivation{(int)moe->shape.n_ff, moe->activation, moe->alpha, moe->limit, moe->gate_bias, moe->up_bias};
+    r.x.x = x_dev;
+    r.x.ldx = ldx;
+    r.x.x_is_bf16 = x_dtype == B200Q_TYPE_BF16;
+    r.x.vec_ok = (reinterpret_cast<uintptr_t>(x_dev) & 15) == 0 && (ldx * act_size(x_dtype)) % 16 == 0;
+    r.x.rows = (int)M;
+    r.x.K = (int)moe->shape.n_embd;
+    r.choice = MoeChoice{ids_dev, ld_ids, weights_dev, ld_weights, (int)M, (int)moe->shape.top_k, (int)moe->shape.n_experts};
+    r.out = MoeOutput{y_dev, ldy, moe->down_bias, y_dtype == B200Q_TYPE_BF16, (flags & B200Q_MOE_ACCUMULATE) != 0, (int)moe->shape.n_embd};
     int launches = 0;
     cudaError_t e = moe_run(r, (cudaStream_t)stream, &launches);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "expert layer launch");

@@ -2,7 +2,7 @@
 // activations' images.
 #include <algorithm>
 
-#include "moe_types.h"
+#include "moe_image.cuh"
 #include "kernels.h"
 
 namespace b200q {
@@ -124,76 +124,8 @@ __global__ void __launch_bounds__(256) moe_repack_kernel(const MoeRepack p, long
 
 // ---- activations -> images --------------------------------------------------------------------------
 
-// 256 elements, eight a lane, into their image
-template <int P> __device__ __forceinline__ void moe_image(const float (&v)[8], int lane, uint8_t *img) {
-    uint32_t top = 0;                    // largest magnitude as bits: orders infinities and NaN above every number
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    top = __reduce_max_sync(0xFFFFFFFFu, top);
-    const bool bad = top > __float_as_uint(3.0e38f);
-    float mul, unit;
-    if (P == 2) {
-        // 16 bits: steps of largest / 32512 (127 * 256, so that the upper byte stays signed); below kTiny a fixed step
-        constexpr float kMax = 32512.f, kTiny = 9.6e-35f;
-        const float amax = fmaxf(__uint_as_float(top), kTiny);
-        mul = kMax / amax;
-        unit = amax * (1.f / kMax);
-    } else {
-        // a power of two that brings the largest to 2^29 .. 2^30: fp32 elements down to 2^-6 of it enter whole
-        const int e = max((int)(top >> 23) - 127, -97);
-        mul = __uint_as_float((uint32_t)(29 - e + 127) << 23);
-        unit = __uint_as_float((uint32_t)(e - 29 + 127) << 23);
-    }
-    const int b = lane >> 2, l4 = lane & 3;
-    uint32_t word[P][2];
-#pragma unroll
-    for (int p = 0; p < P; ++p) word[p][0] = word[p][1] = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        int q = bad ? 0 : __float2int_rn(v[i] * mul);
-#pragma unroll
-        for (int p = P - 1; p >= 0; --p) {         // lowest plane last in the row
-            const int d = p == 0 ? q : (int)(int8_t)q;
-            word[p][i >> 2] |= (uint32_t)(d & 0xFF) << (8 * (i & 3));
-            q = (q - d) >> 8;
-        }
-    }
-    uint8_t *at = img + (b >> 1) * (64 * P) + (b & 1) * 8 + (l4 >> 1) * 4 + 32 * (l4 & 1);
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-        *reinterpret_cast<uint32_t *>(at + 64 * p) = word[p][0];
-        *reinterpret_cast<uint32_t *>(at + 64 * p + 16) = word[p][1];
-        int s = dp4a_ss(word[p][0], 0x01010101u, dp4a_ss(word[p][1], 0x01010101u, 0));
-        s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
-        s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
-        if (l4 == 0) {
-            const int a = (s + 32) >> 6;
-            uint8_t *sums = img + 256 * P + 16 * p + 8 * (b >> 2) + (b & 3);
-            sums[0] = (uint8_t)a;
-            sums[4] = (uint8_t)(s - 64 * a);
-        }
-    }
-    if (lane < P / 2) {
-        const float u = bad ? __int_as_float(0x7FC00000) : unit * (P == 4 && lane == 0 ? 65536.f : 1.f);
-        reinterpret_cast<float *>(img + 272 * P)[lane] = u;
-    }
-}
-
-struct MoeRows {
-    const void *x;
-    long long ldx;
-    int x_is_bf16, vec_ok;
-    int rows, K, nrec;
-    uint8_t *img;
-    unsigned img_stride;
-    const int *ids;                      // rows are slots: those whose expert is none are left out
-    long long ld_ids;
-    int top_k, experts;
-};
-
 template <int P> __device__ __forceinline__ void moe_make_image(const MoeRows &p, long long task, int lane) {
     const int row = (int)(task / p.nrec), rec = (int)(task - (long long)row * p.nrec);
-    if (p.ids && (unsigned)p.ids[row / p.top_k * p.ld_ids + row % p.top_k] >= (unsigned)p.experts) return;
     const int k0 = rec * 256 + lane * 8;
     float v[8];
     if (k0 >= p.K) {
@@ -229,30 +161,50 @@ template <int P> __device__ __forceinline__ void moe_make_image(const MoeRows &p
 
 struct MoePrep {
     MoeRows rows;
-    const int *ids;
-    long long ld_ids;
-    int m, top_k, experts, group;        // group: rows of a group at most
+    MoeChoice choice;
+    int group;                           // rows of a group at most
     MoeLists lists;
 };
 
-// Slots by expert, in ascending order within one, so that the same choice gives the same groups every time.  The block's threads own
-// consecutive experts and read all ids.
-__device__ void moe_make_lists(const MoePrep &p) {
-    __shared__ int ids[kMoeMaxSlots];
-    __shared__ int sums[8];
-    const int slots = p.m * p.top_k, tid = threadIdx.x, lane = tid & 31;
-    for (int s = tid; s < slots; s += 256) ids[s] = p.ids[s / p.top_k * p.ld_ids + s % p.top_k];
-    __syncthreads();
-    const int per = (p.experts + 255) / 256, e0 = tid * per;
-    int count[kMoeMaxExperts / 256];
-    int mine = 0;                        // groups
-#pragma unroll
-    for (int i = 0; i < kMoeMaxExperts / 256; ++i) {
-        count[i] = 0;
-        if (i < per && e0 + i < p.experts) {
-            for (int s = 0; s < slots; ++s) count[i] += ids[s] == e0 + i;
-            mine += (count[i] + p.group - 1) / p.group;
+// Slots by expert and, within one, in ascending order, so that the same choice gives the same groups every time.  A counting sort by
+// one block: warps take equal runs of slots, a slot's place among its warp's slots of the same expert comes from a match within 32 and a count
+// of those before, its warp's from a sum over the warps.
+constexpr int kPrepThreads = 1024, kPrepWarps = kPrepThreads / 32;
+struct MoeSort {
+    uint16_t count[kPrepWarps][kMoeMaxExperts];      // slots of the warp so far; then: of the warps before
+    uint16_t place[kMoeMaxSlots];
+    uint16_t groups[kMoeMaxExperts];                 // an expert's first group
+    uint16_t all[kMoeMaxExperts];
+    int sums[kPrepWarps];
+};
+__device__ void moe_make_lists(const MoePrep &p, MoeSort &m) {
+    const MoeChoice &c = p.choice;
+    const int slots = c.m * c.top_k, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int chunks = (slots + 31) / 32, k0 = chunks * warp / kPrepWarps, k1 = chunks * (warp + 1) / kPrepWarps;
+    for (int e = lane; e < c.experts; e += 32) m.count[warp][e] = 0;
+    __syncwarp();
+    for (int k = k0; k < k1; ++k) {
+        const int s = k * 32 + lane;
+        int e = s < slots ? c.ids[s / c.top_k * c.ld_ids + s % c.top_k] : -1;
+        if ((unsigned)e >= (unsigned)c.experts) e = -1;
+        const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
+        const int before = e < 0 ? 0 : m.count[warp][e], rank = __popc(same & ((1u << lane) - 1));
+        __syncwarp();
+        if (e >= 0) {
+            m.place[s] = (uint16_t)(before + rank);
+            if (rank == 0) m.count[warp][e] = (uint16_t)(before + __popc(same));
         }
+        __syncwarp();
+    }
+    __syncthreads();
+    int mine = 0, all = 0;                           // thread e: expert e
+    if (tid < c.experts) {
+        for (int w = 0; w < kPrepWarps; ++w) {
+            const int n = m.count[w][tid];
+            m.count[w][tid] = (uint16_t)all;
+            all += n;
+        }
+        mine = (all + p.group - 1) / p.group;
     }
     int run = mine;
 #pragma unroll
@@ -260,40 +212,40 @@ __device__ void moe_make_lists(const MoePrep &p) {
         const int y = __shfl_up_sync(0xFFFFFFFFu, run, d);
         if (lane >= d) run += y;
     }
-    if (lane == 31) sums[tid >> 5] = run;
+    if (lane == 31) m.sums[warp] = run;
     __syncthreads();
-    int at = run - mine;
-    for (int w = 0; w < (tid >> 5); ++w) at += sums[w];
-    if (tid == 255) *p.lists.ngroups = at + mine;
-#pragma unroll
-    for (int i = 0; i < kMoeMaxExperts / 256; ++i) {
-        if (i >= per || count[i] == 0) continue;
-        int n = 0;
-        for (int s = 0; s < slots; ++s)
-            if (ids[s] == e0 + i) {
-                MoeGroup &g = p.lists.groups[at];
-                g.slot[n++] = s;
-                --count[i];
-                if (n == p.group || count[i] == 0) {
-                    g.expert = e0 + i;
-                    g.n = n;
-                    n = 0;
-                    ++at;
-                }
-            }
+    for (int w = 0; w < warp; ++w) run += m.sums[w];
+    if (tid < c.experts) {
+        m.groups[tid] = (uint16_t)(run - mine);
+        m.all[tid] = (uint16_t)all;
+    }
+    if (tid == kPrepThreads - 1) *p.lists.ngroups = run;
+    __syncthreads();
+    for (int k = k0; k < k1; ++k) {
+        const int s = k * 32 + lane;
+        const int e = s < slots ? c.ids[s / c.top_k * c.ld_ids + s % c.top_k] : -1;
+        if ((unsigned)e >= (unsigned)c.experts) continue;
+        const int at = m.count[warp][e] + m.place[s], r = at % p.group;
+        MoeGroup &g = p.lists.groups[m.groups[e] + at / p.group];
+        g.slot[r] = s;
+        if (r == 0) {
+            g.expert = e;
+            g.n = min(p.group, m.all[e] - at);
+        }
     }
 }
 
 // block 0: the lists; the others: the rows' images, one warp per record
-template <int P> __global__ void __launch_bounds__(256) moe_prep_kernel(const __grid_constant__ MoePrep p) {
+template <int P> __global__ void __launch_bounds__(kPrepThreads) moe_prep_kernel(const __grid_constant__ MoePrep p) {
+    extern __shared__ __align__(16) uint8_t smem[];
     pdl_launch_dependents();
     pdl_wait();
     if (blockIdx.x == 0) {
-        moe_make_lists(p);
+        moe_make_lists(p, *reinterpret_cast<MoeSort *>(smem));
         return;
     }
     const long long tasks = (long long)p.rows.rows * p.rows.nrec;
-    for (long long task = (long long)(blockIdx.x - 1) * 8 + (threadIdx.x >> 5); task < tasks; task += (long long)(gridDim.x - 1) * 8)
+    for (long long task = (long long)(blockIdx.x - 1) * kPrepWarps + (threadIdx.x >> 5); task < tasks; task += (long long)(gridDim.x - 1) * kPrepWarps)
         moe_make_image<P>(p.rows, task, threadIdx.x & 31);
 }
 
@@ -305,46 +257,33 @@ template <int P> __global__ void __launch_bounds__(256) moe_image_kernel(const _
         moe_make_image<P>(p, task, threadIdx.x & 31);
 }
 
-// y[m] = sum over the row's choices, in their order
-struct MoeCombine {
-    const float *z;
-    long long ld_z;
-    const int *ids;
-    long long ld_ids;
-    const float *weights;
-    long long ld_weights;
-    const float *bias;                   // [expert][n] or null
-    void *y;
-    long long ldy;
-    int y_is_bf16, accumulate, n, m, top_k, experts;
-};
 __global__ void __launch_bounds__(256) moe_combine_kernel(const __grid_constant__ MoeCombine p) {
     pdl_launch_dependents();
     pdl_wait();
     const int n = blockIdx.x * 256 + threadIdx.x, m = blockIdx.y;
-    if (n >= p.n) return;
+    const MoeChoice &c = p.choice;
+    const MoeOutput &o = p.out;
+    if (n >= o.n) return;
     float sum = 0.f;
-    for (int j = 0; j < p.top_k; ++j) {
-        const int e = p.ids[m * p.ld_ids + j];
-        if ((unsigned)e >= (unsigned)p.experts) continue;
-        float v = p.z[(long long)(m * p.top_k + j) * p.ld_z + n];
-        if (p.bias) v += p.bias[(long long)e * p.n + n];
-        sum = fmaf(p.weights[m * p.ld_weights + j], v, sum);
+    for (int j = 0; j < c.top_k; ++j) {
+        const int e = c.ids[m * c.ld_ids + j];
+        if ((unsigned)e >= (unsigned)c.experts) continue;
+        float v = p.z[(long long)(m * c.top_k + j) * p.ld_z + n];
+        if (o.bias) v += o.bias[(long long)e * o.n + n];
+        sum = fmaf(c.weights[m * c.ld_weights + j], v, sum);
     }
-    const long long at = m * p.ldy + n;
-    if (p.y_is_bf16) {
-        __nv_bfloat16 *y = reinterpret_cast<__nv_bfloat16 *>(p.y) + at;
-        *y = __float2bfloat16_rn(p.accumulate ? __bfloat162float(*y) + sum : sum);
-    } else {
-        float *y = reinterpret_cast<float *>(p.y) + at;
-        *y = p.accumulate ? *y + sum : sum;
-    }
+    moe_store(o, m, n, sum);
 }
 
-template <typename Kernel, typename Params> cudaError_t launch(Kernel kern, const Params &p, dim3 grid, cudaStream_t st) {
+template <typename Kernel, typename Params> cudaError_t launch(Kernel kern, const Params &p, dim3 grid, int threads, cudaStream_t st, size_t smem = 0) {
+    if (smem > 48 * 1024) {
+        cudaError_t e = moe_configure(reinterpret_cast<const void *>(kern), smem);
+        if (e != cudaSuccess) return e;
+    }
     cudaLaunchConfig_t cfg{};
+    cfg.dynamicSmemBytes = smem;
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -357,26 +296,18 @@ template <typename Kernel, typename Params> cudaError_t launch(Kernel kern, cons
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-cudaError_t gate_up_launch(int qt, const MoeGateUp &p, const MoeConfig &c, int grid, cudaStream_t st) {
-    switch (qt) {
-    case QT_Q4_K: return moe_gate_up_q4_k(p, c, grid, st);
-    case QT_Q5_K: return moe_gate_up_q5_k(p, c, grid, st);
-    case QT_Q6_K: return moe_gate_up_q6_k(p, c, grid, st);
-    case QT_Q8_0: return moe_gate_up_q8_0(p, c, grid, st);
-    case QT_Q4_0: return moe_gate_up_q4_0(p, c, grid, st);
-    default: return moe_gate_up_mxfp4(p, c, grid, st);
+#define MOE_BY_TYPE(CALL, ...)                       \
+    switch (qt) {                                    \
+    case QT_Q4_K: return CALL##_q4_k(__VA_ARGS__);   \
+    case QT_Q5_K: return CALL##_q5_k(__VA_ARGS__);   \
+    case QT_Q6_K: return CALL##_q6_k(__VA_ARGS__);   \
+    case QT_Q8_0: return CALL##_q8_0(__VA_ARGS__);   \
+    case QT_Q4_0: return CALL##_q4_0(__VA_ARGS__);   \
+    default: return CALL##_mxfp4(__VA_ARGS__);       \
     }
-}
-cudaError_t down_launch(int qt, const MoeDown &p, const MoeConfig &c, int grid, cudaStream_t st) {
-    switch (qt) {
-    case QT_Q4_K: return moe_down_q4_k(p, c, grid, st);
-    case QT_Q5_K: return moe_down_q5_k(p, c, grid, st);
-    case QT_Q6_K: return moe_down_q6_k(p, c, grid, st);
-    case QT_Q8_0: return moe_down_q8_0(p, c, grid, st);
-    case QT_Q4_0: return moe_down_q4_0(p, c, grid, st);
-    default: return moe_down_mxfp4(p, c, grid, st);
-    }
-}
+cudaError_t few_down(int qt, const MoeFewDown &p, int planes, int tiles, int grid, cudaStream_t st) { MOE_BY_TYPE(moe_few_down, p, planes, tiles, grid, st) }
+cudaError_t gate_up_launch(int qt, const MoeGateUp &p, int planes, int tiles, int grid, cudaStream_t st) { MOE_BY_TYPE(moe_gate_up, p, planes, tiles, grid, st) }
+cudaError_t many_down(int qt, const MoeDown &p, int planes, int grid, cudaStream_t st) { MOE_BY_TYPE(moe_down, p, planes, grid, st) }
 
 }  // namespace
 
@@ -419,113 +350,56 @@ size_t moe_workspace(const MoeShapeInfo &s, MoeBuffers *out, uint8_t *base) {
     b.x_img = take((size_t)s.max_rows * ceil_div(s.n_embd, SB) * moe_image_bytes(4));
     b.h_img = take((size_t)slots * ceil_div(s.n_ff, SB) * moe_image_bytes(4));
     b.z = reinterpret_cast<float *>(take((size_t)slots * ceil_div(s.n_embd, 16) * 16 * sizeof(float)));
+    b.partial = reinterpret_cast<float *>(take((size_t)2 * s.sm_count * 2 * kMoeWarps * kMoePart * sizeof(float)));
+    b.count = reinterpret_cast<unsigned *>(take((size_t)2 * s.sm_count * kMoeWarps * sizeof(unsigned)));
     if (out) *out = b;
     return at;
 }
 
 cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches) {
     const MoeShapeInfo &s = r.shape;
-    const int slots = r.m * (int)s.top_k;
+    const int slots = r.choice.m * (int)s.top_k, grid = 2 * s.sm_count;
     // 31-bit activations for fp32 results, 16 bits where the result is rounded to bf16
-    MoeConfig c{};
-    c.planes = r.y_is_bf16 ? 2 : 4;
-    c.column_tiles = r.m * c.planes <= 8 ? 1 : 4;
+    const int planes = r.out.y_is_bf16 ? 2 : 4;
     const int x_rec = (int)ceil_div(s.n_embd, SB), h_rec = (int)ceil_div(s.n_ff, SB);
-
-    MoePrep pr{};
-    pr.rows.x = r.x;
-    pr.rows.ldx = r.ldx;
-    pr.rows.x_is_bf16 = r.x_is_bf16;
-    pr.rows.vec_ok = (reinterpret_cast<uintptr_t>(r.x) & 15) == 0 && (r.ldx * (r.x_is_bf16 ? 2 : 4)) % 16 == 0;
-    pr.rows.rows = r.m;
-    pr.rows.K = (int)s.n_embd;
-    pr.rows.nrec = x_rec;
-    pr.rows.img = r.buf.x_img;
-    pr.rows.img_stride = (unsigned)(x_rec * moe_image_bytes(c.planes));
-    pr.ids = r.ids;
-    pr.ld_ids = r.ld_ids;
-    pr.m = r.m;
-    pr.top_k = (int)s.top_k;
-    pr.experts = (int)s.n_experts;
-    pr.group = moe_group_rows(c.planes, c.column_tiles);
-    pr.lists = r.buf.lists;
-    const int prep_grid = 1 + (int)std::min<long long>(ceil_div((long long)r.m * x_rec, 8), 4 * s.sm_count);
-    cudaError_t e = c.planes == 2 ? launch(moe_prep_kernel<2>, pr, prep_grid, st) : launch(moe_prep_kernel<4>, pr, prep_grid, st);
+    auto weights = [&](const uint8_t *w, int qt, int64_t tiles, int nrec) { return MoeWeights{w, tiles * nrec * moe_rec_bytes(qt), (int)tiles, nrec}; };
+    const MoeWeights gate_up = weights(r.gate_up, r.gate_up_type, ceil_div(s.n_ff, 8), x_rec), down = weights(r.down, r.down_type, ceil_div(s.n_embd, 16), h_rec);
+    MoeRows x = r.x, h{};
+    x.nrec = x_rec;
+    h.x = r.buf.h;
+    h.ldx = s.n_ff;
+    h.vec_ok = s.n_ff % 4 == 0;
+    h.rows = slots;
+    h.K = (int)s.n_ff;
+    h.nrec = h_rec;
+    x.img = r.buf.x_img;
+    x.img_stride = (unsigned)(x_rec * moe_image_bytes(planes));
+    h.img = r.buf.h_img;
+    h.img_stride = (unsigned)(h_rec * moe_image_bytes(planes));
+    const bool few = r.choice.m <= kMoeFewRows;
+    const int tiles = !few ? kMoeManyTiles : r.choice.m * planes <= 8 ? 1 : 2;
+    const int warps = kPrepThreads / 32, spread = s.sm_count;
+    const MoePrep pr{x, r.choice, moe_group_rows(planes, tiles), r.buf.lists};
+    const unsigned x_grid = 1 + (unsigned)std::min<long long>(ceil_div((long long)r.choice.m * x_rec, warps), spread);
+    cudaError_t e = planes == 2 ? launch(moe_prep_kernel<2>, pr, x_grid, kPrepThreads, st, sizeof(MoeSort)) : launch(moe_prep_kernel<4>, pr, x_grid, kPrepThreads, st, sizeof(MoeSort));
     if (e != cudaSuccess) return e;
-
-    const int used = (int)std::min<long long>(slots, s.n_experts);      // experts that may have been chosen
-    // Records of a tile are shared by as many warps as it takes to give every warp of the chip work
-    auto product = [&](const uint8_t *w, int qt, int tiles, int nrec, const uint8_t *img, unsigned stride, int per_row) {
-        MoeProduct p{};
-        p.w = w;
-        p.tiles = tiles;
-        p.nrec = nrec;
-        p.expert_bytes = (long long)tiles * nrec * moe_rec_bytes(qt);
-        p.lists = r.buf.lists;
-        p.img = img;
-        p.img_stride = stride;
-        p.slots_per_row = per_row;
-        p.status = r.status;
-        p.split = 1;
-        while (p.split < moe_max_split(qt, c.planes, c.column_tiles) && 2 * p.split <= nrec && (long long)used * tiles * p.split < 2ll * kMoeWarps * s.sm_count) p.split *= 2;
-        return p;
+    auto product = [&](const MoeWeights &w, const MoeRows &rows, int per_row) {
+        return MoeProduct{w, r.buf.lists, rows.img, rows.img_stride, per_row, r.buf.partial, r.buf.count, r.status};
     };
-    auto grid_of = [&](const MoeProduct &p) {
-        return (int)std::min<long long>(2 * s.sm_count, (long long)slots * ceil_div(p.tiles, kMoeWarps / p.split));
-    };
-    MoeGateUp gu{};
-    gu.product = product(r.gate_up, r.gate_up_type, (int)ceil_div(s.n_ff, 8), x_rec, r.buf.x_img, pr.rows.img_stride, (int)s.top_k);
-    gu.h = r.buf.h;
-    gu.ff = (int)s.n_ff;
-    gu.activation = r.activation;
-    gu.alpha = r.alpha;
-    gu.limit = r.limit;
-    gu.gate_bias = r.gate_bias;
-    gu.up_bias = r.up_bias;
-    if ((e = gate_up_launch(r.gate_up_type, gu, c, grid_of(gu.product), st)) != cudaSuccess) return e;
-
-    MoeRows hr{};
-    hr.x = r.buf.h;
-    hr.ldx = s.n_ff;
-    hr.vec_ok = s.n_ff % 4 == 0;
-    hr.rows = slots;
-    hr.K = (int)s.n_ff;
-    hr.nrec = h_rec;
-    hr.img = r.buf.h_img;
-    hr.img_stride = (unsigned)(h_rec * moe_image_bytes(c.planes));
-    hr.ids = r.ids;
-    hr.ld_ids = r.ld_ids;
-    hr.top_k = (int)s.top_k;
-    hr.experts = (int)s.n_experts;
-    const int h_grid = (int)std::min<long long>(ceil_div((long long)slots * h_rec, 8), 4 * s.sm_count);
-    e = c.planes == 2 ? launch(moe_image_kernel<2>, hr, h_grid, st) : launch(moe_image_kernel<4>, hr, h_grid, st);
-    if (e != cudaSuccess) return e;
-
-    MoeDown d{};
-    d.product = product(r.down, r.down_type, (int)ceil_div(s.n_embd, 16), h_rec, r.buf.h_img, hr.img_stride, 1);
-    d.z = r.buf.z;
-    d.ld_z = ceil_div(s.n_embd, 16) * 16;
-    if ((e = down_launch(r.down_type, d, c, grid_of(d.product), st)) != cudaSuccess) return e;
-
-    MoeCombine cb{};
-    cb.z = d.z;
-    cb.ld_z = d.ld_z;
-    cb.ids = r.ids;
-    cb.ld_ids = r.ld_ids;
-    cb.weights = r.weights;
-    cb.ld_weights = r.ld_weights;
-    cb.bias = r.down_bias;
-    cb.y = r.y;
-    cb.ldy = r.ldy;
-    cb.y_is_bf16 = r.y_is_bf16;
-    cb.accumulate = r.accumulate;
-    cb.n = (int)s.n_embd;
-    cb.m = r.m;
-    cb.top_k = (int)s.top_k;
-    cb.experts = (int)s.n_experts;
-    if ((e = launch(moe_combine_kernel, cb, dim3((unsigned)ceil_div(s.n_embd, 256), (unsigned)r.m), st)) != cudaSuccess) return e;
+    const MoeGateUp gu{product(gate_up, x, (int)s.top_k), r.act, r.buf.h};
+    if ((e = gate_up_launch(r.gate_up_type, gu, planes, tiles, grid, st)) != cudaSuccess) return e;
+    const unsigned h_grid = (unsigned)std::min<long long>(ceil_div((long long)slots * h_rec, 8), 4 * spread);
+    if ((e = planes == 2 ? launch(moe_image_kernel<2>, h, h_grid, 256, st) : launch(moe_image_kernel<4>, h, h_grid, 256, st)) != cudaSuccess) return e;
+    if (few) {
+        const MoeFewDown d{product(down, h, 1), r.choice, r.out};
+        *launches = 4;
+        return few_down(r.down_type, d, planes, tiles, grid, st);
+    }
+    const MoeDown d{product(down, h, 1), r.buf.z, ceil_div(s.n_embd, 16) * 16};
+    if ((e = many_down(r.down_type, d, planes, grid, st)) != cudaSuccess) return e;
+    const MoeCombine cb{r.choice, r.out, r.buf.z, d.ld_z};
     *launches = 5;
-    return cudaSuccess;
+    return launch(moe_combine_kernel, cb, dim3((unsigned)ceil_div(s.n_embd, 256), (unsigned)r.choice.m), 256, st);
 }
 
 cudaError_t moe_set_wait_limit_ns(unsigned long long ns) {

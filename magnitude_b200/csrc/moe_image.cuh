@@ -1,0 +1,94 @@
+// Device pieces that the launches of an expert layer share: activations into images, a row's output.
+#pragma once
+
+#include "moe_types.h"
+
+namespace b200q {
+namespace {
+
+// 256 elements, eight a lane, into their image
+template <int P> __device__ __forceinline__ void moe_image(const float (&v)[8], int lane, uint8_t *img) {
+    uint32_t top = 0;                    // largest magnitude as bits: orders infinities and NaN above every number
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    const bool bad = top > __float_as_uint(3.0e38f);
+    float mul, unit;
+    if (P == 2) {
+        // 16 bits: steps of largest / 32512 (127 * 256, so that the upper byte stays signed); below kTiny a fixed step
+        constexpr float kMax = 32512.f, kTiny = 9.6e-35f;
+        const float amax = fmaxf(__uint_as_float(top), kTiny);
+        mul = kMax / amax;
+        unit = amax * (1.f / kMax);
+    } else {
+        // a power of two that brings the largest to 2^29 .. 2^30: fp32 elements down to 2^-6 of it enter whole
+        const int e = max((int)(top >> 23) - 127, -97);
+        mul = __uint_as_float((uint32_t)(29 - e + 127) << 23);
+        unit = __uint_as_float((uint32_t)(e - 29 + 127) << 23);
+    }
+    const int b = lane >> 2, l4 = lane & 3;
+    uint32_t word[P][2];
+#pragma unroll
+    for (int p = 0; p < P; ++p) word[p][0] = word[p][1] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        int q = bad ? 0 : __float2int_rn(v[i] * mul);
+#pragma unroll
+        for (int p = P - 1; p >= 0; --p) {         // lowest plane last in the row
+            const int d = p == 0 ? q : (int)(int8_t)q;
+            word[p][i >> 2] |= (uint32_t)(d & 0xFF) << (8 * (i & 3));
+            q = (q - d) >> 8;
+        }
+    }
+    uint8_t *at = img + (b >> 1) * (64 * P) + (b & 1) * 8 + (l4 >> 1) * 4 + 32 * (l4 & 1);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        *reinterpret_cast<uint32_t *>(at + 64 * p) = word[p][0];
+        *reinterpret_cast<uint32_t *>(at + 64 * p + 16) = word[p][1];
+        int s = dp4a_ss(word[p][0], 0x01010101u, dp4a_ss(word[p][1], 0x01010101u, 0));
+        s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
+        s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
+        if (l4 == 0) {
+            const int a = (s + 32) >> 6;
+            uint8_t *sums = img + 256 * P + 16 * p + 8 * (b >> 2) + (b & 3);
+            sums[0] = (uint8_t)a;
+            sums[4] = (uint8_t)(s - 64 * a);
+        }
+    }
+    if (lane < P / 2) {
+        const float u = bad ? __int_as_float(0x7FC00000) : unit * (P == 4 && lane == 0 ? 65536.f : 1.f);
+        reinterpret_cast<float *>(img + 272 * P)[lane] = u;
+    }
+}
+
+__device__ __forceinline__ void moe_store(const MoeOutput &o, int row, int n, float v) {
+    const long long at = row * o.ldy + n;
+    if (o.y_is_bf16) {
+        __nv_bfloat16 *y = reinterpret_cast<__nv_bfloat16 *>(o.y) + at;
+        *y = __float2bfloat16_rn(o.accumulate ? __bfloat162float(*y) + v : v);
+    } else {
+        float *y = reinterpret_cast<float *>(o.y) + at;
+        *y = o.accumulate ? *y + v : v;
+    }
+}
+
+// A kernel's shared memory is set once per device
+inline cudaError_t moe_configure(const void *kern, size_t smem) {
+    struct Done {
+        const void *kern;
+        int device;
+    };
+    static thread_local Done done[16];       // this thread's last ones
+    static thread_local int next = 0;
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    for (const Done &d : done)
+        if (d.kern == kern && d.device == device) return cudaSuccess;
+    if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
+    done[next++ % 16] = Done{kern, device};
+    return cudaSuccess;
+}
+
+}  // namespace
+}  // namespace b200q

@@ -6,12 +6,12 @@
 // 16); its integer sums are multiplied by the block's integer scale and added up as integers over the record (Q4_K, Q5_K,
 // Q6_K), or scaled in fp32 (types with an fp16 or power-of-two scale per block), so nothing is multiplied per weight.  The
 // minima of Q4_K and Q5_K are two more MMAs with the sums of the activations' blocks.
-// A block takes one group and the records of eight tile rows a step: a producer warp copies the weights and the group's activations
-// into a ring of stages, eight warps multiply, one record each, and share the activations.
+// A block takes one group and the records of eight tiles a step: a producer warp fills a ring of stages with weights and the group's
+// activations, eight warps multiply, one record each, and share the activations.
 #pragma once
 
 #include "kernels.h"
-#include "moe_types.h"
+#include "moe_image.cuh"
 
 namespace b200q {
 namespace {
@@ -47,8 +47,9 @@ __device__ __forceinline__ int byte_s(uint32_t w, int i) {
 // How a warp's columns are used.  NL column tiles hold 8 / P rows each.  A group of few rows needs only half or a quarter
 // of one tile: then the columns also tell F blocks apart (column = class F, row, plane; class f holds blocks f, f + F, .. and zeros for the
 // others), F MMAs add up into the same sums, and a lane has 1 / F of the scaling to do.
-template <int NL_, int F_> struct MoeMode {
-    static constexpr int NL = NL_, F = F_;
+// O: the first of the NL tiles (more than two tiles are multiplied two at a time: with four the sums do not fit into registers).
+template <int NL_, int F_, int O_ = 0> struct MoeMode {
+    static constexpr int NL = NL_, F = F_, O = O_;
 };
 
 // where a lane finds its column in the group's images: byte offsets
@@ -89,7 +90,7 @@ template <int QT, int P> struct MoeRecordK {
     }
     template <typename Mode, int NT>
     static __device__ __forceinline__ void run(const uint8_t *rec, int lane, const uint8_t *img, const uint8_t *zero, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
-        constexpr int NL = Mode::NL, F = Mode::F;
+        constexpr int NL = Mode::NL, F = Mode::F, O = Mode::O;
         const int g = lane >> 2, t = lane & 3;
         constexpr int kHead = QT == QT_Q5_K ? 2560 : 2048;
         uint4 hd[2], f = make_uint4(0, 0, 0, 0);
@@ -114,7 +115,7 @@ template <int QT, int P> struct MoeRecordK {
                 words(rec, lane, j, f, lo, hi);
 #pragma unroll
                 for (int nt = 0; nt < NL; ++nt) {
-                    const uint4 b = moe_b<P>(img + col.b[nt], j);
+                    const uint4 b = moe_b<P>(img + col.b[O + nt], j);
                     int c[4];
                     moe_mma<false>(c, lo[0], lo[2], lo[1], lo[3], b.x, b.y, true);
 #pragma unroll
@@ -165,16 +166,16 @@ template <int QT, int P> struct MoeRecordK {
             // block sums 64 a + b: lanes t < 2 bring a and b of blocks 4 t .. 4 t + 3, the others' A words are zero.  (class F's bytes begin
             // where the image does, so the plane follows from the offset)
             const int plane = F == 1 ? g % P : g % (8 / F) % P;
-            const uint2 bs = *reinterpret_cast<const uint2 *>(img + col.b[nt] + 256 * P - 48 * plane - 16 * t + 8 * (t & 1));
+            const uint2 bs = *reinterpret_cast<const uint2 *>(img + col.b[O + nt] + 256 * P - 48 * plane - 16 * t + 8 * (t & 1));
             int ma[4], mb[4];
             moe_mma<false>(ma, am[0], am[1], 0u, 0u, bs.x, 0u, true);
             moe_mma<false>(mb, am[0], am[1], 0u, 0u, bs.y, 0u, true);
-            const float s = *reinterpret_cast<const float *>(img + col.s[nt]);
+            const float s = *reinterpret_cast<const float *>(img + col.s[O + nt]);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const float v = fmaf(256.f, (float)sum[nt][2 * i], (float)sum[nt][2 * i + 1]);
                 const float m = fmaf(256.f, (float)(64 * ma[2 * i] + mb[2 * i]), (float)(64 * ma[2 * i + 1] + mb[2 * i + 1]));
-                acc[nt][i] = fmaf(s, fmaf(d[i], v, -dmin[i] * m), acc[nt][i]);
+                acc[O + nt][i] = fmaf(s, fmaf(d[i], v, -dmin[i] * m), acc[O + nt][i]);
             }
         }
     }
@@ -185,7 +186,7 @@ template <int P> struct MoeRecord<QT_Q5_K, P> : MoeRecordK<QT_Q5_K, P> {};
 template <int P> struct MoeRecord<QT_Q6_K, P> {
     template <typename Mode, int NT>
     static __device__ __forceinline__ void run(const uint8_t *rec, int lane, const uint8_t *img, const uint8_t *zero, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
-        constexpr int NL = Mode::NL, F = Mode::F;
+        constexpr int NL = Mode::NL, F = Mode::F, O = Mode::O;
         const int g = lane >> 2;
         const uint4 s0 = moe_lds(rec + 3072 + 16 * g), s1 = moe_lds(rec + 3072 + 16 * g + 128);
         const float d[2] = {half_bits_to_float(*reinterpret_cast<const uint16_t *>(rec + 3328 + 2 * g)) * 0.25f,
@@ -222,7 +223,7 @@ template <int P> struct MoeRecord<QT_Q6_K, P> {
                 if (F == 1) {
 #pragma unroll
                     for (int nt = 0; nt < NL; ++nt) {
-                        const uint4 b = moe_b<P>(img + col.b[nt], j);
+                        const uint4 b = moe_b<P>(img + col.b[O + nt], j);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             int c[4];
@@ -245,9 +246,9 @@ template <int P> struct MoeRecord<QT_Q6_K, P> {
         }
 #pragma unroll
         for (int nt = 0; nt < NL; ++nt) {
-            const float s = *reinterpret_cast<const float *>(img + col.s[nt]);
+            const float s = *reinterpret_cast<const float *>(img + col.s[O + nt]);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) acc[nt][i] = fmaf(s, d[i] * fmaf(256.f, (float)sum[nt][2 * i], (float)sum[nt][2 * i + 1]), acc[nt][i]);
+            for (int i = 0; i < 2; ++i) acc[O + nt][i] = fmaf(s, d[i] * fmaf(256.f, (float)sum[nt][2 * i], (float)sum[nt][2 * i + 1]), acc[O + nt][i]);
         }
     }
 };
@@ -261,7 +262,7 @@ template <int QT, int P> struct MoeRecordBlock {
     }
     template <typename Mode, int NT>
     static __device__ __forceinline__ void run(const uint8_t *rec, int lane, const uint8_t *img, const uint8_t *zero, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
-        constexpr int NL = Mode::NL, F = Mode::F;
+        constexpr int NL = Mode::NL, F = Mode::F, O = Mode::O;
         const int g = lane >> 2;
         uint4 hd[2];                                  // eight fp16 d (MXFP4: eight scale bytes)
         if (QT == QT_MXFP4) {
@@ -308,7 +309,7 @@ template <int QT, int P> struct MoeRecordBlock {
                     const float d0 = scale_of(hd[0], 2 * j + k), d1 = scale_of(hd[1], 2 * j + k);
 #pragma unroll
                     for (int nt = 0; nt < NL; ++nt) {
-                        const uint2 b = moe_b_block<P>(img + col.b[nt], 2 * j + k);
+                        const uint2 b = moe_b_block<P>(img + col.b[O + nt], 2 * j + k);
                         int c[4];
                         moe_mma<true>(c, a[k][0], a[k][2], a[k][1], a[k][3], b.x, b.y, true);
                         e[nt][0] = fmaf(d0, (float)(256 * c[0] + c[1]), e[nt][0]);
@@ -335,9 +336,9 @@ template <int QT, int P> struct MoeRecordBlock {
         constexpr float scale = QT == QT_Q8_0 ? 1.f : QT == QT_Q4_0 ? 0.0625f : 0.5f;
 #pragma unroll
         for (int nt = 0; nt < NL; ++nt) {
-            const float s = *reinterpret_cast<const float *>(img + col.s[nt]) * scale;
-            acc[nt][0] = fmaf(s, e[nt][0], acc[nt][0]);
-            acc[nt][1] = fmaf(s, e[nt][1], acc[nt][1]);
+            const float s = *reinterpret_cast<const float *>(img + col.s[O + nt]) * scale;
+            acc[O + nt][0] = fmaf(s, e[nt][0], acc[O + nt][0]);
+            acc[O + nt][1] = fmaf(s, e[nt][1], acc[O + nt][1]);
         }
     }
 };
@@ -395,21 +396,9 @@ __device__ __forceinline__ bool moe_wait(uint32_t bar, uint32_t parity, volatile
     return false;
 }
 
-// A product's part of one block: units (group, run of tiles) in turn, every unit's records a step at a time.  With `split` warps a tile
-// (few tiles in all), a step takes as many records of 8 / split tiles, and the warps' sums are added up in order.
-//   finish(unit's group, tile, slots, acc): one warp per tile; the lane holds the sums of rows g, g + 8 of slots[nt] (-1: of none)
-template <int QT, int P, int NT, typename Finish> __device__ __forceinline__ void moe_product(const MoeProduct &p, uint8_t *smem, Finish finish) {
-    constexpr int REC = moe_rec_bytes(QT), D = moe_depth(QT, P, NT), IMG = moe_image_bytes(P), kGroup = moe_group_rows(P, NT);
-    __shared__ MoeHead head;
-    __shared__ __align__(16) uint8_t zero[256 * P];
-    __shared__ float part[NT == 1 ? 2 : 1][NT == 1 ? kMoeWarps : 1][2][32];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int split = NT == 1 ? p.split : 1, per = kMoeWarps / split;
-    const int runs = (p.tiles + per - 1) / per, units = *p.lists.ngroups * runs, steps = (p.nrec + split - 1) / split;
-    const int stage_bytes = moe_stage_bytes(QT, P, NT, split);
-    volatile int *fail = &head.fail;
-    if (tid == 0) {
-        for (int i = 0; i < D; ++i) {
+__device__ __forceinline__ void moe_ring_init(MoeHead &head, int depth) {
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < depth; ++i) {
             mbar_init(smem_u32(&head.full[i]), 1);
             mbar_init(smem_u32(&head.empty[i]), kMoeWarps);
         }
@@ -417,144 +406,233 @@ template <int QT, int P, int NT, typename Finish> __device__ __forceinline__ voi
         mbar_fence_init();
         fence_proxy_async();
     }
-    for (int i = tid; i < 64 * P; i += kMoeThreads) reinterpret_cast<uint32_t *>(zero)[i] = 0u;
-    __syncthreads();
+}
 
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    if (warp == kMoeWarps) {
-        // ===== producer ==================================================================================
-        bool full_ring = false;
-        for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
-            const int gi = u / runs, tile0 = (u - gi * runs) * per, tiles = min(per, p.tiles - tile0);
-            const int word = lane < (int)(sizeof(MoeGroup) / 4) ? reinterpret_cast<const int *>(p.lists.groups + gi)[lane] : 0;
-            const int expert = __shfl_sync(0xFFFFFFFFu, word, 0), n = __shfl_sync(0xFFFFFFFFu, word, 1);
-            const uint8_t *w = p.w + expert * p.expert_bytes + (long long)tile0 * p.nrec * REC;
-            const int slot = __shfl_sync(0xFFFFFFFFu, word, 2 + lane % 16);          // of row lane % 16
-            const uint8_t *img = p.img + (size_t)(lane % 16 < n ? slot / p.slots_per_row : 0) * p.img_stride;
-            for (int s = 0; s < steps; ++s) {
-                if (full_ring) {
-                    ok = __all_sync(0xFFFFFFFFu, moe_wait(smem_u32(&head.empty[stage]), phase ^ 1, fail, p.status));
-                    if (!ok) break;
-                }
-                const int recs = min(split, p.nrec - s * split);
-                const uint32_t bar = smem_u32(&head.full[stage]), dst = smem_u32(smem + stage * stage_bytes);
-                if (lane < (int)(sizeof(MoeGroup) / 4)) reinterpret_cast<int *>(&head.group[stage])[lane] = word;
-                fence_proxy_async();         // the readers' last accesses precede the copies
-                __syncwarp();
-                if (lane == 0) mbar_expect_tx(bar, recs * (tiles * REC + n * IMG));
-                __syncwarp();
-                if (lane < kMoeWarps) {      // warp lane's record
-                    const int t = lane / split, r = lane % split;
-                    if (t < tiles && r < recs) bulk_g2s(dst + lane * REC, w + ((long long)t * p.nrec + s * split + r) * REC, REC, bar);
-                }
-                if (lane % 16 < n)           // row lane % 16 of the group, every other record
-                    for (int r = lane / 16; r < recs; r += 2)
-                        bulk_g2s(dst + kMoeWarps * REC + (r * kGroup + lane % 16) * IMG, img + (size_t)(s * split + r) * IMG, IMG, bar);
-                if (++stage == D) stage = 0, phase ^= 1, full_ring = true;
-            }
-        }
-    } else {
-        // ===== products ===================================================================================
-        const int ws = warp % split, wt = warp / split;     // the warp's record of a step and tile of a unit
-        int turn = 0;
-        for (int u = blockIdx.x; u < units; u += gridDim.x) {
-            const int gi = u / runs, tile = (u - gi * runs) * per + wt;
-            MoeGroup grp;
-            float acc[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = 0.f;
-            // after a failure the products are left out, but the warps still meet
-            ok = ok && __all_sync(0xFFFFFFFFu, moe_wait(smem_u32(&head.full[stage]), phase, fail, p.status));
-            grp.expert = ok ? head.group[stage].expert : 0;
-            grp.n = ok ? head.group[stage].n : 0;
-            const int n = __shfl_sync(0xFFFFFFFFu, grp.n, 0);
-            const MoeColumns<NT> col = moe_columns<P, NT>(max(n, 1), lane);
-            int slot[NT];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const int r = nt * (8 / P) + col.row;
-                slot[nt] = ok && col.row >= 0 && r < n ? head.group[stage].slot[r] : -1;
-            }
-            auto work = [&](auto mode) {
-                for (int s = 0; s < steps; ++s) {
-                    if (s > 0) ok = ok && __all_sync(0xFFFFFFFFu, moe_wait(smem_u32(&head.full[stage]), phase, fail, p.status));
-                    if (!ok) break;
-                    const uint8_t *at = smem + stage * stage_bytes;
-                    if (tile < p.tiles && s * split + ws < p.nrec)
-                        MoeRecord<QT, P>::template run<decltype(mode)>(at + warp * REC, lane, at + kMoeWarps * REC + ws * kGroup * IMG, zero, col, acc);
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&head.empty[stage]));
-                    if (++stage == D) stage = 0, phase ^= 1;
-                }
-            };
-            const int used = n * P;              // columns
-            if (P == 2 && used <= 2) work(MoeMode<1, 4>{});
-            else if (used <= 4) work(MoeMode<1, 2>{});
-            else if (used <= 8 || NT == 1) work(MoeMode<1, 1>{});
-            else if (used <= 16) work(MoeMode<NT == 1 ? 1 : 2, 1>{});
-            else work(MoeMode<NT, 1>{});
-            moe_join<P, NT>(col, acc);
-            if (NT == 1 && split > 1) {
-                part[turn][warp][0][lane] = acc[0][0];
-                part[turn][warp][1][lane] = acc[0][1];
-                // a tile's warps meet.  (The next unit's sums go to the other half; that half's readers have met here since.)
-                asm volatile("bar.sync %0, %1;" ::"r"(1 + wt), "r"(32 * split) : "memory");
-                if (ws == 0)
-                    for (int k = 1; k < split; ++k) acc[0][0] += part[turn][warp + k][0][lane], acc[0][1] += part[turn][warp + k][1][lane];
-                turn ^= 1;
-            }
-            if (ok && ws == 0 && tile < p.tiles) finish(grp, tile, slot, acc);
-        }
-    }
-    // After a failure copies may still be on their way: they get time to land (far above a copy's latency) before the block's
-    // shared memory is released.
+// After a failure copies may still be on their way: they get time to land (far above a copy's latency) before the block's shared
+// memory is released.
+__device__ __forceinline__ void moe_leave(MoeHead &head) {
     __syncthreads();
-    if (*fail) {
+    if (*(volatile int *)&head.fail) {
         const uint64_t t0 = globaltimer_ns();
         while (globaltimer_ns() - t0 < 100000) {
         }
     }
 }
 
-// ---- gate, up and the activation function --------------------------------------------------------
-template <int QT, int P, int NT>
-__global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __grid_constant__ MoeGateUp p) {
-    extern __shared__ __align__(128) uint8_t smem[];
-    const int lane = threadIdx.x & 31, g = lane >> 2;
+// Called by a whole warp after its stores: true in the warp that is the last of `parts` to come here for `count`, which then sees the
+// stores of all.  The count is zero again.
+__device__ __forceinline__ bool moe_last(unsigned *count, int parts, int lane) {
+    __syncwarp();
+    unsigned old = 0;
+    if (lane == 0)       // releases the warp's stores, acquires the others'
+        asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;" : "=r"(old) : "l"(count), "r"((unsigned)(parts - 1)) : "memory");
+    const bool last = __shfl_sync(0xFFFFFFFFu, old, 0) == (unsigned)(parts - 1);
+    __syncwarp();        // what lane 0 acquired is ordered before the other lanes' reads, too
+    return last;
+}
+
+// Equal runs of `total` steps for the blocks (of few steps, one each): block b has [begin(b), begin(b + 1))
+struct MoeShare {
+    long long total, blocks;
+    __device__ __forceinline__ MoeShare(long long steps) : total(steps), blocks(min((long long)gridDim.x, steps)) {}
+    __device__ __forceinline__ long long begin(long long b) const { return b < blocks ? total * b / blocks : total; }
+    __device__ __forceinline__ long long owner(long long step) const { return ((step + 1) * blocks - 1) / total; }
+};
+
+// A warp's way through the ring
+template <int D> struct MoeRing {
+    uint32_t phase = 0;
+    int stage = 0;
+    bool ok = true;
+    __device__ __forceinline__ void next() {
+        if (++stage == D) stage = 0, phase ^= 1;
+    }
+};
+
+// `steps` records of a group of n rows: acc of the warp's tile (active: there is one)
+template <int QT, int P, int NT, int D>
+__device__ __forceinline__ void moe_multiply(MoeRing<D> &ring, MoeHead &head, const uint8_t *smem, int stage_bytes, const uint8_t *zero, int *status, int steps,
+                                             int n, bool active, int warp, int lane, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
+    constexpr int REC = moe_rec_bytes(QT);
+    auto work = [&](auto mode, auto more) {
+        for (int s = 0; s < steps; ++s) {
+            // after a failure the products are left out, but shared sums are still counted
+            ring.ok = ring.ok && __all_sync(0xFFFFFFFFu, moe_wait(smem_u32(&head.full[ring.stage]), ring.phase, &head.fail, status));
+            if (!ring.ok) break;
+            if (active) {
+                uint32_t at = ring.stage * stage_bytes;
+                MoeRecord<QT, P>::template run<decltype(mode)>(smem + at + warp * REC, lane, smem + at + kMoeWarps * REC, zero, col, acc);
+                if constexpr (decltype(more)::NL > 0) {
+                    asm volatile("" : "+r"(at)::"memory");       // the weights are unpacked again, not kept
+                    MoeRecord<QT, P>::template run<decltype(more)>(smem + at + warp * REC, lane, smem + at + kMoeWarps * REC, zero, col, acc);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&head.empty[ring.stage]));
+            ring.next();
+        }
+    };
+    using None = MoeMode<0, 1>;
+    const int used = n * P;              // columns
+    if (P == 2 && used <= 2) work(MoeMode<1, 4>{}, None{});
+    else if (used <= 4) work(MoeMode<1, 2>{}, None{});
+    else if (used <= 8 || NT == 1) work(MoeMode<1, 1>{}, None{});
+    else if constexpr (NT > 1) {
+        if (used <= 16 || NT == 2) work(MoeMode<2, 1>{}, None{});
+        else if constexpr (NT > 2) {
+            if (used <= 24) work(MoeMode<2, 1>{}, MoeMode<1, 1, 2>{});
+            else work(MoeMode<2, 1>{}, MoeMode<2, 1, 2>{});
+        }
+    }
+    moe_join<P, NT>(col, acc);
+}
+
+__device__ __forceinline__ float moe_activate(const MoeActivation &p, long long at, float a, float b) {
+    if (p.gate_bias) a += p.gate_bias[at];
+    if (p.up_bias) b += p.up_bias[at];
+    if (p.kind == B200Q_MOE_SWIGLU_CLAMPED) {
+        // (comparisons that keep NaN)
+        a = a > p.limit ? p.limit : a;
+        b = b > p.limit ? p.limit : b < -p.limit ? -p.limit : b;
+        return a / (1.f + expf(-p.alpha * a)) * (b + 1.f);
+    }
+    return a / (1.f + expf(-a)) * b;
+}
+
+// ---- the producer ------------------------------------------------------------------------------------
+// One stretch of steps of the producer warp: records from r0 on of a group's rows and of eight tiles from tile0 on.  `word`: lane i holds word i
+// of the group.
+template <int QT, int P, int NT, int D>
+__device__ __forceinline__ void moe_produce(MoeRing<D> &ring, bool &full_ring, MoeHead &head, uint8_t *smem, const MoeProduct &p, int word, int tile0, int r0, int steps,
+                                            int lane) {
+    constexpr int REC = moe_rec_bytes(QT), IMG = moe_image_bytes(P), STAGE = moe_stage_bytes(QT, P, NT);
+    const MoeWeights &w = p.weights;
+    const int expert = __shfl_sync(0xFFFFFFFFu, word, 0), n = __shfl_sync(0xFFFFFFFFu, word, 1);
+    const int slot = __shfl_sync(0xFFFFFFFFu, word, 2 + lane % kMoeGroupRows);      // of row lane % 16
+    const int tiles = min(kMoeWarps, w.tiles - tile0);
+    // lanes 0 .. 7: the record of a tile; lanes 16 .. 31: the image of a row
+    const bool copies = lane < 16 ? lane < tiles : lane - 16 < n;
+    const uint8_t *src = lane < 16 ? w.w + expert * w.expert_bytes + ((long long)(tile0 + lane) * w.nrec + r0) * REC
+                                   : p.img + (size_t)(lane - 16 < n ? slot / p.slots_per_row : 0) * p.img_stride + (size_t)r0 * IMG;
+    const uint32_t at = lane < 16 ? lane * REC : kMoeWarps * REC + (lane - 16) * IMG, size = lane < 16 ? REC : IMG;
+    for (int s = 0; s < steps; ++s) {
+        if (full_ring) {
+            ring.ok = __all_sync(0xFFFFFFFFu, moe_wait(smem_u32(&head.empty[ring.stage]), ring.phase ^ 1, &head.fail, p.status));
+            if (!ring.ok) return;
+        }
+        const uint32_t bar = smem_u32(&head.full[ring.stage]);
+        if (lane < (int)(sizeof(MoeGroup) / 4)) reinterpret_cast<int *>(&head.group[ring.stage])[lane] = word;
+        fence_proxy_async();                 // the readers' last accesses precede the copies
+        __syncwarp();
+        if (lane == 0) mbar_expect_tx(bar, tiles * REC + n * IMG);
+        __syncwarp();
+        if (copies) bulk_g2s(smem_u32(smem + ring.stage * STAGE) + at, src, size, bar);
+        src += size;
+        ring.next();
+        if (ring.stage == 0) full_ring = true;
+    }
+}
+__device__ __forceinline__ int moe_group_word(const MoeProduct &p, int gi, int lane) {
+    return lane < (int)(sizeof(MoeGroup) / 4) ? reinterpret_cast<const int *>(p.lists.groups + gi)[lane] : 0;
+}
+
+// The group of the ring's next stage as the multiplying warps see it
+template <int NT> struct MoeView {
+    int expert, n, slot[NT];             // slot of the row of the lane's columns in every tile, -1: none
+};
+template <int P, int NT, int D>
+__device__ __forceinline__ MoeView<NT> moe_view(MoeRing<D> &ring, MoeHead &head, int *status, int lane, MoeColumns<NT> &col) {
+    ring.ok = ring.ok && __all_sync(0xFFFFFFFFu, moe_wait(smem_u32(&head.full[ring.stage]), ring.phase, &head.fail, status));
+    const MoeGroup &grp = head.group[ring.stage];
+    MoeView<NT> v;
+    v.expert = ring.ok ? grp.expert : 0;
+    v.n = ring.ok ? grp.n : 1;
+    const int slot = ring.ok ? grp.slot[lane % kMoeGroupRows] : 0;
+    col = moe_columns<P, NT>(v.n, lane);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = nt * (8 / P) + col.row, sl = __shfl_sync(0xFFFFFFFFu, slot, max(r, 0));
+        v.slot[nt] = ring.ok && col.row >= 0 && r < v.n ? sl : -1;
+    }
+    return v;
+}
+
+// ---- sums per slot -------------------------------------------------------------------------------------
+// A unit is a group and eight tiles; all units' steps are dealt to the blocks as equal runs.  Where a run ends inside a unit, every warp
+// leaves its sums in memory, and the one that is the last to come adds them up in the order of K, so that results do not depend on
+// who that is.
+//   finish(expert, tile, slots, acc): one warp per tile; the lane holds the sums of rows g, g + 8 of slots[nt] (-1: of none)
+template <int QT, int P, int NT, typename Finish> __device__ __forceinline__ void moe_slots(const MoeProduct &p, uint8_t *smem, Finish finish) {
+    constexpr int D = moe_depth(QT, P, NT, kMoeSmem), STAGE = moe_stage_bytes(QT, P, NT);
+    __shared__ MoeHead head;
+    __shared__ __align__(16) uint8_t zero[256 * P];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    moe_ring_init(head, D);
+    for (int i = tid; i < 64 * P; i += kMoeThreads) reinterpret_cast<uint32_t *>(zero)[i] = 0u;
     pdl_launch_dependents();
     pdl_wait();
-    moe_product<QT, P, NT>(p.product, smem, [&](const MoeGroup &grp, int tile, const int (&slot)[NT], const float (&acc)[NT][2]) {
+    __syncthreads();
+    const MoeWeights &w = p.weights;
+    const int runs = (w.tiles + kMoeWarps - 1) / kMoeWarps, steps = w.nrec;
+    const MoeShare share((long long)*p.lists.ngroups * runs * steps);
+    long long pos = share.begin(blockIdx.x);
+    const long long end = share.begin(blockIdx.x + 1);
+    MoeRing<D> ring;
+    bool full_ring = false;
+    for (int s1; pos < end; pos += s1) {
+        const int u = (int)(pos / steps), s0 = (int)(pos - (long long)u * steps), gi = u / runs, tile0 = (u - gi * runs) * kMoeWarps, tile = tile0 + warp;
+        s1 = (int)min((long long)(steps - s0), end - pos);
+        if (warp == kMoeWarps) {
+            if (!ring.ok) break;
+            moe_produce<QT, P, NT, D>(ring, full_ring, head, smem, p, moe_group_word(p, gi, lane), tile0, s0, s1, lane);
+            continue;
+        }
+        MoeColumns<NT> col;
+        const MoeView<NT> v = moe_view<P, NT, D>(ring, head, p.status, lane, col);
+        float acc[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = 0.f;
+        moe_multiply<QT, P, NT, D>(ring, head, smem, STAGE, zero, p.status, s1, v.n, tile < w.tiles, warp, lane, col, acc);
+        if (tile >= w.tiles) continue;
+        if (s1 < steps) {
+            // this block's share: [block][unit that began in an earlier block, unit that goes on in the next][warp]
+            auto part = [&](long long b, int later) { return p.partial + ((b * 2 + later) * kMoeWarps + warp) * kMoePart + lane; };
+            float *mine = part(blockIdx.x, s0 == 0);
+#pragma unroll
+            for (int i = 0; i < NT * 2; ++i) __stcg(mine + i * 32, acc[i >> 1][i & 1]);
+            const long long b0 = share.owner(pos - s0), b1 = share.owner(pos - s0 + steps - 1);
+            if (!moe_last(p.count + b0 * kMoeWarps + warp, (int)(b1 - b0) + 1, lane)) continue;
+#pragma unroll
+            for (int i = 0; i < NT * 2; ++i) acc[i >> 1][i & 1] = 0.f;
+            for (long long b = b0; b <= b1; ++b) {
+                const float *from = part(b, b == b0);
+#pragma unroll
+                for (int i = 0; i < NT * 2; ++i) acc[i >> 1][i & 1] += __ldcg(from + i * 32);
+            }
+        }
+        finish(v.expert, tile, v.slot, acc);
+    }
+    moe_leave(head);
+}
+
+// gate, up and the activation function
+template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __grid_constant__ MoeGateUp p) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int g = (threadIdx.x & 31) >> 2;
+    moe_slots<QT, P, NT>(p.product, smem, [&](int expert, int tile, const int (&slot)[NT], const float (&acc)[NT][2]) {
         const int f = tile * 8 + g;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            if (f >= p.ff || slot[nt] < 0) continue;
-            float a = acc[nt][0], b = acc[nt][1];
-            if (p.gate_bias) a += p.gate_bias[(long long)grp.expert * p.ff + f];
-            if (p.up_bias) b += p.up_bias[(long long)grp.expert * p.ff + f];
-            float h;
-            if (p.activation == B200Q_MOE_SWIGLU_CLAMPED) {
-                // (comparisons that keep NaN)
-                a = a > p.limit ? p.limit : a;
-                b = b > p.limit ? p.limit : b < -p.limit ? -p.limit : b;
-                h = a / (1.f + expf(-p.alpha * a)) * (b + 1.f);
-            } else {
-                h = a / (1.f + expf(-a)) * b;
-            }
-            p.h[(long long)slot[nt] * p.ff + f] = h;
-        }
+        for (int nt = 0; nt < NT; ++nt)
+            if (f < p.act.ff && slot[nt] >= 0)
+                p.h[(long long)slot[nt] * p.act.ff + f] = moe_activate(p.act, (long long)expert * p.act.ff + f, acc[nt][0], acc[nt][1]);
     });
 }
 
-// ---- down ------------------------------------------------------------------------------------------
-template <int QT, int P, int NT>
-__global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(const __grid_constant__ MoeDown p) {
+// down, more rows: every slot's outputs go to memory
+template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(const __grid_constant__ MoeDown p) {
     extern __shared__ __align__(128) uint8_t smem[];
-    const int lane = threadIdx.x & 31, g = lane >> 2;
-    pdl_launch_dependents();
-    pdl_wait();
-    moe_product<QT, P, NT>(p.product, smem, [&](const MoeGroup &grp, int tile, const int (&slot)[NT], const float (&acc)[NT][2]) {
+    const int g = (threadIdx.x & 31) >> 2;
+    moe_slots<QT, P, NT>(p.product, smem, [&](int, int tile, const int (&slot)[NT], const float (&acc)[NT][2]) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             if (slot[nt] < 0) continue;
@@ -565,8 +643,102 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(const __grid_c
     });
 }
 
+// ---- down and the weighted sums of few rows ----------------------------------------------------------------
+// Run after run of eight tiles, all groups: a warp keeps its tile's outputs of all rows in shared memory and adds every group's to them, so that
+// the sums over experts cost neither memory nor meetings; blocks that share a run add up their parts as above.
+template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 2) moe_few_down_kernel(const __grid_constant__ MoeFewDown p) {
+    constexpr int D = moe_depth(QT, P, NT, kMoeFewSmem), STAGE = moe_stage_bytes(QT, P, NT);
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ MoeHead head;
+    __shared__ __align__(16) uint8_t zero[256 * P];
+    __shared__ float outputs[kMoeWarps][kMoeFewRows][16];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    moe_ring_init(head, D);
+    for (int i = tid; i < 64 * P; i += kMoeThreads) reinterpret_cast<uint32_t *>(zero)[i] = 0u;
+    for (int i = tid; i < kMoeWarps * kMoeFewRows * 16; i += kMoeThreads) (&outputs[0][0][0])[i] = 0.f;
+    pdl_launch_dependents();
+    pdl_wait();
+    __syncthreads();
+    const MoeProduct &pr = p.product;
+    const MoeWeights &w = pr.weights;
+    const MoeOutput &o = p.out;
+    const int groups = *pr.lists.ngroups, runs = (w.tiles + kMoeWarps - 1) / kMoeWarps, steps = w.nrec, m = p.choice.m;
+    if (groups == 0)                     // no row has a choice
+        for (int i = blockIdx.x * kMoeThreads + tid; i < m * o.n; i += gridDim.x * kMoeThreads) moe_store(o, i / o.n, i % o.n, 0.f);
+    const long long run_steps = (long long)groups * steps;
+    const MoeShare share(run_steps * runs);
+    long long pos = share.begin(blockIdx.x);
+    const long long end = share.begin(blockIdx.x + 1);
+    MoeRing<D> ring;
+    bool full_ring = false;
+    bool whole = false;                  // the run's first step was this block's
+    for (int s1; pos < end; pos += s1) {
+        const int run = (int)(pos / run_steps), gi = (int)((pos - run * run_steps) / steps), s0 = (int)(pos - run * run_steps - (long long)gi * steps);
+        const int tile0 = run * kMoeWarps, tile = tile0 + warp;
+        s1 = (int)min((long long)(steps - s0), end - pos);
+        if (warp == kMoeWarps) {
+            if (!ring.ok) break;
+            moe_produce<QT, P, NT, D>(ring, full_ring, head, smem, pr, moe_group_word(pr, gi, lane), tile0, s0, s1, lane);
+            continue;
+        }
+        if (gi == 0 && s0 == 0) whole = true;
+        MoeColumns<NT> col;
+        const MoeView<NT> v = moe_view<P, NT, D>(ring, head, pr.status, lane, col);
+        float acc[NT][2], weight[NT], bias[2] = {0.f, 0.f};
+        int row[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            acc[nt][0] = acc[nt][1] = 0.f;
+            row[nt] = v.slot[nt] < 0 ? -1 : v.slot[nt] / p.choice.top_k;
+            weight[nt] = v.slot[nt] < 0 ? 0.f : p.choice.weights[row[nt] * p.choice.ld_weights + v.slot[nt] % p.choice.top_k];
+        }
+        if (o.bias && s0 == 0)           // (once, with the group's first record)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (tile * 16 + g + 8 * i < o.n) bias[i] = o.bias[(long long)v.expert * o.n + tile * 16 + g + 8 * i];
+        moe_multiply<QT, P, NT, D>(ring, head, smem, STAGE, zero, pr.status, s1, v.n, tile < w.tiles, warp, lane, col, acc);
+        if (tile >= w.tiles) continue;
+        // one lane group after the other: a row that chose the expert twice has two columns
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (t == i && row[nt] >= 0) {
+                    float *out = outputs[warp][row[nt]];
+                    out[g] = fmaf(weight[nt], acc[nt][0] + bias[0], out[g]);
+                    out[g + 8] = fmaf(weight[nt], acc[nt][1] + bias[1], out[g + 8]);
+                }
+                __syncwarp();
+            }
+        const bool last_step = gi == groups - 1 && s0 + s1 == steps;
+        if (!last_step && pos + s1 < end) continue;
+        // the run ends here, or this block's part of it
+        float *own = &outputs[warp][0][0];
+        const long long begin = run * run_steps, b0 = share.owner(begin), b1 = share.owner(begin + run_steps - 1);
+        auto part = [&](long long b, int later) { return pr.partial + ((b * 2 + later) * kMoeWarps + warp) * kMoePart; };
+        bool mine = true;
+        if (b1 > b0) {
+            float *to = part(blockIdx.x, whole);
+            for (int i = lane; i < m * 16; i += 32) __stcg(to + i, own[i]);
+            mine = moe_last(pr.count + b0 * kMoeWarps + warp, (int)(b1 - b0) + 1, lane);
+        }
+        if (mine)
+            for (int i = lane; i < m * 16; i += 32) {
+                float sum = b1 == b0 ? own[i] : 0.f;
+                if (b1 > b0)
+#pragma unroll 8
+                    for (long long b = b0; b <= b1; ++b) sum += __ldcg(part(b, b == b0) + i);
+                if (tile * 16 + (i & 15) < o.n && ring.ok) moe_store(o, i >> 4, tile * 16 + (i & 15), sum);
+            }
+        for (int i = lane; i < m * 16; i += 32) own[i] = 0.f;
+        __syncwarp();
+        whole = false;
+    }
+    moe_leave(head);
+}
+
 template <typename Kernel, typename Params> cudaError_t moe_launch(Kernel kern, const Params &p, int grid, size_t smem, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = moe_configure(reinterpret_cast<const void *>(kern), smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
@@ -586,26 +758,27 @@ template <typename Kernel, typename Params> cudaError_t moe_launch(Kernel kern, 
 }  // namespace b200q
 
 // one source file per weight type (they compile side by side)
-#define MOE_INSTANTIATE(NAME, QT)                                                                                                     \
-    namespace b200q {                                                                                                                 \
-    namespace {                                                                                                                       \
-    size_t moe_smem(const MoeProduct &p, const MoeConfig &c) {                                                                          \
-        return (size_t)moe_depth(QT, c.planes, c.column_tiles) * moe_stage_bytes(QT, c.planes, c.column_tiles, p.split);                   \
-    }                                                                                                                                 \
-    }                                                                                                                                 \
-    cudaError_t moe_gate_up_##NAME(const MoeGateUp &p, const MoeConfig &c, int grid, cudaStream_t st) {                                 \
-        const size_t smem = moe_smem(p.product, c);                                                                                     \
-        if (c.planes == 2) return c.column_tiles == 1 ? moe_launch(moe_gate_up_kernel<QT, 2, 1>, p, grid, smem, st)                     \
-                                                      : moe_launch(moe_gate_up_kernel<QT, 2, 4>, p, grid, smem, st);                    \
-        return c.column_tiles == 1 ? moe_launch(moe_gate_up_kernel<QT, 4, 1>, p, grid, smem, st)                                        \
-                                   : moe_launch(moe_gate_up_kernel<QT, 4, 4>, p, grid, smem, st);                                       \
-    }                                                                                                                                 \
-    cudaError_t moe_down_##NAME(const MoeDown &p, const MoeConfig &c, int grid, cudaStream_t st) {                                      \
-        const size_t smem = moe_smem(p.product, c);                                                                                     \
-        if (c.planes == 2) return c.column_tiles == 1 ? moe_launch(moe_down_kernel<QT, 2, 1>, p, grid, smem, st)                        \
-                                                      : moe_launch(moe_down_kernel<QT, 2, 4>, p, grid, smem, st);                       \
-        return c.column_tiles == 1 ? moe_launch(moe_down_kernel<QT, 4, 1>, p, grid, smem, st)                                           \
-                                   : moe_launch(moe_down_kernel<QT, 4, 4>, p, grid, smem, st);                                          \
-    }                                                                                                                                 \
-    cudaError_t moe_wait_limit_##NAME(unsigned long long ns) { return cudaMemcpyToSymbol(s_wait_limit_ns, &ns, sizeof(ns)); }            \
+#define MOE_INSTANTIATE(NAME, QT)                                                                                                 \
+    namespace b200q {                                                                                                             \
+    namespace {                                                                                                                   \
+    template <int P, int NT> constexpr size_t moe_smem(int room) { return (size_t)moe_depth(QT, P, NT, room) * moe_stage_bytes(QT, P, NT); } \
+    template <int P, int NT> struct MoeKernels {                                                                                    \
+        static cudaError_t run(const MoeGateUp &p, int grid, cudaStream_t st) { return moe_launch(moe_gate_up_kernel<QT, P, NT>, p, grid, moe_smem<P, NT>(kMoeSmem), st); } \
+        static cudaError_t run(const MoeDown &p, int grid, cudaStream_t st) { return moe_launch(moe_down_kernel<QT, P, NT>, p, grid, moe_smem<P, NT>(kMoeSmem), st); } \
+        static cudaError_t run(const MoeFewDown &p, int grid, cudaStream_t st) { return moe_launch(moe_few_down_kernel<QT, P, NT>, p, grid, moe_smem<P, NT>(kMoeFewSmem), st); } \
+    };                                                                                                                            \
+    template <typename Params> cudaError_t few(const Params &p, int planes, int tiles, int grid, cudaStream_t st) {                 \
+        if (planes == 2) return tiles == 1 ? MoeKernels<2, 1>::run(p, grid, st) : MoeKernels<2, 2>::run(p, grid, st);                 \
+        return tiles == 1 ? MoeKernels<4, 1>::run(p, grid, st) : MoeKernels<4, 2>::run(p, grid, st);                                  \
+    }                                                                                                                             \
+    template <typename Params> cudaError_t many(const Params &p, int planes, int grid, cudaStream_t st) {                           \
+        return planes == 2 ? MoeKernels<2, 4>::run(p, grid, st) : MoeKernels<4, 4>::run(p, grid, st);                                 \
+    }                                                                                                                             \
+    }                                                                                                                             \
+    cudaError_t moe_gate_up_##NAME(const MoeGateUp &p, int planes, int tiles, int grid, cudaStream_t st) {                          \
+        return tiles <= 2 ? few(p, planes, tiles, grid, st) : many(p, planes, grid, st);                                              \
+    }                                                                                                                             \
+    cudaError_t moe_few_down_##NAME(const MoeFewDown &p, int planes, int tiles, int grid, cudaStream_t st) { return few(p, planes, tiles, grid, st); } \
+    cudaError_t moe_down_##NAME(const MoeDown &p, int planes, int grid, cudaStream_t st) { return many(p, planes, grid, st); }       \
+    cudaError_t moe_wait_limit_##NAME(unsigned long long ns) { return cudaMemcpyToSymbol(s_wait_limit_ns, &ns, sizeof(ns)); }        \
     }

@@ -27,7 +27,7 @@ namespace b200q {
 //           then the rows' 16 int8 scales, then their d
 // The byte count is GGUF's (blocks of 32 weights: K padded to 256, rows to 16 with zeros).
 // ---------------------------------------------------------------------------------------------
-constexpr int kMoeWarps = 8, kMoeThreads = 32 * (kMoeWarps + 1);      // warps that multiply; with the producer
+constexpr int kMoeWarps = 8;             // warps that multiply
 __host__ __device__ constexpr int moe_rec_bytes(int qt) { return 16 * (qt == QT_Q4_K || qt == QT_Q4_0 ? 144 : qt == QT_Q5_K ? 176 : qt == QT_Q6_K ? 210 : qt == QT_Q8_0 ? 272 : 136); }
 // ---------------------------------------------------------------------------------------------
 // Activations
@@ -40,22 +40,21 @@ __host__ __device__ constexpr int moe_rec_bytes(int qt) { return 16 * (qt == QT_
 // ---------------------------------------------------------------------------------------------
 __host__ __device__ constexpr int moe_image_bytes(int planes) { return planes * (256 + 16) + 16; }
 
-// A block's ring: a stage holds eight records and the images of a group's rows, once per record of a tile in it.  As many stages (2 to
-// 4) as leave room for two blocks an SM: half of 228 KB each, less 1 KB that a block costs by itself and 6 KB of its own.
-constexpr int kMoeSmem = 109568, kMoeMaxDepth = 4;
+constexpr int kMoeThreads = 32 * (kMoeWarps + 1);      // with the producer
+constexpr int kMoeFewRows = 16;          // up to so many rows their outputs are added up inside the down product
+constexpr int kMoeManyTiles = 4;         // column tiles of a group of more rows
+
+// A block's ring: a stage holds eight records and the images of a group's rows.  As many stages (2 to 4) as leave room for two blocks an
+// SM: half of 228 KB each, less 1 KB that a block costs by itself and what it has beside the ring (few rows: 8 KB of outputs).
+constexpr int kMoeSmem = 113664, kMoeFewSmem = 105472, kMoeMaxDepth = 4;
+constexpr int kMoePart = 256;            // floats of a warp's share of a cut unit: two per lane and column tile, or 16 outputs of 16 rows
 __host__ __device__ constexpr int moe_group_rows(int planes, int column_tiles) { return column_tiles * 8 / planes; }
-__host__ __device__ constexpr int moe_stage_bytes(int qt, int planes, int column_tiles, int split) {
-    return kMoeWarps * moe_rec_bytes(qt) + split * moe_group_rows(planes, column_tiles) * moe_image_bytes(planes);
+__host__ __device__ constexpr int moe_stage_bytes(int qt, int planes, int column_tiles) {
+    return kMoeWarps * moe_rec_bytes(qt) + moe_group_rows(planes, column_tiles) * moe_image_bytes(planes);
 }
-__host__ __device__ constexpr int moe_depth(int qt, int planes, int column_tiles) {
-    const int d = kMoeSmem / moe_stage_bytes(qt, planes, column_tiles, 1);
+__host__ __device__ constexpr int moe_depth(int qt, int planes, int column_tiles, int room) {
+    const int d = room / moe_stage_bytes(qt, planes, column_tiles);
     return d < 2 ? 2 : d > kMoeMaxDepth ? kMoeMaxDepth : d;
-}
-// warps that may share a tile's records: with one column tile only, and while the stages fit
-__host__ __device__ constexpr int moe_max_split(int qt, int planes, int column_tiles) {
-    int s = column_tiles == 1 ? kMoeWarps : 1;
-    while (s > 1 && moe_depth(qt, planes, column_tiles) * moe_stage_bytes(qt, planes, column_tiles, s) > kMoeSmem) s /= 2;
-    return s;
 }
 
 constexpr int kMoeMaxRows = 512, kMoeMaxTopK = 16, kMoeMaxSlots = kMoeMaxRows * kMoeMaxTopK, kMoeMaxExperts = 1024;
@@ -72,34 +71,74 @@ struct MoeLists {
     MoeGroup *groups;
 };
 
-struct MoeProduct {
+struct MoeWeights {
     const uint8_t *w;
     long long expert_bytes;
-    int tiles, nrec, split;              // split: warps that share a tile's records
-    MoeLists lists;
-    const uint8_t *img;                  // images
-    unsigned img_stride;                 // bytes of a row's image
-    int slots_per_row;                   // slot / slots_per_row = row of the images
-    int *status;
+    int tiles, nrec;
 };
 
-struct MoeGateUp {
-    MoeProduct product;
-    float *h;                            // [slot][ff]
-    int ff;
-    int activation;
+struct MoeActivation {
+    int ff, kind;
     float alpha, limit;
     const float *gate_bias, *up_bias;    // [expert][ff] or null
 };
 
+// rows that become images
+struct MoeRows {
+    const void *x;
+    long long ldx;
+    int x_is_bf16, vec_ok;               // vec_ok: rows are 16-byte aligned
+    int rows, K, nrec;
+    uint8_t *img;                        // where to
+    unsigned img_stride;
+};
+
+struct MoeChoice {
+    const int *ids;
+    long long ld_ids;
+    const float *weights;
+    long long ld_weights;
+    int m, top_k, experts;
+};
+
+struct MoeOutput {
+    void *y;
+    long long ldy;
+    const float *bias;                   // [expert][n] or null
+    int y_is_bf16, accumulate, n;
+};
+
+struct MoeProduct {
+    MoeWeights weights;
+    MoeLists lists;
+    const uint8_t *img;                  // images
+    unsigned img_stride;                 // bytes of a row's image
+    int slots_per_row;                   // slot / slots_per_row = row of the images
+    float *partial;                      // [block][2][warp][kMoePart]: shares of cut units
+    unsigned *count;                     // [block][warp]: shares seen so far; zero between launches
+    int *status;
+};
+struct MoeGateUp {
+    MoeProduct product;
+    MoeActivation act;
+    float *h;                            // [slot][ff]
+};
+struct MoeFewDown {
+    MoeProduct product;
+    MoeChoice choice;
+    MoeOutput out;
+};
 struct MoeDown {
     MoeProduct product;
     float *z;                            // [slot][ld_z]
     long long ld_z;
 };
-
-struct MoeConfig {                       // what picks a kernel
-    int planes, column_tiles;
+// y[m] = sum over the row's choices, in their order
+struct MoeCombine {
+    MoeChoice choice;
+    MoeOutput out;
+    const float *z;
+    long long ld_z;
 };
 
 // ---- moe.cu: what the C ABI layer calls ----------------------------------------------------------
@@ -111,7 +150,8 @@ struct MoeBuffers {
     MoeLists lists;
     float *h;
     uint8_t *x_img, *h_img;
-    float *z;
+    float *z, *partial;
+    unsigned *count;
 };
 struct MoeRun {
     MoeShapeInfo shape;
@@ -119,19 +159,10 @@ struct MoeRun {
     MoeBuffers buf;
     int gate_up_type, down_type;
     const uint8_t *gate_up, *down;
-    const float *gate_bias, *up_bias, *down_bias;
-    int activation;
-    float alpha, limit;
-    const void *x;
-    long long ldx;
-    int x_is_bf16, m;
-    const int *ids;
-    long long ld_ids;
-    const float *weights;
-    long long ld_weights;
-    void *y;
-    long long ldy;
-    int y_is_bf16, accumulate;
+    MoeActivation act;
+    MoeRows x;                           // nrec and images are filled in
+    MoeChoice choice;
+    MoeOutput out;
 };
 size_t moe_matrix_bytes(int qt, int64_t experts, int64_t rows, int64_t K, bool paired);
 // GGUF rows [expert][row] in device memory -> records; src1: the up matrix that shares tiles with src0, or null
@@ -140,9 +171,10 @@ cudaError_t moe_repack(int qt, const uint8_t *src0, const uint8_t *src1, uint8_t
 size_t moe_workspace(const MoeShapeInfo &s, MoeBuffers *out, uint8_t *base);
 cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches);
 
-#define MOE_DECLARE(NAME)                                                                                     \
-    cudaError_t moe_gate_up_##NAME(const MoeGateUp &p, const MoeConfig &c, int grid, cudaStream_t st);          \
-    cudaError_t moe_down_##NAME(const MoeDown &p, const MoeConfig &c, int grid, cudaStream_t st);               \
+#define MOE_DECLARE(NAME)                                                                                               \
+    cudaError_t moe_gate_up_##NAME(const MoeGateUp &p, int planes, int tiles, int grid, cudaStream_t st);                 \
+    cudaError_t moe_few_down_##NAME(const MoeFewDown &p, int planes, int tiles, int grid, cudaStream_t st);               \
+    cudaError_t moe_down_##NAME(const MoeDown &p, int planes, int grid, cudaStream_t st);                                 \
     cudaError_t moe_wait_limit_##NAME(unsigned long long ns);
 MOE_DECLARE(q4_k)
 MOE_DECLARE(q5_k)
