@@ -24,7 +24,6 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 256, kWarps = 8, kCluster = 8;
-constexpr int kRankBlock = 64;           // ranks whose sums a warp holds at a time
 constexpr int kLeaderRows = 512;
 
 // D += A (16 x 16 bf16, row) * B (16 x 8 bf16, col)
@@ -65,147 +64,184 @@ struct RowList {
     int n;
 };
 
-// eight elements of an activation row from k0 on as planes of four words; zeros beyond K and for missing rows
-template <bool XF32, int PX> __device__ __forceinline__ void load_x(const AdaptersParams &p, int row, int k0, uint32_t (&out)[PX][4]) {
-    if (row < 0 || k0 >= p.K) {
+// eight elements of an activation row from k0 on, loaded ahead; zeros beyond K and for missing rows
+template <bool XF32> struct XPiece {
+    uint4 w[XF32 ? 2 : 1];
+    __device__ __forceinline__ void load(const AdaptersParams &p, int row, int k0, bool wanted) {
 #pragma unroll
-        for (int i = 0; i < PX; ++i)
+        for (int i = 0; i < (XF32 ? 2 : 1); ++i) w[i] = make_uint4(0, 0, 0, 0);
+        if (row < 0 || !wanted) return;
+        if (XF32) {
+            const uint32_t *src = reinterpret_cast<const uint32_t *>(p.x) + row * p.ldx + k0;
+            if (p.x_vec && k0 + 8 <= p.K) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) out[i][j] = 0u;
-        return;
-    }
-    if (XF32) {
-        float v[8];
-        const float *src = reinterpret_cast<const float *>(p.x) + row * p.ldx + k0;
-        if (p.x_vec && k0 + 8 <= p.K) {
-            const float4 a = reinterpret_cast<const float4 *>(src)[0], b = reinterpret_cast<const float4 *>(src)[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+                for (int i = 0; i < (XF32 ? 2 : 1); ++i) w[i] = reinterpret_cast<const uint4 *>(src)[i];
+            } else {
+                uint32_t v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = k0 + i < p.K ? src[i] : 0u;
+#pragma unroll
+                for (int i = 0; i < (XF32 ? 2 : 1); ++i) w[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            }
         } else {
+            const unsigned short *src = reinterpret_cast<const unsigned short *>(p.x) + row * p.ldx + k0;
+            if (p.x_vec && k0 + 8 <= p.K) {
+                w[0] = *reinterpret_cast<const uint4 *>(src);
+            } else {
+                uint32_t v[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = k0 + i < p.K ? src[i] : 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t w[PX];
-            split<PX>(v[2 * j], v[2 * j + 1], w);
-#pragma unroll
-            for (int i = 0; i < PX; ++i) out[i][j] = w[i];
-        }
-    } else {
-        const unsigned short *src = reinterpret_cast<const unsigned short *>(p.x) + row * p.ldx + k0;
-        if (p.x_vec && k0 + 8 <= p.K) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(src);
-            out[0][0] = w.x, out[0][1] = w.y, out[0][2] = w.z, out[0][3] = w.w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t lo = k0 + 2 * j < p.K ? src[2 * j] : 0u, hi = k0 + 2 * j + 1 < p.K ? src[2 * j + 1] : 0u;
-                out[0][j] = lo | hi << 16;
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t lo = k0 + 2 * j < p.K ? src[2 * j] : 0u, hi = k0 + 2 * j + 1 < p.K ? src[2 * j + 1] : 0u;
+                    v[j] = lo | hi << 16;
+                }
+                w[0] = make_uint4(v[0], v[1], v[2], v[3]);
             }
         }
     }
-}
-
-// eight outputs of a row from n0 on: y += scale * v
-template <bool YF32> __device__ __forceinline__ void add_y(const AdapterSet &s, int row, int n0, float scale, const float (&v)[8]) {
-    if (YF32) {
-        float *y = reinterpret_cast<float *>(s.y) + row * s.ldy + n0;
-        if (s.y_vec && n0 + 8 <= s.n) {
-            float4 a = reinterpret_cast<float4 *>(y)[0], b = reinterpret_cast<float4 *>(y)[1];
-            a.x = fmaf(scale, v[0], a.x), a.y = fmaf(scale, v[1], a.y), a.z = fmaf(scale, v[2], a.z), a.w = fmaf(scale, v[3], a.w);
-            b.x = fmaf(scale, v[4], b.x), b.y = fmaf(scale, v[5], b.y), b.z = fmaf(scale, v[6], b.z), b.w = fmaf(scale, v[7], b.w);
-            reinterpret_cast<float4 *>(y)[0] = a;
-            reinterpret_cast<float4 *>(y)[1] = b;
+    // as planes of four words (pairs of elements)
+    __device__ __forceinline__ void planes(uint32_t (&out)[XF32 ? 3 : 1][4]) const {
+        if (XF32) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t v[XF32 ? 3 : 1];
+                const uint4 &p = w[XF32 ? j >> 1 : 0];
+                split(__uint_as_float(word_of(p, 2 * (j & 1))), __uint_as_float(word_of(p, 2 * (j & 1) + 1)), v);
+#pragma unroll
+                for (int i = 0; i < (XF32 ? 3 : 1); ++i) out[i][j] = v[i];
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (n0 + i < s.n) y[i] = fmaf(scale, v[i], y[i]);
+            for (int j = 0; j < 4; ++j) out[0][j] = word_of(w[0], j);
         }
-    } else {
-        __nv_bfloat16 *y = reinterpret_cast<__nv_bfloat16 *>(s.y) + row * s.ldy + n0;
-        if (s.y_vec && n0 + 8 <= s.n) {
-            uint4 w = *reinterpret_cast<uint4 *>(y);
+    }
+};
+
+// Eight outputs of a row from n0 on, loaded ahead (rows of whole 16-byte pieces) and put back with scale * v added
+template <bool YF32> struct OutputPiece {
+    uint4 w[YF32 ? 2 : 1];
+    static __device__ __forceinline__ uint4 *at(const AdapterSet &s, int row, int n0) {
+        return reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(s.y) + (row * s.ldy + n0) * (YF32 ? 4 : 2));
+    }
+    __device__ __forceinline__ void load(const AdapterSet &s, int row, int n0) {
+        const uint4 *y = at(s, row, n0);
+#pragma unroll
+        for (int i = 0; i < (YF32 ? 2 : 1); ++i) w[i] = y[i];
+    }
+    __device__ __forceinline__ void add(const AdapterSet &s, int row, int n0, float scale, const float (&v)[8]) {
+        uint4 *y = at(s, row, n0);
+        if (YF32) {
+#pragma unroll
+            for (int i = 0; i < (YF32 ? 2 : 1); ++i)
+                y[i] = make_uint4(__float_as_uint(fmaf(scale, v[4 * i], __uint_as_float(w[i].x))), __float_as_uint(fmaf(scale, v[4 * i + 1], __uint_as_float(w[i].y))),
+                                  __float_as_uint(fmaf(scale, v[4 * i + 2], __uint_as_float(w[i].z))), __float_as_uint(fmaf(scale, v[4 * i + 3], __uint_as_float(w[i].w))));
+        } else {
             uint32_t o[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t u = word_of(w, i);
+                const uint32_t u = word_of(w[0], i);
                 o[i] = last_plane(fmaf(scale, v[2 * i], __uint_as_float(u << 16)), fmaf(scale, v[2 * i + 1], __uint_as_float(u & 0xFFFF0000u)));
             }
-            *reinterpret_cast<uint4 *>(y) = make_uint4(o[0], o[1], o[2], o[3]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (n0 + i < s.n) y[i] = __float2bfloat16_rn(fmaf(scale, v[i], __bfloat162float(y[i])));
+            y[0] = make_uint4(o[0], o[1], o[2], o[3]);
         }
+    }
+};
+// one output
+template <bool YF32> __device__ __forceinline__ void add_y(const AdapterSet &s, int row, int n, float scale, float v) {
+    if (YF32) {
+        float *y = reinterpret_cast<float *>(s.y) + row * s.ldy + n;
+        *y = fmaf(scale, v, *y);
+    } else {
+        __nv_bfloat16 *y = reinterpret_cast<__nv_bfloat16 *>(s.y) + row * s.ldy + n;
+        *y = __float2bfloat16_rn(fmaf(scale, v, __bfloat162float(*y)));
     }
 }
 
-// shared memory: the warps' sums of a rank block, this block's t, t as operand fragments
+// Shared memory: the warps' sums of a rank block (later a 16 x 32 piece of outputs per warp), this block's t, t as operand fragments.
+// kRanks: ranks whose sums a warp holds at a time.
+constexpr int kTileLd = 33;
 template <int MT> struct Smem {
-    static constexpr int kRows = 16 * MT, kKWarps = kWarps / MT;
-    static constexpr size_t kSums = size_t(kKWarps) * kRows * kRankBlock * 4;
+    static constexpr int kRows = 16 * MT, kKWarps = kWarps / MT, kRanks = MT == 1 ? 32 : 64;
+    static constexpr size_t kSums = size_t(kKWarps) * kRows * kRanks * 4 > size_t(kWarps) * 16 * kTileLd * 4 ? size_t(kKWarps) * kRows * kRanks * 4
+                                                                                                          : size_t(kWarps) * 16 * kTileLd * 4;
     static size_t bytes(int rank_pad, int planes) { return kSums + size_t(kRows) * rank_pad * 4 + size_t(MT) * (rank_pad / 16) * planes * 512; }
 };
+
+__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 // one adapter against the rows of `list`
 template <bool F16, bool XF32, bool YF32, int MT>
 __device__ __forceinline__ void adapter_pass(const AdaptersParams &p, const AdapterSet &s, int slot, const RowList &list, int rank_pad_max, uint8_t *smem) {
     using S = Smem<MT>;
-    constexpr int PX = XF32 ? 3 : 1, PA = F16 ? 2 : 1, PT = YF32 ? 3 : 2;
+    constexpr int PX = XF32 ? 3 : 1, PA = F16 ? 2 : 1, PT = YF32 ? 3 : 2, RT = S::kRanks / 8;
     cg::cluster_group cluster = cg::this_cluster();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, part = (int)cluster.block_rank();
     const int rank = s.rank[slot], rt = (rank + 7) / 8, rk = (rank + 15) / 16, rank_pad = 16 * rk;
     float *sums = reinterpret_cast<float *>(smem);
     float *tpart = reinterpret_cast<float *>(smem + S::kSums);
     uint4 *frag = reinterpret_cast<uint4 *>(smem + S::kSums + (size_t)S::kRows * rank_pad_max * 4);
+    const float scale = s.scale[slot];
+    const uint4 *b = reinterpret_cast<const uint4 *>(s.b + slot * s.b_stride);
+    const int nc0 = (int)((long long)s.nchunks * part / kCluster), nc1 = (int)((long long)s.nchunks * (part + 1) / kCluster);
+    if (MT == 1)                             // B and y start their way while A is multiplied: 128 bytes a thread and turn
+        for (long long i = (long long)nc0 * rk * 1024 + threadIdx.x * 128, end = min((long long)nc1 * rk * 1024, i + 64 * 1024); i < end; i += kThreads * 128)
+            prefetch_l2(reinterpret_cast<const uint8_t *>(b) + i);
 
     // ---- t = A x over this block's part of K
     const int mt = warp % MT, kw = warp / MT;
     const int row0 = list.row[mt * 16 + g], row1 = list.row[mt * 16 + g + 8];
     const uint4 *a = reinterpret_cast<const uint4 *>(s.a + slot * s.a_stride);
-    const int kc0 = p.kchunks * part / kCluster, kc1 = p.kchunks * (part + 1) / kCluster;
-    for (int rb = 0; rb < rt; rb += kRankBlock / 8) {
-        const int tiles = min(rt - rb, kRankBlock / 8);
-        float acc[kRankBlock / 8][4];
+    const int kc0 = (int)((long long)p.kchunks * part / kCluster), kc1 = (int)((long long)p.kchunks * (part + 1) / kCluster);
+    for (int rb = 0; rb < rt; rb += RT) {
+        const int tiles = min(rt - rb, RT);
+        float acc[RT][4];
 #pragma unroll
-        for (int i = 0; i < kRankBlock / 8; ++i)
+        for (int i = 0; i < RT; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+        XPiece<XF32> x0, x1;                 // the next chunk's, on their way
+        x0.load(p, row0, (kc0 + kw) * 32 + 8 * t, kc0 + kw < kc1);
+        x1.load(p, row1, (kc0 + kw) * 32 + 8 * t, kc0 + kw < kc1);
         for (int kc = kc0 + kw; kc < kc1; kc += S::kKWarps) {
-            uint32_t x0[PX][4], x1[PX][4];
-            load_x<XF32, PX>(p, row0, kc * 32 + 8 * t, x0);
-            load_x<XF32, PX>(p, row1, kc * 32 + 8 * t, x1);
+            uint32_t f0[PX][4], f1[PX][4];
+            x0.planes(f0);
+            x1.planes(f1);
+            uint4 w[RT];
 #pragma unroll
-            for (int i = 0; i < kRankBlock / 8; ++i) {
+            for (int i = 0; i < RT; ++i)
+                if (i < tiles) w[i] = a[((size_t)kc * rt + rb + i) * 32 + lane];
+            x0.load(p, row0, (kc + S::kKWarps) * 32 + 8 * t, kc + S::kKWarps < kc1);
+            x1.load(p, row1, (kc + S::kKWarps) * 32 + 8 * t, kc + S::kKWarps < kc1);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
                 if (i >= tiles) break;
-                const uint4 w = a[((size_t)kc * rt + rb + i) * 32 + lane];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t b0[PA], b1[PA];
-                    adapter_planes<F16, PA>(h ? w.z : w.x, b0);
-                    adapter_planes<F16, PA>(h ? w.w : w.y, b1);
+                    adapter_planes<F16, PA>(h ? w[i].z : w[i].x, b0);
+                    adapter_planes<F16, PA>(h ? w[i].w : w[i].y, b1);
 #pragma unroll
                     for (int px = 0; px < PX; ++px)
 #pragma unroll
                         for (int pa = 0; pa < PA; ++pa)
-                            mma_bf16(acc[i], x0[px][2 * h], x1[px][2 * h], x0[px][2 * h + 1], x1[px][2 * h + 1], b0[pa], b1[pa]);
+                            mma_bf16(acc[i], f0[px][2 * h], f1[px][2 * h], f0[px][2 * h + 1], f1[px][2 * h + 1], b0[pa], b1[pa]);
                 }
             }
         }
 #pragma unroll
-        for (int i = 0; i < kRankBlock / 8; ++i) {
+        for (int i = 0; i < RT; ++i) {
             if (i >= tiles) break;
-            float *dst = sums + ((size_t)kw * S::kRows + mt * 16 + g) * kRankBlock + 8 * i + 2 * t;
+            float *dst = sums + ((size_t)kw * S::kRows + mt * 16 + g) * S::kRanks + 8 * i + 2 * t;
             *reinterpret_cast<float2 *>(dst) = make_float2(acc[i][0], acc[i][1]);
-            *reinterpret_cast<float2 *>(dst + 8 * kRankBlock) = make_float2(acc[i][2], acc[i][3]);
+            *reinterpret_cast<float2 *>(dst + 8 * S::kRanks) = make_float2(acc[i][2], acc[i][3]);
         }
         __syncthreads();
-        const int width = min(rank_pad - 8 * rb, kRankBlock);        // the last tile of 16 may be half there
+        const int width = min(rank_pad - 8 * rb, S::kRanks);        // the last tile of 16 may be half there
         for (int i = threadIdx.x; i < S::kRows * width; i += kThreads) {
             const int r = i / width, c = i - r * width;
             float v = 0.f;
             if (c < 8 * tiles)
-                for (int w = 0; w < S::kKWarps; ++w) v += sums[((size_t)w * S::kRows + r) * kRankBlock + c];
+#pragma unroll
+                for (int w = 0; w < S::kKWarps; ++w) v += sums[((size_t)w * S::kRows + r) * S::kRanks + c];
             tpart[r * rank_pad + 8 * rb + c] = v;
         }
         __syncthreads();
@@ -219,12 +255,11 @@ __device__ __forceinline__ void adapter_pass(const AdaptersParams &p, const Adap
 #pragma unroll
         for (int e = 0; e < 4; ++e) {                            // (row g, ranks 2 t), (row g + 8, ..), (row g, ranks 2 t + 8), (..)
             const int at = (m * 16 + (l >> 2) + 8 * (e & 1)) * rank_pad + k * 16 + 2 * (l & 3) + 8 * (e >> 1);
-            float2 v = make_float2(0.f, 0.f);
-            for (int b = 0; b < kCluster; ++b) {
-                const float2 o = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(tpart, b) + at);
-                v.x += o.x;
-                v.y += o.y;
-            }
+            float2 o[kCluster], v = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < kCluster; ++c) o[c] = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(tpart, c) + at);
+#pragma unroll
+            for (int c = 0; c < kCluster; ++c) v.x += o[c].x, v.y += o[c].y;
             split<PT>(v.x, v.y, w[e]);
         }
 #pragma unroll
@@ -234,10 +269,19 @@ __device__ __forceinline__ void adapter_pass(const AdaptersParams &p, const Adap
     auto arrived = cluster.barrier_arrive();                      // this block has read the others' parts
 
     // ---- y += scale B t over this block's part of N
-    const float scale = s.scale[slot];
-    const uint4 *b = reinterpret_cast<const uint4 *>(s.b + slot * s.b_stride);
-    const int nc0 = s.nchunks * part / kCluster, nc1 = s.nchunks * (part + 1) / kCluster;
+    float *piece = sums + warp * 16 * kTileLd;
     for (int nc = nc0 + warp; nc < nc1; nc += kWarps) {
+        const bool vec = s.y_vec && nc * 32 + 32 <= s.n;
+        OutputPiece<YF32> y[MT][2];
+        if (vec) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int row = list.row[m * 16 + g + 8 * h];
+                    if (row >= 0) y[m][h].load(s, row, nc * 32 + 8 * t);
+                }
+        }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             float acc[4][4];
@@ -245,6 +289,7 @@ __device__ __forceinline__ void adapter_pass(const AdaptersParams &p, const Adap
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+#pragma unroll 2
             for (int k = 0; k < rk; ++k) {
                 const uint4 w0 = b[(((size_t)nc * rk + k) * 2) * 32 + lane], w1 = b[(((size_t)nc * rk + k) * 2 + 1) * 32 + lane];
                 uint4 f[PT];
@@ -262,14 +307,29 @@ __device__ __forceinline__ void adapter_pass(const AdaptersParams &p, const Adap
                         for (int pa = 0; pa < PA; ++pa) mma_bf16(acc[i], f[q].x, f[q].y, f[q].z, f[q].w, b0[pa], b1[pa]);
                 }
             }
+            if (vec) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int row = list.row[m * 16 + g + 8 * h];
-                if (row < 0) continue;
-                float v[8];
+                for (int h = 0; h < 2; ++h) {
+                    const int row = list.row[m * 16 + g + 8 * h];
+                    if (row < 0) continue;
+                    float v[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[2 * i] = acc[i][2 * h], v[2 * i + 1] = acc[i][2 * h + 1];
-                add_y<YF32>(s, row, nc * 32 + 8 * t, scale, v);
+                    for (int i = 0; i < 4; ++i) v[2 * i] = acc[i][2 * h], v[2 * i + 1] = acc[i][2 * h + 1];
+                    y[m][h].add(s, row, nc * 32 + 8 * t, scale, v);
+                }
+            } else {                         // a row's 32 outputs by 32 lanes: neighbouring lanes, neighbouring outputs
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) piece[(g + 8 * (j >> 1)) * kTileLd + 8 * t + 2 * i + (j & 1)] = acc[i][j];
+                __syncwarp();
+                if (nc * 32 + lane < s.n)
+#pragma unroll 8
+                    for (int r = 0; r < 16; ++r) {
+                        const int row = list.row[m * 16 + r];
+                        if (row >= 0) add_y<YF32>(s, row, nc * 32 + lane, scale, piece[r * kTileLd + lane]);
+                    }
             }
         }
     }
@@ -277,7 +337,7 @@ __device__ __forceinline__ void adapter_pass(const AdaptersParams &p, const Adap
 }
 
 template <bool F16, bool XF32, bool YF32, int MT>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) adapters_kernel(const __grid_constant__ AdaptersParams p) {
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, MT == 1 && !XF32 && !F16 ? 3 : 2) adapters_kernel(const __grid_constant__ AdaptersParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ RowList list;
     __shared__ int s_slot[64];
