@@ -61,7 +61,7 @@ template <bool F16, int PLANES> __device__ __forceinline__ void adapter_planes(u
 
 struct RowList {
     int row[64];                 // -1: no row
-    int n;
+    int base;                    // more than sixteen: row[i] is base + i or none
 };
 
 // eight elements of an activation row from k0 on, loaded ahead; zeros beyond K and for missing rows
@@ -116,24 +116,20 @@ template <bool XF32> struct XPiece {
     }
 };
 
-// Eight outputs of a row from n0 on, loaded ahead (rows of whole 16-byte pieces) and put back with scale * v added
+// Eight neighbouring outputs (16-byte aligned), loaded ahead and put back with scale * v added
 template <bool YF32> struct OutputPiece {
     uint4 w[YF32 ? 2 : 1];
-    static __device__ __forceinline__ uint4 *at(const AdapterSet &s, int row, int n0) {
-        return reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(s.y) + (row * s.ldy + n0) * (YF32 ? 4 : 2));
-    }
-    __device__ __forceinline__ void load(const AdapterSet &s, int row, int n0) {
-        const uint4 *y = at(s, row, n0);
+    __device__ __forceinline__ void load(const uint8_t *y) {
 #pragma unroll
-        for (int i = 0; i < (YF32 ? 2 : 1); ++i) w[i] = y[i];
+        for (int i = 0; i < (YF32 ? 2 : 1); ++i) w[i] = reinterpret_cast<const uint4 *>(y)[i];
     }
-    __device__ __forceinline__ void add(const AdapterSet &s, int row, int n0, float scale, const float (&v)[8]) {
-        uint4 *y = at(s, row, n0);
+    __device__ __forceinline__ void add(uint8_t *y, float scale, const float (&v)[8]) const {
+        uint4 *out = reinterpret_cast<uint4 *>(y);
         if (YF32) {
 #pragma unroll
             for (int i = 0; i < (YF32 ? 2 : 1); ++i)
-                y[i] = make_uint4(__float_as_uint(fmaf(scale, v[4 * i], __uint_as_float(w[i].x))), __float_as_uint(fmaf(scale, v[4 * i + 1], __uint_as_float(w[i].y))),
-                                  __float_as_uint(fmaf(scale, v[4 * i + 2], __uint_as_float(w[i].z))), __float_as_uint(fmaf(scale, v[4 * i + 3], __uint_as_float(w[i].w))));
+                out[i] = make_uint4(__float_as_uint(fmaf(scale, v[4 * i], __uint_as_float(w[i].x))), __float_as_uint(fmaf(scale, v[4 * i + 1], __uint_as_float(w[i].y))),
+                                    __float_as_uint(fmaf(scale, v[4 * i + 2], __uint_as_float(w[i].z))), __float_as_uint(fmaf(scale, v[4 * i + 3], __uint_as_float(w[i].w))));
         } else {
             uint32_t o[4];
 #pragma unroll
@@ -141,7 +137,7 @@ template <bool YF32> struct OutputPiece {
                 const uint32_t u = word_of(w[0], i);
                 o[i] = last_plane(fmaf(scale, v[2 * i], __uint_as_float(u << 16)), fmaf(scale, v[2 * i + 1], __uint_as_float(u & 0xFFFF0000u)));
             }
-            y[0] = make_uint4(o[0], o[1], o[2], o[3]);
+            out[0] = make_uint4(o[0], o[1], o[2], o[3]);
         }
     }
 };
@@ -269,70 +265,90 @@ __device__ __forceinline__ void adapter_pass(const AdaptersParams &p, const Adap
     auto arrived = cluster.barrier_arrive();                      // this block has read the others' parts
 
     // ---- y += scale B t over this block's part of N
-    float *piece = sums + warp * 16 * kTileLd;
-    for (int nc = nc0 + warp; nc < nc1; nc += kWarps) {
-        const bool vec = s.y_vec && nc * 32 + 32 <= s.n;
-        OutputPiece<YF32> y[MT][2];
-        if (vec) {
+    // acc of column tile i: rows g, g + 8 of row tile m, outputs 8 t + 2 i, + 1 of the chunk
+    auto multiply = [&](int nc, int m, float (&acc)[4][4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+        const uint4 *bp = b + (size_t)nc * rk * 64 + lane, *fp = frag + (size_t)m * rk * PT * 32 + lane;
+#pragma unroll 2
+        for (int k = 0; k < rk; ++k, bp += 64, fp += PT * 32) {
+            const uint4 w[2] = {bp[0], bp[32]};
+            uint4 f[PT];
+#pragma unroll
+            for (int q = 0; q < PT; ++q) f[q] = fp[q * 32];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t b0[PA], b1[PA];
+                adapter_planes<F16, PA>(i & 1 ? w[i >> 1].z : w[i >> 1].x, b0);
+                adapter_planes<F16, PA>(i & 1 ? w[i >> 1].w : w[i >> 1].y, b1);
+#pragma unroll
+                for (int q = 0; q < PT; ++q)
+#pragma unroll
+                    for (int pa = 0; pa < PA; ++pa) mma_bf16(acc[i], f[q].x, f[q].y, f[q].z, f[q].w, b0[pa], b1[pa]);
+            }
+        }
+    };
+    int nc = nc0 + warp;
+    if (s.y_vec) {
+        constexpr int YB = YF32 ? 4 : 2;
+        bool have[MT][2];
+        uint8_t *row[MT == 1 ? 2 : 1];       // sixteen rows: their addresses; more: neighbours of the first
+        const long long ld = s.ldy * YB;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = list.row[m * 16 + g + 8 * h];
+                have[m][h] = r >= 0;
+                if (MT == 1) row[MT == 1 ? h : 0] = reinterpret_cast<uint8_t *>(s.y) + r * ld + (nc * 32 + 8 * t) * YB;
+            }
+        if (MT > 1) row[0] = reinterpret_cast<uint8_t *>(s.y) + (list.base + g) * ld + ((long long)nc * 32 + 8 * t) * YB;
+        auto at = [&](int m, int h) { return MT == 1 ? row[MT == 1 ? h : 0] : row[0] + (16 * m + 8 * h) * ld; };
+        for (; nc < nc1 && nc * 32 + 32 <= s.n; nc += kWarps) {
+            OutputPiece<YF32> y[MT][2];
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int row = list.row[m * 16 + g + 8 * h];
-                    if (row >= 0) y[m][h].load(s, row, nc * 32 + 8 * t);
-                }
-        }
+                for (int h = 0; h < 2; ++h)
+                    if (have[m][h]) y[m][h].load(at(m, h));
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            float acc[4][4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-#pragma unroll 2
-            for (int k = 0; k < rk; ++k) {
-                const uint4 w0 = b[(((size_t)nc * rk + k) * 2) * 32 + lane], w1 = b[(((size_t)nc * rk + k) * 2 + 1) * 32 + lane];
-                uint4 f[PT];
-#pragma unroll
-                for (int q = 0; q < PT; ++q) f[q] = frag[((size_t)(m * rk + k) * PT + q) * 32 + lane];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t b0[PA], b1[PA];
-                    const uint4 w = i < 2 ? w0 : w1;
-                    adapter_planes<F16, PA>(i & 1 ? w.z : w.x, b0);
-                    adapter_planes<F16, PA>(i & 1 ? w.w : w.y, b1);
-#pragma unroll
-                    for (int q = 0; q < PT; ++q)
-#pragma unroll
-                        for (int pa = 0; pa < PA; ++pa) mma_bf16(acc[i], f[q].x, f[q].y, f[q].z, f[q].w, b0[pa], b1[pa]);
-                }
-            }
-            if (vec) {
+            for (int m = 0; m < MT; ++m) {
+                float acc[4][4];
+                multiply(nc, m, acc);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int row = list.row[m * 16 + g + 8 * h];
-                    if (row < 0) continue;
                     float v[8];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) v[2 * i] = acc[i][2 * h], v[2 * i + 1] = acc[i][2 * h + 1];
-                    y[m][h].add(s, row, nc * 32 + 8 * t, scale, v);
+                    if (have[m][h]) y[m][h].add(at(m, h), scale, v);
                 }
-            } else {                         // a row's 32 outputs by 32 lanes: neighbouring lanes, neighbouring outputs
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) piece[(g + 8 * (j >> 1)) * kTileLd + 8 * t + 2 * i + (j & 1)] = acc[i][j];
-                __syncwarp();
-                if (nc * 32 + lane < s.n)
-#pragma unroll 8
-                    for (int r = 0; r < 16; ++r) {
-                        const int row = list.row[m * 16 + r];
-                        if (row >= 0) add_y<YF32>(s, row, nc * 32 + lane, scale, piece[r * kTileLd + lane]);
-                    }
             }
+#pragma unroll
+            for (int i = 0; i < (MT == 1 ? 2 : 1); ++i) row[i] += kWarps * 32 * YB;
         }
     }
+    // rows that are not aligned, the last outputs: a row's 32 by 32 lanes
+    float *piece = sums + warp * 16 * kTileLd;
+    for (; nc < nc1; nc += kWarps)
+#pragma unroll 1
+        for (int m = 0; m < MT; ++m) {
+            float acc[4][4];
+            multiply(nc, m, acc);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) piece[(g + 8 * (j >> 1)) * kTileLd + 8 * t + 2 * i + (j & 1)] = acc[i][j];
+            __syncwarp();
+            if (nc * 32 + lane < s.n)
+#pragma unroll 8
+                for (int r = 0; r < 16; ++r) {
+                    const int to = list.row[m * 16 + r];
+                    if (to >= 0) add_y<YF32>(s, to, nc * 32 + lane, scale, piece[r * kTileLd + lane]);
+                }
+        }
     cluster.barrier_wait(std::move(arrived));
 }
 
@@ -374,19 +390,28 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, MT 
         __syncthreads();
         adapter_pass<F16, XF32, YF32, MT>(p, s, slot, list, p.rank_pad, smem);
     } else {
-        const int base = id * 16 * MT;
-        if (tid < 16 * MT) s_slot[tid] = base + tid < p.m && active(p.rows[base + tid]) ? p.rows[base + tid] : -1;
+        static_assert(MT == 1 || MT == 4, "two warps look the rows over");
+        const int base = id * 64;
+        if (tid < 64) s_slot[tid] = base + tid < p.m && active(p.rows[base + tid]) ? p.rows[base + tid] : -1;
         __syncthreads();
-        for (int r = 0; r < 16 * MT; ++r) {
-            const int slot = s_slot[r];
-            if (slot < 0) continue;
-            bool seen = false;
-            for (int q = 0; q < r; ++q) seen |= s_slot[q] == slot;
-            if (seen) continue;
-            __syncthreads();
-            if (tid < 16 * MT) list.row[tid] = s_slot[tid] == slot ? base + tid : -1;
+        if (warp < 2) {                      // the rows that are the first of their adapter
+            const int slot = s_slot[tid];
+            const unsigned same = __match_any_sync(0xFFFFFFFFu, slot);      // (all lanes take part, rows without an adapter too)
+            bool first = slot >= 0 && __ffs(same) - 1 == lane;
+            if (warp == 1)
+                for (int q = 0; q < 32; ++q) first &= s_slot[q] != slot;
+            const unsigned all = __ballot_sync(0xFFFFFFFFu, first);
+            if (lane == 0) s_count[warp] = (int)all;
+        }
+        __syncthreads();
+        unsigned long long left = (unsigned long long)(unsigned)s_count[1] << 32 | (unsigned)s_count[0];
+        for (; left; left &= left - 1) {
+            const int slot = s_slot[__ffsll((long long)left) - 1];
+            if (tid < 64) list.row[tid] = s_slot[tid] == slot ? base + tid : -1;
+            if (tid == 0) list.base = base;
             __syncthreads();
             adapter_pass<F16, XF32, YF32, MT>(p, s, slot, list, p.rank_pad, smem);
+            __syncthreads();
         }
     }
 }
