@@ -6,7 +6,7 @@
 //   * up to kLeaderRows rows (sequences decoding together, in any order): the cluster of row i counts the rows before it that have the same
 //     adapter; every sixteenth leads a cluster of the next sixteen of them, the others' clusters end at once.  No list has to be
 //     made first, and the grouping depends on the choices alone.
-//   * more rows (prompts: long runs of one adapter): a cluster owns 64 neighbouring rows and takes the adapters that occur among
+//   * more rows (prompts: long runs of one adapter): a cluster owns 32 neighbouring rows and takes the adapters that occur among
 //     them one after the other.
 // Both products run on mma.sync.m16n8k16 with bf16 operands and fp32 sums, the rows as M.  Operands of more bits are cut into
 // bf16 planes: fp32 activations three (exact), fp16 adapters two (exact), t three where y is fp32 (exact) and two where y
@@ -24,7 +24,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 256, kWarps = 8, kCluster = 8;
-constexpr int kLeaderRows = 512;
+constexpr int kLeaderRows = 512, kTileRows = 32;
 
 // D += A (16 x 16 bf16, row) * B (16 x 8 bf16, col)
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -60,8 +60,7 @@ template <bool F16, int PLANES> __device__ __forceinline__ void adapter_planes(u
 }
 
 struct RowList {
-    int row[64];                 // -1: no row
-    int base;                    // more than sixteen: row[i] is base + i or none
+    int row[kTileRows];          // -1: no row
 };
 
 // eight elements of an activation row from k0 on, loaded ahead; zeros beyond K and for missing rows
@@ -156,7 +155,7 @@ template <bool YF32> __device__ __forceinline__ void add_y(const AdapterSet &s, 
 // kRanks: ranks whose sums a warp holds at a time.
 constexpr int kTileLd = 33;
 template <int MT> struct Smem {
-    static constexpr int kRows = 16 * MT, kKWarps = kWarps / MT, kRanks = MT == 1 ? 32 : 64;
+    static constexpr int kRows = 16 * MT, kKWarps = kWarps / MT, kRanks = MT == 1 ? 32 : 64, kChunks = MT == 1 ? 1 : 4;
     static constexpr size_t kSums = size_t(kKWarps) * kRows * kRanks * 4 > size_t(kWarps) * 16 * kTileLd * 4 ? size_t(kKWarps) * kRows * kRanks * 4
                                                                                                           : size_t(kWarps) * 16 * kTileLd * 4;
     static size_t bytes(int rank_pad, int planes) { return kSums + size_t(kRows) * rank_pad * 4 + size_t(MT) * (rank_pad / 16) * planes * 512; }
@@ -177,7 +176,8 @@ __device__ __forceinline__ void adapter_pass(const AdaptersParams &p, const Adap
     uint4 *frag = reinterpret_cast<uint4 *>(smem + S::kSums + (size_t)S::kRows * rank_pad_max * 4);
     const float scale = s.scale[slot];
     const uint4 *b = reinterpret_cast<const uint4 *>(s.b + slot * s.b_stride);
-    const int nc0 = (int)((long long)s.nchunks * part / kCluster), nc1 = (int)((long long)s.nchunks * (part + 1) / kCluster);
+    const long long pieces = (s.nchunks + S::kChunks - 1) / S::kChunks;
+    const int nc0 = (int)(pieces * part / kCluster) * S::kChunks, nc1 = min((int)(pieces * (part + 1) / kCluster) * S::kChunks, s.nchunks);
     if (MT == 1)                             // B and y start their way while A is multiplied: 128 bytes a thread and turn
         for (long long i = (long long)nc0 * rk * 1024 + threadIdx.x * 128, end = min((long long)nc1 * rk * 1024, i + 64 * 1024); i < end; i += kThreads * 128)
             prefetch_l2(reinterpret_cast<const uint8_t *>(b) + i);
@@ -290,63 +290,57 @@ __device__ __forceinline__ void adapter_pass(const AdaptersParams &p, const Adap
             }
         }
     };
-    int nc = nc0 + warp;
+    // Warps share the row tiles and the chunks; with many rows a warp takes four neighbouring chunks of sixteen rows at a time: whole
+    // 256-byte pieces of bf16 rows.
+    constexpr int CH = S::kChunks, kStep = S::kKWarps * CH;
+    const int m = warp % MT;
+    int nc = nc0 + (warp / MT) * CH;
     if (s.y_vec) {
         constexpr int YB = YF32 ? 4 : 2;
-        bool have[MT][2];
-        uint8_t *row[MT == 1 ? 2 : 1];       // sixteen rows: their addresses; more: neighbours of the first
-        const long long ld = s.ldy * YB;
+        const int r0 = list.row[m * 16 + g], r1 = list.row[m * 16 + g + 8];
+        uint8_t *row[2] = {reinterpret_cast<uint8_t *>(s.y) + (r0 * s.ldy + nc * 32 + 8 * t) * YB, reinterpret_cast<uint8_t *>(s.y) + (r1 * s.ldy + nc * 32 + 8 * t) * YB};
+        const bool have[2] = {r0 >= 0, r1 >= 0};
+        for (; nc + CH <= nc1 && (nc + CH) * 32 <= s.n; nc += kStep) {
+            OutputPiece<YF32> y[CH][2];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = list.row[m * 16 + g + 8 * h];
-                have[m][h] = r >= 0;
-                if (MT == 1) row[MT == 1 ? h : 0] = reinterpret_cast<uint8_t *>(s.y) + r * ld + (nc * 32 + 8 * t) * YB;
-            }
-        if (MT > 1) row[0] = reinterpret_cast<uint8_t *>(s.y) + (list.base + g) * ld + ((long long)nc * 32 + 8 * t) * YB;
-        auto at = [&](int m, int h) { return MT == 1 ? row[MT == 1 ? h : 0] : row[0] + (16 * m + 8 * h) * ld; };
-        for (; nc < nc1 && nc * 32 + 32 <= s.n; nc += kWarps) {
-            OutputPiece<YF32> y[MT][2];
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int c = 0; c < CH; ++c)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    if (have[m][h]) y[m][h].load(at(m, h));
+                    if (have[h]) y[c][h].load(row[h] + c * 32 * YB);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
+            for (int c = 0; c < CH; ++c) {
                 float acc[4][4];
-                multiply(nc, m, acc);
+                multiply(nc + c, m, acc);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float v[8];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) v[2 * i] = acc[i][2 * h], v[2 * i + 1] = acc[i][2 * h + 1];
-                    if (have[m][h]) y[m][h].add(at(m, h), scale, v);
+                    if (have[h]) y[c][h].add(row[h] + c * 32 * YB, scale, v);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < (MT == 1 ? 2 : 1); ++i) row[i] += kWarps * 32 * YB;
+            row[0] += kStep * 32 * YB;
+            row[1] += kStep * 32 * YB;
         }
     }
     // rows that are not aligned, the last outputs: a row's 32 by 32 lanes
     float *piece = sums + warp * 16 * kTileLd;
-    for (; nc < nc1; nc += kWarps)
+    for (; nc < nc1; nc += kStep)
 #pragma unroll 1
-        for (int m = 0; m < MT; ++m) {
+        for (int c = nc; c < min(nc + CH, nc1); ++c) {
             float acc[4][4];
-            multiply(nc, m, acc);
+            multiply(c, m, acc);
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) piece[(g + 8 * (j >> 1)) * kTileLd + 8 * t + 2 * i + (j & 1)] = acc[i][j];
             __syncwarp();
-            if (nc * 32 + lane < s.n)
+            if (c * 32 + lane < s.n)
 #pragma unroll 8
                 for (int r = 0; r < 16; ++r) {
                     const int to = list.row[m * 16 + r];
-                    if (to >= 0) add_y<YF32>(s, to, nc * 32 + lane, scale, piece[r * kTileLd + lane]);
+                    if (to >= 0) add_y<YF32>(s, to, c * 32 + lane, scale, piece[r * kTileLd + lane]);
                 }
         }
     cluster.barrier_wait(std::move(arrived));
@@ -356,7 +350,7 @@ template <bool F16, bool XF32, bool YF32, int MT>
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, MT == 1 && !XF32 && !F16 ? 3 : 2) adapters_kernel(const __grid_constant__ AdaptersParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ RowList list;
-    __shared__ int s_slot[64];
+    __shared__ int s_slot[kTileRows];
     __shared__ int s_count[kWarps];
     const AdapterSet &s = p.set[blockIdx.y];
     const int id = blockIdx.x / kCluster, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -372,7 +366,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, MT 
         for (int i = tid; i < id; i += kThreads) before += p.rows[i] == slot;
         before = __reduce_add_sync(0xFFFFFFFFu, before);
         if (lane == 0) s_count[warp] = before;
-        if (tid < 64) list.row[tid] = -1;
+        if (tid < kTileRows) list.row[tid] = -1;
         __syncthreads();
         before = 0;
         for (int w = 0; w < kWarps; ++w) before += s_count[w];
@@ -390,25 +384,20 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, MT 
         __syncthreads();
         adapter_pass<F16, XF32, YF32, MT>(p, s, slot, list, p.rank_pad, smem);
     } else {
-        static_assert(MT == 1 || MT == 4, "two warps look the rows over");
-        const int base = id * 64;
-        if (tid < 64) s_slot[tid] = base + tid < p.m && active(p.rows[base + tid]) ? p.rows[base + tid] : -1;
-        __syncthreads();
-        if (warp < 2) {                      // the rows that are the first of their adapter
-            const int slot = s_slot[tid];
+        static_assert(MT <= 2, "one warp looks the rows over");
+        const int base = id * kTileRows;
+        if (warp == 0) {
+            int slot = base + lane < p.m ? p.rows[base + lane] : -1;
+            if (!active(slot)) slot = -1;
+            s_slot[lane] = slot;
             const unsigned same = __match_any_sync(0xFFFFFFFFu, slot);      // (all lanes take part, rows without an adapter too)
-            bool first = slot >= 0 && __ffs(same) - 1 == lane;
-            if (warp == 1)
-                for (int q = 0; q < 32; ++q) first &= s_slot[q] != slot;
-            const unsigned all = __ballot_sync(0xFFFFFFFFu, first);
-            if (lane == 0) s_count[warp] = (int)all;
+            const unsigned first = __ballot_sync(0xFFFFFFFFu, slot >= 0 && __ffs(same) - 1 == lane);
+            if (lane == 0) s_count[0] = (int)first;
         }
         __syncthreads();
-        unsigned long long left = (unsigned long long)(unsigned)s_count[1] << 32 | (unsigned)s_count[0];
-        for (; left; left &= left - 1) {
-            const int slot = s_slot[__ffsll((long long)left) - 1];
-            if (tid < 64) list.row[tid] = s_slot[tid] == slot ? base + tid : -1;
-            if (tid == 0) list.base = base;
+        for (unsigned left = (unsigned)s_count[0]; left; left &= left - 1) {      // the rows that are the first of their adapter
+            const int slot = s_slot[__ffs((int)left) - 1];
+            if (tid < kTileRows) list.row[tid] = s_slot[tid] == slot ? base + tid : -1;
             __syncthreads();
             adapter_pass<F16, XF32, YF32, MT>(p, s, slot, list, p.rank_pad, smem);
             __syncthreads();
@@ -436,7 +425,7 @@ template <bool F16, bool XF32, bool YF32, int MT> cudaError_t launch(const Adapt
 
 template <bool F16, bool XF32, bool YF32> cudaError_t launch_rows(const AdaptersParams &p, cudaStream_t st) {
     if (p.m <= kLeaderRows) return launch<F16, XF32, YF32, 1>(p, p.m, st);
-    return launch<F16, XF32, YF32, 4>(p, (p.m + 63) / 64, st);
+    return launch<F16, XF32, YF32, kTileRows / 16>(p, (p.m + kTileRows - 1) / kTileRows, st);
 }
 
 // A[rank][K], B[N][rank] (row-major) -> fragments
