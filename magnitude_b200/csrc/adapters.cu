@@ -1,13 +1,11 @@
 // Low-rank adapters of many requests beside a shared projection: y[m] += scale * B (A x[m]) with the adapter that row m picks.
 //
-// One launch.  A cluster of eight blocks owns a few rows of one adapter: its blocks split K for t = A x, add their parts up through
-// distributed shared memory in the order of the blocks, and split N for y += scale * B t.  So t never leaves the SMs, an adapter
-// is read once per cluster, and no launch or device-wide wait stands between the two products.
-//   * up to kLeaderRows rows (sequences decoding together, in any order): the cluster of row i counts the rows before it that have the same
-//     adapter; every sixteenth leads a cluster of the next sixteen of them, the others' clusters end at once.  No list has to be
-//     made first, and the grouping depends on the choices alone.
-//   * more rows (prompts: long runs of one adapter): a cluster owns 32 neighbouring rows and takes the adapters that occur among
-//     them one after the other.
+//   * up to kFewRows rows (sequences decoding together, in any order, or the pieces of a few prompts): one launch of clusters of eight blocks.
+//     A cluster takes up to sixteen rows of one adapter and one projection at a time; its blocks split K for t = A x, add their parts
+//     up through distributed shared memory in the order of the blocks, and split N for y += scale * B t, so t never leaves the SMs.
+//     Every block finds the rows of each adapter for itself.
+//   * more rows (long runs of one adapter): two launches, t = A x for tiles of 32 rows (K cut into a few ranges to fill the chip), then
+//     y += scale * B t as one stream over y.  A tile takes the adapters that occur among its rows one after the other.
 // Both products run on mma.sync.m16n8k16 with bf16 operands and fp32 sums, the rows as M.  Operands of more bits are cut into
 // bf16 planes: fp32 activations three (exact), fp16 adapters two (exact), t three where y is fp32 (exact) and two where y
 // is rounded to bf16 anyway (an error of at most 2^-15 of t).  The adapters are kept in fragment order, so a load is 512 bytes a warp.
@@ -16,6 +14,7 @@
 #include <algorithm>
 
 #include "adapters.h"
+#include "launch.h"
 
 namespace b200q {
 
@@ -24,7 +23,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 256, kWarps = 8, kCluster = 8;
-constexpr int kLeaderRows = 512, kTileRows = 32;
+constexpr int kFewRows = 512;
 
 // D += A (16 x 16 bf16, row) * B (16 x 8 bf16, col)
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -59,14 +58,10 @@ template <bool F16, int PLANES> __device__ __forceinline__ void adapter_planes(u
     }
 }
 
-struct RowList {
-    int row[kTileRows];          // -1: no row
-};
-
 // eight elements of an activation row from k0 on, loaded ahead; zeros beyond K and for missing rows
 template <bool XF32> struct XPiece {
     uint4 w[XF32 ? 2 : 1];
-    __device__ __forceinline__ void load(const AdaptersParams &p, int row, int k0, bool wanted) {
+    __device__ __forceinline__ void load(const AdaptersParams &p, long long row, int k0, bool wanted) {
 #pragma unroll
         for (int i = 0; i < (XF32 ? 2 : 1); ++i) w[i] = make_uint4(0, 0, 0, 0);
         if (row < 0 || !wanted) return;
@@ -151,185 +146,112 @@ template <bool YF32> __device__ __forceinline__ void add_y(const AdapterSet &s, 
     }
 }
 
-// Shared memory: the warps' sums of a rank block (later a 16 x 32 piece of outputs per warp), this block's t, t as operand fragments.
-// kRanks: ranks whose sums a warp holds at a time.
-constexpr int kTileLd = 33;
-template <int MT> struct Smem {
-    static constexpr int kRows = 16 * MT, kKWarps = kWarps / MT, kRanks = MT == 1 ? 32 : 64, kChunks = MT == 1 ? 1 : 4;
-    static constexpr size_t kSums = size_t(kKWarps) * kRows * kRanks * 4 > size_t(kWarps) * 16 * kTileLd * 4 ? size_t(kKWarps) * kRows * kRanks * 4
-                                                                                                          : size_t(kWarps) * 16 * kTileLd * 4;
-    static size_t bytes(int rank_pad, int planes) { return kSums + size_t(kRows) * rank_pad * 4 + size_t(MT) * (rank_pad / 16) * planes * 512; }
-};
-
-__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
-
-// one adapter against the rows of `list`
-template <bool F16, bool XF32, bool YF32, int MT>
-__device__ __forceinline__ void adapter_pass(const AdaptersParams &p, const AdapterSet &s, int slot, const RowList &list, int rank_pad_max, uint8_t *smem) {
-    using S = Smem<MT>;
-    constexpr int PX = XF32 ? 3 : 1, PA = F16 ? 2 : 1, PT = YF32 ? 3 : 2, RT = S::kRanks / 8;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, part = (int)cluster.block_rank();
-    const int rank = s.rank[slot], rt = (rank + 7) / 8, rk = (rank + 15) / 16, rank_pad = 16 * rk;
-    float *sums = reinterpret_cast<float *>(smem);
-    float *tpart = reinterpret_cast<float *>(smem + S::kSums);
-    uint4 *frag = reinterpret_cast<uint4 *>(smem + S::kSums + (size_t)S::kRows * rank_pad_max * 4);
-    const float scale = s.scale[slot];
-    const uint4 *b = reinterpret_cast<const uint4 *>(s.b + slot * s.b_stride);
-    const long long pieces = (s.nchunks + S::kChunks - 1) / S::kChunks;
-    const int nc0 = (int)(pieces * part / kCluster) * S::kChunks, nc1 = min((int)(pieces * (part + 1) / kCluster) * S::kChunks, s.nchunks);
-    if (MT == 1)                             // B and y start their way while A is multiplied: 128 bytes a thread and turn
-        for (long long i = (long long)nc0 * rk * 1024 + threadIdx.x * 128, end = min((long long)nc1 * rk * 1024, i + 64 * 1024); i < end; i += kThreads * 128)
-            prefetch_l2(reinterpret_cast<const uint8_t *>(b) + i);
-
-    // ---- t = A x over this block's part of K
-    const int mt = warp % MT, kw = warp / MT;
-    const int row0 = list.row[mt * 16 + g], row1 = list.row[mt * 16 + g + 8];
-    const uint4 *a = reinterpret_cast<const uint4 *>(s.a + slot * s.a_stride);
-    const int kc0 = (int)((long long)p.kchunks * part / kCluster), kc1 = (int)((long long)p.kchunks * (part + 1) / kCluster);
-    for (int rb = 0; rb < rt; rb += RT) {
-        const int tiles = min(rt - rb, RT);
-        float acc[RT][4];
+// A piece of t = A x for sixteen rows: tiles of eight ranks, chunks kc, kc + step, .. below kc1.  r0, r1: the lane's rows, -1: none;
+// w(i, kc): the lane's fragment of tile i.
+template <bool F16, bool XF32, int RT, typename Fragment>
+__device__ __forceinline__ void shrink(const AdaptersParams &p, long long r0, long long r1, int kc, int kc1, int step, int tiles, int t, Fragment fragment, float (&acc)[RT][4]) {
+    constexpr int PX = XF32 ? 3 : 1, PA = F16 ? 2 : 1;
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+    XPiece<XF32> x0, x1;                     // the next chunk's, on their way
+    x0.load(p, r0, kc * 32 + 8 * t, kc < kc1);
+    x1.load(p, r1, kc * 32 + 8 * t, kc < kc1);
+    for (; kc < kc1; kc += step) {
+        uint32_t f0[PX][4], f1[PX][4];
+        x0.planes(f0);
+        x1.planes(f1);
+        uint4 w[RT];
 #pragma unroll
         for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-        XPiece<XF32> x0, x1;                 // the next chunk's, on their way
-        x0.load(p, row0, (kc0 + kw) * 32 + 8 * t, kc0 + kw < kc1);
-        x1.load(p, row1, (kc0 + kw) * 32 + 8 * t, kc0 + kw < kc1);
-        for (int kc = kc0 + kw; kc < kc1; kc += S::kKWarps) {
-            uint32_t f0[PX][4], f1[PX][4];
-            x0.planes(f0);
-            x1.planes(f1);
-            uint4 w[RT];
-#pragma unroll
-            for (int i = 0; i < RT; ++i)
-                if (i < tiles) w[i] = a[((size_t)kc * rt + rb + i) * 32 + lane];
-            x0.load(p, row0, (kc + S::kKWarps) * 32 + 8 * t, kc + S::kKWarps < kc1);
-            x1.load(p, row1, (kc + S::kKWarps) * 32 + 8 * t, kc + S::kKWarps < kc1);
-#pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                if (i >= tiles) break;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t b0[PA], b1[PA];
-                    adapter_planes<F16, PA>(h ? w[i].z : w[i].x, b0);
-                    adapter_planes<F16, PA>(h ? w[i].w : w[i].y, b1);
-#pragma unroll
-                    for (int px = 0; px < PX; ++px)
-#pragma unroll
-                        for (int pa = 0; pa < PA; ++pa)
-                            mma_bf16(acc[i], f0[px][2 * h], f1[px][2 * h], f0[px][2 * h + 1], f1[px][2 * h + 1], b0[pa], b1[pa]);
-                }
-            }
-        }
+            if (i < tiles) w[i] = fragment(i, kc);
+        x0.load(p, r0, (kc + step) * 32 + 8 * t, kc + step < kc1);
+        x1.load(p, r1, (kc + step) * 32 + 8 * t, kc + step < kc1);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             if (i >= tiles) break;
-            float *dst = sums + ((size_t)kw * S::kRows + mt * 16 + g) * S::kRanks + 8 * i + 2 * t;
-            *reinterpret_cast<float2 *>(dst) = make_float2(acc[i][0], acc[i][1]);
-            *reinterpret_cast<float2 *>(dst + 8 * S::kRanks) = make_float2(acc[i][2], acc[i][3]);
-        }
-        __syncthreads();
-        const int width = min(rank_pad - 8 * rb, S::kRanks);        // the last tile of 16 may be half there
-        for (int i = threadIdx.x; i < S::kRows * width; i += kThreads) {
-            const int r = i / width, c = i - r * width;
-            float v = 0.f;
-            if (c < 8 * tiles)
 #pragma unroll
-                for (int w = 0; w < S::kKWarps; ++w) v += sums[((size_t)w * S::kRows + r) * S::kRanks + c];
-            tpart[r * rank_pad + 8 * rb + c] = v;
-        }
-        __syncthreads();
-    }
-    cluster.sync();
-
-    // ---- t over all of K, as operand fragments: [row tile][rank tile][plane][lane]
-    for (int i = threadIdx.x; i < MT * rk * 32; i += kThreads) {
-        const int l = i & 31, tile = i >> 5, m = tile / rk, k = tile - m * rk;
-        uint32_t w[4][PT];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {                            // (row g, ranks 2 t), (row g + 8, ..), (row g, ranks 2 t + 8), (..)
-            const int at = (m * 16 + (l >> 2) + 8 * (e & 1)) * rank_pad + k * 16 + 2 * (l & 3) + 8 * (e >> 1);
-            float2 o[kCluster], v = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int c = 0; c < kCluster; ++c) o[c] = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(tpart, c) + at);
-#pragma unroll
-            for (int c = 0; c < kCluster; ++c) v.x += o[c].x, v.y += o[c].y;
-            split<PT>(v.x, v.y, w[e]);
-        }
-#pragma unroll
-        for (int q = 0; q < PT; ++q) frag[((size_t)tile * PT + q) * 32 + l] = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
-    }
-    __syncthreads();
-    auto arrived = cluster.barrier_arrive();                      // this block has read the others' parts
-
-    // ---- y += scale B t over this block's part of N
-    // acc of column tile i: rows g, g + 8 of row tile m, outputs 8 t + 2 i, + 1 of the chunk
-    auto multiply = [&](int nc, int m, float (&acc)[4][4]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-        const uint4 *bp = b + (size_t)nc * rk * 64 + lane, *fp = frag + (size_t)m * rk * PT * 32 + lane;
-#pragma unroll 2
-        for (int k = 0; k < rk; ++k, bp += 64, fp += PT * 32) {
-            const uint4 w[2] = {bp[0], bp[32]};
-            uint4 f[PT];
-#pragma unroll
-            for (int q = 0; q < PT; ++q) f[q] = fp[q * 32];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int h = 0; h < 2; ++h) {
                 uint32_t b0[PA], b1[PA];
-                adapter_planes<F16, PA>(i & 1 ? w[i >> 1].z : w[i >> 1].x, b0);
-                adapter_planes<F16, PA>(i & 1 ? w[i >> 1].w : w[i >> 1].y, b1);
+                adapter_planes<F16, PA>(h ? w[i].z : w[i].x, b0);
+                adapter_planes<F16, PA>(h ? w[i].w : w[i].y, b1);
 #pragma unroll
-                for (int q = 0; q < PT; ++q)
+                for (int px = 0; px < PX; ++px)
 #pragma unroll
-                    for (int pa = 0; pa < PA; ++pa) mma_bf16(acc[i], f[q].x, f[q].y, f[q].z, f[q].w, b0[pa], b1[pa]);
+                    for (int pa = 0; pa < PA; ++pa) mma_bf16(acc[i], f0[px][2 * h], f1[px][2 * h], f0[px][2 * h + 1], f1[px][2 * h + 1], b0[pa], b1[pa]);
             }
         }
-    };
-    // Warps share the row tiles and the chunks; with many rows a warp takes four neighbouring chunks of sixteen rows at a time: whole
-    // 256-byte pieces of bf16 rows.
-    constexpr int CH = S::kChunks, kStep = S::kKWarps * CH;
-    const int m = warp % MT;
-    int nc = nc0 + (warp / MT) * CH;
+    }
+}
+
+// B t of sixteen rows and a chunk of 32 outputs: acc of column tile i: rows g, g + 8, outputs 8 t + 2 i, + 1.  bp: the lane's fragments of the
+// chunk, fp: of the rows' t
+template <bool F16, int PT> __device__ __forceinline__ void expand(const uint4 *bp, const uint4 *fp, int rk, float (&acc)[4][4]) {
+    constexpr int PA = F16 ? 2 : 1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+#pragma unroll 2
+    for (int k = 0; k < rk; ++k, bp += 64, fp += PT * 32) {
+        const uint4 w[2] = {bp[0], bp[32]};
+        uint4 f[PT];
+#pragma unroll
+        for (int q = 0; q < PT; ++q) f[q] = fp[q * 32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t b0[PA], b1[PA];
+            adapter_planes<F16, PA>(i & 1 ? w[i >> 1].z : w[i >> 1].x, b0);
+            adapter_planes<F16, PA>(i & 1 ? w[i >> 1].w : w[i >> 1].y, b1);
+#pragma unroll
+            for (int q = 0; q < PT; ++q)
+#pragma unroll
+                for (int pa = 0; pa < PA; ++pa) mma_bf16(acc[i], f[q].x, f[q].y, f[q].z, f[q].w, b0[pa], b1[pa]);
+        }
+    }
+}
+
+// y of sixteen rows += scale B t over the chunks nc, nc + step, .. below nc1, CH neighbouring ones at a time.  row[16]: the rows, -1: none;
+// piece: 16 x kTileLd floats of the warp
+constexpr int kTileLd = 33;
+template <bool F16, bool YF32, int CH>
+__device__ __forceinline__ void add_chunks(const AdapterSet &s, const uint4 *b, const uint4 *frag, int rk, float scale, const int *row, int nc, int nc1, int step, float *piece,
+                                           int lane) {
+    constexpr int PT = YF32 ? 3 : 2, YB = YF32 ? 4 : 2;
+    const int g = lane >> 2, t = lane & 3;
     if (s.y_vec) {
-        constexpr int YB = YF32 ? 4 : 2;
-        const int r0 = list.row[m * 16 + g], r1 = list.row[m * 16 + g + 8];
-        uint8_t *row[2] = {reinterpret_cast<uint8_t *>(s.y) + (r0 * s.ldy + nc * 32 + 8 * t) * YB, reinterpret_cast<uint8_t *>(s.y) + (r1 * s.ldy + nc * 32 + 8 * t) * YB};
-        const bool have[2] = {r0 >= 0, r1 >= 0};
-        for (; nc + CH <= nc1 && (nc + CH) * 32 <= s.n; nc += kStep) {
+        const int r0 = row[g], r1 = row[g + 8];
+        uint8_t *to[2] = {reinterpret_cast<uint8_t *>(s.y) + (r0 * s.ldy + nc * 32 + 8 * t) * YB, reinterpret_cast<uint8_t *>(s.y) + (r1 * s.ldy + nc * 32 + 8 * t) * YB};
+        for (; nc + CH <= nc1 && (nc + CH) * 32 <= s.n; nc += step) {
             OutputPiece<YF32> y[CH][2];
 #pragma unroll
-            for (int c = 0; c < CH; ++c)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    if (have[h]) y[c][h].load(row[h] + c * 32 * YB);
+            for (int c = 0; c < CH; ++c) {
+                if (r0 >= 0) y[c][0].load(to[0] + c * 32 * YB);
+                if (r1 >= 0) y[c][1].load(to[1] + c * 32 * YB);
+            }
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 float acc[4][4];
-                multiply(nc + c, m, acc);
+                expand<F16, PT>(b + (size_t)(nc + c) * rk * 64 + lane, frag + lane, rk, acc);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float v[8];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) v[2 * i] = acc[i][2 * h], v[2 * i + 1] = acc[i][2 * h + 1];
-                    if (have[h]) y[c][h].add(row[h] + c * 32 * YB, scale, v);
+                    if ((h ? r1 : r0) >= 0) y[c][h].add(to[h] + c * 32 * YB, scale, v);
                 }
             }
-            row[0] += kStep * 32 * YB;
-            row[1] += kStep * 32 * YB;
+            to[0] += step * 32 * YB;
+            to[1] += step * 32 * YB;
         }
     }
     // rows that are not aligned, the last outputs: a row's 32 by 32 lanes
-    float *piece = sums + warp * 16 * kTileLd;
-    for (; nc < nc1; nc += kStep)
+    for (; nc < nc1; nc += step)
 #pragma unroll 1
         for (int c = nc; c < min(nc + CH, nc1); ++c) {
             float acc[4][4];
-            multiply(c, m, acc);
+            expand<F16, PT>(b + (size_t)c * rk * 64 + lane, frag + lane, rk, acc);
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -338,80 +260,308 @@ __device__ __forceinline__ void adapter_pass(const AdaptersParams &p, const Adap
             __syncwarp();
             if (c * 32 + lane < s.n)
 #pragma unroll 8
-                for (int r = 0; r < 16; ++r) {
-                    const int to = list.row[m * 16 + r];
-                    if (to >= 0) add_y<YF32>(s, to, c * 32 + lane, scale, piece[r * kTileLd + lane]);
-                }
+                for (int r = 0; r < 16; ++r)
+                    if (row[r] >= 0) add_y<YF32>(s, row[r], c * 32 + lane, scale, piece[r * kTileLd + lane]);
         }
+}
+
+// an adapter that takes part: within the set and loaded
+__device__ __forceinline__ bool active(const AdapterSet &s, int slot) { return (unsigned)slot < (unsigned)s.slots && s.rank[slot] > 0; }
+
+// ---- up to kFewRows rows ---------------------------------------------------------------------------------
+
+// The rows by adapter: groups of up to sixteen, in the order of their first rows
+struct FewRows {
+    int slot[kFewRows];
+    short sorted[kFewRows], first[kFewRows + 1];     // rows of group i: sorted[first[i]] .. sorted[first[i + 1] - 1]
+    short lead[kFewRows];                            // of every row: the first row of its group; then: where that group's rows begin
+    int2 sums[kWarps];
+    int n;
+};
+__device__ __forceinline__ void few_groups(FewRows &l, const AdaptersParams &p) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int i = tid; i < kFewRows; i += kThreads) l.slot[i] = i < p.m ? p.rows[i] : -1;
+    __syncthreads();
+    int groups = 0, rows = 0;                        // of the rows before these
+    for (int i0 = 0; i0 < p.m; i0 += kThreads) {
+        const int i = i0 + tid, slot = i < p.m ? l.slot[i] : -1;
+        int before = 0, all = 0, lead = i;
+        if (slot >= 0)
+            for (int j = 0; j < p.m; j += 4) {
+                const int4 v = *reinterpret_cast<const int4 *>(l.slot + j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if ((e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w) == slot) {
+                        if (j + e <= i && all % 16 == 0) lead = j + e;
+                        before += j + e < i;
+                        ++all;
+                    }
+            }
+        const bool leads = slot >= 0 && lead == i;
+        const int n = leads ? min(16, all - before) : 0;
+        int2 run = make_int2(leads, n);
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int x = __shfl_up_sync(0xFFFFFFFFu, run.x, d), y = __shfl_up_sync(0xFFFFFFFFu, run.y, d);
+            if (lane >= d) run.x += x, run.y += y;
+        }
+        if (lane == 31) l.sums[warp] = run;
+        __syncthreads();
+        int2 total = make_int2(0, 0);
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) run.x += l.sums[w].x, run.y += l.sums[w].y;
+            total.x += l.sums[w].x, total.y += l.sums[w].y;
+        }
+        if (leads) {
+            l.first[groups + run.x - 1] = (short)(rows + run.y - n);
+            l.lead[i] = (short)(rows + run.y - n);
+        }
+        __syncthreads();                             // groups that begin among these rows or before
+        if (slot >= 0) l.sorted[l.lead[lead] + before % 16] = (short)i;
+        groups += total.x;
+        rows += total.y;
+        __syncthreads();
+    }
+    if (tid == 0) {
+        l.n = groups;
+        l.first[groups] = (short)rows;
+    }
+    __syncthreads();
+}
+
+// Shared memory beside the rows: the warps' sums of a rank block (later a 16 x 32 piece of outputs each), this block's t, t as fragments
+constexpr int kFewRanks = 32;                        // ranks whose sums a warp holds at a time
+constexpr size_t kFewSums = size_t(kWarps) * 16 * kTileLd * 4;
+static_assert(kFewSums >= size_t(kWarps) * 16 * kFewRanks * 4, "sums");
+size_t few_smem(int rank_pad, int planes) { return kFewSums + size_t(16) * rank_pad * 4 + size_t(rank_pad / 16) * planes * 512; }
+
+__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+// one adapter against up to sixteen rows
+template <bool F16, bool XF32, bool YF32>
+__device__ __forceinline__ void few_pass(const AdaptersParams &p, const AdapterSet &s, int slot, const int *row, uint8_t *smem) {
+    constexpr int PT = YF32 ? 3 : 2, RT = kFewRanks / 8;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, part = (int)cluster.block_rank();
+    const int rank = s.rank[slot], rt = (rank + 7) / 8, rk = (rank + 15) / 16, rank_pad = 16 * rk;
+    float *sums = reinterpret_cast<float *>(smem);
+    float *tpart = reinterpret_cast<float *>(smem + kFewSums);
+    uint4 *frag = reinterpret_cast<uint4 *>(smem + kFewSums + (size_t)16 * p.rank_pad * 4);
+    const float scale = s.scale[slot];
+    const uint4 *a = reinterpret_cast<const uint4 *>(s.a + slot * s.a_stride), *b = reinterpret_cast<const uint4 *>(s.b + slot * s.b_stride);
+    const int nc0 = (int)((long long)s.nchunks * part / kCluster), nc1 = (int)((long long)s.nchunks * (part + 1) / kCluster);
+    // B starts its way while A is multiplied: 128 bytes a thread and turn
+    for (long long i = (long long)nc0 * rk * 1024 + threadIdx.x * 128, end = min((long long)nc1 * rk * 1024, i + 64 * 1024); i < end; i += kThreads * 128)
+        prefetch_l2(reinterpret_cast<const uint8_t *>(b) + i);
+
+    // ---- t = A x over this block's part of K
+    const int kc0 = (int)((long long)p.kchunks * part / kCluster), kc1 = (int)((long long)p.kchunks * (part + 1) / kCluster);
+    for (int rb = 0; rb < rt; rb += RT) {
+        const int tiles = min(rt - rb, RT);
+        float acc[RT][4];
+        shrink<F16, XF32, RT>(p, row[g], row[g + 8], kc0 + warp, kc1, kWarps, tiles, t, [&](int i, int kc) { return a[((size_t)kc * rt + rb + i) * 32 + lane]; }, acc);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            if (i >= tiles) break;
+            float *dst = sums + (warp * 16 + g) * kFewRanks + 8 * i + 2 * t;
+            *reinterpret_cast<float2 *>(dst) = make_float2(acc[i][0], acc[i][1]);
+            *reinterpret_cast<float2 *>(dst + 8 * kFewRanks) = make_float2(acc[i][2], acc[i][3]);
+        }
+        __syncthreads();
+        const int width = min(rank_pad - 8 * rb, kFewRanks);        // the last tile of 16 may be half there
+        for (int i = threadIdx.x; i < 16 * width; i += kThreads) {
+            const int r = i / width, c = i - r * width;
+            float v = 0.f;
+            if (c < 8 * tiles)
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) v += sums[(w * 16 + r) * kFewRanks + c];
+            tpart[r * rank_pad + 8 * rb + c] = v;
+        }
+        __syncthreads();
+    }
+    cluster.sync();
+
+    // ---- t over all of K, as operand fragments: [rank tile][plane][lane]
+    for (int i = threadIdx.x; i < rk * 32; i += kThreads) {
+        const int l = i & 31, k = i >> 5;
+        uint32_t w[4][PT];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {                            // (row g, ranks 2 t), (row g + 8, ..), (row g, ranks 2 t + 8), (..)
+            const int at = ((l >> 2) + 8 * (e & 1)) * rank_pad + k * 16 + 2 * (l & 3) + 8 * (e >> 1);
+            float2 o[kCluster], v = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < kCluster; ++c) o[c] = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(tpart, c) + at);
+#pragma unroll
+            for (int c = 0; c < kCluster; ++c) v.x += o[c].x, v.y += o[c].y;
+            split<PT>(v.x, v.y, w[e]);
+        }
+#pragma unroll
+        for (int q = 0; q < PT; ++q) frag[((size_t)k * PT + q) * 32 + l] = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
+    }
+    __syncthreads();
+    auto arrived = cluster.barrier_arrive();                      // this block has read the others' parts
+
+    // ---- y += scale B t over this block's part of N
+    add_chunks<F16, YF32, 1>(s, b, frag, rk, scale, row, nc0 + warp, nc1, kWarps, sums + warp * 16 * kTileLd, lane);
     cluster.barrier_wait(std::move(arrived));
 }
 
-template <bool F16, bool XF32, bool YF32, int MT>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, MT == 1 && !XF32 && !F16 ? 3 : 2) adapters_kernel(const __grid_constant__ AdaptersParams p) {
+template <bool F16, bool XF32, bool YF32>
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) adapters_few_kernel(const __grid_constant__ AdaptersParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ RowList list;
-    __shared__ int s_slot[kTileRows];
-    __shared__ int s_count[kWarps];
-    const AdapterSet &s = p.set[blockIdx.y];
-    const int id = blockIdx.x / kCluster, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    __shared__ __align__(16) FewRows rows;
+    __shared__ int row[16];
     pdl_launch_dependents();
     pdl_wait();
-    // an adapter that takes part: within the set and loaded
-    auto active = [&](int slot) { return (unsigned)slot < (unsigned)s.slots && s.rank[slot] > 0; };
-    // (every block of a cluster sees the same rows and takes the same way)
-    if (MT == 1) {
-        const int slot = p.rows[id];
-        if (!active(slot)) return;
-        int before = 0;
-        for (int i = tid; i < id; i += kThreads) before += p.rows[i] == slot;
-        before = __reduce_add_sync(0xFFFFFFFFu, before);
-        if (lane == 0) s_count[warp] = before;
-        if (tid < kTileRows) list.row[tid] = -1;
+    few_groups(rows, p);
+    // (every block of a cluster has the same groups and takes the same way)
+    const int clusters = gridDim.x / kCluster, items = rows.n * p.sets;
+    for (int item = blockIdx.x / kCluster; item < items; item += clusters) {
+        const int group = item / p.sets;
+        const AdapterSet &s = p.set[item - group * p.sets];
+        const int first = rows.first[group], slot = rows.slot[rows.sorted[first]];
+        if (!active(s, slot)) continue;
+        const int n = rows.first[group + 1] - first;
+        if (threadIdx.x < 16) row[threadIdx.x] = threadIdx.x < n ? rows.sorted[first + threadIdx.x] : -1;
         __syncthreads();
-        before = 0;
-        for (int w = 0; w < kWarps; ++w) before += s_count[w];
-        if (before % 16) return;
-        if (warp == 0) {
-            int found = 0;
-            for (int i0 = id; i0 < p.m && found < 16; i0 += 32) {
-                const bool mine = i0 + lane < p.m && p.rows[i0 + lane] == slot;
-                const unsigned all = __ballot_sync(0xFFFFFFFFu, mine);
-                const int at = found + __popc(all & ((1u << lane) - 1));
-                if (mine && at < 16) list.row[at] = i0 + lane;
-                found += __popc(all);
+        few_pass<F16, XF32, YF32>(p, s, slot, row, smem);
+        __syncthreads();
+    }
+}
+
+// ---- more rows ---------------------------------------------------------------------------------------------
+constexpr int kTileRows = 32, kSumTiles = 8;         // rows of a block; tiles of eight ranks whose sums a warp holds at a time
+
+// The rows of a block's tile that are the first of an adapter of some set: bit mask (a warp; rows of a tile at most 32)
+__device__ __forceinline__ unsigned first_rows(int slot, int lane) {
+    const unsigned same = __match_any_sync(0xFFFFFFFFu, slot);      // (all lanes take part, rows without an adapter too)
+    return __ballot_sync(0xFFFFFFFFu, slot >= 0 && __ffs(same) - 1 == lane);
+}
+
+// t[range of K][row][ranks of all sets]
+template <bool F16, bool XF32> __global__ void __launch_bounds__(kThreads, 2) adapters_shrink_kernel(const __grid_constant__ AdaptersParams p) {
+    __shared__ float sums[4][kTileRows][8 * kSumTiles];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int base = blockIdx.x * kTileRows, m = warp & 1, kw = warp >> 1;
+    const int kc0 = (int)((long long)p.kchunks * blockIdx.y / gridDim.y), kc1 = (int)((long long)p.kchunks * (blockIdx.y + 1) / gridDim.y);
+    pdl_launch_dependents();
+    pdl_wait();
+    const int mine = base + lane < p.m ? p.rows[base + lane] : -1;
+    for (unsigned left = first_rows(mine, lane); left; left &= left - 1) {
+        const int slot = __shfl_sync(0xFFFFFFFFu, mine, __ffs((int)left) - 1);
+        const unsigned have = __ballot_sync(0xFFFFFFFFu, mine == slot);
+        const int i0 = m * 16 + g, i1 = i0 + 8;
+        const int r0 = (have >> i0) & 1 ? base + i0 : -1, r1 = (have >> i1) & 1 ? base + i1 : -1;
+        // tiles of eight ranks, set after set, kSumTiles at a time
+        int set = 0, tile = 0;
+        while (true) {
+            const uint4 *from[kSumTiles];
+            int to[kSumTiles], rt[kSumTiles], tiles = 0;
+#pragma unroll
+            for (int i = 0; i < kSumTiles; ++i) {
+                from[i] = nullptr;
+                to[i] = rt[i] = 0;
+                while (set < p.sets && (!active(p.set[set], slot) || tile >= (p.set[set].rank[slot] + 7) / 8)) ++set, tile = 0;
+                if (set < p.sets) {
+                    const AdapterSet &s = p.set[set];
+                    rt[i] = (s.rank[slot] + 7) / 8;
+                    from[i] = reinterpret_cast<const uint4 *>(s.a + slot * s.a_stride) + tile * 32 + lane;
+                    to[i] = s.t_at + 8 * tile;
+                    ++tile;
+                    ++tiles;
+                }
             }
-        }
-        __syncthreads();
-        adapter_pass<F16, XF32, YF32, MT>(p, s, slot, list, p.rank_pad, smem);
-    } else {
-        static_assert(MT <= 2, "one warp looks the rows over");
-        const int base = id * kTileRows;
-        if (warp == 0) {
-            int slot = base + lane < p.m ? p.rows[base + lane] : -1;
-            if (!active(slot)) slot = -1;
-            s_slot[lane] = slot;
-            const unsigned same = __match_any_sync(0xFFFFFFFFu, slot);      // (all lanes take part, rows without an adapter too)
-            const unsigned first = __ballot_sync(0xFFFFFFFFu, slot >= 0 && __ffs(same) - 1 == lane);
-            if (lane == 0) s_count[0] = (int)first;
-        }
-        __syncthreads();
-        for (unsigned left = (unsigned)s_count[0]; left; left &= left - 1) {      // the rows that are the first of their adapter
-            const int slot = s_slot[__ffs((int)left) - 1];
-            if (tid < kTileRows) list.row[tid] = s_slot[tid] == slot ? base + tid : -1;
+            if (tiles == 0) break;
+            float acc[kSumTiles][4];
+            shrink<F16, XF32, kSumTiles>(p, r0, r1, kc0 + kw, kc1, 4, tiles, t, [&](int i, int kc) { return from[i][(size_t)kc * rt[i] * 32]; }, acc);
+#pragma unroll
+            for (int i = 0; i < kSumTiles; ++i) {
+                *reinterpret_cast<float2 *>(&sums[kw][i0][8 * i + 2 * t]) = make_float2(acc[i][0], acc[i][1]);
+                *reinterpret_cast<float2 *>(&sums[kw][i1][8 * i + 2 * t]) = make_float2(acc[i][2], acc[i][3]);
+            }
             __syncthreads();
-            adapter_pass<F16, XF32, YF32, MT>(p, s, slot, list, p.rank_pad, smem);
+            // lane = rank of a tile and row: eight ranks of four rows a turn
+#pragma unroll
+            for (int i = 0; i < kSumTiles; ++i) {
+                if (i >= tiles) break;
+                const int r = warp * 4 + (lane >> 3), c = lane & 7;
+                if ((have >> r) & 1)
+                    p.t[((long long)blockIdx.y * p.m + base + r) * p.t_ld + to[i] + c] =
+                        sums[0][r][8 * i + c] + sums[1][r][8 * i + c] + sums[2][r][8 * i + c] + sums[3][r][8 * i + c];
+            }
             __syncthreads();
         }
     }
 }
 
-template <bool F16, bool XF32, bool YF32, int MT> cudaError_t launch(const AdaptersParams &p, int clusters, cudaStream_t st) {
-    auto kern = adapters_kernel<F16, XF32, YF32, MT>;
-    const size_t smem = Smem<MT>::bytes(p.rank_pad, YF32 ? 3 : 2);
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
+// y += scale B t: a block takes 64 rows and kStreamChunks chunks of 32 outputs; four warps side by side in the rows, two in the outputs
+constexpr int kStreamRows = 64, kStreamChunks = 32, kStreamStep = 4;
+constexpr size_t kPieces = size_t(kWarps) * 16 * kTileLd * 4;
+template <bool F16, bool YF32> __global__ void __launch_bounds__(kThreads, 2) adapters_stream_kernel(const __grid_constant__ AdaptersParams p) {
+    constexpr int PT = YF32 ? 3 : 2;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int slots[kStreamRows], row[kStreamRows];
+    __shared__ unsigned firsts[2];
+    uint4 *frag = reinterpret_cast<uint4 *>(smem + kPieces);
+    const AdapterSet &s = p.set[blockIdx.z];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, base = blockIdx.y * kStreamRows;
+    const int nc0 = blockIdx.x * kStreamChunks, nc1 = min(nc0 + kStreamChunks, s.nchunks);
+    if (nc0 >= nc1) return;                  // (another set is wider)
+    pdl_launch_dependents();
+    pdl_wait();
+    if (warp < 2) {
+        const int i = warp * 32 + lane;
+        int slot = base + i < p.m ? p.rows[base + i] : -1;
+        if (!active(s, slot)) slot = -1;
+        slots[i] = slot;
+        const unsigned first = first_rows(slot, lane);
+        if (lane == 0) firsts[warp] = first;
+    }
+    __syncthreads();
+    for (int half = 0; half < 2; ++half)
+        for (unsigned left = firsts[half]; left; left &= left - 1) {
+            const int slot = slots[half * 32 + __ffs((int)left) - 1];
+            if (half == 1) {                 // had its turn among the first rows?
+                bool seen = false;
+                for (int q = 0; q < 32; ++q) seen |= slots[q] == slot;
+                if (seen) continue;
+            }
+            const int rk = (s.rank[slot] + 15) / 16, ranks = (s.rank[slot] + 7) / 8 * 8;
+            if (threadIdx.x < kStreamRows) row[threadIdx.x] = slots[threadIdx.x] == slot ? base + (int)threadIdx.x : -1;
+            __syncthreads();
+            // t, added up over the ranges of K, as fragments: [row tile][rank tile][plane][lane]
+            for (int i = threadIdx.x; i < 4 * rk * 32; i += kThreads) {
+                const int l = i & 31, tile = i >> 5, m = tile / rk, k = tile - m * rk;
+                uint32_t w[4][PT];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = row[m * 16 + (l >> 2) + 8 * (e & 1)], c = k * 16 + 2 * (l & 3) + 8 * (e >> 1);
+                    float2 v = make_float2(0.f, 0.f);
+                    if (r >= 0 && c < ranks)
+                        for (int q = 0; q < p.t_ranges; ++q) {
+                            const float2 o = *reinterpret_cast<const float2 *>(p.t + ((long long)q * p.m + r) * p.t_ld + s.t_at + c);
+                            v.x += o.x, v.y += o.y;
+                        }
+                    split<PT>(v.x, v.y, w[e]);
+                }
+#pragma unroll
+                for (int q = 0; q < PT; ++q) frag[((size_t)tile * PT + q) * 32 + l] = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
+            }
+            __syncthreads();
+            const int m = warp & 3;
+            add_chunks<F16, YF32, kStreamStep>(s, reinterpret_cast<const uint4 *>(s.b + slot * s.b_stride), frag + (size_t)m * rk * PT * 32, rk, s.scale[slot], row + m * 16,
+                                               nc0 + (warp >> 2) * kStreamStep, nc1, 2 * kStreamStep, reinterpret_cast<float *>(smem) + warp * 16 * kTileLd, lane);
+            __syncthreads();
+        }
+}
+
+template <typename Kernel> cudaError_t launch(Kernel kern, const AdaptersParams &p, dim3 grid, size_t smem, cudaStream_t st) {
+    if (smem > 32 * 1024) {
+        cudaError_t e = configure_smem(reinterpret_cast<const void *>(kern), smem);
+        if (e != cudaSuccess) return e;
+    }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(clusters * kCluster), (unsigned)p.sets);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -423,9 +573,32 @@ template <bool F16, bool XF32, bool YF32, int MT> cudaError_t launch(const Adapt
     return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
-template <bool F16, bool XF32, bool YF32> cudaError_t launch_rows(const AdaptersParams &p, cudaStream_t st) {
-    if (p.m <= kLeaderRows) return launch<F16, XF32, YF32, 1>(p, p.m, st);
-    return launch<F16, XF32, YF32, kTileRows / 16>(p, (p.m + kTileRows - 1) / kTileRows, st);
+template <bool F16, bool XF32, bool YF32> cudaError_t run(AdaptersParams p, int sm_count, size_t t_floats, cudaStream_t st) {
+    constexpr int PT = YF32 ? 3 : 2;
+    if (p.m <= kFewRows) {
+        const int clusters = std::min(p.m * p.sets, sm_count * 2 / kCluster);
+        return launch(adapters_few_kernel<F16, XF32, YF32>, p, dim3((unsigned)(clusters * kCluster)), few_smem(p.rank_pad, PT), st);
+    }
+    // ranges of K: as many blocks as run at a time
+    const int tiles = (p.m + kTileRows - 1) / kTileRows;
+    p.t_ranges = std::max(1, std::min({2 * sm_count / tiles, p.kchunks / 16, 8}));
+    int widest = 0;
+    for (int i = 0; i < p.sets; ++i) widest = std::max(widest, p.set[i].nchunks);
+    // t of as many rows at a time as there is room for
+    const int room = (int)std::min<size_t>(t_floats / ((size_t)p.t_ranges * p.t_ld) / kStreamRows * kStreamRows, size_t(32767) * kStreamRows);
+    for (int done = 0, all = p.m; done < all; done += room) {
+        p.m = std::min(room, all - done);
+        cudaError_t e = launch(adapters_shrink_kernel<F16, XF32>, p, dim3((unsigned)((p.m + kTileRows - 1) / kTileRows), (unsigned)p.t_ranges), 0, st);
+        if (e != cudaSuccess) return e;
+        e = launch(adapters_stream_kernel<F16, YF32>, p,
+                   dim3((unsigned)((widest + kStreamChunks - 1) / kStreamChunks), (unsigned)((p.m + kStreamRows - 1) / kStreamRows), (unsigned)p.sets),
+                   kPieces + size_t(4) * (p.rank_pad / 16) * PT * 512, st);
+        if (e != cudaSuccess) return e;
+        p.rows += p.m;
+        p.x = reinterpret_cast<const uint8_t *>(p.x) + (long long)p.m * p.ldx * (XF32 ? 4 : 2);
+        for (int i = 0; i < p.sets; ++i) p.set[i].y = reinterpret_cast<uint8_t *>(p.set[i].y) + (long long)p.m * p.set[i].ldy * (YF32 ? 4 : 2);
+    }
+    return cudaSuccess;
 }
 
 // A[rank][K], B[N][rank] (row-major) -> fragments
@@ -462,11 +635,11 @@ cudaError_t adapter_pack(const void *a, const void *b, uint8_t *pa, uint8_t *pb,
     return cudaGetLastError();
 }
 
-cudaError_t adapters_run(const AdaptersParams &p, bool f16, bool x_f32, bool y_f32, cudaStream_t st) {
-    if (f16) return x_f32 ? (y_f32 ? launch_rows<true, true, true>(p, st) : launch_rows<true, true, false>(p, st))
-                          : (y_f32 ? launch_rows<true, false, true>(p, st) : launch_rows<true, false, false>(p, st));
-    return x_f32 ? (y_f32 ? launch_rows<false, true, true>(p, st) : launch_rows<false, true, false>(p, st))
-                 : (y_f32 ? launch_rows<false, false, true>(p, st) : launch_rows<false, false, false>(p, st));
+cudaError_t adapters_run(const AdaptersParams &p, bool f16, bool x_f32, bool y_f32, int sm_count, size_t t_floats, cudaStream_t st) {
+    if (f16) return x_f32 ? (y_f32 ? run<true, true, true>(p, sm_count, t_floats, st) : run<true, true, false>(p, sm_count, t_floats, st))
+                          : (y_f32 ? run<true, false, true>(p, sm_count, t_floats, st) : run<true, false, false>(p, sm_count, t_floats, st));
+    return x_f32 ? (y_f32 ? run<false, true, true>(p, sm_count, t_floats, st) : run<false, true, false>(p, sm_count, t_floats, st))
+                 : (y_f32 ? run<false, false, true>(p, sm_count, t_floats, st) : run<false, false, false>(p, sm_count, t_floats, st));
 }
 
 }  // namespace b200q

@@ -6,6 +6,7 @@
 namespace b200q {
 
 constexpr int kAdapterMaxRank = 256, kAdapterMaxSets = 4;
+constexpr size_t kAdapterTFloats = size_t(4) << 20;      // a context's room for t: 512 rows of 1024 ranks in eight ranges
 
 // Fragments of an adapter, 16 bytes a lane (lane 4 g + t):
 //   A  [chunk of 32 of K][rank tile of 8][lane]: rank g of the tile, K 8 t .. 8 t + 7 of the chunk
@@ -23,6 +24,7 @@ struct AdapterSet {
     void *y;
     long long ldy;
     int y_vec;                       // rows of y are 16-byte aligned
+    int t_at;                        // more rows: where the set's ranks begin in a row of t
 };
 
 struct AdaptersParams {
@@ -35,9 +37,13 @@ struct AdaptersParams {
     const int *rows;                 // [m]: every row's slot
     int m;
     int rank_pad;                    // largest rank of the sets, in multiples of 16
+    // more rows: t = A x on its way from one launch to the next, [range of K][row][t_ld]
+    float *t;
+    int t_ld, t_ranges;
 };
 
 cudaError_t adapter_pack(const void *a, const void *b, uint8_t *pa, uint8_t *pb, int rank, int K, int n, cudaStream_t st);
-cudaError_t adapters_run(const AdaptersParams &p, bool f16, bool x_f32, bool y_f32, cudaStream_t st);
+// t_floats: room at p.t
+cudaError_t adapters_run(const AdaptersParams &p, bool f16, bool x_f32, bool y_f32, int sm_count, size_t t_floats, cudaStream_t st);
 
 }  // namespace b200q

@@ -690,6 +690,7 @@ void b200q_ctx_destroy(b200q_ctx *ctx) {
     if (ctx->hy_dev) cudaFree(ctx->hy_dev);
     ctx->scratch.free_all();
     ctx->hscratch.free_all();
+    if (ctx->adapter_t) cudaFree(ctx->adapter_t);
     if (ctx->status_dev) cudaFree(ctx->status_dev);
     delete ctx;
 }

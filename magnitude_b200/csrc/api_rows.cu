@@ -316,6 +316,7 @@ b200q_status b200q_adapters_create(b200q_ctx *ctx, int64_t N, int64_t K, int32_t
     if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void **>(&a->b), a->b_stride * max_adapters);
     if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void **>(&a->rank), max_adapters * sizeof(int));
     if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void **>(&a->scale), max_adapters * sizeof(float));
+    if (e == cudaSuccess && !ctx->adapter_t) e = cudaMalloc(reinterpret_cast<void **>(&ctx->adapter_t), kAdapterTFloats * sizeof(float));
     if (e == cudaSuccess) e = cudaMemset(a->rank, 0, max_adapters * sizeof(int));
     if (e == cudaSuccess) e = cudaMemset(a->scale, 0, max_adapters * sizeof(float));
     if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
@@ -405,9 +406,14 @@ b200q_status b200q_adapters_apply(b200q_ctx *ctx, const b200q_adapters *const *s
         d.y = y_dev[i];
         d.ldy = ldy[i];
         d.y_vec = (reinterpret_cast<uintptr_t>(y_dev[i]) & 15) == 0 && (ldy[i] * act_size(y_dtype)) % 16 == 0;
-        p.rank_pad = std::max(p.rank_pad, (sets[i]->max_rank + 15) / 16 * 16);
+        d.t_at = p.t_ld;
+        const int pad = (sets[i]->max_rank + 15) / 16 * 16;
+        p.t_ld += pad;
+        p.rank_pad = std::max(p.rank_pad, pad);
     }
-    cudaError_t e = adapters_run(p, sets[0]->dtype == B200Q_TYPE_F16, x_dtype == B200Q_TYPE_F32, y_dtype == B200Q_TYPE_F32, (cudaStream_t)stream);
+    p.t = ctx->adapter_t;
+    cudaError_t e = adapters_run(p, sets[0]->dtype == B200Q_TYPE_F16, x_dtype == B200Q_TYPE_F32, y_dtype == B200Q_TYPE_F32, ctx->sm_count, kAdapterTFloats,
+                                 (cudaStream_t)stream);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "adapter launch");
     return B200Q_OK;
 }

@@ -55,6 +55,7 @@ struct b200q_ctx {
     int gemm_bn = 0, gemm_debug = 0, gemm_pair = 0, gemm_ksplit = 1, gemm_dense = -1;
     // tunables (environment overrides for experiments)
     int gemv_grid = 0, gemv_smem = 0, gemv_pdl = 1, gemv_xprep = 1;
+    float *adapter_t = nullptr;       // A x of large adapter calls (allocated with the first adapter set)
     // tensor parallel
     void *comm = nullptr;            // ncclComm_t
     int tp_rank = 0, tp_world = 1;

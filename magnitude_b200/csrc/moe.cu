@@ -4,6 +4,7 @@
 
 #include "moe_image.cuh"
 #include "kernels.h"
+#include "launch.h"
 
 namespace b200q {
 
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(const __grid_constant_
 
 template <typename Kernel, typename Params> cudaError_t launch(Kernel kern, const Params &p, dim3 grid, int threads, cudaStream_t st, size_t smem = 0) {
     if (smem > 48 * 1024) {
-        cudaError_t e = moe_configure(reinterpret_cast<const void *>(kern), smem);
+        cudaError_t e = configure_smem(reinterpret_cast<const void *>(kern), smem);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg{};

@@ -72,23 +72,5 @@ __device__ __forceinline__ void moe_store(const MoeOutput &o, int row, int n, fl
     }
 }
 
-// A kernel's shared memory is set once per device
-inline cudaError_t moe_configure(const void *kern, size_t smem) {
-    struct Done {
-        const void *kern;
-        int device;
-    };
-    static thread_local Done done[16];       // this thread's last ones
-    static thread_local int next = 0;
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e != cudaSuccess) return e;
-    for (const Done &d : done)
-        if (d.kern == kern && d.device == device) return cudaSuccess;
-    if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
-    done[next++ % 16] = Done{kern, device};
-    return cudaSuccess;
-}
-
 }  // namespace
 }  // namespace b200q

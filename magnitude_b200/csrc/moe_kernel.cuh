@@ -11,6 +11,7 @@
 #pragma once
 
 #include "kernels.h"
+#include "launch.h"
 #include "moe_image.cuh"
 
 namespace b200q {
@@ -738,7 +739,7 @@ template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 
 }
 
 template <typename Kernel, typename Params> cudaError_t moe_launch(Kernel kern, const Params &p, int grid, size_t smem, cudaStream_t st) {
-    cudaError_t e = moe_configure(reinterpret_cast<const void *>(kern), smem);
+    cudaError_t e = configure_smem(reinterpret_cast<const void *>(kern), smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
