@@ -136,14 +136,13 @@ template <bool YF32> struct OutputPiece {
     }
 };
 // one output
-template <bool YF32> __device__ __forceinline__ void add_y(const AdapterSet &s, int row, int n, float scale, float v) {
-    if (YF32) {
-        float *y = reinterpret_cast<float *>(s.y) + row * s.ldy + n;
-        *y = fmaf(scale, v, *y);
-    } else {
-        __nv_bfloat16 *y = reinterpret_cast<__nv_bfloat16 *>(s.y) + row * s.ldy + n;
-        *y = __float2bfloat16_rn(fmaf(scale, v, __bfloat162float(*y)));
-    }
+template <bool YF32> __device__ __forceinline__ float load_y(const AdapterSet &s, long long row, int n) {
+    if (YF32) return reinterpret_cast<const float *>(s.y)[row * s.ldy + n];
+    return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(s.y)[row * s.ldy + n]);
+}
+template <bool YF32> __device__ __forceinline__ void store_y(const AdapterSet &s, long long row, int n, float v) {
+    if (YF32) reinterpret_cast<float *>(s.y)[row * s.ldy + n] = v;
+    else reinterpret_cast<__nv_bfloat16 *>(s.y)[row * s.ldy + n] = __float2bfloat16_rn(v);
 }
 
 // A piece of t = A x for sixteen rows: tiles of eight ranks, chunks kc, kc + step, .. below kc1.  r0, r1: the lane's rows, -1: none;
@@ -259,9 +258,15 @@ __device__ __forceinline__ void add_chunks(const AdapterSet &s, const uint4 *b, 
                 for (int j = 0; j < 4; ++j) piece[(g + 8 * (j >> 1)) * kTileLd + 8 * t + 2 * i + (j & 1)] = acc[i][j];
             __syncwarp();
             if (c * 32 + lane < s.n)
-#pragma unroll 8
-                for (int r = 0; r < 16; ++r)
-                    if (row[r] >= 0) add_y<YF32>(s, row[r], c * 32 + lane, scale, piece[r * kTileLd + lane]);
+#pragma unroll
+                for (int r0 = 0; r0 < 16; r0 += 8) {         // eight loads, then eight stores
+                    float old[8];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) old[r] = row[r0 + r] >= 0 ? load_y<YF32>(s, row[r0 + r], c * 32 + lane) : 0.f;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                        if (row[r0 + r] >= 0) store_y<YF32>(s, row[r0 + r], c * 32 + lane, fmaf(scale, piece[(r0 + r) * kTileLd + lane], old[r]));
+                }
         }
 }
 
@@ -270,61 +275,111 @@ __device__ __forceinline__ bool active(const AdapterSet &s, int slot) { return (
 
 // ---- up to kFewRows rows ---------------------------------------------------------------------------------
 
-// The rows by adapter: groups of up to sixteen, in the order of their first rows
+// The rows by adapter: groups of up to sixteen, adapters in the order of their first rows.  Warp w owns rows 64 w .. 64 w + 63.
+constexpr int kKeys = 2 * kFewRows;
 struct FewRows {
     int slot[kFewRows];
+    int key[kKeys];                                  // a table of the slots that occur: open addressing
+    int first_row[kKeys];                            // of every key
+    short row_base[kKeys], group_base[kKeys];        // where its rows, its groups begin
+    uint8_t count[kWarps][kKeys];                    // its rows in every warp
     short sorted[kFewRows], first[kFewRows + 1];     // rows of group i: sorted[first[i]] .. sorted[first[i + 1] - 1]
-    short lead[kFewRows];                            // of every row: the first row of its group; then: where that group's rows begin
     int2 sums[kWarps];
     int n;
 };
 __device__ __forceinline__ void few_groups(FewRows &l, const AdaptersParams &p) {
+    static_assert(kFewRows == 64 * kWarps, "rows of a warp");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    for (int i = tid; i < kFewRows; i += kThreads) l.slot[i] = i < p.m ? p.rows[i] : -1;
+    if (p.m == 1) {                                  // nothing to sort
+        if (tid == 0) {
+            l.slot[0] = p.rows[0];
+            l.sorted[0] = l.first[0] = 0;
+            l.first[1] = 1;
+            l.n = 1;
+        }
+        __syncthreads();
+        return;
+    }
+    for (int i = tid; i < kKeys; i += kThreads) {
+        l.key[i] = -1;
+        l.first_row[i] = kFewRows;
+    }
+    for (int i = tid; i < kWarps * kKeys / 4; i += kThreads) reinterpret_cast<uint32_t *>(l.count)[i] = 0u;
     __syncthreads();
-    int groups = 0, rows = 0;                        // of the rows before these
-    for (int i0 = 0; i0 < p.m; i0 += kThreads) {
-        const int i = i0 + tid, slot = i < p.m ? l.slot[i] : -1;
-        int before = 0, all = 0, lead = i;
-        if (slot >= 0)
-            for (int j = 0; j < p.m; j += 4) {
-                const int4 v = *reinterpret_cast<const int4 *>(l.slot + j);
+    int at[2], rank[2];                              // key and place among the warp's rows of the same slot
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if ((e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w) == slot) {
-                        if (j + e <= i && all % 16 == 0) lead = j + e;
-                        before += j + e < i;
-                        ++all;
-                    }
+    for (int h = 0; h < 2; ++h) {
+        const int i = warp * 64 + h * 32 + lane, slot = i < p.m ? p.rows[i] : -1;
+        l.slot[i] = slot;
+        at[h] = -1;
+        if (slot >= 0) {
+            int k = (int)(((unsigned)slot * 2654435761u) >> 22);      // (Fibonacci hashing: the upper ten bits)
+            while (true) {
+                const int old = atomicCAS(&l.key[k], -1, slot);
+                if (old == -1 || old == slot) break;
+                k = (k + 1) & (kKeys - 1);
             }
-        const bool leads = slot >= 0 && lead == i;
-        const int n = leads ? min(16, all - before) : 0;
-        int2 run = make_int2(leads, n);
+            at[h] = k;
+            atomicMin(&l.first_row[k], i);
+        }
+        __syncwarp();
+        const unsigned same = __match_any_sync(0xFFFFFFFFu, at[h]);
+        const int before = at[h] >= 0 ? l.count[warp][at[h]] : 0;
+        rank[h] = before + __popc(same & ((1u << lane) - 1));
+        __syncwarp();
+        if (at[h] >= 0 && (same >> lane) == 1u) l.count[warp][at[h]] = (uint8_t)(rank[h] + 1);      // the last lane of those
+        __syncwarp();
+    }
+    __syncthreads();
+    int all[2];
+    int2 mine = make_int2(0, 0), run[2];             // rows and groups that begin with this thread's rows
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        all[h] = 0;
+        int before = 0;
+        if (at[h] >= 0)
+            for (int w = 0; w < kWarps; ++w) {
+                const int n = l.count[w][at[h]];
+                all[h] += n;
+                before += w < warp ? n : 0;
+            }
+        rank[h] += before;
+        const bool begins = at[h] >= 0 && l.first_row[at[h]] == warp * 64 + h * 32 + lane;
+        run[h] = begins ? make_int2(all[h], (all[h] + 15) / 16) : make_int2(0, 0);
+        const int2 own = run[h];
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
-            const int x = __shfl_up_sync(0xFFFFFFFFu, run.x, d), y = __shfl_up_sync(0xFFFFFFFFu, run.y, d);
-            if (lane >= d) run.x += x, run.y += y;
+            const int x = __shfl_up_sync(0xFFFFFFFFu, run[h].x, d), y = __shfl_up_sync(0xFFFFFFFFu, run[h].y, d);
+            if (lane >= d) run[h].x += x, run[h].y += y;
         }
-        if (lane == 31) l.sums[warp] = run;
-        __syncthreads();
-        int2 total = make_int2(0, 0);
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) run.x += l.sums[w].x, run.y += l.sums[w].y;
-            total.x += l.sums[w].x, total.y += l.sums[w].y;
-        }
-        if (leads) {
-            l.first[groups + run.x - 1] = (short)(rows + run.y - n);
-            l.lead[i] = (short)(rows + run.y - n);
-        }
-        __syncthreads();                             // groups that begin among these rows or before
-        if (slot >= 0) l.sorted[l.lead[lead] + before % 16] = (short)i;
-        groups += total.x;
-        rows += total.y;
-        __syncthreads();
+        const int2 sum = make_int2(__shfl_sync(0xFFFFFFFFu, run[h].x, 31), __shfl_sync(0xFFFFFFFFu, run[h].y, 31));
+        run[h].x += mine.x - own.x, run[h].y += mine.y - own.y;
+        mine.x += sum.x, mine.y += sum.y;
     }
+    if (lane == 0) l.sums[warp] = mine;
+    __syncthreads();
+    int2 base = make_int2(0, 0), total = make_int2(0, 0);
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) base.x += l.sums[w].x, base.y += l.sums[w].y;
+        total.x += l.sums[w].x, total.y += l.sums[w].y;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (at[h] >= 0 && l.first_row[at[h]] == warp * 64 + h * 32 + lane) {
+            l.row_base[at[h]] = (short)(base.x + run[h].x);
+            l.group_base[at[h]] = (short)(base.y + run[h].y);
+        }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (at[h] >= 0) {
+            const int to = l.row_base[at[h]] + rank[h];
+            l.sorted[to] = (short)(warp * 64 + h * 32 + lane);
+            if (rank[h] % 16 == 0) l.first[l.group_base[at[h]] + rank[h] / 16] = (short)to;
+        }
     if (tid == 0) {
-        l.n = groups;
-        l.first[groups] = (short)rows;
+        l.n = total.y;
+        l.first[total.y] = (short)total.x;
     }
     __syncthreads();
 }
@@ -335,27 +390,31 @@ constexpr size_t kFewSums = size_t(kWarps) * 16 * kTileLd * 4;
 static_assert(kFewSums >= size_t(kWarps) * 16 * kFewRanks * 4, "sums");
 size_t few_smem(int rank_pad, int planes) { return kFewSums + size_t(16) * rank_pad * 4 + size_t(rank_pad / 16) * planes * 512; }
 
-__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+// the block's threads ask for a piece of memory, 128 bytes each and turn (at most 64 KB)
+__device__ __forceinline__ void prefetch_bytes(const uint8_t *p, long long bytes) {
+    for (int i = threadIdx.x * 128; i < min(bytes, 65536ll); i += kThreads * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
+}
 
 // one adapter against up to sixteen rows
 template <bool F16, bool XF32, bool YF32>
-__device__ __forceinline__ void few_pass(const AdaptersParams &p, const AdapterSet &s, int slot, const int *row, uint8_t *smem) {
+__device__ __forceinline__ void few_pass(const AdaptersParams &p, const AdapterSet &s, int slot, const int *row, int parts, uint8_t *smem) {
     constexpr int PT = YF32 ? 3 : 2, RT = kFewRanks / 8;
     cg::cluster_group cluster = cg::this_cluster();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, part = (int)cluster.block_rank();
-    const int rank = s.rank[slot], rt = (rank + 7) / 8, rk = (rank + 15) / 16, rank_pad = 16 * rk;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int block = (int)cluster.block_rank(), part = block & (parts - 1), lead = block - part;
+    const int rank = slot < 0 ? 0 : s.rank[slot], rt = (rank + 7) / 8, rk = (rank + 15) / 16, rank_pad = 16 * rk;
     float *sums = reinterpret_cast<float *>(smem);
     float *tpart = reinterpret_cast<float *>(smem + kFewSums);
     uint4 *frag = reinterpret_cast<uint4 *>(smem + kFewSums + (size_t)16 * p.rank_pad * 4);
-    const float scale = s.scale[slot];
+    const float scale = slot < 0 ? 0.f : s.scale[slot];
     const uint4 *a = reinterpret_cast<const uint4 *>(s.a + slot * s.a_stride), *b = reinterpret_cast<const uint4 *>(s.b + slot * s.b_stride);
-    const int nc0 = (int)((long long)s.nchunks * part / kCluster), nc1 = (int)((long long)s.nchunks * (part + 1) / kCluster);
-    // B starts its way while A is multiplied: 128 bytes a thread and turn
-    for (long long i = (long long)nc0 * rk * 1024 + threadIdx.x * 128, end = min((long long)nc1 * rk * 1024, i + 64 * 1024); i < end; i += kThreads * 128)
-        prefetch_l2(reinterpret_cast<const uint8_t *>(b) + i);
+    const int nc0 = (int)((long long)s.nchunks * part / parts), nc1 = slot < 0 ? nc0 : (int)((long long)s.nchunks * (part + 1) / parts);
+    const int kc0 = (int)((long long)p.kchunks * part / parts), kc1 = (int)((long long)p.kchunks * (part + 1) / parts);
+    // the block's parts of A (what is not read at once) and B all start their way
+    prefetch_bytes(reinterpret_cast<const uint8_t *>(a) + (long long)(kc0 + kWarps) * rt * 512, (long long)(kc1 - kc0 - kWarps) * rt * 512);
+    prefetch_bytes(reinterpret_cast<const uint8_t *>(b) + (long long)nc0 * rk * 1024, (long long)(nc1 - nc0) * rk * 1024);
 
     // ---- t = A x over this block's part of K
-    const int kc0 = (int)((long long)p.kchunks * part / kCluster), kc1 = (int)((long long)p.kchunks * (part + 1) / kCluster);
     for (int rb = 0; rb < rt; rb += RT) {
         const int tiles = min(rt - rb, RT);
         float acc[RT][4];
@@ -390,9 +449,11 @@ __device__ __forceinline__ void few_pass(const AdaptersParams &p, const AdapterS
             const int at = ((l >> 2) + 8 * (e & 1)) * rank_pad + k * 16 + 2 * (l & 3) + 8 * (e >> 1);
             float2 o[kCluster], v = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int c = 0; c < kCluster; ++c) o[c] = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(tpart, c) + at);
+            for (int c = 0; c < kCluster; ++c)
+                if (c < parts) o[c] = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(tpart, lead + c) + at);
 #pragma unroll
-            for (int c = 0; c < kCluster; ++c) v.x += o[c].x, v.y += o[c].y;
+            for (int c = 0; c < kCluster; ++c)
+                if (c < parts) v.x += o[c].x, v.y += o[c].y;
             split<PT>(v.x, v.y, w[e]);
         }
 #pragma unroll
@@ -414,44 +475,55 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
     pdl_launch_dependents();
     pdl_wait();
     few_groups(rows, p);
-    // (every block of a cluster has the same groups and takes the same way)
-    const int clusters = gridDim.x / kCluster, items = rows.n * p.sets;
-    for (int item = blockIdx.x / kCluster; item < items; item += clusters) {
-        const int group = item / p.sets;
-        const AdapterSet &s = p.set[item - group * p.sets];
-        const int first = rows.first[group], slot = rows.slot[rows.sorted[first]];
-        if (!active(s, slot)) continue;
-        const int n = rows.first[group + 1] - first;
-        if (threadIdx.x < 16) row[threadIdx.x] = threadIdx.x < n ? rows.sorted[first + threadIdx.x] : -1;
+    // As many blocks of a cluster share an item (a group and a set) as there are blocks for all items: eight of few, one of many.  (Every
+    // block has the same groups; those of a cluster meet the same number of times.)
+    const int items = rows.n * p.sets, block = (int)(blockIdx.x % kCluster);
+    int parts = kCluster;
+    while (parts > 1 && items * parts > (int)gridDim.x) parts /= 2;
+    const int at_a_time = gridDim.x / parts, rounds = (items + at_a_time - 1) / at_a_time;
+    for (int round = 0; round < rounds; ++round) {
+        const int item = round * at_a_time + blockIdx.x / kCluster * (kCluster / parts) + block / parts;
+        const int group = min(item, items - 1) / p.sets, set = min(item, items - 1) - group * p.sets;
+        const AdapterSet &s = p.set[set];
+        const int first = rows.first[group], n = rows.first[group + 1] - first;
+        int slot = item < items ? rows.slot[rows.sorted[first]] : -1;
+        if (!active(s, slot)) slot = -1;
+        if (threadIdx.x < 16) row[threadIdx.x] = slot >= 0 && threadIdx.x < n ? rows.sorted[first + threadIdx.x] : -1;
         __syncthreads();
-        few_pass<F16, XF32, YF32>(p, s, slot, row, smem);
+        few_pass<F16, XF32, YF32>(p, s, slot, row, parts, smem);
         __syncthreads();
     }
 }
 
 // ---- more rows ---------------------------------------------------------------------------------------------
-constexpr int kTileRows = 32, kSumTiles = 8;         // rows of a block; tiles of eight ranks whose sums a warp holds at a time
-
-// The rows of a block's tile that are the first of an adapter of some set: bit mask (a warp; rows of a tile at most 32)
+// bit mask of the warp's lanes whose slot is the first of its kind
 __device__ __forceinline__ unsigned first_rows(int slot, int lane) {
     const unsigned same = __match_any_sync(0xFFFFFFFFu, slot);      // (all lanes take part, rows without an adapter too)
     return __ballot_sync(0xFFFFFFFFu, slot >= 0 && __ffs(same) - 1 == lane);
 }
 
-// t[range of K][row][ranks of all sets]
+// t[range of K][row][ranks of all sets].  A warp takes sixteen rows; the eight of a block read the same fragments of A at about the same
+// time, so that all but one find them in L1 (with 32 rows a block and K shared by its warps A came from L2 for every 32 rows: 4096 rows of
+// 5120, 64 ranks, 49 us).
+constexpr int kSumTiles = 8, kShrinkRows = 16 * kWarps;      // tiles of eight ranks whose sums a warp holds at a time
 template <bool F16, bool XF32> __global__ void __launch_bounds__(kThreads, 2) adapters_shrink_kernel(const __grid_constant__ AdaptersParams p) {
-    __shared__ float sums[4][kTileRows][8 * kSumTiles];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int base = blockIdx.x * kTileRows, m = warp & 1, kw = warp >> 1;
+    const int base = blockIdx.x * kShrinkRows + warp * 16;
     const int kc0 = (int)((long long)p.kchunks * blockIdx.y / gridDim.y), kc1 = (int)((long long)p.kchunks * (blockIdx.y + 1) / gridDim.y);
     pdl_launch_dependents();
     pdl_wait();
-    const int mine = base + lane < p.m ? p.rows[base + lane] : -1;
+    if (base >= p.m) return;
+    {                                        // the rows of x all start their way at once
+        const long long from = kc0 * 32ll * (XF32 ? 4 : 2), to = min(kc1 * 32ll, (long long)p.K) * (XF32 ? 4 : 2);
+        const uint8_t *x = reinterpret_cast<const uint8_t *>(p.x) + (base + (lane & 15)) * p.ldx * (XF32 ? 4 : 2);
+        if (base + (lane & 15) < p.m)
+            for (long long i = from + (lane >> 4) * 128; i < to; i += 256) asm volatile("prefetch.global.L2 [%0];" ::"l"(x + i));
+    }
+    const int mine = lane < 16 && base + lane < p.m ? p.rows[base + lane] : -1;
     for (unsigned left = first_rows(mine, lane); left; left &= left - 1) {
         const int slot = __shfl_sync(0xFFFFFFFFu, mine, __ffs((int)left) - 1);
         const unsigned have = __ballot_sync(0xFFFFFFFFu, mine == slot);
-        const int i0 = m * 16 + g, i1 = i0 + 8;
-        const int r0 = (have >> i0) & 1 ? base + i0 : -1, r1 = (have >> i1) & 1 ? base + i1 : -1;
+        const long long r0 = (have >> g) & 1 ? base + g : -1, r1 = (have >> (g + 8)) & 1 ? base + g + 8 : -1;
         // tiles of eight ranks, set after set, kSumTiles at a time
         int set = 0, tile = 0;
         while (true) {
@@ -464,7 +536,7 @@ template <bool F16, bool XF32> __global__ void __launch_bounds__(kThreads, 2) ad
                 while (set < p.sets && (!active(p.set[set], slot) || tile >= (p.set[set].rank[slot] + 7) / 8)) ++set, tile = 0;
                 if (set < p.sets) {
                     const AdapterSet &s = p.set[set];
-                    rt[i] = (s.rank[slot] + 7) / 8;
+                    rt[i] = (s.rank[slot] + 7) / 8 * 32;
                     from[i] = reinterpret_cast<const uint4 *>(s.a + slot * s.a_stride) + tile * 32 + lane;
                     to[i] = s.t_at + 8 * tile;
                     ++tile;
@@ -473,29 +545,20 @@ template <bool F16, bool XF32> __global__ void __launch_bounds__(kThreads, 2) ad
             }
             if (tiles == 0) break;
             float acc[kSumTiles][4];
-            shrink<F16, XF32, kSumTiles>(p, r0, r1, kc0 + kw, kc1, 4, tiles, t, [&](int i, int kc) { return from[i][(size_t)kc * rt[i] * 32]; }, acc);
-#pragma unroll
-            for (int i = 0; i < kSumTiles; ++i) {
-                *reinterpret_cast<float2 *>(&sums[kw][i0][8 * i + 2 * t]) = make_float2(acc[i][0], acc[i][1]);
-                *reinterpret_cast<float2 *>(&sums[kw][i1][8 * i + 2 * t]) = make_float2(acc[i][2], acc[i][3]);
-            }
-            __syncthreads();
-            // lane = rank of a tile and row: eight ranks of four rows a turn
+            shrink<F16, XF32, kSumTiles>(p, r0, r1, kc0, kc1, 1, tiles, t, [&](int i, int kc) { return from[i][(unsigned)kc * (unsigned)rt[i]]; }, acc);
+            float *out = p.t + (long long)blockIdx.y * p.m * p.t_ld + 2 * t;
 #pragma unroll
             for (int i = 0; i < kSumTiles; ++i) {
                 if (i >= tiles) break;
-                const int r = warp * 4 + (lane >> 3), c = lane & 7;
-                if ((have >> r) & 1)
-                    p.t[((long long)blockIdx.y * p.m + base + r) * p.t_ld + to[i] + c] =
-                        sums[0][r][8 * i + c] + sums[1][r][8 * i + c] + sums[2][r][8 * i + c] + sums[3][r][8 * i + c];
+                if (r0 >= 0) *reinterpret_cast<float2 *>(out + r0 * p.t_ld + to[i]) = make_float2(acc[i][0], acc[i][1]);
+                if (r1 >= 0) *reinterpret_cast<float2 *>(out + r1 * p.t_ld + to[i]) = make_float2(acc[i][2], acc[i][3]);
             }
-            __syncthreads();
         }
     }
 }
 
-// y += scale B t: a block takes 64 rows and kStreamChunks chunks of 32 outputs; four warps side by side in the rows, two in the outputs
-constexpr int kStreamRows = 64, kStreamChunks = 32, kStreamStep = 4;
+// y += scale B t: a block takes 64 rows and p.stream_chunks chunks of 32 outputs; four warps side by side in the rows, two in the outputs
+constexpr int kStreamRows = 64, kStreamStep = 4;
 constexpr size_t kPieces = size_t(kWarps) * 16 * kTileLd * 4;
 template <bool F16, bool YF32> __global__ void __launch_bounds__(kThreads, 2) adapters_stream_kernel(const __grid_constant__ AdaptersParams p) {
     constexpr int PT = YF32 ? 3 : 2;
@@ -505,7 +568,7 @@ template <bool F16, bool YF32> __global__ void __launch_bounds__(kThreads, 2) ad
     uint4 *frag = reinterpret_cast<uint4 *>(smem + kPieces);
     const AdapterSet &s = p.set[blockIdx.z];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, base = blockIdx.y * kStreamRows;
-    const int nc0 = blockIdx.x * kStreamChunks, nc1 = min(nc0 + kStreamChunks, s.nchunks);
+    const int nc0 = blockIdx.x * p.stream_chunks, nc1 = min(nc0 + p.stream_chunks, s.nchunks);
     if (nc0 >= nc1) return;                  // (another set is wider)
     pdl_launch_dependents();
     pdl_wait();
@@ -556,10 +619,8 @@ template <bool F16, bool YF32> __global__ void __launch_bounds__(kThreads, 2) ad
 }
 
 template <typename Kernel> cudaError_t launch(Kernel kern, const AdaptersParams &p, dim3 grid, size_t smem, cudaStream_t st) {
-    if (smem > 32 * 1024) {
-        cudaError_t e = configure_smem(reinterpret_cast<const void *>(kern), smem);
-        if (e != cudaSuccess) return e;
-    }
+    cudaError_t e = configure_smem(reinterpret_cast<const void *>(kern), smem);
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(kThreads);
@@ -579,19 +640,20 @@ template <bool F16, bool XF32, bool YF32> cudaError_t run(AdaptersParams p, int 
         const int clusters = std::min(p.m * p.sets, sm_count * 2 / kCluster);
         return launch(adapters_few_kernel<F16, XF32, YF32>, p, dim3((unsigned)(clusters * kCluster)), few_smem(p.rank_pad, PT), st);
     }
-    // ranges of K: as many blocks as run at a time
-    const int tiles = (p.m + kTileRows - 1) / kTileRows;
-    p.t_ranges = std::max(1, std::min({2 * sm_count / tiles, p.kchunks / 16, 8}));
+    // ranges of K: as many blocks as run at a time, of eight chunks at least
+    p.t_ranges = std::max(1, std::min({2 * sm_count / ((p.m + kShrinkRows - 1) / kShrinkRows), p.kchunks / 8, 16}));
+    // 32 chunks a block read t seldom; 8 where that leaves blocks out of work
     int widest = 0;
     for (int i = 0; i < p.sets; ++i) widest = std::max(widest, p.set[i].nchunks);
+    p.stream_chunks = (long long)((p.m + kStreamRows - 1) / kStreamRows) * p.sets * ((widest + 31) / 32) >= 4ll * sm_count ? 32 : 8;
     // t of as many rows at a time as there is room for
     const int room = (int)std::min<size_t>(t_floats / ((size_t)p.t_ranges * p.t_ld) / kStreamRows * kStreamRows, size_t(32767) * kStreamRows);
     for (int done = 0, all = p.m; done < all; done += room) {
         p.m = std::min(room, all - done);
-        cudaError_t e = launch(adapters_shrink_kernel<F16, XF32>, p, dim3((unsigned)((p.m + kTileRows - 1) / kTileRows), (unsigned)p.t_ranges), 0, st);
+        cudaError_t e = launch(adapters_shrink_kernel<F16, XF32>, p, dim3((unsigned)((p.m + kShrinkRows - 1) / kShrinkRows), (unsigned)p.t_ranges), 0, st);
         if (e != cudaSuccess) return e;
         e = launch(adapters_stream_kernel<F16, YF32>, p,
-                   dim3((unsigned)((widest + kStreamChunks - 1) / kStreamChunks), (unsigned)((p.m + kStreamRows - 1) / kStreamRows), (unsigned)p.sets),
+                   dim3((unsigned)((widest + p.stream_chunks - 1) / p.stream_chunks), (unsigned)((p.m + kStreamRows - 1) / kStreamRows), (unsigned)p.sets),
                    kPieces + size_t(4) * (p.rank_pad / 16) * PT * 512, st);
         if (e != cudaSuccess) return e;
         p.rows += p.m;

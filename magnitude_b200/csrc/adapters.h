@@ -6,7 +6,7 @@
 namespace b200q {
 
 constexpr int kAdapterMaxRank = 256, kAdapterMaxSets = 4;
-constexpr size_t kAdapterTFloats = size_t(4) << 20;      // a context's room for t: 512 rows of 1024 ranks in eight ranges
+constexpr size_t kAdapterTFloats = size_t(8) << 20;      // a context's room for t: 512 rows of 1024 ranks in sixteen ranges
 
 // Fragments of an adapter, 16 bytes a lane (lane 4 g + t):
 //   A  [chunk of 32 of K][rank tile of 8][lane]: rank g of the tile, K 8 t .. 8 t + 7 of the chunk
@@ -40,6 +40,7 @@ struct AdaptersParams {
     // more rows: t = A x on its way from one launch to the next, [range of K][row][t_ld]
     float *t;
     int t_ld, t_ranges;
+    int stream_chunks;               // chunks of 32 outputs of a block
 };
 
 cudaError_t adapter_pack(const void *a, const void *b, uint8_t *pa, uint8_t *pb, int rank, int K, int n, cudaStream_t st);
