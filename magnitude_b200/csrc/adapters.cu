@@ -145,15 +145,26 @@ template <bool YF32> __device__ __forceinline__ void store_y(const AdapterSet &s
     else reinterpret_cast<__nv_bfloat16 *>(s.y)[row * s.ldy + n] = __float2bfloat16_rn(v);
 }
 
-// A piece of t = A x for sixteen rows: tiles of eight ranks, chunks kc, kc + step, .. below kc1.  r0, r1: the lane's rows, -1: none;
+// acc += sixteen rows (planes of eight elements of rows g, g + 8) times a fragment of A: 32 of K, eight ranks
+template <bool F16, int PX> __device__ __forceinline__ void multiply_tile(const uint32_t (&f0)[PX][4], const uint32_t (&f1)[PX][4], const uint4 &w, float (&acc)[4]) {
+    constexpr int PA = F16 ? 2 : 1;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t b0[PA], b1[PA];
+        adapter_planes<F16, PA>(h ? w.z : w.x, b0);
+        adapter_planes<F16, PA>(h ? w.w : w.y, b1);
+#pragma unroll
+        for (int px = 0; px < PX; ++px)
+#pragma unroll
+            for (int pa = 0; pa < PA; ++pa) mma_bf16(acc, f0[px][2 * h], f1[px][2 * h], f0[px][2 * h + 1], f1[px][2 * h + 1], b0[pa], b1[pa]);
+    }
+}
+
+// acc += a piece of t = A x for sixteen rows: tiles of eight ranks, chunks kc, kc + step, .. below kc1.  r0, r1: the lane's rows, -1: none;
 // w(i, kc): the lane's fragment of tile i.
 template <bool F16, bool XF32, int RT, typename Fragment>
 __device__ __forceinline__ void shrink(const AdaptersParams &p, long long r0, long long r1, int kc, int kc1, int step, int tiles, int t, Fragment fragment, float (&acc)[RT][4]) {
-    constexpr int PX = XF32 ? 3 : 1, PA = F16 ? 2 : 1;
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+    constexpr int PX = XF32 ? 3 : 1;
     XPiece<XF32> x0, x1;                     // the next chunk's, on their way
     x0.load(p, r0, kc * 32 + 8 * t, kc < kc1);
     x1.load(p, r1, kc * 32 + 8 * t, kc < kc1);
@@ -170,16 +181,7 @@ __device__ __forceinline__ void shrink(const AdaptersParams &p, long long r0, lo
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             if (i >= tiles) break;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t b0[PA], b1[PA];
-                adapter_planes<F16, PA>(h ? w[i].z : w[i].x, b0);
-                adapter_planes<F16, PA>(h ? w[i].w : w[i].y, b1);
-#pragma unroll
-                for (int px = 0; px < PX; ++px)
-#pragma unroll
-                    for (int pa = 0; pa < PA; ++pa) mma_bf16(acc[i], f0[px][2 * h], f1[px][2 * h], f0[px][2 * h + 1], f1[px][2 * h + 1], b0[pa], b1[pa]);
-            }
+            multiply_tile<F16, PX>(f0, f1, w[i], acc[i]);
         }
     }
 }
@@ -418,6 +420,10 @@ __device__ __forceinline__ void few_pass(const AdaptersParams &p, const AdapterS
     for (int rb = 0; rb < rt; rb += RT) {
         const int tiles = min(rt - rb, RT);
         float acc[RT][4];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
         shrink<F16, XF32, RT>(p, row[g], row[g + 8], kc0 + warp, kc1, kWarps, tiles, t, [&](int i, int kc) { return a[((size_t)kc * rt + rb + i) * 32 + lane]; }, acc);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
@@ -468,7 +474,7 @@ __device__ __forceinline__ void few_pass(const AdaptersParams &p, const AdapterS
 }
 
 template <bool F16, bool XF32, bool YF32>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) adapters_few_kernel(const __grid_constant__ AdaptersParams p) {
+__global__ void __launch_bounds__(kThreads, 2) adapters_few_kernel(const __grid_constant__ AdaptersParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(16) FewRows rows;
     __shared__ int row[16];
@@ -502,59 +508,147 @@ __device__ __forceinline__ unsigned first_rows(int slot, int lane) {
     return __ballot_sync(0xFFFFFFFFu, slot >= 0 && __ffs(same) - 1 == lane);
 }
 
-// t[range of K][row][ranks of all sets].  A warp takes sixteen rows; the eight of a block read the same fragments of A at about the same
-// time, so that all but one find them in L1 (with 32 rows a block and K shared by its warps A came from L2 for every 32 rows: 4096 rows of
-// 5120, 64 ranks, 49 us).
+// t[row][ranks of all sets].  A cluster takes 128 rows, sixteen a warp, and one adapter of them after the other; its blocks split K and add their
+// parts up through distributed shared memory, each for some of the rows.  x and the fragments of A come into shared memory by cp.async, 512
+// bytes of every row at a time.  (With x in registers, a chunk ahead, the way from L2 set the pace: 4096 rows of 5120, 64 ranks, 54 us.)
 constexpr int kSumTiles = 8, kShrinkRows = 16 * kWarps;      // tiles of eight ranks whose sums a warp holds at a time
+constexpr int kSumLd = 8 * kSumTiles + 2;
+constexpr int kXLd = 512 + 64;                               // bytes from row to row: two rows' pieces lie in different banks
+constexpr size_t kShrinkX = size_t(kShrinkRows) * kXLd;
+__host__ __device__ constexpr int batch_chunks(bool f32) { return f32 ? 4 : 8; }
+constexpr size_t kShrinkSmem = kShrinkX + size_t(8) * kSumTiles * 512;
+static_assert(kShrinkX >= size_t(kShrinkRows) * kSumLd * 4, "sums");
+struct AdapterTile {
+    const uint4 *from;                   // its fragment of the first chunk
+    int step, to;                        // 16-byte words from chunk to chunk; its place in a row of t
+};
 template <bool F16, bool XF32> __global__ void __launch_bounds__(kThreads, 2) adapters_shrink_kernel(const __grid_constant__ AdaptersParams p) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int base = blockIdx.x * kShrinkRows + warp * 16;
-    const int kc0 = (int)((long long)p.kchunks * blockIdx.y / gridDim.y), kc1 = (int)((long long)p.kchunks * (blockIdx.y + 1) / gridDim.y);
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int slots[kShrinkRows];
+    __shared__ unsigned firsts[kShrinkRows / 32];
+    __shared__ AdapterTile tiles_of[kAdapterMaxSets * kAdapterMaxRank / 8];
+    __shared__ int all_tiles;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int base = blockIdx.x * kShrinkRows, mine = warp * 16;
+    const int parts = gridDim.y, part0 = blockIdx.y;      // the cluster
+    const int kc0 = (int)((long long)p.kchunks * part0 / parts), kc1 = (int)((long long)p.kchunks * (part0 + 1) / parts);
+    cg::cluster_group cluster = cg::this_cluster();
+    float *sums = reinterpret_cast<float *>(smem);        // [row][rank of the tiles at hand], where x was
+    uint8_t *afrag = smem + kShrinkX;
+    constexpr int PX = XF32 ? 3 : 1, XB = XF32 ? 4 : 2, BATCH = batch_chunks(XF32);
     pdl_launch_dependents();
     pdl_wait();
-    if (base >= p.m) return;
-    {                                        // the rows of x all start their way at once
-        const long long from = kc0 * 32ll * (XF32 ? 4 : 2), to = min(kc1 * 32ll, (long long)p.K) * (XF32 ? 4 : 2);
-        const uint8_t *x = reinterpret_cast<const uint8_t *>(p.x) + (base + (lane & 15)) * p.ldx * (XF32 ? 4 : 2);
-        if (base + (lane & 15) < p.m)
-            for (long long i = from + (lane >> 4) * 128; i < to; i += 256) asm volatile("prefetch.global.L2 [%0];" ::"l"(x + i));
+    if (tid < kShrinkRows) {
+        const int slot = base + tid < p.m ? p.rows[base + tid] : -1;
+        slots[tid] = slot;
+        const unsigned first = first_rows(slot, lane);
+        if (lane == 0) firsts[warp] = first;
     }
-    const int mine = lane < 16 && base + lane < p.m ? p.rows[base + lane] : -1;
-    for (unsigned left = first_rows(mine, lane); left; left &= left - 1) {
-        const int slot = __shfl_sync(0xFFFFFFFFu, mine, __ffs((int)left) - 1);
-        const unsigned have = __ballot_sync(0xFFFFFFFFu, mine == slot);
-        const long long r0 = (have >> g) & 1 ? base + g : -1, r1 = (have >> (g + 8)) & 1 ? base + g + 8 : -1;
-        // tiles of eight ranks, set after set, kSumTiles at a time
-        int set = 0, tile = 0;
-        while (true) {
-            const uint4 *from[kSumTiles];
-            int to[kSumTiles], rt[kSumTiles], tiles = 0;
-#pragma unroll
-            for (int i = 0; i < kSumTiles; ++i) {
-                from[i] = nullptr;
-                to[i] = rt[i] = 0;
-                while (set < p.sets && (!active(p.set[set], slot) || tile >= (p.set[set].rank[slot] + 7) / 8)) ++set, tile = 0;
-                if (set < p.sets) {
+    __syncthreads();
+    for (int part = 0; part < kShrinkRows / 32; ++part)
+        for (unsigned left = firsts[part]; left; left &= left - 1) {
+            const int slot = slots[part * 32 + __ffs((int)left) - 1];
+            bool seen = false;               // had its turn among earlier rows?
+            for (int q = lane; q < part * 32; q += 32) seen |= slots[q] == slot;
+            if (__any_sync(0xFFFFFFFFu, seen)) continue;
+            const bool any = __any_sync(0xFFFFFFFFu, lane < 16 && slots[mine + (lane & 15)] == slot);
+            // tiles of eight ranks, set after set
+            if (tid < p.sets * (kAdapterMaxRank / 8)) {
+                int at = 0, tile = tid;
+                for (int set = 0; set < p.sets; ++set) {
                     const AdapterSet &s = p.set[set];
-                    rt[i] = (s.rank[slot] + 7) / 8 * 32;
-                    from[i] = reinterpret_cast<const uint4 *>(s.a + slot * s.a_stride) + tile * 32 + lane;
-                    to[i] = s.t_at + 8 * tile;
-                    ++tile;
-                    ++tiles;
+                    const int rt = active(s, slot) ? (s.rank[slot] + 7) / 8 : 0;
+                    if (tile >= 0 && tile < rt) {
+                        tiles_of[tid].from = reinterpret_cast<const uint4 *>(s.a + slot * s.a_stride) + tile * 32;
+                        tiles_of[tid].step = rt * 32;
+                        tiles_of[tid].to = s.t_at + 8 * tile;
+                    }
+                    at += rt;
+                    tile -= rt;
                 }
+                if (tid == 0) all_tiles = at;
             }
-            if (tiles == 0) break;
-            float acc[kSumTiles][4];
-            shrink<F16, XF32, kSumTiles>(p, r0, r1, kc0, kc1, 1, tiles, t, [&](int i, int kc) { return from[i][(unsigned)kc * (unsigned)rt[i]]; }, acc);
-            float *out = p.t + (long long)blockIdx.y * p.m * p.t_ld + 2 * t;
+            __syncthreads();
+            for (int first = 0; first < all_tiles; first += kSumTiles) {
+                const int tiles = min(all_tiles - first, kSumTiles);
+                float acc[kSumTiles][4];
 #pragma unroll
-            for (int i = 0; i < kSumTiles; ++i) {
-                if (i >= tiles) break;
-                if (r0 >= 0) *reinterpret_cast<float2 *>(out + r0 * p.t_ld + to[i]) = make_float2(acc[i][0], acc[i][1]);
-                if (r1 >= 0) *reinterpret_cast<float2 *>(out + r1 * p.t_ld + to[i]) = make_float2(acc[i][2], acc[i][3]);
+                for (int i = 0; i < kSumTiles; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+                for (int kc = kc0; kc < kc1; kc += BATCH) {
+                    const int chunks = min(BATCH, kc1 - kc);
+                    __syncthreads();         // what was there has been read
+                    for (int i = tid; i < kShrinkRows * 32; i += kThreads) {      // 16 bytes of a row; zeros beyond the rows and K
+                        const int r = i >> 5, at = (i & 31) * 16, k = kc * 32 + at / XB;
+                        const long long row = base + r;
+                        const uint8_t *from = reinterpret_cast<const uint8_t *>(p.x) + (row * p.ldx + k) * XB;
+                        uint8_t *to = smem + r * kXLd + at;
+                        const int left = row < p.m && at < chunks * 32 * XB ? min(max((p.K - k) * XB, 0), 16) : 0;
+                        if (p.x_vec) {
+                            if (left == 0) from = reinterpret_cast<const uint8_t *>(p.x);
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(left) : "memory");
+                        } else {
+#pragma unroll
+                            for (int b = 0; b < 16; b += XB) {
+                                if (XF32) *reinterpret_cast<uint32_t *>(to + b) = b < left ? *reinterpret_cast<const uint32_t *>(from + b) : 0u;
+                                else *reinterpret_cast<uint16_t *>(to + b) = b < left ? *reinterpret_cast<const uint16_t *>(from + b) : (uint16_t)0;
+                            }
+                        }
+                    }
+                    for (int i = warp; i < tiles; i += kWarps) {
+                        const AdapterTile tile = tiles_of[first + i];
+                        for (int c = 0; c < chunks; ++c)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(afrag + ((c * kSumTiles + i) * 32 + lane) * 16)),
+                                         "l"(tile.from + (size_t)(kc + c) * tile.step + lane)
+                                         : "memory");
+                    }
+                    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+                    __syncthreads();
+                    if (any)
+                        for (int c = 0; c < chunks; ++c) {
+                            uint32_t f0[PX][4], f1[PX][4];
+                            XPiece<XF32> x0, x1;
+                            const uint8_t *at = smem + (mine + g) * kXLd + (c * 32 + 8 * t) * XB;
+#pragma unroll
+                            for (int i = 0; i < (XF32 ? 2 : 1); ++i) {
+                                x0.w[i] = *reinterpret_cast<const uint4 *>(at + 16 * i);
+                                x1.w[i] = *reinterpret_cast<const uint4 *>(at + 8 * kXLd + 16 * i);
+                            }
+                            x0.planes(f0);
+                            x1.planes(f1);
+#pragma unroll
+                            for (int i = 0; i < kSumTiles; ++i) {
+                                if (i >= tiles) break;
+                                multiply_tile<F16, PX>(f0, f1, *reinterpret_cast<const uint4 *>(afrag + ((c * kSumTiles + i) * 32 + lane) * 16), acc[i]);
+                            }
+                        }
+                }
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < kSumTiles; ++i) {
+                    float *to = sums + (mine + g) * kSumLd + 8 * i + 2 * t;
+                    *reinterpret_cast<float2 *>(to) = make_float2(acc[i][0], acc[i][1]);
+                    *reinterpret_cast<float2 *>(to + 8 * kSumLd) = make_float2(acc[i][2], acc[i][3]);
+                }
+                cluster.sync();
+                const int rows = kShrinkRows / parts;
+                for (int i = tid; i < rows * tiles * 4; i += kThreads) {
+                    const int r = part0 * rows + i / (tiles * 4), c = 2 * (i % (tiles * 4));
+                    if (slots[r] != slot) continue;
+                    float2 o[kCluster], v = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int q = 0; q < kCluster; ++q)
+                        if (q < parts) o[q] = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(sums, q) + r * kSumLd + c);
+#pragma unroll
+                    for (int q = 0; q < kCluster; ++q)
+                        if (q < parts) v.x += o[q].x, v.y += o[q].y;
+                    *reinterpret_cast<float2 *>(p.t + (long long)(base + r) * p.t_ld + tiles_of[first + c / 8].to + c % 8) = v;
+                }
+                cluster.sync();
             }
+            __syncthreads();                 // the tiles' list has been read
         }
-    }
 }
 
 // y += scale B t: a block takes 64 rows and p.stream_chunks chunks of 32 outputs; four warps side by side in the rows, two in the outputs
@@ -592,7 +686,7 @@ template <bool F16, bool YF32> __global__ void __launch_bounds__(kThreads, 2) ad
             const int rk = (s.rank[slot] + 15) / 16, ranks = (s.rank[slot] + 7) / 8 * 8;
             if (threadIdx.x < kStreamRows) row[threadIdx.x] = slots[threadIdx.x] == slot ? base + (int)threadIdx.x : -1;
             __syncthreads();
-            // t, added up over the ranges of K, as fragments: [row tile][rank tile][plane][lane]
+            // t as fragments: [row tile][rank tile][plane][lane]
             for (int i = threadIdx.x; i < 4 * rk * 32; i += kThreads) {
                 const int l = i & 31, tile = i >> 5, m = tile / rk, k = tile - m * rk;
                 uint32_t w[4][PT];
@@ -600,11 +694,7 @@ template <bool F16, bool YF32> __global__ void __launch_bounds__(kThreads, 2) ad
                 for (int e = 0; e < 4; ++e) {
                     const int r = row[m * 16 + (l >> 2) + 8 * (e & 1)], c = k * 16 + 2 * (l & 3) + 8 * (e >> 1);
                     float2 v = make_float2(0.f, 0.f);
-                    if (r >= 0 && c < ranks)
-                        for (int q = 0; q < p.t_ranges; ++q) {
-                            const float2 o = *reinterpret_cast<const float2 *>(p.t + ((long long)q * p.m + r) * p.t_ld + s.t_at + c);
-                            v.x += o.x, v.y += o.y;
-                        }
+                    if (r >= 0 && c < ranks) v = *reinterpret_cast<const float2 *>(p.t + (long long)r * p.t_ld + s.t_at + c);
                     split<PT>(v.x, v.y, w[e]);
                 }
 #pragma unroll
@@ -618,7 +708,7 @@ template <bool F16, bool YF32> __global__ void __launch_bounds__(kThreads, 2) ad
         }
 }
 
-template <typename Kernel> cudaError_t launch(Kernel kern, const AdaptersParams &p, dim3 grid, size_t smem, cudaStream_t st) {
+template <typename Kernel> cudaError_t launch(Kernel kern, const AdaptersParams &p, dim3 grid, dim3 cluster, size_t smem, cudaStream_t st) {
     cudaError_t e = configure_smem(reinterpret_cast<const void *>(kern), smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
@@ -626,11 +716,15 @@ template <typename Kernel> cudaError_t launch(Kernel kern, const AdaptersParams 
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster.x;
+    attr[1].val.clusterDim.y = cluster.y;
+    attr[1].val.clusterDim.z = cluster.z;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
@@ -638,22 +732,26 @@ template <bool F16, bool XF32, bool YF32> cudaError_t run(AdaptersParams p, int 
     constexpr int PT = YF32 ? 3 : 2;
     if (p.m <= kFewRows) {
         const int clusters = std::min(p.m * p.sets, sm_count * 2 / kCluster);
-        return launch(adapters_few_kernel<F16, XF32, YF32>, p, dim3((unsigned)(clusters * kCluster)), few_smem(p.rank_pad, PT), st);
+        return launch(adapters_few_kernel<F16, XF32, YF32>, p, dim3((unsigned)(clusters * kCluster)), dim3(kCluster), few_smem(p.rank_pad, PT), st);
     }
-    // ranges of K: as many blocks as run at a time, of eight chunks at least
-    p.t_ranges = std::max(1, std::min({2 * sm_count / ((p.m + kShrinkRows - 1) / kShrinkRows), p.kchunks / 8, 16}));
-    // 32 chunks a block read t seldom; 8 where that leaves blocks out of work
+    // blocks that split K: as many as run at a time, of eight chunks each at least
+    int parts = kCluster;
+    while (parts > 1 && (parts * ((p.m + kShrinkRows - 1) / kShrinkRows) > 2 * sm_count || p.kchunks < 8 * parts)) parts /= 2;
+    // A block reads t before its outputs: the more chunks of them, the better, while the SMs have some ten blocks each to share out
     int widest = 0;
     for (int i = 0; i < p.sets; ++i) widest = std::max(widest, p.set[i].nchunks);
-    p.stream_chunks = (long long)((p.m + kStreamRows - 1) / kStreamRows) * p.sets * ((widest + 31) / 32) >= 4ll * sm_count ? 32 : 8;
+    p.stream_chunks = 64;
+    while (p.stream_chunks > 8 && (long long)((p.m + kStreamRows - 1) / kStreamRows) * p.sets * ((widest + p.stream_chunks - 1) / p.stream_chunks) < 20ll * sm_count)
+        p.stream_chunks /= 2;
     // t of as many rows at a time as there is room for
-    const int room = (int)std::min<size_t>(t_floats / ((size_t)p.t_ranges * p.t_ld) / kStreamRows * kStreamRows, size_t(32767) * kStreamRows);
+    const int room = (int)std::min<size_t>(t_floats / (size_t)p.t_ld / kStreamRows * kStreamRows, size_t(32767) * kStreamRows);
     for (int done = 0, all = p.m; done < all; done += room) {
         p.m = std::min(room, all - done);
-        cudaError_t e = launch(adapters_shrink_kernel<F16, XF32>, p, dim3((unsigned)((p.m + kShrinkRows - 1) / kShrinkRows), (unsigned)p.t_ranges), 0, st);
+        cudaError_t e = launch(adapters_shrink_kernel<F16, XF32>, p, dim3((unsigned)((p.m + kShrinkRows - 1) / kShrinkRows), (unsigned)parts), dim3(1, (unsigned)parts),
+                               kShrinkSmem, st);
         if (e != cudaSuccess) return e;
         e = launch(adapters_stream_kernel<F16, YF32>, p,
-                   dim3((unsigned)((widest + p.stream_chunks - 1) / p.stream_chunks), (unsigned)((p.m + kStreamRows - 1) / kStreamRows), (unsigned)p.sets),
+                   dim3((unsigned)((widest + p.stream_chunks - 1) / p.stream_chunks), (unsigned)((p.m + kStreamRows - 1) / kStreamRows), (unsigned)p.sets), dim3(1),
                    kPieces + size_t(4) * (p.rank_pad / 16) * PT * 512, st);
         if (e != cudaSuccess) return e;
         p.rows += p.m;

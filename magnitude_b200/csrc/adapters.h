@@ -6,7 +6,7 @@
 namespace b200q {
 
 constexpr int kAdapterMaxRank = 256, kAdapterMaxSets = 4;
-constexpr size_t kAdapterTFloats = size_t(8) << 20;      // a context's room for t: 512 rows of 1024 ranks in sixteen ranges
+constexpr size_t kAdapterTFloats = size_t(2) << 20;      // a context's room for t: 2048 rows of 1024 ranks
 
 // Fragments of an adapter, 16 bytes a lane (lane 4 g + t):
 //   A  [chunk of 32 of K][rank tile of 8][lane]: rank g of the tile, K 8 t .. 8 t + 7 of the chunk
@@ -37,9 +37,9 @@ struct AdaptersParams {
     const int *rows;                 // [m]: every row's slot
     int m;
     int rank_pad;                    // largest rank of the sets, in multiples of 16
-    // more rows: t = A x on its way from one launch to the next, [range of K][row][t_ld]
+    // more rows: t = A x on its way from one launch to the next, [row][t_ld]
     float *t;
-    int t_ld, t_ranges;
+    int t_ld;
     int stream_chunks;               // chunks of 32 outputs of a block
 };
 
