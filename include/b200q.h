@@ -420,7 +420,7 @@ typedef struct b200q_router_config {
     int32_t n_experts;             /* 1..1024 */
     int32_t top_k;                 /* 1..32, at most n_experts */
     int64_t n_embd;
-    int64_t max_rows;              /* 1..1048576 */
+    int64_t max_rows;              /* 1..131072; the workspace holds 32 bytes for every row and expert */
     int32_t w_dtype;               /* F32 or BF16 */
     int32_t scoring;               /* B200Q_SCORING_* */
     int32_t normalise;             /* non-zero: the chosen weights are divided by their sum */

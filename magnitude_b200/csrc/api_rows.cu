@@ -215,7 +215,7 @@ b200q_status b200q_router_create(b200q_ctx *ctx, const b200q_router_config *c, b
         return fail(ctx, B200Q_ERR_INVALID_CONFIG, "router: 1..%d experts and 1..%d choices (at most the experts); got %d and %d", kRouterMaxExperts,
                     kRouterMaxTopK, c->n_experts, c->top_k);
     if (c->n_embd < 1 || c->n_embd > (1 << 20)) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "router: n_embd must be 1..%d", 1 << 20);
-    if (c->max_rows < 1 || c->max_rows > (1 << 20)) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "router: max_rows must be 1..%d", 1 << 20);
+    if (c->max_rows < 1 || c->max_rows > (1 << 17)) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "router: max_rows must be 1..%d", 1 << 17);
     if (c->scoring != B200Q_SCORING_SOFTMAX && c->scoring != B200Q_SCORING_SIGMOID) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "unknown scoring %d", c->scoring);
     if (c->scoring == B200Q_SCORING_SOFTMAX && c->select_bias)
         return fail(ctx, B200Q_ERR_INVALID_CONFIG, "a bias of the choice goes with sigmoid scores; softmax takes logit_bias");
@@ -228,12 +228,14 @@ b200q_status b200q_router_create(b200q_ctx *ctx, const b200q_router_config *c, b
     r->max_rows = c->max_rows;
     const size_t elt = act_size(c->w_dtype), row = (size_t)c->n_embd * elt;
     const int64_t ld = (c->n_embd + 31) / 32 * 32;
+    const size_t logit_bytes = (size_t)kRouterMaxRanges * c->max_rows * c->n_experts * sizeof(double);
     cudaError_t e = cudaMalloc(&r->w, c->n_experts * ld * elt);
     if (e == cudaSuccess) e = cudaMemset(r->w, 0, c->n_experts * ld * elt);
     if (e == cudaSuccess) e = cudaMemcpy2D(r->w, ld * elt, c->w, row, row, c->n_experts, cudaMemcpyDefault);
     if (e == cudaSuccess) e = upload_floats(c->logit_bias, c->n_experts, &r->logit_bias);
     if (e == cudaSuccess) e = upload_floats(c->select_bias, c->n_experts, &r->select_bias);
-    if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void **>(&r->logits), (size_t)c->max_rows * c->n_experts * sizeof(double));
+    if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void **>(&r->logits), logit_bytes + 256);
+    if (e == cudaSuccess) e = cudaMemset(reinterpret_cast<uint8_t *>(r->logits) + logit_bytes, 0, 256);
     if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);      // in place before a call on any stream reads it
     if (e != cudaSuccess) {
         b200q_router_destroy(r);
@@ -251,6 +253,7 @@ b200q_status b200q_router_create(b200q_ctx *ctx, const b200q_router_config *c, b
     r->run.normalise = c->normalise != 0;
     r->run.scale = c->scale;
     r->run.logits = r->logits;
+    r->run.count = reinterpret_cast<unsigned *>(reinterpret_cast<uint8_t *>(r->logits) + logit_bytes);
     *out = r;
     return B200Q_OK;
 }

@@ -47,9 +47,134 @@ __device__ __forceinline__ void load8(const void *base, long long at, int k0, in
     }
 }
 
-// A block owns RT x 16 rows and ET x 8 experts; its warps split K in turns of 32 and are added up in order.
+constexpr double kMax = 1.7976931348623157e308;
+
+// A double as an unsigned number that orders the same way
+__device__ __forceinline__ unsigned long long ordered(double v) {
+    const long long b = __double_as_longlong(v);
+    return (unsigned long long)(b ^ ((b >> 63) | (long long)0x8000000000000000ull));
+}
+
+// One row's choice by a warp: expert e belongs to lane e % 32.  logits(e): the row's.
+template <int PER, typename Logits> __device__ __forceinline__ void choose(const RouterRun &p, int row, int lane, Logits logits) {
+    double score[PER], top = -kMax;
+    unsigned long long key[PER];             // what is compared; 0: taken, or beyond the last expert
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int e = 32 * i + lane;
+        double l = -kMax;
+        if (e < p.experts) {
+            l = logits(e) + (p.logit_bias ? (double)p.logit_bias[e] : 0.0);
+            l = isnan(l) ? -kMax : fmin(fmax(l, -kMax), kMax);
+        }
+        top = fmax(top, l);
+        score[i] = p.sigmoid ? 1.0 / (1.0 + exp(-l)) : l;
+        double k = score[i] + (p.select_bias && e < p.experts ? (double)p.select_bias[e] : 0.0);
+        key[i] = e < p.experts ? ordered(isnan(k) ? -kMax : fmin(fmax(k, -kMax), kMax)) : 0ull;
+    }
+    float all = 0.f;                          // softmax over all experts
+    if (!p.sigmoid) {
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+        if (!p.normalise) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (32 * i + lane < p.experts) all += expf((float)(score[i] - top));
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(0xFFFFFFFFu, all, d);
+        }
+    }
+    float mine = 0.f, sum = 0.f;              // lane j keeps choice j's weight
+    int pick = 0;
+    for (int j = 0; j < p.top_k; ++j) {
+        unsigned long long best = 0;
+        int at = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (key[i] > best) best = key[i], at = i;
+        // the largest of the warp, of equal ones the lowest index: 32 bits at a time
+        const unsigned hi = __reduce_max_sync(0xFFFFFFFFu, (unsigned)(best >> 32));
+        const unsigned lo = __reduce_max_sync(0xFFFFFFFFu, (unsigned)(best >> 32) == hi ? (unsigned)best : 0u);
+        const bool has = best == ((unsigned long long)hi << 32 | lo) && best != 0;
+        const int e = (int)__reduce_min_sync(0xFFFFFFFFu, has ? 32u * at + lane : 0x7FFFFFFFu);
+        double s = 0.0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (e == 32 * i + lane) s = score[i], key[i] = 0ull;
+        const float v = __shfl_sync(0xFFFFFFFFu, p.sigmoid ? (float)s : expf((float)(s - top)), e & 31);
+        sum += v;
+        if (lane == j) mine = v, pick = e;
+    }
+    if (lane < p.top_k) {
+        const float by = p.normalise ? sum : p.sigmoid ? 1.f : all;
+        p.ids[row * p.ld_ids + lane] = pick;
+        p.weights[row * p.ld_weights + lane] = by > 0.f ? mine / by * p.scale : 0.f;
+    }
+}
+template <typename Logits> __device__ __forceinline__ void choose_any(const RouterRun &p, int row, int lane, Logits logits) {
+    if (p.experts <= 128) choose<4>(p, row, lane, logits);
+    else if (p.experts <= 256) choose<8>(p, row, lane, logits);
+    else choose<32>(p, row, lane, logits);
+}
+
+// ---- up to kFewRows rows: one launch ---------------------------------------------------------------------
+// A block per expert, its threads split K; the block that is the last to leave its logits makes the choice.
+constexpr int kFewRows = 16;
+__global__ void __launch_bounds__(kThreads) router_few_kernel(const __grid_constant__ RouterRun p) {
+    __shared__ double part[kWarps][kFewRows];
+    __shared__ int last;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, e = blockIdx.x;
+    pdl_launch_dependents();
+    float w[8];
+    const int first = tid * 8;
+    if (first < p.w_ld) load8(p.w, (long long)e * p.w_ld, first, (int)p.w_ld, p.w_is_bf16, true, w);      // (weights depend on no earlier launch)
+    pdl_wait();
+    double acc[kFewRows];
+#pragma unroll
+    for (int m = 0; m < kFewRows; ++m) acc[m] = 0.0;
+    for (int k0 = first; k0 < p.w_ld; k0 += kThreads * 8) {
+        if (k0 > first) load8(p.w, (long long)e * p.w_ld, k0, (int)p.w_ld, p.w_is_bf16, true, w);
+#pragma unroll
+        for (int m = 0; m < kFewRows; ++m) {
+            if (m >= p.m) break;
+            float x[8];
+            load8(p.x, m * p.ldx, k0, p.K, p.x_is_bf16, p.x_vec, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[m] = fma((double)w[i], (double)x[i], acc[m]);
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < kFewRows; ++m) {
+        if (m >= p.m) break;
+        double s = acc[m];
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
+        if (lane == 0) part[warp][m] = s;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        if (lane < p.m) {
+            double s = 0.0;
+            for (int v = 0; v < kWarps; ++v) s += part[v][lane];
+            __stcg(p.logits + (long long)lane * p.experts + e, s);
+        }
+        __syncwarp();
+        if (lane == 0) {                     // releases the warp's stores, acquires the other blocks'
+            unsigned old;
+            asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;" : "=r"(old) : "l"(p.count), "r"((unsigned)(p.experts - 1)) : "memory");
+            last = old == (unsigned)(p.experts - 1);
+        }
+    }
+    __syncthreads();
+    if (!last) return;
+    for (int m = warp; m < p.m; m += kWarps) choose_any(p, m, lane, [&](int i) { return __ldcg(p.logits + (long long)m * p.experts + i); });
+}
+
+// ---- more rows: two launches -------------------------------------------------------------------------------
+// A block owns RT x 16 rows and ET x 8 experts, and one of gridDim.z ranges of K (so that every SM has two blocks); its warps split that in
+// turns of 32 and are added up in order.  p.logits: [range][row][expert]
 template <int RT, int ET>
-__global__ void __launch_bounds__(kThreads) router_logits_kernel(const __grid_constant__ RouterRun p) {
+__global__ void __launch_bounds__(kThreads, 2) router_logits_kernel(const __grid_constant__ RouterRun p) {
     __shared__ double part[kWarps][32][4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int row0 = blockIdx.y * 16 * RT, e0 = blockIdx.x * 8 * ET;
@@ -62,8 +187,8 @@ __global__ void __launch_bounds__(kThreads) router_logits_kernel(const __grid_co
         for (int e = 0; e < ET; ++e)
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[r][e][i] = 0.0;
-    const int chunks = (p.K + 31) / 32;
-    for (int c = warp; c < chunks; c += kWarps) {
+    const int chunks = (p.K + 31) / 32, c1 = (int)((long long)chunks * (blockIdx.z + 1) / gridDim.z);
+    for (int c = (int)((long long)chunks * blockIdx.z / gridDim.z) + warp; c < c1; c += kWarps) {
         const int k0 = c * 32 + 8 * t;
         float w[ET][8];
 #pragma unroll
@@ -79,6 +204,7 @@ __global__ void __launch_bounds__(kThreads) router_logits_kernel(const __grid_co
                 for (int e = 0; e < ET; ++e) mma_f64(acc[r][e], x[0][2 * j], x[1][2 * j], x[0][2 * j + 1], x[1][2 * j + 1], w[e][2 * j], w[e][2 * j + 1]);
         }
     }
+    double *logits = p.logits + (long long)blockIdx.z * p.m * p.experts;
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -91,78 +217,31 @@ __global__ void __launch_bounds__(kThreads) router_logits_kernel(const __grid_co
                 double s = 0.0;
                 for (int v = 0; v < kWarps; ++v) s += part[v][l][i];
                 const int row = row0 + 16 * r + (l >> 2) + 8 * (i >> 1), ex = e0 + 8 * e + 2 * (l & 3) + (i & 1);
-                if (row < p.m && ex < p.experts) p.logits[(long long)row * p.experts + ex] = s + (p.logit_bias ? (double)p.logit_bias[ex] : 0.0);
+                if (row < p.m && ex < p.experts) logits[(long long)row * p.experts + ex] = s;
             }
             __syncthreads();
         }
 }
 
-// One warp per row: expert e belongs to lane e % 32.
-template <int PER> __global__ void __launch_bounds__(kThreads) router_choose_kernel(const __grid_constant__ RouterRun p) {
-    const int row = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+// one warp per row
+constexpr int kChooseWarps = 4;
+__global__ void __launch_bounds__(32 * kChooseWarps) router_choose_kernel(const __grid_constant__ RouterRun p) {
+    const int row = blockIdx.x * kChooseWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     pdl_launch_dependents();
     pdl_wait();
     if (row >= p.m) return;
-    constexpr double kMax = 1.7976931348623157e308;
-    double score[PER], key[PER];             // key: what is compared; taken ones and those beyond the last expert fall below all others
-    double top = -kMax;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int e = 32 * i + lane;
-        double l = e < p.experts ? p.logits[(long long)row * p.experts + e] : -kMax;
-        l = isnan(l) ? -kMax : fmin(fmax(l, -kMax), kMax);
-        top = fmax(top, l);
-        score[i] = p.sigmoid ? 1.0 / (1.0 + exp(-l)) : l;
-        double k = score[i] + (p.select_bias && e < p.experts ? (double)p.select_bias[e] : 0.0);
-        key[i] = isnan(k) ? -kMax : fmin(fmax(k, -kMax), kMax);
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    float all = 0.f;                          // softmax over all experts
-    if (!p.sigmoid && !p.normalise) {
-        double s = 0.0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (32 * i + lane < p.experts) s += exp(score[i] - top);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
-        all = (float)s;
-    }
-    unsigned left = 0;                        // experts of this lane that are still to have
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-        if (32 * i + lane < p.experts) left |= 1u << i;
-    float mine = 0.f, sum = 0.f;              // lane j keeps choice j's weight
-    for (int j = 0; j < p.top_k; ++j) {
-        double best = -kMax, s = 0.0;
-        int at = 0x7FFFFFFF;
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (((left >> i) & 1) && (at == 0x7FFFFFFF || key[i] > best)) best = key[i], at = 32 * i + lane, s = score[i];
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-            const double ob = __shfl_xor_sync(0xFFFFFFFFu, best, d), os = __shfl_xor_sync(0xFFFFFFFFu, s, d);
-            const int oa = __shfl_xor_sync(0xFFFFFFFFu, at, d);
-            if (oa != 0x7FFFFFFF && (at == 0x7FFFFFFF || ob > best || (ob == best && oa < at))) best = ob, at = oa, s = os;
-        }
-        if ((at & 31) == lane) left &= ~(1u << (at >> 5));
-        const float v = p.sigmoid ? (float)s : (float)exp(s - top);
-        sum += v;
-        if (lane == j) {
-            mine = v;
-            p.ids[row * p.ld_ids + j] = at;
-        }
-    }
-    if (lane < p.top_k) {
-        const float by = p.normalise ? sum : p.sigmoid ? 1.f : all;
-        p.weights[row * p.ld_weights + lane] = by > 0.f ? mine / by * p.scale : 0.f;
-    }
+    choose_any(p, row, lane, [&](int e) {
+        const double *from = p.logits + (long long)row * p.experts + e;
+        double s = from[0];
+        for (int r = 1; r < p.ranges; ++r) s += from[(long long)r * p.m * p.experts];
+        return s;
+    });
 }
 
-template <typename Kernel> cudaError_t launch(Kernel kern, const RouterRun &p, dim3 grid, cudaStream_t st) {
+template <typename Kernel> cudaError_t launch(Kernel kern, const RouterRun &p, dim3 grid, cudaStream_t st, int threads = kThreads) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -174,16 +253,17 @@ template <typename Kernel> cudaError_t launch(Kernel kern, const RouterRun &p, d
 
 }  // namespace
 
-cudaError_t router_run(const RouterRun &r, int sm_count, cudaStream_t st) {
+cudaError_t router_run(RouterRun r, int sm_count, cudaStream_t st) {
+    if (r.m <= kFewRows) return launch(router_few_kernel, r, dim3((unsigned)r.experts), st);
     const unsigned rows16 = (unsigned)((r.m + 15) / 16), e8 = (unsigned)((r.experts + 7) / 8);
-    // two row tiles and four expert tiles a block where that still gives every SM one: each operand is then converted once for several products
-    cudaError_t e = (rows16 + 1) / 2 * ((e8 + 3) / 4) >= (unsigned)sm_count / 2 ? launch(router_logits_kernel<2, 4>, r, dim3((e8 + 3) / 4, (rows16 + 1) / 2), st)
-                                                                              : launch(router_logits_kernel<1, 1>, r, dim3(e8, rows16), st);
+    // two row tiles and two expert tiles a block where that still gives every SM one: an operand is then converted once for two products
+    const bool large = (rows16 + 1) / 2 * ((e8 + 1) / 2) >= (unsigned)sm_count;
+    dim3 grid = large ? dim3((e8 + 1) / 2, (rows16 + 1) / 2) : dim3(e8, rows16);
+    while (grid.z < kRouterMaxRanges && grid.x * grid.y * grid.z * 2 <= 2 * (unsigned)sm_count && r.K >= 512 * (int)grid.z) grid.z *= 2;
+    r.ranges = (int)grid.z;
+    cudaError_t e = large ? launch(router_logits_kernel<2, 2>, r, grid, st) : launch(router_logits_kernel<1, 1>, r, grid, st);
     if (e != cudaSuccess) return e;
-    const dim3 grid((unsigned)((r.m + kWarps - 1) / kWarps));
-    if (r.experts <= 128) return launch(router_choose_kernel<4>, r, grid, st);
-    if (r.experts <= 256) return launch(router_choose_kernel<8>, r, grid, st);
-    return launch(router_choose_kernel<32>, r, grid, st);
+    return launch(router_choose_kernel, r, dim3((unsigned)((r.m + kChooseWarps - 1) / kChooseWarps)), st, 32 * kChooseWarps);
 }
 
 }  // namespace b200q

@@ -5,7 +5,7 @@
 
 namespace b200q {
 
-constexpr int kRouterMaxExperts = 1024, kRouterMaxTopK = 32;
+constexpr int kRouterMaxExperts = 1024, kRouterMaxTopK = 32, kRouterMaxRanges = 4;
 
 struct RouterRun {
     const void *w;                   // [experts][w_ld], zeros beyond K
@@ -23,9 +23,11 @@ struct RouterRun {
     long long ld_ids;
     float *weights;
     long long ld_weights;
-    double *logits;                  // [m][experts]
+    double *logits;                  // [range of K][m][experts]
+    int ranges;
+    unsigned *count;                 // zero between launches
 };
 
-cudaError_t router_run(const RouterRun &r, int sm_count, cudaStream_t st);
+cudaError_t router_run(RouterRun r, int sm_count, cudaStream_t st);
 
 }  // namespace b200q
