@@ -112,6 +112,8 @@ b200q_status b200q_moe_create(b200q_ctx *ctx, const b200q_moe_config *c, b200q_m
     if (c->n_ff % gguf_block_elems(c->down_type))
         return fail(ctx, B200Q_ERR_INVALID_CONFIG, "n_ff=%lld is not a multiple of the %d-weight block", (long long)c->n_ff, gguf_block_elems(c->down_type));
     if (!c->gate || !c->up || !c->down) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null weight pointer");
+    if (moe_most_steps(MoeShapeInfo{c->n_experts, c->top_k, c->n_embd, c->n_ff, c->max_rows, 0}) > 0x7FFFFFFF)
+        return fail(ctx, B200Q_ERR_INVALID_CONFIG, "expert layer: too many rows for matrices of %lld x %lld", (long long)c->n_ff, (long long)c->n_embd);
     const int64_t elems = (int64_t)c->n_experts * c->n_embd * c->n_ff;
     const int64_t gu = b200q_tensor_storage_bytes(c->gate_up_type, elems), dn = b200q_tensor_storage_bytes(c->down_type, elems);
     if ((int64_t)c->gate_bytes != gu || (int64_t)c->up_bytes != gu || (int64_t)c->down_bytes != dn)

@@ -335,6 +335,11 @@ cudaError_t moe_repack(int qt, const uint8_t *src0, const uint8_t *src1, uint8_t
     return cudaGetLastError();
 }
 
+// Steps (a record of eight tiles) of a product at most: every slot a group of its own
+int64_t moe_most_steps(const MoeShapeInfo &s) {
+    return s.max_rows * s.top_k * std::max(ceil_div(ceil_div(s.n_ff, 8), kMoeWarps) * ceil_div(s.n_embd, SB), ceil_div(ceil_div(s.n_embd, 16), kMoeWarps) * ceil_div(s.n_ff, SB));
+}
+
 // Bytes of the workspace of a layer of up to max_rows rows, and where its parts lie.
 size_t moe_workspace(const MoeShapeInfo &s, MoeBuffers *out, uint8_t *base) {
     const int64_t slots = s.max_rows * s.top_k;

@@ -432,12 +432,15 @@ __device__ __forceinline__ bool moe_last(unsigned *count, int parts, int lane) {
     return last;
 }
 
-// Equal runs of `total` steps for the blocks (of few steps, one each): block b has [begin(b), begin(b + 1))
+// Equal runs of `total` steps for the blocks (of few steps, one each; the first few blocks have one more): block b has [begin(b), begin(b + 1))
 struct MoeShare {
-    long long total, blocks;
-    __device__ __forceinline__ MoeShare(long long steps) : total(steps), blocks(min((long long)gridDim.x, steps)) {}
-    __device__ __forceinline__ long long begin(long long b) const { return b < blocks ? total * b / blocks : total; }
-    __device__ __forceinline__ long long owner(long long step) const { return ((step + 1) * blocks - 1) / total; }
+    int each, more;
+    __device__ __forceinline__ MoeShare(int total) : each(total / (int)gridDim.x), more(total - each * (int)gridDim.x) {}
+    __device__ __forceinline__ int begin(int b) const { return b * each + min(b, more); }
+    __device__ __forceinline__ int owner(int step) const {
+        const int longer = more * (each + 1);
+        return step < longer ? step / (each + 1) : more + (step - longer) / each;
+    }
 };
 
 // A warp's way through the ring
@@ -575,14 +578,14 @@ template <int QT, int P, int NT, typename Finish> __device__ __forceinline__ voi
     __syncthreads();
     const MoeWeights &w = p.weights;
     const int runs = (w.tiles + kMoeWarps - 1) / kMoeWarps, steps = w.nrec;
-    const MoeShare share((long long)*p.lists.ngroups * runs * steps);
-    long long pos = share.begin(blockIdx.x);
-    const long long end = share.begin(blockIdx.x + 1);
+    const MoeShare share(*p.lists.ngroups * runs * steps);
+    int pos = share.begin(blockIdx.x);
+    const int end = share.begin(blockIdx.x + 1);
     MoeRing<D> ring;
     bool full_ring = false;
     for (int s1; pos < end; pos += s1) {
-        const int u = (int)(pos / steps), s0 = (int)(pos - (long long)u * steps), gi = u / runs, tile0 = (u - gi * runs) * kMoeWarps, tile = tile0 + warp;
-        s1 = (int)min((long long)(steps - s0), end - pos);
+        const int u = pos / steps, s0 = pos - u * steps, gi = u / runs, tile0 = (u - gi * runs) * kMoeWarps, tile = tile0 + warp;
+        s1 = min(steps - s0, end - pos);
         if (warp == kMoeWarps) {
             if (!ring.ok) break;
             moe_produce<QT, P, NT, D>(ring, full_ring, head, smem, p, moe_group_word(p, gi, lane), tile0, s0, s1, lane);
@@ -597,15 +600,15 @@ template <int QT, int P, int NT, typename Finish> __device__ __forceinline__ voi
         if (tile >= w.tiles) continue;
         if (s1 < steps) {
             // this block's share: [block][unit that began in an earlier block, unit that goes on in the next][warp]
-            auto part = [&](long long b, int later) { return p.partial + ((b * 2 + later) * kMoeWarps + warp) * kMoePart + lane; };
+            auto part = [&](int b, int later) { return p.partial + ((b * 2 + later) * kMoeWarps + warp) * kMoePart + lane; };
             float *mine = part(blockIdx.x, s0 == 0);
 #pragma unroll
             for (int i = 0; i < NT * 2; ++i) __stcg(mine + i * 32, acc[i >> 1][i & 1]);
-            const long long b0 = share.owner(pos - s0), b1 = share.owner(pos - s0 + steps - 1);
-            if (!moe_last(p.count + b0 * kMoeWarps + warp, (int)(b1 - b0) + 1, lane)) continue;
+            const int b0 = share.owner(pos - s0), b1 = share.owner(pos - s0 + steps - 1);
+            if (!moe_last(p.count + b0 * kMoeWarps + warp, b1 - b0 + 1, lane)) continue;
 #pragma unroll
             for (int i = 0; i < NT * 2; ++i) acc[i >> 1][i & 1] = 0.f;
-            for (long long b = b0; b <= b1; ++b) {
+            for (int b = b0; b <= b1; ++b) {
                 const float *from = part(b, b == b0);
 #pragma unroll
                 for (int i = 0; i < NT * 2; ++i) acc[i >> 1][i & 1] += __ldcg(from + i * 32);
@@ -666,17 +669,17 @@ template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 
     const int groups = *pr.lists.ngroups, runs = (w.tiles + kMoeWarps - 1) / kMoeWarps, steps = w.nrec, m = p.choice.m;
     if (groups == 0)                     // no row has a choice
         for (int i = blockIdx.x * kMoeThreads + tid; i < m * o.n; i += gridDim.x * kMoeThreads) moe_store(o, i / o.n, i % o.n, 0.f);
-    const long long run_steps = (long long)groups * steps;
+    const int run_steps = groups * steps;
     const MoeShare share(run_steps * runs);
-    long long pos = share.begin(blockIdx.x);
-    const long long end = share.begin(blockIdx.x + 1);
+    int pos = share.begin(blockIdx.x);
+    const int end = share.begin(blockIdx.x + 1);
     MoeRing<D> ring;
     bool full_ring = false;
     bool whole = false;                  // the run's first step was this block's
     for (int s1; pos < end; pos += s1) {
-        const int run = (int)(pos / run_steps), gi = (int)((pos - run * run_steps) / steps), s0 = (int)(pos - run * run_steps - (long long)gi * steps);
+        const int run = pos / run_steps, gi = (pos - run * run_steps) / steps, s0 = pos - run * run_steps - gi * steps;
         const int tile0 = run * kMoeWarps, tile = tile0 + warp;
-        s1 = (int)min((long long)(steps - s0), end - pos);
+        s1 = min(steps - s0, end - pos);
         if (warp == kMoeWarps) {
             if (!ring.ok) break;
             moe_produce<QT, P, NT, D>(ring, full_ring, head, smem, pr, moe_group_word(pr, gi, lane), tile0, s0, s1, lane);
@@ -715,20 +718,20 @@ template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 
         if (!last_step && pos + s1 < end) continue;
         // the run ends here, or this block's part of it
         float *own = &outputs[warp][0][0];
-        const long long begin = run * run_steps, b0 = share.owner(begin), b1 = share.owner(begin + run_steps - 1);
-        auto part = [&](long long b, int later) { return pr.partial + ((b * 2 + later) * kMoeWarps + warp) * kMoePart; };
+        const int begin = run * run_steps, b0 = share.owner(begin), b1 = share.owner(begin + run_steps - 1);
+        auto part = [&](int b, int later) { return pr.partial + ((b * 2 + later) * kMoeWarps + warp) * kMoePart; };
         bool mine = true;
         if (b1 > b0) {
             float *to = part(blockIdx.x, whole);
             for (int i = lane; i < m * 16; i += 32) __stcg(to + i, own[i]);
-            mine = moe_last(pr.count + b0 * kMoeWarps + warp, (int)(b1 - b0) + 1, lane);
+            mine = moe_last(pr.count + b0 * kMoeWarps + warp, b1 - b0 + 1, lane);
         }
         if (mine)
             for (int i = lane; i < m * 16; i += 32) {
                 float sum = b1 == b0 ? own[i] : 0.f;
                 if (b1 > b0)
 #pragma unroll 8
-                    for (long long b = b0; b <= b1; ++b) sum += __ldcg(part(b, b == b0) + i);
+                    for (int b = b0; b <= b1; ++b) sum += __ldcg(part(b, b == b0) + i);
                 if (tile * 16 + (i & 15) < o.n && ring.ok) moe_store(o, i >> 4, tile * 16 + (i & 15), sum);
             }
         for (int i = lane; i < m * 16; i += 32) own[i] = 0.f;

@@ -167,6 +167,7 @@ struct MoeRun {
 size_t moe_matrix_bytes(int qt, int64_t experts, int64_t rows, int64_t K, bool paired);
 // GGUF rows [expert][row] in device memory -> records; src1: the up matrix that shares tiles with src0, or null
 cudaError_t moe_repack(int qt, const uint8_t *src0, const uint8_t *src1, uint8_t *dst, int64_t experts, int64_t rows, int64_t K, cudaStream_t st);
+int64_t moe_most_steps(const MoeShapeInfo &s);
 // bytes of a layer's workspace, and its parts from `base` on
 size_t moe_workspace(const MoeShapeInfo &s, MoeBuffers *out, uint8_t *base);
 cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches);

@@ -40,18 +40,19 @@ class Source:
 
 def matrix(t, what: str, device: int, columns: int, dtypes: dict, rows: int | None = None):
     """(pointer, dtype id, leading dimension) of a CUDA tensor [rows, columns] whose rows are contiguous."""
-    if not t.is_cuda or t.device.index != device:
-        raise invalid(f"{what} is on {t.device}, not on cuda:{device}")
-    d = dtypes.get(t.dtype)
-    if d is None:
-        raise invalid(f"{what} is {t.dtype}, not one of {', '.join(map(str, dtypes))}")
-    if t.dim() != 2 or t.shape[1] != columns or (rows is not None and t.shape[0] != rows):
-        raise invalid(f"{what} has shape {tuple(t.shape)}, not ({'rows' if rows is None else rows}, {columns})")
-    m = t.shape[0]
-    if columns > 1 and t.stride(1) != 1:
+    d, shape = dtypes.get(t.dtype), t.shape
+    if d is None or t.get_device() != device or len(shape) != 2 or shape[1] != columns or (rows is not None and shape[0] != rows):
+        if t.get_device() != device:
+            raise invalid(f"{what} is on {t.device}, not on cuda:{device}")
+        if d is None:
+            raise invalid(f"{what} is {t.dtype}, not one of {', '.join(map(str, dtypes))}")
+        raise invalid(f"{what} has shape {tuple(shape)}, not ({'rows' if rows is None else rows}, {columns})")
+    ld, one = t.stride()
+    if one != 1 and columns > 1:
         raise invalid(f"the rows of {what} are not contiguous")
-    ld = t.stride(0) if m > 1 else columns
-    if ld < columns:
+    if shape[0] <= 1:
+        ld = columns
+    elif ld < columns:
         raise invalid(f"the rows of {what} overlap")
     return t.data_ptr(), d, ld
 
