@@ -228,7 +228,9 @@ __device__ void moe_make_lists(const MoePrep &p, MoeSort &m) {
         if ((unsigned)e >= (unsigned)c.experts) continue;
         const int at = m.count[warp][e] + m.place[s], r = at % p.group;
         MoeGroup &g = p.lists.groups[m.groups[e] + at / p.group];
-        g.slot[r] = s;
+        const int row = s / c.top_k;
+        g.slot[r] = s | row << 16;
+        g.weight[r] = c.weights[row * c.ld_weights + s % c.top_k];
         if (r == 0) {
             g.expert = e;
             g.n = min(p.group, m.all[e] - at);
@@ -309,6 +311,9 @@ long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 cudaError_t few_down(int qt, const MoeFewDown &p, int planes, int tiles, int grid, cudaStream_t st) { MOE_BY_TYPE(moe_few_down, p, planes, tiles, grid, st) }
 cudaError_t gate_up_launch(int qt, const MoeGateUp &p, int planes, int tiles, int grid, cudaStream_t st) { MOE_BY_TYPE(moe_gate_up, p, planes, tiles, grid, st) }
 cudaError_t many_down(int qt, const MoeDown &p, int planes, int grid, cudaStream_t st) { MOE_BY_TYPE(moe_down, p, planes, grid, st) }
+size_t one_smem(int qt, int planes, int records) { MOE_BY_TYPE(moe_one_smem, planes, records) }
+cudaError_t one_gate_up(int qt, const MoeOneGateUp &p, int planes, int grid, cudaStream_t st) { MOE_BY_TYPE(moe_one_gate_up, p, planes, grid, st) }
+cudaError_t one_down(int qt, const MoeOneDown &p, int planes, int grid, cudaStream_t st) { MOE_BY_TYPE(moe_one_down, p, planes, grid, st) }
 
 }  // namespace
 
@@ -372,6 +377,12 @@ cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches) {
     const MoeWeights gate_up = weights(r.gate_up, r.gate_up_type, ceil_div(s.n_ff, 8), x_rec), down = weights(r.down, r.down_type, ceil_div(s.n_embd, 16), h_rec);
     MoeRows x = r.x, h{};
     x.nrec = x_rec;
+    // One row whose images lie beside the rings of records in half of an SM's shared memory
+    if (r.choice.m == 1 && one_smem(r.gate_up_type, planes, x_rec) <= kMoeOneSmem && one_smem(r.down_type, planes, (int)s.top_k * h_rec) <= kMoeOneSmem) {
+        *launches = 2;
+        cudaError_t e = one_gate_up(r.gate_up_type, MoeOneGateUp{gate_up, x, r.choice, r.act, r.buf.h, r.status}, planes, grid, st);
+        return e != cudaSuccess ? e : one_down(r.down_type, MoeOneDown{down, r.buf.h, (int)s.n_ff, r.choice, r.out, r.status}, planes, grid, st);
+    }
     h.x = r.buf.h;
     h.ldx = s.n_ff;
     h.vec_ok = s.n_ff % 4 == 0;
@@ -389,19 +400,19 @@ cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches) {
     const unsigned x_grid = 1 + (unsigned)std::min<long long>(ceil_div((long long)r.choice.m * x_rec, warps), spread);
     cudaError_t e = planes == 2 ? launch(moe_prep_kernel<2>, pr, x_grid, kPrepThreads, st, sizeof(MoeSort)) : launch(moe_prep_kernel<4>, pr, x_grid, kPrepThreads, st, sizeof(MoeSort));
     if (e != cudaSuccess) return e;
-    auto product = [&](const MoeWeights &w, const MoeRows &rows, int per_row) {
-        return MoeProduct{w, r.buf.lists, rows.img, rows.img_stride, per_row, r.buf.partial, r.buf.count, r.status};
+    auto product = [&](const MoeWeights &w, const MoeRows &rows, int shift) {
+        return MoeProduct{w, r.buf.lists, rows.img, rows.img_stride, shift, r.buf.partial, r.buf.count, r.status};
     };
-    const MoeGateUp gu{product(gate_up, x, (int)s.top_k), r.act, r.buf.h};
+    const MoeGateUp gu{product(gate_up, x, 16), r.act, r.buf.h};
     if ((e = gate_up_launch(r.gate_up_type, gu, planes, tiles, grid, st)) != cudaSuccess) return e;
     const unsigned h_grid = (unsigned)std::min<long long>(ceil_div((long long)slots * h_rec, 8), 4 * spread);
     if ((e = planes == 2 ? launch(moe_image_kernel<2>, h, h_grid, 256, st) : launch(moe_image_kernel<4>, h, h_grid, 256, st)) != cudaSuccess) return e;
     if (few) {
-        const MoeFewDown d{product(down, h, 1), r.choice, r.out};
+        const MoeFewDown d{product(down, h, 0), r.choice, r.out};
         *launches = 4;
         return few_down(r.down_type, d, planes, tiles, grid, st);
     }
-    const MoeDown d{product(down, h, 1), r.buf.z, ceil_div(s.n_embd, 16) * 16};
+    const MoeDown d{product(down, h, 0), r.buf.z, ceil_div(s.n_embd, 16) * 16};
     if ((e = many_down(r.down_type, d, planes, grid, st)) != cudaSuccess) return e;
     const MoeCombine cb{r.choice, r.out, r.buf.z, d.ld_z};
     *launches = 5;

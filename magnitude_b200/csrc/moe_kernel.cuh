@@ -352,11 +352,11 @@ template <int P, int NT> __device__ __forceinline__ MoeColumns<NT> moe_columns(i
     constexpr int IMG = moe_image_bytes(P);
     const int g = lane >> 2, t = lane & 3;
     MoeColumns<NT> c;
-    const int width = P == 2 && n * P <= 2 ? 2 : n * P <= 4 ? 4 : 8;      // columns of a class
-    c.classes = 8 / width;
-    c.class_b = g / width;
-    c.class_s = 2 * t / width;
-    const int gc = g % width, tc = 2 * t % width;
+    const int lw = P == 2 && n * P <= 2 ? 1 : n * P <= 4 ? 2 : 3, width = 1 << lw;      // columns of a class
+    c.classes = 8 >> lw;
+    c.class_b = g >> lw;
+    c.class_s = 2 * t >> lw;
+    const int gc = g & (width - 1), tc = 2 * t & (width - 1);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         c.b[nt] = min(nt * (8 / P) + gc / P, n - 1) * IMG + (gc % P) * 64 + t * 16;
@@ -443,6 +443,29 @@ struct MoeShare {
     }
 };
 
+// A block's way through its steps: units in turn (inner fastest), `steps` each
+struct MoeWalk {
+    int steps, inners, pos, end, outer, inner, s0;
+    __device__ __forceinline__ MoeWalk(const MoeShare &share, int steps_, int inners_) : steps(steps_), inners(inners_) {
+        pos = share.begin(blockIdx.x);
+        end = share.begin(blockIdx.x + 1);
+        const int u = pos / steps;
+        s0 = pos - u * steps;
+        outer = u / inners;
+        inner = u - outer * inners;
+    }
+    __device__ __forceinline__ bool done() const { return pos >= end; }
+    __device__ __forceinline__ int here() const { return min(steps - s0, end - pos); }       // steps of this unit
+    __device__ __forceinline__ void next(int n) {
+        pos += n;
+        s0 += n;
+        if (s0 == steps) {
+            s0 = 0;
+            if (++inner == inners) inner = 0, ++outer;
+        }
+    }
+};
+
 // A warp's way through the ring
 template <int D> struct MoeRing {
     uint32_t phase = 0;
@@ -504,20 +527,27 @@ __device__ __forceinline__ float moe_activate(const MoeActivation &p, long long 
 }
 
 // ---- the producer ------------------------------------------------------------------------------------
-// One stretch of steps of the producer warp: records from r0 on of a group's rows and of eight tiles from tile0 on.  `word`: lane i holds word i
-// of the group.
+// A lane's two words of a group (lanes 0 .. 16)
+constexpr int kMoeGroupLanes = sizeof(MoeGroup) / 8;
+__device__ __forceinline__ int2 moe_group_words(const MoeProduct &p, int gi, int lane) {
+    return lane < kMoeGroupLanes ? __ldcg(reinterpret_cast<const int2 *>(p.lists.groups + gi) + lane) : make_int2(0, 0);
+}
+// One stretch of steps of the producer warp: records from r0 on of a group's rows and of eight tiles from tile0 on: both, the weights alone, or
+// only the images
+enum { kMoeWeightsAlone = 1, kMoeImagesAlone = 2, kMoeBoth = 3 };
 template <int QT, int P, int NT, int D>
-__device__ __forceinline__ void moe_produce(MoeRing<D> &ring, bool &full_ring, MoeHead &head, uint8_t *smem, const MoeProduct &p, int word, int tile0, int r0, int steps,
-                                            int lane) {
+__device__ __forceinline__ void moe_produce(MoeRing<D> &ring, bool &full_ring, MoeHead &head, uint8_t *smem, const MoeProduct &p, int what, int2 words, int tile0, int r0,
+                                            int steps, int lane) {
     constexpr int REC = moe_rec_bytes(QT), IMG = moe_image_bytes(P), STAGE = moe_stage_bytes(QT, P, NT);
     const MoeWeights &w = p.weights;
-    const int expert = __shfl_sync(0xFFFFFFFFu, word, 0), n = __shfl_sync(0xFFFFFFFFu, word, 1);
-    const int slot = __shfl_sync(0xFFFFFFFFu, word, 2 + lane % kMoeGroupRows);      // of row lane % 16
+    const int expert = __shfl_sync(0xFFFFFFFFu, words.x, 0), n = __shfl_sync(0xFFFFFFFFu, words.y, 0);
+    const int even = __shfl_sync(0xFFFFFFFFu, words.x, 1 + lane % kMoeGroupRows / 2), odd = __shfl_sync(0xFFFFFFFFu, words.y, 1 + lane % kMoeGroupRows / 2);
+    const int row = ((lane & 1 ? odd : even) >> p.shift) & 0xFFFF;      // of the images
     const int tiles = min(kMoeWarps, w.tiles - tile0);
     // lanes 0 .. 7: the record of a tile; lanes 16 .. 31: the image of a row
-    const bool copies = lane < 16 ? lane < tiles : lane - 16 < n;
+    const bool copies = lane < 16 ? (what & kMoeWeightsAlone) && lane < tiles : (what & kMoeImagesAlone) && lane - 16 < n;
     const uint8_t *src = lane < 16 ? w.w + expert * w.expert_bytes + ((long long)(tile0 + lane) * w.nrec + r0) * REC
-                                   : p.img + (size_t)(lane - 16 < n ? slot / p.slots_per_row : 0) * p.img_stride + (size_t)r0 * IMG;
+                                   : p.img + (size_t)(lane - 16 < n ? row : 0) * p.img_stride + (size_t)r0 * IMG;
     const uint32_t at = lane < 16 ? lane * REC : kMoeWarps * REC + (lane - 16) * IMG, size = lane < 16 ? REC : IMG;
     for (int s = 0; s < steps; ++s) {
         if (full_ring) {
@@ -525,10 +555,12 @@ __device__ __forceinline__ void moe_produce(MoeRing<D> &ring, bool &full_ring, M
             if (!ring.ok) return;
         }
         const uint32_t bar = smem_u32(&head.full[ring.stage]);
-        if (lane < (int)(sizeof(MoeGroup) / 4)) reinterpret_cast<int *>(&head.group[ring.stage])[lane] = word;
-        fence_proxy_async();                 // the readers' last accesses precede the copies
-        __syncwarp();
-        if (lane == 0) mbar_expect_tx(bar, tiles * REC + n * IMG);
+        if (what & kMoeWeightsAlone) {
+            if (lane < kMoeGroupLanes) reinterpret_cast<int2 *>(&head.group[ring.stage])[lane] = words;
+            fence_proxy_async();             // the readers' last accesses precede the copies
+            __syncwarp();
+            if (lane == 0) mbar_expect_tx(bar, tiles * REC + n * IMG);
+        }
         __syncwarp();
         if (copies) bulk_g2s(smem_u32(smem + ring.stage * STAGE) + at, src, size, bar);
         src += size;
@@ -536,13 +568,43 @@ __device__ __forceinline__ void moe_produce(MoeRing<D> &ring, bool &full_ring, M
         if (ring.stage == 0) full_ring = true;
     }
 }
-__device__ __forceinline__ int moe_group_word(const MoeProduct &p, int gi, int lane) {
-    return lane < (int)(sizeof(MoeGroup) / 4) ? reinterpret_cast<const int *>(p.lists.groups + gi)[lane] : 0;
+// The producer warp's walk.  Group and eight tiles of a unit: place(walk).  EARLY: the block may have started before the images are there
+// (but not before the lists are): it fills the ring with weights, then waits.
+template <int QT, int P, int NT, int D, bool EARLY, typename Place>
+__device__ __forceinline__ void moe_producer(MoeHead &head, uint8_t *smem, const MoeProduct &p, MoeWalk walk, Place place, int lane) {
+    MoeRing<D> ring;
+    bool full_ring = false;
+    auto pass = [&](int limit, int what) {
+        if (walk.done()) return;
+        int2 words = moe_group_words(p, place(walk).x, lane);
+        while (limit > 0 && !walk.done() && ring.ok) {
+            const int n = min(limit, walk.here());
+            const int2 at = place(walk);
+            const int r0 = walk.s0;
+            walk.next(n);
+            const int2 then = walk.done() ? words : moe_group_words(p, place(walk).x, lane);
+            moe_produce<QT, P, NT, D>(ring, full_ring, head, smem, p, what, words, at.y * kMoeWarps, r0, n, lane);
+            words = then;
+            limit -= n;
+        }
+    };
+    if (EARLY) {
+        const MoeWalk from = walk;
+        pass(D, kMoeWeightsAlone);
+        pdl_wait();
+        walk = from;
+        ring = MoeRing<D>();
+        full_ring = false;
+        pass(D, kMoeImagesAlone);
+    }
+    pass(0x7FFFFFFF, kMoeBoth);
 }
 
 // The group of the ring's next stage as the multiplying warps see it
 template <int NT> struct MoeView {
-    int expert, n, slot[NT];             // slot of the row of the lane's columns in every tile, -1: none
+    int expert, n;
+    int slot[NT], row[NT];               // of the lane's columns in every tile, -1: none
+    float weight[NT];                    // 0: none
 };
 template <int P, int NT, int D>
 __device__ __forceinline__ MoeView<NT> moe_view(MoeRing<D> &ring, MoeHead &head, int *status, int lane, MoeColumns<NT> &col) {
@@ -551,12 +613,15 @@ __device__ __forceinline__ MoeView<NT> moe_view(MoeRing<D> &ring, MoeHead &head,
     MoeView<NT> v;
     v.expert = ring.ok ? grp.expert : 0;
     v.n = ring.ok ? grp.n : 1;
-    const int slot = ring.ok ? grp.slot[lane % kMoeGroupRows] : 0;
     col = moe_columns<P, NT>(v.n, lane);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int r = nt * (8 / P) + col.row, sl = __shfl_sync(0xFFFFFFFFu, slot, max(r, 0));
-        v.slot[nt] = ring.ok && col.row >= 0 && r < v.n ? sl : -1;
+        const int r = nt * (8 / P) + col.row;
+        const bool has = ring.ok && col.row >= 0 && r < v.n;
+        const int slot = has ? grp.slot[r] : -1;
+        v.slot[nt] = has ? slot & 0xFFFF : -1;
+        v.row[nt] = slot >> 16;
+        v.weight[nt] = has ? grp.weight[r] : 0.f;
     }
     return v;
 }
@@ -566,31 +631,30 @@ __device__ __forceinline__ MoeView<NT> moe_view(MoeRing<D> &ring, MoeHead &head,
 // leaves its sums in memory, and the one that is the last to come adds them up in the order of K, so that results do not depend on
 // who that is.
 //   finish(expert, tile, slots, acc): one warp per tile; the lane holds the sums of rows g, g + 8 of slots[nt] (-1: of none)
-template <int QT, int P, int NT, typename Finish> __device__ __forceinline__ void moe_slots(const MoeProduct &p, uint8_t *smem, Finish finish) {
+template <int QT, int P, int NT, bool EARLY, typename Finish> __device__ __forceinline__ void moe_slots(const MoeProduct &p, uint8_t *smem, Finish finish) {
     constexpr int D = moe_depth(QT, P, NT, kMoeSmem), STAGE = moe_stage_bytes(QT, P, NT);
     __shared__ MoeHead head;
     __shared__ __align__(16) uint8_t zero[256 * P];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     moe_ring_init(head, D);
     for (int i = tid; i < 64 * P; i += kMoeThreads) reinterpret_cast<uint32_t *>(zero)[i] = 0u;
-    pdl_launch_dependents();
-    pdl_wait();
+    if (!EARLY) pdl_wait();
+    pdl_launch_dependents();             // (not EARLY: the launch after the next may then read the lists before it waits)
     __syncthreads();
     const MoeWeights &w = p.weights;
     const int runs = (w.tiles + kMoeWarps - 1) / kMoeWarps, steps = w.nrec;
-    const MoeShare share(*p.lists.ngroups * runs * steps);
-    int pos = share.begin(blockIdx.x);
-    const int end = share.begin(blockIdx.x + 1);
+    const MoeShare share(__ldcg(p.lists.ngroups) * runs * steps);
+    MoeWalk walk(share, steps, runs);
+    if (warp == kMoeWarps) {
+        moe_producer<QT, P, NT, D, EARLY>(head, smem, p, walk, [](const MoeWalk &k) { return make_int2(k.outer, k.inner); }, lane);
+        moe_leave(head);
+        return;
+    }
+    if (EARLY) pdl_wait();
     MoeRing<D> ring;
-    bool full_ring = false;
-    for (int s1; pos < end; pos += s1) {
-        const int u = pos / steps, s0 = pos - u * steps, gi = u / runs, tile0 = (u - gi * runs) * kMoeWarps, tile = tile0 + warp;
-        s1 = min(steps - s0, end - pos);
-        if (warp == kMoeWarps) {
-            if (!ring.ok) break;
-            moe_produce<QT, P, NT, D>(ring, full_ring, head, smem, p, moe_group_word(p, gi, lane), tile0, s0, s1, lane);
-            continue;
-        }
+    for (int s1; !walk.done(); walk.next(s1)) {
+        const int pos = walk.pos, s0 = walk.s0, tile = walk.inner * kMoeWarps + warp;
+        s1 = walk.here();
         MoeColumns<NT> col;
         const MoeView<NT> v = moe_view<P, NT, D>(ring, head, p.status, lane, col);
         float acc[NT][2];
@@ -623,7 +687,7 @@ template <int QT, int P, int NT, typename Finish> __device__ __forceinline__ voi
 template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __grid_constant__ MoeGateUp p) {
     extern __shared__ __align__(128) uint8_t smem[];
     const int g = (threadIdx.x & 31) >> 2;
-    moe_slots<QT, P, NT>(p.product, smem, [&](int expert, int tile, const int (&slot)[NT], const float (&acc)[NT][2]) {
+    moe_slots<QT, P, NT, false>(p.product, smem, [&](int expert, int tile, const int (&slot)[NT], const float (&acc)[NT][2]) {
         const int f = tile * 8 + g;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -636,7 +700,7 @@ template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 
 template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(const __grid_constant__ MoeDown p) {
     extern __shared__ __align__(128) uint8_t smem[];
     const int g = (threadIdx.x & 31) >> 2;
-    moe_slots<QT, P, NT>(p.product, smem, [&](int, int tile, const int (&slot)[NT], const float (&acc)[NT][2]) {
+    moe_slots<QT, P, NT, true>(p.product, smem, [&](int, int tile, const int (&slot)[NT], const float (&acc)[NT][2]) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             if (slot[nt] < 0) continue;
@@ -661,41 +725,33 @@ template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 
     for (int i = tid; i < 64 * P; i += kMoeThreads) reinterpret_cast<uint32_t *>(zero)[i] = 0u;
     for (int i = tid; i < kMoeWarps * kMoeFewRows * 16; i += kMoeThreads) (&outputs[0][0][0])[i] = 0.f;
     pdl_launch_dependents();
-    pdl_wait();
     __syncthreads();
     const MoeProduct &pr = p.product;
     const MoeWeights &w = pr.weights;
     const MoeOutput &o = p.out;
-    const int groups = *pr.lists.ngroups, runs = (w.tiles + kMoeWarps - 1) / kMoeWarps, steps = w.nrec, m = p.choice.m;
-    if (groups == 0)                     // no row has a choice
-        for (int i = blockIdx.x * kMoeThreads + tid; i < m * o.n; i += gridDim.x * kMoeThreads) moe_store(o, i / o.n, i % o.n, 0.f);
+    const int groups = __ldcg(pr.lists.ngroups), runs = (w.tiles + kMoeWarps - 1) / kMoeWarps, steps = w.nrec, m = p.choice.m;
     const int run_steps = groups * steps;
     const MoeShare share(run_steps * runs);
-    int pos = share.begin(blockIdx.x);
-    const int end = share.begin(blockIdx.x + 1);
+    MoeWalk walk(share, steps, max(groups, 1));
+    if (warp == kMoeWarps) {
+        moe_producer<QT, P, NT, D, true>(head, smem, pr, walk, [](const MoeWalk &k) { return make_int2(k.inner, k.outer); }, lane);
+        moe_leave(head);
+        return;
+    }
+    pdl_wait();
+    if (groups == 0)                     // no row has a choice
+        for (int i = blockIdx.x * 32 * kMoeWarps + tid; i < m * o.n; i += gridDim.x * 32 * kMoeWarps) moe_store(o, i / o.n, i % o.n, 0.f);
     MoeRing<D> ring;
-    bool full_ring = false;
     bool whole = false;                  // the run's first step was this block's
-    for (int s1; pos < end; pos += s1) {
-        const int run = pos / run_steps, gi = (pos - run * run_steps) / steps, s0 = pos - run * run_steps - gi * steps;
-        const int tile0 = run * kMoeWarps, tile = tile0 + warp;
-        s1 = min(steps - s0, end - pos);
-        if (warp == kMoeWarps) {
-            if (!ring.ok) break;
-            moe_produce<QT, P, NT, D>(ring, full_ring, head, smem, pr, moe_group_word(pr, gi, lane), tile0, s0, s1, lane);
-            continue;
-        }
+    for (int s1; !walk.done(); walk.next(s1)) {
+        const int run = walk.outer, gi = walk.inner, s0 = walk.s0, tile = run * kMoeWarps + warp;
+        s1 = walk.here();
         if (gi == 0 && s0 == 0) whole = true;
         MoeColumns<NT> col;
         const MoeView<NT> v = moe_view<P, NT, D>(ring, head, pr.status, lane, col);
-        float acc[NT][2], weight[NT], bias[2] = {0.f, 0.f};
-        int row[NT];
+        float acc[NT][2], bias[2] = {0.f, 0.f};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            acc[nt][0] = acc[nt][1] = 0.f;
-            row[nt] = v.slot[nt] < 0 ? -1 : v.slot[nt] / p.choice.top_k;
-            weight[nt] = v.slot[nt] < 0 ? 0.f : p.choice.weights[row[nt] * p.choice.ld_weights + v.slot[nt] % p.choice.top_k];
-        }
+        for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = 0.f;
         if (o.bias && s0 == 0)           // (once, with the group's first record)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -707,15 +763,15 @@ template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (t == i && row[nt] >= 0) {
-                    float *out = outputs[warp][row[nt]];
-                    out[g] = fmaf(weight[nt], acc[nt][0] + bias[0], out[g]);
-                    out[g + 8] = fmaf(weight[nt], acc[nt][1] + bias[1], out[g + 8]);
+                if (t == i && v.row[nt] >= 0) {
+                    float *out = outputs[warp][v.row[nt]];
+                    out[g] = fmaf(v.weight[nt], acc[nt][0] + bias[0], out[g]);
+                    out[g + 8] = fmaf(v.weight[nt], acc[nt][1] + bias[1], out[g + 8]);
                 }
                 __syncwarp();
             }
         const bool last_step = gi == groups - 1 && s0 + s1 == steps;
-        if (!last_step && pos + s1 < end) continue;
+        if (!last_step && walk.pos + s1 < walk.end) continue;
         // the run ends here, or this block's part of it
         float *own = &outputs[warp][0][0];
         const int begin = run * run_steps, b0 = share.owner(begin), b1 = share.owner(begin + run_steps - 1);
@@ -741,12 +797,12 @@ template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 
     moe_leave(head);
 }
 
-template <typename Kernel, typename Params> cudaError_t moe_launch(Kernel kern, const Params &p, int grid, size_t smem, cudaStream_t st) {
+template <typename Kernel, typename Params> cudaError_t moe_launch(Kernel kern, const Params &p, int grid, size_t smem, cudaStream_t st, int threads = kMoeThreads) {
     cudaError_t e = configure_smem(reinterpret_cast<const void *>(kern), smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(kMoeThreads);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];

@@ -1,4 +1,5 @@
 // Expert layers: MXFP4 weights.
-#include "moe_kernel.cuh"
+#include "moe_one.cuh"
 
 MOE_INSTANTIATE(mxfp4, QT_MXFP4)
+MOE_ONE_INSTANTIATE(mxfp4, QT_MXFP4)

@@ -47,6 +47,7 @@ constexpr int kMoeManyTiles = 4;         // column tiles of a group of more rows
 // A block's ring: a stage holds eight records and the images of a group's rows.  As many stages (2 to 4) as leave room for two blocks an
 // SM: half of 228 KB each, less 1 KB that a block costs by itself and what it has beside the ring (few rows: 8 KB of outputs).
 constexpr int kMoeSmem = 113664, kMoeFewSmem = 105472, kMoeMaxDepth = 4;
+constexpr int kMoeOneSmem = 112640;      // (the same for one row, less what is beside)
 constexpr int kMoePart = 256;            // floats of a warp's share of a cut unit: two per lane and column tile, or 16 outputs of 16 rows
 __host__ __device__ constexpr int moe_group_rows(int planes, int column_tiles) { return column_tiles * 8 / planes; }
 __host__ __device__ constexpr int moe_stage_bytes(int qt, int planes, int column_tiles) {
@@ -63,8 +64,10 @@ constexpr int kMoeMaxRows = 512, kMoeMaxTopK = 16, kMoeMaxSlots = kMoeMaxRows * 
 constexpr int kMoeGroupRows = 16;
 struct MoeGroup {
     int expert, n;
-    int slot[kMoeGroupRows];             // row * top_k + choice
+    int slot[kMoeGroupRows];             // row * top_k + choice, and the row from bit 16 on
+    float weight[kMoeGroupRows];
 };
+static_assert(kMoeMaxSlots <= 1 << 16 && kMoeMaxRows <= 1 << 15, "a slot and its row in one word");
 
 struct MoeLists {
     int *ngroups;
@@ -113,7 +116,7 @@ struct MoeProduct {
     MoeLists lists;
     const uint8_t *img;                  // images
     unsigned img_stride;                 // bytes of a row's image
-    int slots_per_row;                   // slot / slots_per_row = row of the images
+    int shift;                           // 16: images are the rows', 0: the slots'
     float *partial;                      // [block][2][warp][kMoePart]: shares of cut units
     unsigned *count;                     // [block][warp]: shares seen so far; zero between launches
     int *status;
@@ -132,6 +135,23 @@ struct MoeDown {
     MoeProduct product;
     float *z;                            // [slot][ld_z]
     long long ld_z;
+};
+// one row
+struct MoeOneGateUp {
+    MoeWeights weights;
+    MoeRows x;
+    MoeChoice choice;
+    MoeActivation act;
+    float *h;                            // [choice][ff]
+    int *status;
+};
+struct MoeOneDown {
+    MoeWeights weights;
+    const float *h;
+    int ff;
+    MoeChoice choice;
+    MoeOutput out;
+    int *status;
 };
 // y[m] = sum over the row's choices, in their order
 struct MoeCombine {
@@ -176,6 +196,9 @@ cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches);
     cudaError_t moe_gate_up_##NAME(const MoeGateUp &p, int planes, int tiles, int grid, cudaStream_t st);                 \
     cudaError_t moe_few_down_##NAME(const MoeFewDown &p, int planes, int tiles, int grid, cudaStream_t st);               \
     cudaError_t moe_down_##NAME(const MoeDown &p, int planes, int grid, cudaStream_t st);                                 \
+    size_t moe_one_smem_##NAME(int planes, int records);                                                                  \
+    cudaError_t moe_one_gate_up_##NAME(const MoeOneGateUp &p, int planes, int grid, cudaStream_t st);                     \
+    cudaError_t moe_one_down_##NAME(const MoeOneDown &p, int planes, int grid, cudaStream_t st);                          \
     cudaError_t moe_wait_limit_##NAME(unsigned long long ns);
 MOE_DECLARE(q4_k)
 MOE_DECLARE(q5_k)

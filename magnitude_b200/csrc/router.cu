@@ -135,21 +135,34 @@ __global__ void __launch_bounds__(kThreads) router_few_kernel(const __grid_const
     for (int k0 = first; k0 < p.w_ld; k0 += kThreads * 8) {
         if (k0 > first) load8(p.w, (long long)e * p.w_ld, k0, (int)p.w_ld, p.w_is_bf16, true, w);
 #pragma unroll
-        for (int m = 0; m < kFewRows; ++m) {
+        for (int m = 0; m < kFewRows; m += 4) {       // four rows' loads at once
             if (m >= p.m) break;
-            float x[8];
-            load8(p.x, m * p.ldx, k0, p.K, p.x_is_bf16, p.x_vec, x);
+            float x[4][8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[m] = fma((double)w[i], (double)x[i], acc[m]);
+            for (int r = 0; r < 4; ++r) load8(p.x, (long long)min(m + r, p.m - 1) * p.ldx, k0, p.K, p.x_is_bf16, p.x_vec, x[r]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[m + r] = fma((double)w[i], (double)x[r][i], acc[m + r]);
         }
     }
-#pragma unroll
-    for (int m = 0; m < kFewRows; ++m) {
-        if (m >= p.m) break;
-        double s = acc[m];
+    // Sums over the lanes, always in the same pairs.  Several rows: at every step a lane hands half of its rows to the other one.
+    if (p.m == 1) {
+        double s = acc[0];
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
-        if (lane == 0) part[warp][m] = s;
+        if (lane == 0) part[warp][0] = s;
+    } else {
+#pragma unroll
+        for (int d = 16, n = kFewRows / 2; n > 0; d >>= 1, n >>= 1)
+#pragma unroll
+            for (int i = 0; i < n; ++i) {
+                const bool upper = lane & d;
+                const double give = upper ? acc[i] : acc[i + n], keep = upper ? acc[i + n] : acc[i];
+                acc[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, d);
+            }
+        acc[0] += __shfl_xor_sync(0xFFFFFFFFu, acc[0], 1);
+        if (!(lane & 1)) part[warp][lane >> 1] = acc[0];
     }
     __syncthreads();
     if (warp == 0) {
