@@ -719,8 +719,8 @@ template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ MoeHead head;
     __shared__ __align__(16) uint8_t zero[256 * P];
-    __shared__ float outputs[kMoeWarps][kMoeFewRows][16];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    __shared__ __align__(16) float outputs[kMoeWarps][kMoeFewRows][16];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2;
     moe_ring_init(head, D);
     for (int i = tid; i < 64 * P; i += kMoeThreads) reinterpret_cast<uint32_t *>(zero)[i] = 0u;
     for (int i = tid; i < kMoeWarps * kMoeFewRows * 16; i += kMoeThreads) (&outputs[0][0][0])[i] = 0.f;
@@ -758,12 +758,13 @@ template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 
                 if (tile * 16 + g + 8 * i < o.n) bias[i] = o.bias[(long long)v.expert * o.n + tile * 16 + g + 8 * i];
         moe_multiply<QT, P, NT, D>(ring, head, smem, STAGE, zero, pr.status, s1, v.n, tile < w.tiles, warp, lane, col, acc);
         if (tile >= w.tiles) continue;
-        // one lane group after the other: a row that chose the expert twice has two columns
+        // one column after the other: a row that chose the expert twice has two
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (t == i && v.row[nt] >= 0) {
+            for (int i = 0; i < 8 / P; ++i) {
+                if (nt * (8 / P) + i >= v.n) break;
+                if (col.row == i && v.row[nt] >= 0) {
                     float *out = outputs[warp][v.row[nt]];
                     out[g] = fmaf(v.weight[nt], acc[nt][0] + bias[0], out[g]);
                     out[g + 8] = fmaf(v.weight[nt], acc[nt][1] + bias[1], out[g + 8]);
@@ -779,18 +780,30 @@ template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 
         bool mine = true;
         if (b1 > b0) {
             float *to = part(blockIdx.x, whole);
-            for (int i = lane; i < m * 16; i += 32) __stcg(to + i, own[i]);
+            for (int i = 4 * lane; i < m * 16; i += 128) __stcg(reinterpret_cast<float4 *>(to + i), *reinterpret_cast<const float4 *>(own + i));
             mine = moe_last(pr.count + b0 * kMoeWarps + warp, b1 - b0 + 1, lane);
         }
         if (mine)
-            for (int i = lane; i < m * 16; i += 32) {
-                float sum = b1 == b0 ? own[i] : 0.f;
-                if (b1 > b0)
-#pragma unroll 8
-                    for (int b = b0; b <= b1; ++b) sum += __ldcg(part(b, b == b0) + i);
-                if (tile * 16 + (i & 15) < o.n && ring.ok) moe_store(o, i >> 4, tile * 16 + (i & 15), sum);
+            for (int i = 4 * lane; i < m * 16; i += 128) {
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (b1 == b0) sum = *reinterpret_cast<const float4 *>(own + i);
+                else {
+                    // (eight parts on their way at once: one after the other, some twenty blocks' took a third of the launch)
+#pragma unroll 1
+                    for (int b = b0; b <= b1; b += 8) {
+                        float4 v[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[k] = b + k <= b1 ? __ldcg(reinterpret_cast<const float4 *>(part(b + k, b + k == b0) + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) sum.x += v[k].x, sum.y += v[k].y, sum.z += v[k].z, sum.w += v[k].w;
+                    }
+                }
+                const float out[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (tile * 16 + (i & 15) + k < o.n && ring.ok) moe_store(o, i >> 4, tile * 16 + (i & 15) + k, out[k]);
             }
-        for (int i = lane; i < m * 16; i += 32) own[i] = 0.f;
+        for (int i = 4 * lane; i < m * 16; i += 128) *reinterpret_cast<float4 *>(own + i) = make_float4(0.f, 0.f, 0.f, 0.f);
         __syncwarp();
         whole = false;
     }
