@@ -12,9 +12,12 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <mutex>
+#include <vector>
 
 #include "adapters.h"
 #include "launch.h"
+#include "warp_ring.cuh"
 
 namespace b200q {
 
@@ -22,7 +25,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256, kWarps = 8, kCluster = 8;
+constexpr int kThreads = 256, kWarps = 8, kLogCluster = 3, kCluster = 1 << kLogCluster;
 constexpr int kFewRows = 512;
 
 // D += A (16 x 16 bf16, row) * B (16 x 8 bf16, col)
@@ -58,38 +61,38 @@ template <bool F16, int PLANES> __device__ __forceinline__ void adapter_planes(u
     }
 }
 
-// eight elements of an activation row from k0 on, loaded ahead; zeros beyond K and for missing rows
+// 16 bytes element by element, `left` of them; out of line, since it is rare and long
+template <bool F32> __device__ __noinline__ uint4 load_words(const uint8_t *at, int left) {
+    uint32_t v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (F32) {
+            v[j] = j < left ? reinterpret_cast<const uint32_t *>(at)[j] : 0u;
+        } else {
+            const uint32_t lo = 2 * j < left ? reinterpret_cast<const unsigned short *>(at)[2 * j] : 0u;
+            const uint32_t hi = 2 * j + 1 < left ? reinterpret_cast<const unsigned short *>(at)[2 * j + 1] : 0u;
+            v[j] = lo | hi << 16;
+        }
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// eight elements of an activation row from k0 on, loaded ahead; zeros beyond K.  (The piece of a missing row stays as it was made: zeros.)
 template <bool XF32> struct XPiece {
     uint4 w[XF32 ? 2 : 1];
-    __device__ __forceinline__ void load(const AdaptersParams &p, long long row, int k0, bool wanted) {
+    __device__ __forceinline__ XPiece() {
 #pragma unroll
         for (int i = 0; i < (XF32 ? 2 : 1); ++i) w[i] = make_uint4(0, 0, 0, 0);
-        if (row < 0 || !wanted) return;
-        if (XF32) {
-            const uint32_t *src = reinterpret_cast<const uint32_t *>(p.x) + row * p.ldx + k0;
-            if (p.x_vec && k0 + 8 <= p.K) {
+    }
+    __device__ __forceinline__ void load(const uint8_t *row, int k0, int K, bool vec) {
+        if (!row) return;
+        const uint8_t *at = row + (long long)k0 * (XF32 ? 4 : 2);
+        if (vec && k0 + 8 <= K) {
 #pragma unroll
-                for (int i = 0; i < (XF32 ? 2 : 1); ++i) w[i] = reinterpret_cast<const uint4 *>(src)[i];
-            } else {
-                uint32_t v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = k0 + i < p.K ? src[i] : 0u;
-#pragma unroll
-                for (int i = 0; i < (XF32 ? 2 : 1); ++i) w[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-            }
+            for (int i = 0; i < (XF32 ? 2 : 1); ++i) w[i] = reinterpret_cast<const uint4 *>(at)[i];
         } else {
-            const unsigned short *src = reinterpret_cast<const unsigned short *>(p.x) + row * p.ldx + k0;
-            if (p.x_vec && k0 + 8 <= p.K) {
-                w[0] = *reinterpret_cast<const uint4 *>(src);
-            } else {
-                uint32_t v[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t lo = k0 + 2 * j < p.K ? src[2 * j] : 0u, hi = k0 + 2 * j + 1 < p.K ? src[2 * j + 1] : 0u;
-                    v[j] = lo | hi << 16;
-                }
-                w[0] = make_uint4(v[0], v[1], v[2], v[3]);
-            }
+            for (int i = 0; i < (XF32 ? 2 : 1); ++i) w[i] = load_words<XF32>(at + 16 * i, K - k0 - 4 * i);
         }
     }
     // as planes of four words (pairs of elements)
@@ -136,13 +139,12 @@ template <bool YF32> struct OutputPiece {
     }
 };
 // one output
-template <bool YF32> __device__ __forceinline__ float load_y(const AdapterSet &s, long long row, int n) {
-    if (YF32) return reinterpret_cast<const float *>(s.y)[row * s.ldy + n];
-    return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(s.y)[row * s.ldy + n]);
+template <bool YF32> __device__ __forceinline__ float load_y(const uint8_t *y) {
+    return YF32 ? *reinterpret_cast<const float *>(y) : __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(y));
 }
-template <bool YF32> __device__ __forceinline__ void store_y(const AdapterSet &s, long long row, int n, float v) {
-    if (YF32) reinterpret_cast<float *>(s.y)[row * s.ldy + n] = v;
-    else reinterpret_cast<__nv_bfloat16 *>(s.y)[row * s.ldy + n] = __float2bfloat16_rn(v);
+template <bool YF32> __device__ __forceinline__ void store_y(uint8_t *y, float v) {
+    if (YF32) *reinterpret_cast<float *>(y) = v;
+    else *reinterpret_cast<__nv_bfloat16 *>(y) = __float2bfloat16_rn(v);
 }
 
 // acc += sixteen rows (planes of eight elements of rows g, g + 8) times a fragment of A: 32 of K, eight ranks
@@ -160,43 +162,18 @@ template <bool F16, int PX> __device__ __forceinline__ void multiply_tile(const 
     }
 }
 
-// acc += a piece of t = A x for sixteen rows: tiles of eight ranks, chunks kc, kc + step, .. below kc1.  r0, r1: the lane's rows, -1: none;
-// w(i, kc): the lane's fragment of tile i.
-template <bool F16, bool XF32, int RT, typename Fragment>
-__device__ __forceinline__ void shrink(const AdaptersParams &p, long long r0, long long r1, int kc, int kc1, int step, int tiles, int t, Fragment fragment, float (&acc)[RT][4]) {
-    constexpr int PX = XF32 ? 3 : 1;
-    XPiece<XF32> x0, x1;                     // the next chunk's, on their way
-    x0.load(p, r0, kc * 32 + 8 * t, kc < kc1);
-    x1.load(p, r1, kc * 32 + 8 * t, kc < kc1);
-    for (; kc < kc1; kc += step) {
-        uint32_t f0[PX][4], f1[PX][4];
-        x0.planes(f0);
-        x1.planes(f1);
-        uint4 w[RT];
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-            if (i < tiles) w[i] = fragment(i, kc);
-        x0.load(p, r0, (kc + step) * 32 + 8 * t, kc + step < kc1);
-        x1.load(p, r1, (kc + step) * 32 + 8 * t, kc + step < kc1);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            if (i >= tiles) break;
-            multiply_tile<F16, PX>(f0, f1, w[i], acc[i]);
-        }
-    }
-}
-
-// B t of sixteen rows and a chunk of 32 outputs: acc of column tile i: rows g, g + 8, outputs 8 t + 2 i, + 1.  bp: the lane's fragments of the
-// chunk, fp: of the rows' t
-template <bool F16, int PT> __device__ __forceinline__ void expand(const uint4 *bp, const uint4 *fp, int rk, float (&acc)[4][4]) {
+// B t of sixteen rows and a chunk of 32 outputs: acc of column tile i: rows g, g + 8, outputs 8 t + 2 i, + 1.  fragments(k, w): the lane's two
+// of rank tile k, fp: of the rows' t
+template <bool F16, int PT, typename Fragments> __device__ __forceinline__ void expand(Fragments fragments, const uint4 *fp, int rk, float (&acc)[4][4]) {
     constexpr int PA = F16 ? 2 : 1;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-#pragma unroll 2
-    for (int k = 0; k < rk; ++k, bp += 64, fp += PT * 32) {
-        const uint4 w[2] = {bp[0], bp[32]};
+#pragma unroll 1
+    for (int k = 0; k < rk; ++k, fp += PT * 32) {
+        uint4 w[2];
+        fragments(k, w);
         uint4 f[PT];
 #pragma unroll
         for (int q = 0; q < PT; ++q) f[q] = fp[q * 32];
@@ -212,13 +189,44 @@ template <bool F16, int PT> __device__ __forceinline__ void expand(const uint4 *
         }
     }
 }
+template <bool F16, int PT> __device__ __forceinline__ void expand(const uint4 *bp, const uint4 *fp, int rk, float (&acc)[4][4]) {
+    expand<F16, PT>([&](int k, uint4(&w)[2]) { w[0] = bp[k * 64], w[1] = bp[k * 64 + 32]; }, fp, rk, acc);
+}
+
+// Outputs that are not aligned: a row's 32 by 32 lanes, sixteen rows
+template <bool YF32> struct OutputColumn {
+    float v[16];
+    // to[16]: where the rows begin in y, in bytes, -1: there is none
+    __device__ __forceinline__ void load(const AdapterSet &s, const long long *to, int n) {
+        const uint8_t *y = reinterpret_cast<const uint8_t *>(s.y) + (long long)n * (YF32 ? 4 : 2);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) v[r] = n < s.n && to[r] >= 0 ? load_y<YF32>(y + to[r]) : 0.f;
+    }
+    // += scale * acc, which goes through the warp's piece of shared memory (16 x kTileLd floats)
+    __device__ __forceinline__ void add(const AdapterSet &s, const long long *to, int n, float scale, const float (&acc)[4][4], float *piece, int lane) const;
+};
+constexpr int kTileLd = 33;
+template <bool YF32>
+__device__ __forceinline__ void OutputColumn<YF32>::add(const AdapterSet &s, const long long *to, int n, float scale, const float (&acc)[4][4], float *piece, int lane) const {
+    const int g = lane >> 2, t = lane & 3;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) piece[(g + 8 * (j >> 1)) * kTileLd + 8 * t + 2 * i + (j & 1)] = acc[i][j];
+    __syncwarp();
+    uint8_t *y = reinterpret_cast<uint8_t *>(s.y) + (long long)n * (YF32 ? 4 : 2);
+    if (n < s.n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            if (to[r] >= 0) store_y<YF32>(y + to[r], fmaf(scale, piece[r * kTileLd + lane], v[r]));
+}
 
 // y of sixteen rows += scale B t over the chunks nc, nc + step, .. below nc1, CH neighbouring ones at a time.  row[16]: the rows, -1: none;
 // piece: 16 x kTileLd floats of the warp
-constexpr int kTileLd = 33;
 template <bool F16, bool YF32, int CH>
-__device__ __forceinline__ void add_chunks(const AdapterSet &s, const uint4 *b, const uint4 *frag, int rk, float scale, const int *row, int nc, int nc1, int step, float *piece,
-                                           int lane) {
+__device__ __forceinline__ void add_chunks(const AdapterSet &s, const uint4 *b, const uint4 *frag, int rk, float scale, const int *row, const long long *row_at, int nc, int nc1, int step,
+                                           float *piece, int lane) {
     constexpr int PT = YF32 ? 3 : 2, YB = YF32 ? 4 : 2;
     const int g = lane >> 2, t = lane & 3;
     if (s.y_vec) {
@@ -247,28 +255,15 @@ __device__ __forceinline__ void add_chunks(const AdapterSet &s, const uint4 *b, 
             to[1] += step * 32 * YB;
         }
     }
-    // rows that are not aligned, the last outputs: a row's 32 by 32 lanes
+    // rows that are not aligned, the last outputs
     for (; nc < nc1; nc += step)
 #pragma unroll 1
         for (int c = nc; c < min(nc + CH, nc1); ++c) {
+            OutputColumn<YF32> y;
+            y.load(s, row_at, c * 32 + lane);
             float acc[4][4];
             expand<F16, PT>(b + (size_t)c * rk * 64 + lane, frag + lane, rk, acc);
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) piece[(g + 8 * (j >> 1)) * kTileLd + 8 * t + 2 * i + (j & 1)] = acc[i][j];
-            __syncwarp();
-            if (c * 32 + lane < s.n)
-#pragma unroll
-                for (int r0 = 0; r0 < 16; r0 += 8) {         // eight loads, then eight stores
-                    float old[8];
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) old[r] = row[r0 + r] >= 0 ? load_y<YF32>(s, row[r0 + r], c * 32 + lane) : 0.f;
-#pragma unroll
-                    for (int r = 0; r < 8; ++r)
-                        if (row[r0 + r] >= 0) store_y<YF32>(s, row[r0 + r], c * 32 + lane, fmaf(scale, piece[(r0 + r) * kTileLd + lane], old[r]));
-                }
+            y.add(s, row_at, c * 32 + lane, scale, acc, piece, lane);
         }
 }
 
@@ -280,16 +275,21 @@ __device__ __forceinline__ bool active(const AdapterSet &s, int slot) { return (
 // The rows by adapter: groups of up to sixteen, adapters in the order of their first rows.  Warp w owns rows 64 w .. 64 w + 63.
 constexpr int kKeys = 2 * kFewRows;
 struct FewRows {
-    int slot[kFewRows];
-    int key[kKeys];                                  // a table of the slots that occur: open addressing
-    int first_row[kKeys];                            // of every key
-    short row_base[kKeys], group_base[kKeys];        // where its rows, its groups begin
-    uint8_t count[kWarps][kKeys];                    // its rows in every warp
+    __align__(16) int slot[kFewRows];
     short sorted[kFewRows], first[kFewRows + 1];     // rows of group i: sorted[first[i]] .. sorted[first[i + 1] - 1]
     int2 sums[kWarps];
     int n;
+    int item, log_parts;                             // this block's
+    int part_sums[4][kWarps];
+    unsigned long long class_sums[kWarps];
 };
-__device__ __forceinline__ void few_groups(FewRows &l, const AdaptersParams &p) {
+struct FewTables {                                   // while they are made
+    int key[kKeys];                                  // the slots that occur: open addressing
+    int first_row[kKeys];                            // of every key
+    short row_base[kKeys], group_base[kKeys];        // where its rows, its groups begin
+    uint8_t count[kWarps][kKeys];                    // its rows in every warp
+};
+__device__ __forceinline__ void few_groups(FewRows &l, FewTables &m, const AdaptersParams &p) {
     static_assert(kFewRows == 64 * kWarps, "rows of a warp");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (p.m == 1) {                                  // nothing to sort
@@ -302,52 +302,84 @@ __device__ __forceinline__ void few_groups(FewRows &l, const AdaptersParams &p) 
         __syncthreads();
         return;
     }
-    for (int i = tid; i < kKeys; i += kThreads) {
-        l.key[i] = -1;
-        l.first_row[i] = kFewRows;
-    }
-    for (int i = tid; i < kWarps * kKeys / 4; i += kThreads) reinterpret_cast<uint32_t *>(l.count)[i] = 0u;
-    __syncthreads();
-    int at[2], rank[2];                              // key and place among the warp's rows of the same slot
+    int at[2], rank[2], all[2] = {0, 0};             // key, place among the rows of the same slot, those rows
+    bool begins[2];                                  // the first of them
+    int index[2] = {warp * 64 + lane, warp * 64 + 32 + lane};        // this thread's rows
+    if (p.m <= 64) {                                 // a thread a row, which looks at all of them; the key is the first row
+        index[0] = tid;
+        at[0] = at[1] = -1;
+        rank[0] = rank[1] = 0;
+        begins[0] = begins[1] = false;
+        if (tid < 64) l.slot[tid] = tid < p.m ? p.rows[tid] : -1;
+        __syncthreads();
+        if (tid < 64) {
+            const int slot = l.slot[tid];
+            int first = 64;
+#pragma unroll 4
+            for (int q = 0; q < p.m; q += 4) {       // (rows beyond the last are -1)
+                const int4 v = *reinterpret_cast<const int4 *>(l.slot + q);
+                const int o[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int i = warp * 64 + h * 32 + lane, slot = i < p.m ? p.rows[i] : -1;
-        l.slot[i] = slot;
-        at[h] = -1;
-        if (slot >= 0) {
-            int k = (int)(((unsigned)slot * 2654435761u) >> 22);      // (Fibonacci hashing: the upper ten bits)
-            while (true) {
-                const int old = atomicCAS(&l.key[k], -1, slot);
-                if (old == -1 || old == slot) break;
-                k = (k + 1) & (kKeys - 1);
+                for (int j = 0; j < 4; ++j) {
+                    const bool same = o[j] == slot;
+                    first = same ? min(first, q + j) : first;
+                    all[0] += same;
+                    rank[0] += same && q + j < tid;
+                }
             }
-            at[h] = k;
-            atomicMin(&l.first_row[k], i);
+            if (slot >= 0) {
+                at[0] = first;
+                begins[0] = first == tid;
+            }
         }
-        __syncwarp();
-        const unsigned same = __match_any_sync(0xFFFFFFFFu, at[h]);
-        const int before = at[h] >= 0 ? l.count[warp][at[h]] : 0;
-        rank[h] = before + __popc(same & ((1u << lane) - 1));
-        __syncwarp();
-        if (at[h] >= 0 && (same >> lane) == 1u) l.count[warp][at[h]] = (uint8_t)(rank[h] + 1);      // the last lane of those
-        __syncwarp();
+    } else {
+        for (int i = tid; i < kKeys; i += kThreads) {
+            m.key[i] = -1;
+            m.first_row[i] = kFewRows;
+        }
+        for (int i = tid; i < kWarps * kKeys / 4; i += kThreads) reinterpret_cast<uint32_t *>(m.count)[i] = 0u;
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int i = index[h], slot = i < p.m ? p.rows[i] : -1;
+            l.slot[i] = slot;
+            at[h] = -1;
+            if (slot >= 0) {
+                int k = (int)(((unsigned)slot * 2654435761u) >> 22);      // (Fibonacci hashing: the upper ten bits)
+                while (true) {
+                    const int old = atomicCAS(&m.key[k], -1, slot);
+                    if (old == -1 || old == slot) break;
+                    k = (k + 1) & (kKeys - 1);
+                }
+                at[h] = k;
+                atomicMin(&m.first_row[k], i);
+            }
+            __syncwarp();
+            const unsigned same = __match_any_sync(0xFFFFFFFFu, at[h]);
+            const int before = at[h] >= 0 ? m.count[warp][at[h]] : 0;
+            rank[h] = before + __popc(same & ((1u << lane) - 1));
+            __syncwarp();
+            if (at[h] >= 0 && (same >> lane) == 1u) m.count[warp][at[h]] = (uint8_t)(rank[h] + 1);      // the last lane of those
+            __syncwarp();
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            int before = 0;
+            if (at[h] >= 0)
+                for (int w = 0; w < kWarps; ++w) {
+                    const int n = m.count[w][at[h]];
+                    all[h] += n;
+                    before += w < warp ? n : 0;
+                }
+            rank[h] += before;
+            begins[h] = at[h] >= 0 && m.first_row[at[h]] == index[h];
+        }
     }
-    __syncthreads();
-    int all[2];
     int2 mine = make_int2(0, 0), run[2];             // rows and groups that begin with this thread's rows
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        all[h] = 0;
-        int before = 0;
-        if (at[h] >= 0)
-            for (int w = 0; w < kWarps; ++w) {
-                const int n = l.count[w][at[h]];
-                all[h] += n;
-                before += w < warp ? n : 0;
-            }
-        rank[h] += before;
-        const bool begins = at[h] >= 0 && l.first_row[at[h]] == warp * 64 + h * 32 + lane;
-        run[h] = begins ? make_int2(all[h], (all[h] + 15) / 16) : make_int2(0, 0);
+        run[h] = begins[h] ? make_int2(all[h], (all[h] + 15) / 16) : make_int2(0, 0);
         const int2 own = run[h];
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
@@ -367,56 +399,154 @@ __device__ __forceinline__ void few_groups(FewRows &l, const AdaptersParams &p) 
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-        if (at[h] >= 0 && l.first_row[at[h]] == warp * 64 + h * 32 + lane) {
-            l.row_base[at[h]] = (short)(base.x + run[h].x);
-            l.group_base[at[h]] = (short)(base.y + run[h].y);
+        if (begins[h]) {
+            m.row_base[at[h]] = (short)(base.x + run[h].x);
+            m.group_base[at[h]] = (short)(base.y + run[h].y);
         }
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < 2; ++h)
         if (at[h] >= 0) {
-            const int to = l.row_base[at[h]] + rank[h];
-            l.sorted[to] = (short)(warp * 64 + h * 32 + lane);
-            if (rank[h] % 16 == 0) l.first[l.group_base[at[h]] + rank[h] / 16] = (short)to;
+            const int to = m.row_base[at[h]] + rank[h];
+            l.sorted[to] = (short)index[h];
+            if (rank[h] % 16 == 0) l.first[m.group_base[at[h]] + rank[h] / 16] = (short)to;
         }
     if (tid == 0) {
         l.n = total.y;
         l.first[total.y] = (short)total.x;
     }
+    fence_proxy_async();                             // copies come to where the tables are
     __syncthreads();
 }
 
-// Shared memory beside the rows: the warps' sums of a rank block (later a 16 x 32 piece of outputs each), this block's t, t as fragments
-constexpr int kFewRanks = 32;                        // ranks whose sums a warp holds at a time
-constexpr size_t kFewSums = size_t(kWarps) * 16 * kTileLd * 4;
-static_assert(kFewSums >= size_t(kWarps) * 16 * kFewRanks * 4, "sums");
-size_t few_smem(int rank_pad, int planes) { return kFewSums + size_t(16) * rank_pad * 4 + size_t(rank_pad / 16) * planes * 512; }
-
-// the block's threads ask for a piece of memory, 128 bytes each and turn (at most 64 KB)
-__device__ __forceinline__ void prefetch_bytes(const uint8_t *p, long long bytes) {
-    for (int i = threadIdx.x * 128; i < min(bytes, 65536ll); i += kThreads * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
+// One item or none for every block: rows.item, rows.log_parts.  items: no more than blocks, and than kMostShares
+constexpr int kMostShares = 2 * kThreads;
+__device__ __forceinline__ void few_shares(FewRows &l, const AdaptersParams &p, int items, int y_bytes) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grid = (int)gridDim.x;
+    if (tid == 0) l.item = items, l.log_parts = 0;   // none
+    // an item's bytes in units of 512: A, B and twice its outputs.  Thread i has items i and i + kThreads
+    int cost[2] = {0, 0};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = h * kThreads + tid;
+        if (i >= items) continue;
+        const int group = i / p.sets, first = l.first[group];
+        const AdapterSet &s = p.set[i - group * p.sets];
+        const int slot = l.slot[l.sorted[first]], rank = (unsigned)slot < (unsigned)s.slots ? s.rank[slot] : 0;
+        if (rank > 0) cost[h] = (rank + 7) / 8 * p.kchunks + (rank + 15) / 16 * 2 * s.nchunks + (l.first[group + 1] - first) * s.nchunks * y_bytes / 8;
+    }
+    auto add = [&](int v, int at) {                  // towards the block's sum
+        v = __reduce_add_sync(0xFFFFFFFFu, v);
+        if (lane == 0) l.part_sums[at][warp] = v;
+    };
+    auto sum = [&](int at) {
+        int v = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) v += l.part_sums[at][w];
+        return v;
+    };
+    add((cost[0] >> 4) + (cost[1] >> 4), 3);         // (512 items of ranks of 256 and 2^17 outputs stay below 2^31)
+    __syncthreads();
+    const float per_cost = 0.0625f / (float)(sum(3) + 1);
+    // blocks of an item: its part of `share` blocks, at least one, rounded down to a power of two; the largest of four shares that fits
+    auto parts_of = [&](int c, int share) {
+        const float n = (float)c * per_cost * (float)share;
+        return n >= 8.f ? 3 : n >= 4.f ? 2 : n >= 2.f ? 1 : 0;
+    };
+    auto share_of = [&](int k) { return k == 0 ? 2 * grid : k == 1 ? grid + grid / 2 : k == 2 ? grid : grid - items; };      // (the last one always fits)
+#pragma unroll
+    for (int q = 0; q < 3; ++q) add((cost[0] ? 1 << parts_of(cost[0], share_of(q)) : 0) + (cost[1] ? 1 << parts_of(cost[1], share_of(q)) : 0), q);
+    __syncthreads();
+    int share = share_of(3);
+#pragma unroll
+    for (int q = 2; q >= 0; --q)
+        if (sum(q) <= grid) share = share_of(q);
+    // the items of eight blocks first, then those of four, .. : an item begins at a multiple of its blocks
+    const int log[2] = {parts_of(cost[0], share), parts_of(cost[1], share)};
+    const unsigned long long own[2] = {cost[0] ? 1ull << (16 * log[0]) : 0ull, cost[1] ? 1ull << (16 * log[1]) : 0ull};      // items of every class, 16 bits each
+    unsigned long long scan = own[0] + own[1];
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const unsigned long long x = __shfl_up_sync(0xFFFFFFFFu, scan, d);
+        if (lane >= d) scan += x;
+    }
+    if (lane == 31) l.class_sums[warp] = scan;
+    __syncthreads();
+    unsigned long long before = scan - own[0] - own[1], all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        const unsigned long long x = l.class_sums[w];
+        all += x;
+        before += w < warp ? x : 0ull;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (cost[h]) {
+            int start = (int)(before >> (16 * log[h]) & 0xFFFF) << log[h];
+#pragma unroll
+            for (int c = 1; c <= kLogCluster; ++c)
+                if (c > log[h]) start += (int)(all >> (16 * c) & 0xFFFF) << c;
+            if ((int)blockIdx.x >= start && (int)blockIdx.x < start + (1 << log[h])) l.item = h * kThreads + tid, l.log_parts = log[h];
+        }
+        before += own[h];
+    }
+    __syncthreads();
 }
 
-// one adapter against up to sixteen rows
+// Shared memory: the warps' rings, the warps' sums of a rank block (later a 16 x 32 piece of outputs each), this block's t, t as fragments
+constexpr int kFewPiece = 4096, kFewDepth = 2;
+__host__ __device__ constexpr int few_tiles(bool x_f32) { return x_f32 ? 4 : 8; }        // tiles of eight ranks whose sums a warp holds at a time
+constexpr size_t kFewRing = size_t(kWarps) * kFewDepth * kFewPiece;
+static_assert(sizeof(FewTables) <= kFewRing, "tables");
+__host__ __device__ constexpr size_t few_sums(bool x_f32) { return size_t(kWarps) * 16 * (8 * few_tiles(x_f32) + 2) * 4; }
+static_assert(few_sums(true) >= size_t(kWarps) * 16 * kTileLd * 4, "a piece of outputs");
+size_t few_smem(int rank_pad, int planes, bool x_f32) { return kFewRing + few_sums(x_f32) + size_t(16) * rank_pad * 4 + size_t(rank_pad / 16) * planes * 512; }
+
+// One adapter against up to sixteen rows.  A warp takes neighbouring chunks of K, then of N; the fragments of A and then of B come through its ring in
+// pieces of 4 KB (of a small rank, those of several chunks), so that B is on its way while t is joined; rows of x are asked for two chunks ahead,
+// rows of y one.  What a step costs is the instructions of one warp after the other, more than their number: hence few and large pieces, and
+// buffers that take turns (a copy from one to the other would wait for the load).
 template <bool F16, bool XF32, bool YF32>
-__device__ __forceinline__ void few_pass(const AdaptersParams &p, const AdapterSet &s, int slot, const int *row, int parts, uint8_t *smem) {
-    constexpr int PT = YF32 ? 3 : 2, RT = kFewRanks / 8;
+__device__ __forceinline__ void few_pass(const AdaptersParams &p, const AdapterSet &s, int slot, const int *row, const long long *row_at, int log_parts, uint8_t *memory, WarpRing<kFewDepth> &ring,
+                                         volatile int *fail) {
+    constexpr int PT = YF32 ? 3 : 2, PX = XF32 ? 3 : 1, RT = few_tiles(XF32), SUM_LD = 8 * RT + 2, XB = XF32 ? 4 : 2, YB = YF32 ? 4 : 2;
     cg::cluster_group cluster = cg::this_cluster();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int block = (int)cluster.block_rank(), part = block & (parts - 1), lead = block - part;
+    const int parts = 1 << log_parts, block = (int)cluster.block_rank(), part = block & (parts - 1), lead = block - part;
     const int rank = slot < 0 ? 0 : s.rank[slot], rt = (rank + 7) / 8, rk = (rank + 15) / 16, rank_pad = 16 * rk;
+    uint8_t *smem = memory + kFewRing;
     float *sums = reinterpret_cast<float *>(smem);
-    float *tpart = reinterpret_cast<float *>(smem + kFewSums);
-    uint4 *frag = reinterpret_cast<uint4 *>(smem + kFewSums + (size_t)16 * p.rank_pad * 4);
+    float *tpart = reinterpret_cast<float *>(smem + few_sums(XF32));
+    uint4 *frag = reinterpret_cast<uint4 *>(smem + few_sums(XF32) + (size_t)16 * p.rank_pad * 4);
     const float scale = slot < 0 ? 0.f : s.scale[slot];
-    const uint4 *a = reinterpret_cast<const uint4 *>(s.a + slot * s.a_stride), *b = reinterpret_cast<const uint4 *>(s.b + slot * s.b_stride);
-    const int nc0 = (int)((long long)s.nchunks * part / parts), nc1 = slot < 0 ? nc0 : (int)((long long)s.nchunks * (part + 1) / parts);
-    const int kc0 = (int)((long long)p.kchunks * part / parts), kc1 = (int)((long long)p.kchunks * (part + 1) / parts);
-    // the block's parts of A (what is not read at once) and B all start their way
-    prefetch_bytes(reinterpret_cast<const uint8_t *>(a) + (long long)(kc0 + kWarps) * rt * 512, (long long)(kc1 - kc0 - kWarps) * rt * 512);
-    prefetch_bytes(reinterpret_cast<const uint8_t *>(b) + (long long)nc0 * rk * 1024, (long long)(nc1 - nc0) * rk * 1024);
+    // the warp's chunks: of the block's part an eighth
+    auto share = [&](int all, int w) { return (int)((long long)all * (part * kWarps + w) >> (log_parts + 3)); };
+    static_assert(kWarps == 8, "an eighth");
+    const int kc0 = share(p.kchunks, warp), kc1 = share(p.kchunks, warp + 1), nc0 = share(s.nchunks, warp), nc1 = slot < 0 ? nc0 : share(s.nchunks, warp + 1);
+    // chunks of a piece: of A where all rank tiles' sums are held at once, of B where its rank tiles fit
+    const int a_chunks = rt > 0 && rt <= RT ? kFewPiece / 512 / rt : 1, b_chunks = rk > 0 && rk <= kFewPiece / 1024 ? kFewPiece / 1024 / rk : 1;
+    // fetched next: of A chunk fa, tiles from fr on; then of B chunk fn, tiles from fk on
+    int fa = kc0, fr = 0, fn = nc0, fk = 0;
+    bool in_a = rt > 0 && kc0 < kc1;
+    auto fetch = [&]() {
+        if (in_a) {
+            const int n = min(a_chunks, kc1 - fa), tiles = min(rt - fr, RT);
+            ring.fill(s.a + slot * s.a_stride + ((long long)fa * rt + fr) * 512, n * tiles * 512, lane);
+            fa += n;
+            if (fa == kc1) fa = kc0, fr += RT, in_a = fr < rt;
+        } else if (fn < nc1) {
+            const int n = min(b_chunks, nc1 - fn), tiles = min(rk - fk, kFewPiece / 1024);
+            ring.fill(s.b + slot * s.b_stride + ((long long)fn * rk + fk) * 1024, n * tiles * 1024, lane);
+            fk += tiles;
+            if (fk == rk) fk = 0, fn += n;
+        }
+    };
+    for (int i = 0; i < kFewDepth; ++i) fetch();
 
     // ---- t = A x over this block's part of K
+    const uint8_t *xr[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) xr[h] = row[g + 8 * h] < 0 ? nullptr : reinterpret_cast<const uint8_t *>(p.x) + row[g + 8 * h] * p.ldx * XB;
     for (int rb = 0; rb < rt; rb += RT) {
         const int tiles = min(rt - rb, RT);
         float acc[RT][4];
@@ -424,22 +554,51 @@ __device__ __forceinline__ void few_pass(const AdaptersParams &p, const AdapterS
         for (int i = 0; i < RT; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-        shrink<F16, XF32, RT>(p, row[g], row[g + 8], kc0 + warp, kc1, kWarps, tiles, t, [&](int i, int kc) { return a[((size_t)kc * rt + rb + i) * 32 + lane]; }, acc);
+        XPiece<XF32> x[2];
+        int left = 0;                        // chunks of the piece
+        uint32_t w = 0;
+#pragma unroll 1
+        for (int kc = kc0 - 1; kc < kc1; ++kc) {       // (before the first chunk: its load)
+            uint32_t f[2][PX][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) x[h].planes(f[h]);
+            if (kc + 1 < kc1)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) x[h].load(xr[h], (kc + 1) * 32 + 8 * t, p.K, p.x_vec);
+            if (kc < kc0) continue;
+            if (left == 0) {
+                ring.wait(fail, p.status);
+                w = ring.at + ring.stage * kFewPiece + lane * 16;
+                left = min(a_chunks, kc1 - kc);
+            }
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                if (i >= tiles) break;
+                multiply_tile<F16, PX>(f[0], f[1], lds128(w + i * 512), acc[i]);
+            }
+            w += tiles * 512;
+            if (--left == 0) {
+                __syncwarp();
+                fetch();
+                ring.next();
+            }
+        }
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             if (i >= tiles) break;
-            float *dst = sums + (warp * 16 + g) * kFewRanks + 8 * i + 2 * t;
+            float *dst = sums + (warp * 16 + g) * SUM_LD + 8 * i + 2 * t;
             *reinterpret_cast<float2 *>(dst) = make_float2(acc[i][0], acc[i][1]);
-            *reinterpret_cast<float2 *>(dst + 8 * kFewRanks) = make_float2(acc[i][2], acc[i][3]);
+            *reinterpret_cast<float2 *>(dst + 8 * SUM_LD) = make_float2(acc[i][2], acc[i][3]);
         }
         __syncthreads();
-        const int width = min(rank_pad - 8 * rb, kFewRanks);        // the last tile of 16 may be half there
-        for (int i = threadIdx.x; i < 16 * width; i += kThreads) {
-            const int r = i / width, c = i - r * width;
+        // a row a half warp
+        const int width = min(rank_pad - 8 * rb, 8 * RT);        // the last tile of 16 may be half there
+        for (int c = threadIdx.x & 15; c < width; c += 16) {
+            const int r = threadIdx.x >> 4;
             float v = 0.f;
             if (c < 8 * tiles)
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) v += sums[(w * 16 + r) * kFewRanks + c];
+                for (int q = 0; q < kWarps; ++q) v += sums[(q * 16 + r) * SUM_LD + c];
             tpart[r * rank_pad + 8 * rb + c] = v;
         }
         __syncthreads();
@@ -447,29 +606,87 @@ __device__ __forceinline__ void few_pass(const AdaptersParams &p, const AdapterS
     cluster.sync();
 
     // ---- t over all of K, as operand fragments: [rank tile][plane][lane]
-    for (int i = threadIdx.x; i < rk * 32; i += kThreads) {
-        const int l = i & 31, k = i >> 5;
-        uint32_t w[4][PT];
+    for (int i = threadIdx.x; i < rk * 128; i += kThreads) {      // (row g, ranks 2 t), (row g + 8, ..), (row g, ranks 2 t + 8), (..)
+        const int l = i & 31, e = (i >> 5) & 3, k = i >> 7;
+        const int at = ((l >> 2) + 8 * (e & 1)) * rank_pad + k * 16 + 2 * (l & 3) + 8 * (e >> 1);
+        float2 o[kCluster], v = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {                            // (row g, ranks 2 t), (row g + 8, ..), (row g, ranks 2 t + 8), (..)
-            const int at = ((l >> 2) + 8 * (e & 1)) * rank_pad + k * 16 + 2 * (l & 3) + 8 * (e >> 1);
-            float2 o[kCluster], v = make_float2(0.f, 0.f);
+        for (int c = 0; c < kCluster; ++c)
+            if (c < parts) o[c] = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(tpart, lead + c) + at);
 #pragma unroll
-            for (int c = 0; c < kCluster; ++c)
-                if (c < parts) o[c] = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(tpart, lead + c) + at);
+        for (int c = 0; c < kCluster; ++c)
+            if (c < parts) v.x += o[c].x, v.y += o[c].y;
+        uint32_t w[PT];
+        split<PT>(v.x, v.y, w);
 #pragma unroll
-            for (int c = 0; c < kCluster; ++c)
-                if (c < parts) v.x += o[c].x, v.y += o[c].y;
-            split<PT>(v.x, v.y, w[e]);
-        }
-#pragma unroll
-        for (int q = 0; q < PT; ++q) frag[((size_t)k * PT + q) * 32 + l] = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
+        for (int q = 0; q < PT; ++q) reinterpret_cast<uint32_t *>(frag + ((size_t)k * PT + q) * 32 + l)[e] = w[q];
     }
     __syncthreads();
     auto arrived = cluster.barrier_arrive();                      // this block has read the others' parts
 
     // ---- y += scale B t over this block's part of N
-    add_chunks<F16, YF32, 1>(s, b, frag, rk, scale, row, nc0 + warp, nc1, kWarps, sums + warp * 16 * kTileLd, lane);
+    int nc, left = 0;                        // chunk; tiles of the piece
+    uint32_t bw = 0;
+    auto fragments = [&](int k, uint4(&w)[2]) {
+        if (left == 0) {
+            ring.wait(fail, p.status);
+            bw = ring.at + ring.stage * kFewPiece + lane * 16;
+            left = min(b_chunks, nc1 - nc) * min(rk - k, kFewPiece / 1024);
+        }
+        w[0] = lds128(bw), w[1] = lds128(bw + 512);
+        bw += 1024;
+        if (--left == 0) {
+            __syncwarp();
+            fetch();
+            ring.next();
+        }
+    };
+    const int whole = s.y_vec ? min(nc1, s.n / 32) : nc0;       // chunks of outputs whose 16 bytes are aligned; the others: a row's 32 by 32 lanes
+    float *piece = sums + warp * 16 * kTileLd;
+    uint8_t *to[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) to[h] = row[g + 8 * h] < 0 ? nullptr : reinterpret_cast<uint8_t *>(s.y) + row_at[g + 8 * h] + ((long long)nc0 * 32 + 8 * t) * YB;
+#pragma unroll 1
+    for (nc = nc0; nc < nc1; ++nc) {
+        const bool aligned = nc < whole;
+        // one set of registers for both kinds: what does not fit is put by as soon as it is loaded, which waits for every load
+        OutputColumn<YF32> z;
+        if (aligned) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (to[h]) {
+                    OutputPiece<YF32> y;
+                    y.load(to[h]);
+#pragma unroll
+                    for (int i = 0; i < 4 * YB / 2; ++i) z.v[4 * YB / 2 * h + i] = __uint_as_float(word_of(y.w[i / 4], i % 4));
+                }
+        } else {
+            z.load(s, row_at, nc * 32 + lane);
+        }
+        float acc[4][4];
+        expand<F16, PT>(fragments, frag + lane, rk, acc);
+        if (!ring.ok) continue;
+        if (aligned) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[2 * i] = acc[i][2 * h], v[2 * i + 1] = acc[i][2 * h + 1];
+                OutputPiece<YF32> y;
+#pragma unroll
+                for (int i = 0; i < YB / 2; ++i) {
+                    const float *o = z.v + 4 * YB / 2 * h + 4 * i;
+                    y.w[i] = make_uint4(__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3]));
+                }
+                if (to[h]) {
+                    y.add(to[h], scale, v);
+                    to[h] += 32 * YB;
+                }
+            }
+        } else {
+            z.add(s, row_at, nc * 32 + lane, scale, acc, piece, lane);
+        }
+    }
     cluster.barrier_wait(std::move(arrived));
 }
 
@@ -478,27 +695,45 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_few_kernel(const __grid_
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(16) FewRows rows;
     __shared__ int row[16];
+    __shared__ long long row_at[16];
+    __shared__ uint64_t bars[kWarps][kFewDepth];
+    __shared__ int fail;
+    WarpRing<kFewDepth> ring;
+    {
+        const int warp = threadIdx.x >> 5;
+        ring.init(bars[warp], smem + (size_t)warp * kFewDepth * kFewPiece, kFewPiece, threadIdx.x & 31);
+        if (threadIdx.x == 0) fail = 0;
+    }
     pdl_launch_dependents();
     pdl_wait();
-    few_groups(rows, p);
-    // As many blocks of a cluster share an item (a group and a set) as there are blocks for all items: eight of few, one of many.  (Every
-    // block has the same groups; those of a cluster meet the same number of times.)
-    const int items = rows.n * p.sets, block = (int)(blockIdx.x % kCluster);
-    int parts = kCluster;
-    while (parts > 1 && items * parts > (int)gridDim.x) parts /= 2;
-    const int at_a_time = gridDim.x / parts, rounds = (items + at_a_time - 1) / at_a_time;
-    for (int round = 0; round < rounds; ++round) {
-        const int item = round * at_a_time + blockIdx.x / kCluster * (kCluster / parts) + block / parts;
+    // (the tables lie where the rings will be; barriers at the end)
+    few_groups(rows, *reinterpret_cast<FewTables *>(smem), p);
+    // As many blocks of a cluster share an item (a group and a set) as its bytes are of all bytes: one, two, four or eight of them.  (Every block
+    // finds the same; the blocks of a cluster meet the same number of times.)  Of more items than blocks, a block takes one after the other.
+    const int items = rows.n * p.sets, grid = (int)gridDim.x;
+    int log_parts = items * kCluster > grid ? 0 : kLogCluster, mine = (int)blockIdx.x >> log_parts;
+    if (items <= min(grid, kMostShares) && items * kCluster > grid) {
+        few_shares(rows, p, items, YF32 ? 4 : 2);
+        log_parts = rows.log_parts;
+        mine = rows.item;
+    }
+    for (int turn = 0; turn < items; turn += grid) {
+        const int item = turn + mine;
         const int group = min(item, items - 1) / p.sets, set = min(item, items - 1) - group * p.sets;
         const AdapterSet &s = p.set[set];
         const int first = rows.first[group], n = rows.first[group + 1] - first;
         int slot = item < items ? rows.slot[rows.sorted[first]] : -1;
         if (!active(s, slot)) slot = -1;
-        if (threadIdx.x < 16) row[threadIdx.x] = slot >= 0 && threadIdx.x < n ? rows.sorted[first + threadIdx.x] : -1;
+        if (threadIdx.x < 16) {
+            const int r = slot >= 0 && threadIdx.x < n ? rows.sorted[first + threadIdx.x] : -1;
+            row[threadIdx.x] = r;
+            row_at[threadIdx.x] = r < 0 ? -1ll : r * s.ldy * (YF32 ? 4 : 2);
+        }
         __syncthreads();
-        few_pass<F16, XF32, YF32>(p, s, slot, row, parts, smem);
+        few_pass<F16, XF32, YF32>(p, s, slot, row, row_at, log_parts, smem, ring, &fail);
         __syncthreads();
     }
+    ring_leave(&fail);
 }
 
 // ---- more rows ---------------------------------------------------------------------------------------------
@@ -658,6 +893,7 @@ template <bool F16, bool YF32> __global__ void __launch_bounds__(kThreads, 2) ad
     constexpr int PT = YF32 ? 3 : 2;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int slots[kStreamRows], row[kStreamRows];
+    __shared__ long long row_at[kStreamRows];
     __shared__ unsigned firsts[2];
     uint4 *frag = reinterpret_cast<uint4 *>(smem + kPieces);
     const AdapterSet &s = p.set[blockIdx.z];
@@ -684,7 +920,11 @@ template <bool F16, bool YF32> __global__ void __launch_bounds__(kThreads, 2) ad
                 if (seen) continue;
             }
             const int rk = (s.rank[slot] + 15) / 16, ranks = (s.rank[slot] + 7) / 8 * 8;
-            if (threadIdx.x < kStreamRows) row[threadIdx.x] = slots[threadIdx.x] == slot ? base + (int)threadIdx.x : -1;
+            if (threadIdx.x < kStreamRows) {
+                const int r = slots[threadIdx.x] == slot ? base + (int)threadIdx.x : -1;
+                row[threadIdx.x] = r;
+                row_at[threadIdx.x] = r < 0 ? -1ll : r * s.ldy * (YF32 ? 4 : 2);
+            }
             __syncthreads();
             // t as fragments: [row tile][rank tile][plane][lane]
             for (int i = threadIdx.x; i < 4 * rk * 32; i += kThreads) {
@@ -702,7 +942,7 @@ template <bool F16, bool YF32> __global__ void __launch_bounds__(kThreads, 2) ad
             }
             __syncthreads();
             const int m = warp & 3;
-            add_chunks<F16, YF32, kStreamStep>(s, reinterpret_cast<const uint4 *>(s.b + slot * s.b_stride), frag + (size_t)m * rk * PT * 32, rk, s.scale[slot], row + m * 16,
+            add_chunks<F16, YF32, kStreamStep>(s, reinterpret_cast<const uint4 *>(s.b + slot * s.b_stride), frag + (size_t)m * rk * PT * 32, rk, s.scale[slot], row + m * 16, row_at + m * 16,
                                                nc0 + (warp >> 2) * kStreamStep, nc1, 2 * kStreamStep, reinterpret_cast<float *>(smem) + warp * 16 * kTileLd, lane);
             __syncthreads();
         }
@@ -728,11 +968,51 @@ template <typename Kernel> cudaError_t launch(Kernel kern, const AdaptersParams 
     return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
+// Clusters of eight blocks of a kernel that run at a time; asked for once per kernel, shared memory and device
+cudaError_t resident_clusters(const void *kern, size_t smem, int sm_count, int *out) {
+    struct Known {
+        const void *kern;
+        size_t smem;
+        int device, clusters;
+    };
+    static std::mutex mutex;
+    static std::vector<Known> known;
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> lock(mutex);
+    for (const Known &k : known)
+        if (k.kern == kern && k.smem == smem && k.device == device) {
+            *out = k.clusters;
+            return cudaSuccess;
+        }
+    if ((e = configure_smem(kern, smem)) != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(sm_count * 2 / kCluster * kCluster));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kCluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if ((e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg)) != cudaSuccess) return e;
+    *out = std::max(n, 1);
+    known.push_back(Known{kern, smem, device, *out});
+    return cudaSuccess;
+}
+
 template <bool F16, bool XF32, bool YF32> cudaError_t run(AdaptersParams p, int sm_count, size_t t_floats, cudaStream_t st) {
     constexpr int PT = YF32 ? 3 : 2;
     if (p.m <= kFewRows) {
-        const int clusters = std::min(p.m * p.sets, sm_count * 2 / kCluster);
-        return launch(adapters_few_kernel<F16, XF32, YF32>, p, dim3((unsigned)(clusters * kCluster)), dim3(kCluster), few_smem(p.rank_pad, PT), st);
+        // as many clusters as run at a time (they do not fill every SM: one that came later would begin when another ends)
+        const size_t smem = few_smem(p.rank_pad, PT, XF32);
+        int most = 0;
+        cudaError_t e = resident_clusters(reinterpret_cast<const void *>(adapters_few_kernel<F16, XF32, YF32>), smem, sm_count, &most);
+        if (e != cudaSuccess) return e;
+        return launch(adapters_few_kernel<F16, XF32, YF32>, p, dim3((unsigned)(std::min(p.m * p.sets, most) * kCluster)), dim3(kCluster), smem, st);
     }
     // blocks that split K: as many as run at a time, of eight chunks each at least
     int parts = kCluster;
@@ -787,6 +1067,8 @@ __global__ void adapter_pack_kernel(const uint16_t *a, const uint16_t *b, uint4 
 }
 
 }  // namespace
+
+cudaError_t adapters_set_wait_limit_ns(unsigned long long ns) { return cudaMemcpyToSymbol(s_wait_limit_ns, &ns, sizeof(ns)); }
 
 cudaError_t adapter_pack(const void *a, const void *b, uint8_t *pa, uint8_t *pb, int rank, int K, int n, cudaStream_t st) {
     const int kchunks = (K + 31) / 32, nchunks = (n + 31) / 32;

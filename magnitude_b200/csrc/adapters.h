@@ -36,6 +36,7 @@ struct AdaptersParams {
     int K, kchunks;
     const int *rows;                 // [m]: every row's slot
     int m;
+    int *status;
     int rank_pad;                    // largest rank of the sets, in multiples of 16
     // more rows: t = A x on its way from one launch to the next, [row][t_ld]
     float *t;

@@ -713,6 +713,7 @@ b200q_status b200q_ctx_set_option(b200q_ctx *ctx, int32_t option, int64_t value)
         CU_TRY(ctx, dense_set_wait_limit_ns(ns));
         CU_TRY(ctx, peer_set_wait_limit_ns(ns));
         CU_TRY(ctx, moe_set_wait_limit_ns(ns));
+        CU_TRY(ctx, adapters_set_wait_limit_ns(ns));
         return B200Q_OK;
     }
     case B200Q_OPT_TP_INIT_TIMEOUT_MS:

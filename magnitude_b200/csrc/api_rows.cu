@@ -417,6 +417,7 @@ b200q_status b200q_adapters_apply(b200q_ctx *ctx, const b200q_adapters *const *s
         p.rank_pad = std::max(p.rank_pad, pad);
     }
     p.t = ctx->adapter_t;
+    p.status = ctx->status_dev;
     cudaError_t e = adapters_run(p, sets[0]->dtype == B200Q_TYPE_F16, x_dtype == B200Q_TYPE_F32, y_dtype == B200Q_TYPE_F32, ctx->sm_count, kAdapterTFloats,
                                  (cudaStream_t)stream);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "adapter launch");

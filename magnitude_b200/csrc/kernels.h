@@ -14,6 +14,7 @@ cudaError_t gemm_set_wait_limit_ns(unsigned long long ns);
 cudaError_t dense_set_wait_limit_ns(unsigned long long ns);
 cudaError_t peer_set_wait_limit_ns(unsigned long long ns);
 cudaError_t moe_set_wait_limit_ns(unsigned long long ns);
+cudaError_t adapters_set_wait_limit_ns(unsigned long long ns);
 
 // ---- layout.cu ------------------------------------------------------------------------------
 // Host: re-lay rows [r0, r0 + n) x superblocks [sb0, sb1) of a GGUF tensor (row length K) into the

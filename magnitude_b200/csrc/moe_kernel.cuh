@@ -13,6 +13,7 @@
 #include "kernels.h"
 #include "launch.h"
 #include "moe_image.cuh"
+#include "warp_ring.cuh"
 
 namespace b200q {
 namespace {
@@ -387,16 +388,6 @@ struct MoeHead {
     int fail;                        // some wait ran out: every role leaves its work
 };
 
-// one bounded wait of a role; on expiry (or when another role already gave up) the role leaves
-__device__ __forceinline__ bool moe_wait(uint32_t bar, uint32_t parity, volatile int *fail, int *status) {
-    if (mbar_try_wait_hint(bar, parity, 32)) return true;
-    if (*fail) return false;
-    if (mbar_wait_bounded_fast(bar, parity)) return true;
-    atomicMax(status, DEV_ERR_PIPE_TIMEOUT);
-    *fail = 1;
-    return false;
-}
-
 __device__ __forceinline__ void moe_ring_init(MoeHead &head, int depth) {
     if (threadIdx.x == 0) {
         for (int i = 0; i < depth; ++i) {
@@ -406,17 +397,6 @@ __device__ __forceinline__ void moe_ring_init(MoeHead &head, int depth) {
         head.fail = 0;
         mbar_fence_init();
         fence_proxy_async();
-    }
-}
-
-// After a failure copies may still be on their way: they get time to land (far above a copy's latency) before the block's shared
-// memory is released.
-__device__ __forceinline__ void moe_leave(MoeHead &head) {
-    __syncthreads();
-    if (*(volatile int *)&head.fail) {
-        const uint64_t t0 = globaltimer_ns();
-        while (globaltimer_ns() - t0 < 100000) {
-        }
     }
 }
 
@@ -484,7 +464,7 @@ __device__ __forceinline__ void moe_multiply(MoeRing<D> &ring, MoeHead &head, co
     auto work = [&](auto mode, auto more) {
         for (int s = 0; s < steps; ++s) {
             // after a failure the products are left out, but shared sums are still counted
-            ring.ok = ring.ok && __all_sync(0xFFFFFFFFu, moe_wait(smem_u32(&head.full[ring.stage]), ring.phase, &head.fail, status));
+            ring.ok = ring.ok && __all_sync(0xFFFFFFFFu, ring_wait(smem_u32(&head.full[ring.stage]), ring.phase, &head.fail, status));
             if (!ring.ok) break;
             if (active) {
                 uint32_t at = ring.stage * stage_bytes;
@@ -551,7 +531,7 @@ __device__ __forceinline__ void moe_produce(MoeRing<D> &ring, bool &full_ring, M
     const uint32_t at = lane < 16 ? lane * REC : kMoeWarps * REC + (lane - 16) * IMG, size = lane < 16 ? REC : IMG;
     for (int s = 0; s < steps; ++s) {
         if (full_ring) {
-            ring.ok = __all_sync(0xFFFFFFFFu, moe_wait(smem_u32(&head.empty[ring.stage]), ring.phase ^ 1, &head.fail, p.status));
+            ring.ok = __all_sync(0xFFFFFFFFu, ring_wait(smem_u32(&head.empty[ring.stage]), ring.phase ^ 1, &head.fail, p.status));
             if (!ring.ok) return;
         }
         const uint32_t bar = smem_u32(&head.full[ring.stage]);
@@ -608,7 +588,7 @@ template <int NT> struct MoeView {
 };
 template <int P, int NT, int D>
 __device__ __forceinline__ MoeView<NT> moe_view(MoeRing<D> &ring, MoeHead &head, int *status, int lane, MoeColumns<NT> &col) {
-    ring.ok = ring.ok && __all_sync(0xFFFFFFFFu, moe_wait(smem_u32(&head.full[ring.stage]), ring.phase, &head.fail, status));
+    ring.ok = ring.ok && __all_sync(0xFFFFFFFFu, ring_wait(smem_u32(&head.full[ring.stage]), ring.phase, &head.fail, status));
     const MoeGroup &grp = head.group[ring.stage];
     MoeView<NT> v;
     v.expert = ring.ok ? grp.expert : 0;
@@ -647,7 +627,7 @@ template <int QT, int P, int NT, bool EARLY, typename Finish> __device__ __force
     MoeWalk walk(share, steps, runs);
     if (warp == kMoeWarps) {
         moe_producer<QT, P, NT, D, EARLY>(head, smem, p, walk, [](const MoeWalk &k) { return make_int2(k.outer, k.inner); }, lane);
-        moe_leave(head);
+        ring_leave(&head.fail);
         return;
     }
     if (EARLY) pdl_wait();
@@ -680,7 +660,7 @@ template <int QT, int P, int NT, bool EARLY, typename Finish> __device__ __force
         }
         finish(v.expert, tile, v.slot, acc);
     }
-    moe_leave(head);
+    ring_leave(&head.fail);
 }
 
 // gate, up and the activation function
@@ -735,7 +715,7 @@ template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 
     MoeWalk walk(share, steps, max(groups, 1));
     if (warp == kMoeWarps) {
         moe_producer<QT, P, NT, D, true>(head, smem, pr, walk, [](const MoeWalk &k) { return make_int2(k.inner, k.outer); }, lane);
-        moe_leave(head);
+        ring_leave(&head.fail);
         return;
     }
     pdl_wait();
@@ -807,7 +787,7 @@ template <int QT, int P, int NT> __global__ void __launch_bounds__(kMoeThreads, 
         __syncwarp();
         whole = false;
     }
-    moe_leave(head);
+    ring_leave(&head.fail);
 }
 
 template <typename Kernel, typename Params> cudaError_t moe_launch(Kernel kern, const Params &p, int grid, size_t smem, cudaStream_t st, int threads = kMoeThreads) {

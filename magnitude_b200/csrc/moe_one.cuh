@@ -15,38 +15,6 @@ namespace {
 
 constexpr int kOneThreads = 32 * kMoeWarps;
 
-// A warp's ring of records
-template <int D> struct MoeOneRing {
-    uint32_t bars;           // D barriers
-    uint32_t at;             // D records in shared memory
-    int stage = 0, filled = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    __device__ __forceinline__ void init(uint64_t *bar, const uint8_t *smem, int lane) {
-        bars = smem_u32(bar);
-        at = smem_u32(smem);
-        if (lane == 0) {
-            for (int i = 0; i < D; ++i) mbar_init(bars + 8 * i, 1);
-            mbar_fence_init();
-            fence_proxy_async();
-        }
-        __syncwarp();
-    }
-    // the next record into the stage after the last one filled (which is free)
-    __device__ __forceinline__ void fill(const uint8_t *src, uint32_t bytes, int lane) {
-        if (lane == 0) {
-            fence_proxy_async();         // the readers' last accesses precede the copy
-            mbar_expect_tx(bars + 8 * filled, bytes);
-            bulk_g2s(at + filled * bytes, src, bytes, bars + 8 * filled);
-        }
-        if (++filled == D) filled = 0;
-    }
-    __device__ __forceinline__ void wait(volatile int *fail, int *status) { ok = ok && __all_sync(0xFFFFFFFFu, moe_wait(bars + 8 * stage, phase, fail, status)); }
-    __device__ __forceinline__ void next() {
-        if (++stage == D) stage = 0, phase ^= 1;
-    }
-};
-
 template <int QT> constexpr int moe_one_depth() { return QT == QT_Q8_0 ? 2 : 3; }
 template <int QT> constexpr int moe_one_ring() { return kMoeWarps * moe_one_depth<QT>() * moe_rec_bytes(QT); }
 
@@ -93,15 +61,6 @@ template <int P> __device__ __forceinline__ float moe_one_sum(const MoeOneShared
     for (int w = 0; w < kMoeWarps; ++w) sum += s.part[i & 1][w][lane & 15];
     return sum;
 }
-template <int P> __device__ __forceinline__ void moe_one_leave(MoeOneShared<P> &s) {
-    __syncthreads();
-    if (*(volatile int *)&s.fail) {      // copies may still be on their way: as in moe_leave
-        const uint64_t t0 = globaltimer_ns();
-        while (globaltimer_ns() - t0 < 100000) {
-        }
-    }
-}
-
 // gate, up and the activation function.  A unit is a choice and a tile of eight gate and eight up rows; the warps split K record by record,
 // and convert of the row what they multiply.
 template <int QT, int P> __global__ void __launch_bounds__(kOneThreads, 2) moe_one_gate_up_kernel(const __grid_constant__ MoeOneGateUp p) {
@@ -111,8 +70,8 @@ template <int QT, int P> __global__ void __launch_bounds__(kOneThreads, 2) moe_o
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2;
     const MoeWeights &w = p.weights;
     uint8_t *images = smem + moe_one_ring<QT>(), *records = smem + warp * D * REC;
-    MoeOneRing<D> ring;
-    ring.init(sh.bars[warp], records, lane);
+    WarpRing<D> ring;
+    ring.init(sh.bars[warp], records, REC, lane);
     for (int i = tid; i < 64 * P; i += kOneThreads) reinterpret_cast<uint32_t *>(sh.zero)[i] = 0u;
     if (tid == 0) sh.fail = 0;
     __syncthreads();
@@ -175,7 +134,7 @@ template <int QT, int P> __global__ void __launch_bounds__(kOneThreads, 2) moe_o
         }
         ++i;
     }
-    moe_one_leave(sh);
+    ring_leave(&sh.fail);
 }
 
 // down and the weighted sum over the choices.  A unit is a tile of 16 rows, its records are those of all choices one after the other; a warp takes
@@ -189,8 +148,8 @@ template <int QT, int P> __global__ void __launch_bounds__(kOneThreads, 2) moe_o
     const MoeOutput &o = p.out;
     const int ff = p.ff, all = p.choice.top_k * w.nrec, j0 = all * warp / kMoeWarps, j1 = all * (warp + 1) / kMoeWarps;
     uint8_t *images = smem + moe_one_ring<QT>(), *records = smem + warp * D * REC;
-    MoeOneRing<D> ring;
-    ring.init(sh.bars[warp], records, lane);
+    WarpRing<D> ring;
+    ring.init(sh.bars[warp], records, REC, lane);
     for (int i = tid; i < 64 * P; i += kOneThreads) reinterpret_cast<uint32_t *>(sh.zero)[i] = 0u;
     if (tid == 0) sh.fail = 0;
     __syncthreads();
@@ -264,7 +223,7 @@ template <int QT, int P> __global__ void __launch_bounds__(kOneThreads, 2) moe_o
             if (stores && *(volatile int *)&sh.fail == 0) moe_store(o, 0, n, sum);
         }
     }
-    moe_one_leave(sh);
+    ring_leave(&sh.fail);
 }
 
 }  // namespace
