@@ -398,7 +398,8 @@ b200q_status b200q_moe_create(b200q_ctx *ctx, const b200q_moe_config *config, b2
 /* x[M][n_embd] F32 or BF16, ids and weights [M][top_k] in device memory, y[M][n_embd] F32 or BF16; M <= max_rows, M == 0 is a
  * no-op.  A choice outside 0..n_experts-1 (-1 for padding) contributes nothing; the same expert twice in a row counts twice.
  * Activations enter as fixed point, 256 elements to a scale: 16 bits where y is BF16, 31 bits where it is F32; sums are
- * integers and fp32.  A piece of 256 elements that holds an infinity or a NaN makes that row's result NaN, no other row's.
+ * integers and fp32.  A piece of 256 elements that holds an infinity or a NaN makes that row's result NaN, no other row's.  y
+ * may be x itself (of one dtype and leading dimension); other overlaps are not allowed.
  * Results do not depend on the other rows of the call but through the order of sums over K. */
 b200q_status b200q_moe_run(b200q_ctx *ctx, b200q_moe *moe, const void *x_dev, int32_t x_dtype, int64_t M, int64_t ldx,
                            const int32_t *ids_dev, int64_t ld_ids, const float *weights_dev, int64_t ld_weights,
@@ -408,7 +409,8 @@ void b200q_moe_destroy(b200q_moe *moe);     /* may follow b200q_ctx_destroy, lik
 /* The router in front of it: logits l = W x[m] + logit_bias, the top_k experts of every row and their weights, in the form
  * b200q_moe_run takes.  Sums are held in 64 bits, so that the choice depends neither on the batch nor on the order of a sum;
  * of equal ones the lower index is chosen first.  A NaN among the logits counts as the lowest number, infinities as the largest.
- * Two calls of one router must not overlap (it has a workspace for max_rows rows; calls allocate nothing). */
+ * Two calls of one router must not overlap (it has a workspace for max_rows rows; calls allocate nothing), nor the replays of
+ * graphs that captured them. */
 typedef struct b200q_router b200q_router;
 
 enum {
@@ -452,11 +454,13 @@ b200q_status b200q_adapters_create(b200q_ctx *ctx, int64_t N, int64_t K, int32_t
  * rank 0 empties the slot.  Copied before the call returns; no call that uses the slot may be in flight. */
 b200q_status b200q_adapters_load(b200q_ctx *ctx, b200q_adapters *set, int32_t slot, int32_t rank, float scale, const void *A,
                                  const void *B);
-/* One activation and 1..4 sets of one dtype and K (the adapters of Q, K and V, or of gate and up), one launch: y_i[M][N_i] of the rows whose
+/* One activation and 1..4 sets of one dtype and K (the adapters of Q, K and V, or of gate and up): y_i[M][N_i] of the rows whose
  * slot holds an adapter are added to, other rows (slot -1, beyond the set, or empty) are not touched.  slots_dev [M] in
  * device memory is read by the launch.  Sums are fp32 over exact products (fp32 activations and, for fp32 outputs, A x enter
- * with 24 bits, for bf16 outputs A x with 16); a bf16 result is rounded once.  Calls of any sets may overlap that add to
- * different outputs; a row that holds an infinity or a NaN spoils no other. */
+ * with 24 bits, for bf16 outputs A x with 16); a bf16 result is rounded once.  Outputs overlap neither each other nor x.  A row
+ * that holds an infinity or a NaN spoils no other.  Calls of up to 512 rows may overlap where they add to different outputs; calls
+ * of more take two launches and a workspace of the context, so two of those must not overlap (nor the replays of graphs
+ * that captured them). */
 b200q_status b200q_adapters_apply(b200q_ctx *ctx, const b200q_adapters *const *sets, int32_t n_sets, const void *x_dev,
                                   int32_t x_dtype, int64_t M, int64_t ldx, const int32_t *slots_dev, void *const *y_dev,
                                   int32_t y_dtype, const int64_t *ldy, void *stream);

@@ -396,6 +396,7 @@ b200q_status b200q_adapters_apply(b200q_ctx *ctx, const b200q_adapters *const *s
     for (int i = 0; i < n_sets; ++i) {
         if (!y_dev[i]) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "null output pointer");
         if (ldy[i] < sets[i]->N) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "leading dimension smaller than the row");
+        if (y_dev[i] == x_dev) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "the output is the activation itself");
         for (int j = 0; j < i; ++j)
             if (y_dev[j] == y_dev[i]) return fail(ctx, B200Q_ERR_INVALID_CONFIG, "sets %d and %d of one call add to the same output", j, i);
         AdapterSet &d = p.set[i];
