@@ -164,13 +164,13 @@ template <bool F16, int PX> __device__ __forceinline__ void multiply_tile(const 
 
 // B t of sixteen rows and a chunk of 32 outputs: acc of column tile i: rows g, g + 8, outputs 8 t + 2 i, + 1.  fragments(k, w): the lane's two
 // of rank tile k, fp: of the rows' t
-template <bool F16, int PT, typename Fragments> __device__ __forceinline__ void expand(Fragments fragments, const uint4 *fp, int rk, float (&acc)[4][4]) {
+template <bool F16, int PT, int UNROLL, typename Fragments> __device__ __forceinline__ void expand(Fragments fragments, const uint4 *fp, int rk, float (&acc)[4][4]) {
     constexpr int PA = F16 ? 2 : 1;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-#pragma unroll 1
+#pragma unroll UNROLL
     for (int k = 0; k < rk; ++k, fp += PT * 32) {
         uint4 w[2];
         fragments(k, w);
@@ -190,7 +190,7 @@ template <bool F16, int PT, typename Fragments> __device__ __forceinline__ void 
     }
 }
 template <bool F16, int PT> __device__ __forceinline__ void expand(const uint4 *bp, const uint4 *fp, int rk, float (&acc)[4][4]) {
-    expand<F16, PT>([&](int k, uint4(&w)[2]) { w[0] = bp[k * 64], w[1] = bp[k * 64 + 32]; }, fp, rk, acc);
+    expand<F16, PT, 2>([&](int k, uint4(&w)[2]) { w[0] = bp[k * 64], w[1] = bp[k * 64 + 32]; }, fp, rk, acc);
 }
 
 // Outputs that are not aligned: a row's 32 by 32 lanes, sixteen rows
@@ -220,6 +220,16 @@ __device__ __forceinline__ void OutputColumn<YF32>::add(const AdapterSet &s, con
 #pragma unroll
         for (int r = 0; r < 16; ++r)
             if (to[r] >= 0) store_y<YF32>(y + to[r], fmaf(scale, piece[r * kTileLd + lane], v[r]));
+}
+
+// y of sixteen rows += scale B t for a chunk of outputs that are not aligned
+template <bool F16, bool YF32>
+__device__ __forceinline__ void add_column(const AdapterSet &s, const uint4 *b, const uint4 *frag, int rk, float scale, const long long *row_at, int c, float *piece, int lane) {
+    OutputColumn<YF32> y;
+    y.load(s, row_at, c * 32 + lane);
+    float acc[4][4];
+    expand<F16, (YF32 ? 3 : 2)>(b + (size_t)c * rk * 64 + lane, frag + lane, rk, acc);
+    y.add(s, row_at, c * 32 + lane, scale, acc, piece, lane);
 }
 
 // y of sixteen rows += scale B t over the chunks nc, nc + step, .. below nc1, CH neighbouring ones at a time.  row[16]: the rows, -1: none;
@@ -258,13 +268,7 @@ __device__ __forceinline__ void add_chunks(const AdapterSet &s, const uint4 *b, 
     // rows that are not aligned, the last outputs
     for (; nc < nc1; nc += step)
 #pragma unroll 1
-        for (int c = nc; c < min(nc + CH, nc1); ++c) {
-            OutputColumn<YF32> y;
-            y.load(s, row_at, c * 32 + lane);
-            float acc[4][4];
-            expand<F16, PT>(b + (size_t)c * rk * 64 + lane, frag + lane, rk, acc);
-            y.add(s, row_at, c * 32 + lane, scale, acc, piece, lane);
-        }
+        for (int c = nc; c < min(nc + CH, nc1); ++c) add_column<F16, YF32>(s, b, frag, rk, scale, row_at, c, piece, lane);
 }
 
 // an adapter that takes part: within the set and loaded
@@ -507,7 +511,7 @@ size_t few_smem(int rank_pad, int planes, bool x_f32) { return kFewRing + few_su
 // rows of y one.  What a step costs is the instructions of one warp after the other, more than their number: hence few and large pieces, and
 // buffers that take turns (a copy from one to the other would wait for the load).
 template <bool F16, bool XF32, bool YF32>
-__device__ __forceinline__ void few_pass(const AdaptersParams &p, const AdapterSet &s, int slot, const int *row, const long long *row_at, int log_parts, uint8_t *memory, WarpRing<kFewDepth> &ring,
+__device__ __forceinline__ void few_pass(const AdaptersParams &p, const AdapterSet &s, int slot, const int *row, const long long *row_at, int log_parts, int copy, int copies, uint8_t *memory, WarpRing<kFewDepth> &ring,
                                          volatile int *fail) {
     constexpr int PT = YF32 ? 3 : 2, PX = XF32 ? 3 : 1, RT = few_tiles(XF32), SUM_LD = 8 * RT + 2, XB = XF32 ? 4 : 2, YB = YF32 ? 4 : 2;
     cg::cluster_group cluster = cg::this_cluster();
@@ -522,7 +526,9 @@ __device__ __forceinline__ void few_pass(const AdaptersParams &p, const AdapterS
     // the warp's chunks: of the block's part an eighth
     auto share = [&](int all, int w) { return (int)((long long)all * (part * kWarps + w) >> (log_parts + 3)); };
     static_assert(kWarps == 8, "an eighth");
-    const int kc0 = share(p.kchunks, warp), kc1 = share(p.kchunks, warp + 1), nc0 = share(s.nchunks, warp), nc1 = slot < 0 ? nc0 : share(s.nchunks, warp + 1);
+    const int kc0 = share(p.kchunks, warp), kc1 = share(p.kchunks, warp + 1);
+    const int n_first = s.nchunks * copy / copies, n_all = s.nchunks * (copy + 1) / copies - n_first;
+    const int nc0 = n_first + share(n_all, warp), nc1 = slot < 0 ? nc0 : n_first + share(n_all, warp + 1);
     // chunks of a piece: of A where all rank tiles' sums are held at once, of B where its rank tiles fit
     const int a_chunks = rt > 0 && rt <= RT ? kFewPiece / 512 / rt : 1, b_chunks = rk > 0 && rk <= kFewPiece / 1024 ? kFewPiece / 1024 / rk : 1;
     // fetched next: of A chunk fa, tiles from fr on; then of B chunk fn, tiles from fk on
@@ -664,7 +670,7 @@ __device__ __forceinline__ void few_pass(const AdaptersParams &p, const AdapterS
             z.load(s, row_at, nc * 32 + lane);
         }
         float acc[4][4];
-        expand<F16, PT>(fragments, frag + lane, rk, acc);
+        expand<F16, PT, 1>(fragments, frag + lane, rk, acc);
         if (!ring.ok) continue;
         if (aligned) {
 #pragma unroll
@@ -712,6 +718,14 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_few_kernel(const __grid_
     // finds the same; the blocks of a cluster meet the same number of times.)  Of more items than blocks, a block takes one after the other.
     const int items = rows.n * p.sets, grid = (int)gridDim.x;
     int log_parts = items * kCluster > grid ? 0 : kLogCluster, mine = (int)blockIdx.x >> log_parts;
+    // Of fewer items than clusters several work on one: each makes t for itself and adds some of the outputs, two chunks a warp or more.
+    // (Four rows of two adapters, 22848 outputs: 21 us by two clusters.)
+    int copy = 0, copies = 1;
+    if (log_parts == kLogCluster) {
+        copies = max(1, min(grid / (kCluster * max(items, 1)), p.most_copies));
+        copy = mine % copies;
+        mine /= copies;
+    }
     if (items <= min(grid, kMostShares) && items * kCluster > grid) {
         few_shares(rows, p, items, YF32 ? 4 : 2);
         log_parts = rows.log_parts;
@@ -730,7 +744,7 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_few_kernel(const __grid_
             row_at[threadIdx.x] = r < 0 ? -1ll : r * s.ldy * (YF32 ? 4 : 2);
         }
         __syncthreads();
-        few_pass<F16, XF32, YF32>(p, s, slot, row, row_at, log_parts, smem, ring, &fail);
+        few_pass<F16, XF32, YF32>(p, s, slot, row, row_at, log_parts, copy, copies, smem, ring, &fail);
         __syncthreads();
     }
     ring_leave(&fail);
@@ -743,147 +757,175 @@ __device__ __forceinline__ unsigned first_rows(int slot, int lane) {
     return __ballot_sync(0xFFFFFFFFu, slot >= 0 && __ffs(same) - 1 == lane);
 }
 
-// t[row][ranks of all sets].  A cluster takes 128 rows, sixteen a warp, and one adapter of them after the other; its blocks split K and add their
-// parts up through distributed shared memory, each for some of the rows.  x and the fragments of A come into shared memory by cp.async, 512
-// bytes of every row at a time.  (With x in registers, a chunk ahead, the way from L2 set the pace: 4096 rows of 5120, 64 ranks, 54 us.)
+// t[row][ranks of all sets].  A cluster takes 128 rows, sixteen a warp, and eight rank tiles at a time of whichever adapters they have; its blocks split K and
+// add their parts up through distributed shared memory, each for some of the rows.  x and the fragments of A come into shared memory by cp.async, 256
+// bytes of every row at a time, the next ones while these are multiplied.  (With x in registers, a chunk ahead, the way from L2 set the pace.)
 constexpr int kSumTiles = 8, kShrinkRows = 16 * kWarps;      // tiles of eight ranks whose sums a warp holds at a time
 constexpr int kSumLd = 8 * kSumTiles + 2;
-constexpr int kXLd = 512 + 64;                               // bytes from row to row: two rows' pieces lie in different banks
-constexpr size_t kShrinkX = size_t(kShrinkRows) * kXLd;
-__host__ __device__ constexpr int batch_chunks(bool f32) { return f32 ? 4 : 8; }
-constexpr size_t kShrinkSmem = kShrinkX + size_t(8) * kSumTiles * 512;
-static_assert(kShrinkX >= size_t(kShrinkRows) * kSumLd * 4, "sums");
+constexpr int kXBytes = 256;
+__host__ __device__ constexpr int batch_chunks(bool f32) { return kXBytes / 32 / (f32 ? 4 : 2); }
+constexpr int kShrinkX = kShrinkRows * kXBytes, kShrinkStage = kShrinkX + batch_chunks(false) * kSumTiles * 512;
+constexpr size_t kShrinkSmem = size_t(2) * kShrinkStage;
+static_assert(kShrinkSmem >= size_t(kShrinkRows) * kSumLd * 4, "sums");
+// 16-byte unit of a row's piece: two rows side by side lie in different banks for the eight lanes that read them together
+template <bool F32> __device__ __forceinline__ int x_unit(int row, int unit) { return unit ^ (F32 ? row & 1 : (row & 1) << 2); }
 struct AdapterTile {
     const uint4 *from;                   // its fragment of the first chunk
     int step, to;                        // 16-byte words from chunk to chunk; its place in a row of t
+    int slot;
 };
 template <bool F16, bool XF32> __global__ void __launch_bounds__(kThreads, 2) adapters_shrink_kernel(const __grid_constant__ AdaptersParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int slots[kShrinkRows];
-    __shared__ unsigned firsts[kShrinkRows / 32];
-    __shared__ AdapterTile tiles_of[kAdapterMaxSets * kAdapterMaxRank / 8];
-    __shared__ int all_tiles;
+    __shared__ int kind[kShrinkRows], kind_end[kShrinkRows];      // the slots that occur, and the rank tiles up to the end of each one's
+    __shared__ int2 sums_of[kShrinkRows / 32];
+    __shared__ AdapterTile tiles_of[kSumTiles];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int base = blockIdx.x * kShrinkRows, mine = warp * 16;
     const int parts = gridDim.y, part0 = blockIdx.y;      // the cluster
     const int kc0 = (int)((long long)p.kchunks * part0 / parts), kc1 = (int)((long long)p.kchunks * (part0 + 1) / parts);
     cg::cluster_group cluster = cg::this_cluster();
     float *sums = reinterpret_cast<float *>(smem);        // [row][rank of the tiles at hand], where x was
-    uint8_t *afrag = smem + kShrinkX;
     constexpr int PX = XF32 ? 3 : 1, XB = XF32 ? 4 : 2, BATCH = batch_chunks(XF32);
     pdl_launch_dependents();
     pdl_wait();
+    auto tiles_in = [&](int set, int slot) { return active(p.set[set], slot) ? (p.set[set].rank[slot] + 7) / 8 : 0; };
+    // the slots that occur, in the order of their first rows, and the tiles of each: all sets'
+    int slot = -1;
+    bool first_row = false;
     if (tid < kShrinkRows) {
-        const int slot = base + tid < p.m ? p.rows[base + tid] : -1;
+        slot = base + tid < p.m ? p.rows[base + tid] : -1;
         slots[tid] = slot;
-        const unsigned first = first_rows(slot, lane);
-        if (lane == 0) firsts[warp] = first;
+        first_row = first_rows(slot, lane) >> lane & 1;
     }
     __syncthreads();
-    for (int part = 0; part < kShrinkRows / 32; ++part)
-        for (unsigned left = firsts[part]; left; left &= left - 1) {
-            const int slot = slots[part * 32 + __ffs((int)left) - 1];
-            bool seen = false;               // had its turn among earlier rows?
-            for (int q = lane; q < part * 32; q += 32) seen |= slots[q] == slot;
-            if (__any_sync(0xFFFFFFFFu, seen)) continue;
-            const bool any = __any_sync(0xFFFFFFFFu, lane < 16 && slots[mine + (lane & 15)] == slot);
-            // tiles of eight ranks, set after set
-            if (tid < p.sets * (kAdapterMaxRank / 8)) {
-                int at = 0, tile = tid;
-                for (int set = 0; set < p.sets; ++set) {
-                    const AdapterSet &s = p.set[set];
-                    const int rt = active(s, slot) ? (s.rank[slot] + 7) / 8 : 0;
-                    if (tile >= 0 && tile < rt) {
-                        tiles_of[tid].from = reinterpret_cast<const uint4 *>(s.a + slot * s.a_stride) + tile * 32;
-                        tiles_of[tid].step = rt * 32;
-                        tiles_of[tid].to = s.t_at + 8 * tile;
-                    }
-                    at += rt;
-                    tile -= rt;
+    int2 run = make_int2(0, 0);
+    if (tid < kShrinkRows) {
+        if (first_row)
+            for (int q = 0; q < warp * 32; ++q) first_row = first_row && slots[q] != slot;
+        if (first_row) {
+            run.x = 1;
+            for (int set = 0; set < p.sets; ++set) run.y += tiles_in(set, slot);
+        }
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int x = __shfl_up_sync(0xFFFFFFFFu, run.x, d), y = __shfl_up_sync(0xFFFFFFFFu, run.y, d);
+            if (lane >= d) run.x += x, run.y += y;
+        }
+        if (lane == 31) sums_of[warp] = run;
+    }
+    __syncthreads();
+    int all_tiles = 0;
+    for (int w = 0; w < kShrinkRows / 32; ++w) {
+        if (w < warp) run.x += sums_of[w].x, run.y += sums_of[w].y;
+        all_tiles += sums_of[w].y;
+    }
+    if (first_row) kind[run.x - 1] = slot, kind_end[run.x - 1] = run.y;
+    __syncthreads();
+    // eight tiles at a time, of whichever adapters: x is read once for all of them
+    for (int first = 0; first < all_tiles; first += kSumTiles) {
+        const int tiles = min(all_tiles - first, kSumTiles);
+        if (tid < tiles) {
+            int k = 0;
+            while (kind_end[k] <= first + tid) ++k;
+            int set = 0, tile = first + tid - (k ? kind_end[k - 1] : 0);
+            while (tile >= tiles_in(set, kind[k])) tile -= tiles_in(set++, kind[k]);
+            const AdapterSet &s = p.set[set];
+            const int rt = tiles_in(set, kind[k]);
+            tiles_of[tid] = AdapterTile{reinterpret_cast<const uint4 *>(s.a + kind[k] * s.a_stride) + tile * 32, rt * 32, s.t_at + 8 * tile, kind[k]};
+        }
+        __syncthreads();
+        // of them, those of this warp's rows
+        unsigned wanted = 0;
+        if (lane < tiles)
+            for (int r = 0; r < 16; ++r) wanted |= slots[mine + r] == tiles_of[lane].slot;
+        wanted = __ballot_sync(0xFFFFFFFFu, wanted != 0);
+        float acc[kSumTiles][4];
+#pragma unroll
+        for (int i = 0; i < kSumTiles; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+        auto fetch = [&](int kc, uint8_t *stage) {
+            const int chunks = min(BATCH, kc1 - kc);
+            for (int i = tid; i < kShrinkRows * (kXBytes / 16); i += kThreads) {      // 16 bytes of a row; zeros beyond the rows and K
+                const int r = i / (kXBytes / 16), unit = i % (kXBytes / 16), k = kc * 32 + unit * 16 / XB;
+                const long long row = base + r;
+                const uint8_t *from = reinterpret_cast<const uint8_t *>(p.x) + (row * p.ldx + k) * XB;
+                uint8_t *to = stage + r * kXBytes + 16 * x_unit<XF32>(r, unit);
+                const int left = row < p.m && unit * 16 < chunks * 32 * XB ? min(max((p.K - k) * XB, 0), 16) : 0;
+                if (p.x_vec) {
+                    if (left == 0) from = reinterpret_cast<const uint8_t *>(p.x);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(left) : "memory");
+                } else {
+                    const uint4 w = load_words<XF32>(from, left / XB);
+                    *reinterpret_cast<uint4 *>(to) = w;
                 }
-                if (tid == 0) all_tiles = at;
+            }
+            for (int i = warp; i < tiles; i += kWarps) {
+                const AdapterTile tile = tiles_of[i];
+                for (int c = 0; c < chunks; ++c)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(stage + kShrinkX + ((c * kSumTiles + i) * 32 + lane) * 16)),
+                                 "l"(tile.from + (size_t)(kc + c) * tile.step + lane)
+                                 : "memory");
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        int turn = 0;
+        if (kc0 < kc1) fetch(kc0, smem);
+        for (int kc = kc0; kc < kc1; kc += BATCH, turn ^= 1) {
+            uint8_t *stage = smem + turn * kShrinkStage;
+            if (kc + BATCH < kc1) {
+                fetch(kc + BATCH, smem + (turn ^ 1) * kShrinkStage);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            } else {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
             }
             __syncthreads();
-            for (int first = 0; first < all_tiles; first += kSumTiles) {
-                const int tiles = min(all_tiles - first, kSumTiles);
-                float acc[kSumTiles][4];
+            const int chunks = min(BATCH, kc1 - kc);
+            if (wanted)
+                for (int c = 0; c < chunks; ++c) {
+                    uint32_t f[2][PX][4];
 #pragma unroll
-                for (int i = 0; i < kSumTiles; ++i)
+                    for (int h = 0; h < 2; ++h) {
+                        XPiece<XF32> x;
+                        const int r = mine + g + 8 * h;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-                for (int kc = kc0; kc < kc1; kc += BATCH) {
-                    const int chunks = min(BATCH, kc1 - kc);
-                    __syncthreads();         // what was there has been read
-                    for (int i = tid; i < kShrinkRows * 32; i += kThreads) {      // 16 bytes of a row; zeros beyond the rows and K
-                        const int r = i >> 5, at = (i & 31) * 16, k = kc * 32 + at / XB;
-                        const long long row = base + r;
-                        const uint8_t *from = reinterpret_cast<const uint8_t *>(p.x) + (row * p.ldx + k) * XB;
-                        uint8_t *to = smem + r * kXLd + at;
-                        const int left = row < p.m && at < chunks * 32 * XB ? min(max((p.K - k) * XB, 0), 16) : 0;
-                        if (p.x_vec) {
-                            if (left == 0) from = reinterpret_cast<const uint8_t *>(p.x);
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(left) : "memory");
-                        } else {
-#pragma unroll
-                            for (int b = 0; b < 16; b += XB) {
-                                if (XF32) *reinterpret_cast<uint32_t *>(to + b) = b < left ? *reinterpret_cast<const uint32_t *>(from + b) : 0u;
-                                else *reinterpret_cast<uint16_t *>(to + b) = b < left ? *reinterpret_cast<const uint16_t *>(from + b) : (uint16_t)0;
-                            }
-                        }
+                        for (int i = 0; i < (XF32 ? 2 : 1); ++i)
+                            x.w[i] = *reinterpret_cast<const uint4 *>(stage + r * kXBytes + 16 * x_unit<XF32>(r, (c * 32 + 8 * t) * XB / 16 + i));
+                        x.planes(f[h]);
                     }
-                    for (int i = warp; i < tiles; i += kWarps) {
-                        const AdapterTile tile = tiles_of[first + i];
-                        for (int c = 0; c < chunks; ++c)
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(afrag + ((c * kSumTiles + i) * 32 + lane) * 16)),
-                                         "l"(tile.from + (size_t)(kc + c) * tile.step + lane)
-                                         : "memory");
+#pragma unroll
+                    for (int i = 0; i < kSumTiles; ++i) {
+                        if (!(wanted >> i & 1)) continue;
+                        multiply_tile<F16, PX>(f[0], f[1], *reinterpret_cast<const uint4 *>(stage + kShrinkX + ((c * kSumTiles + i) * 32 + lane) * 16), acc[i]);
                     }
-                    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-                    __syncthreads();
-                    if (any)
-                        for (int c = 0; c < chunks; ++c) {
-                            uint32_t f0[PX][4], f1[PX][4];
-                            XPiece<XF32> x0, x1;
-                            const uint8_t *at = smem + (mine + g) * kXLd + (c * 32 + 8 * t) * XB;
-#pragma unroll
-                            for (int i = 0; i < (XF32 ? 2 : 1); ++i) {
-                                x0.w[i] = *reinterpret_cast<const uint4 *>(at + 16 * i);
-                                x1.w[i] = *reinterpret_cast<const uint4 *>(at + 8 * kXLd + 16 * i);
-                            }
-                            x0.planes(f0);
-                            x1.planes(f1);
-#pragma unroll
-                            for (int i = 0; i < kSumTiles; ++i) {
-                                if (i >= tiles) break;
-                                multiply_tile<F16, PX>(f0, f1, *reinterpret_cast<const uint4 *>(afrag + ((c * kSumTiles + i) * 32 + lane) * 16), acc[i]);
-                            }
-                        }
                 }
-                __syncthreads();
-#pragma unroll
-                for (int i = 0; i < kSumTiles; ++i) {
-                    float *to = sums + (mine + g) * kSumLd + 8 * i + 2 * t;
-                    *reinterpret_cast<float2 *>(to) = make_float2(acc[i][0], acc[i][1]);
-                    *reinterpret_cast<float2 *>(to + 8 * kSumLd) = make_float2(acc[i][2], acc[i][3]);
-                }
-                cluster.sync();
-                const int rows = kShrinkRows / parts;
-                for (int i = tid; i < rows * tiles * 4; i += kThreads) {
-                    const int r = part0 * rows + i / (tiles * 4), c = 2 * (i % (tiles * 4));
-                    if (slots[r] != slot) continue;
-                    float2 o[kCluster], v = make_float2(0.f, 0.f);
-#pragma unroll
-                    for (int q = 0; q < kCluster; ++q)
-                        if (q < parts) o[q] = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(sums, q) + r * kSumLd + c);
-#pragma unroll
-                    for (int q = 0; q < kCluster; ++q)
-                        if (q < parts) v.x += o[q].x, v.y += o[q].y;
-                    *reinterpret_cast<float2 *>(p.t + (long long)(base + r) * p.t_ld + tiles_of[first + c / 8].to + c % 8) = v;
-                }
-                cluster.sync();
-            }
-            __syncthreads();                 // the tiles' list has been read
+            __syncthreads();         // this stage has been read
         }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kSumTiles; ++i) {
+            float *to = sums + (mine + g) * kSumLd + 8 * i + 2 * t;
+            *reinterpret_cast<float2 *>(to) = make_float2(acc[i][0], acc[i][1]);
+            *reinterpret_cast<float2 *>(to + 8 * kSumLd) = make_float2(acc[i][2], acc[i][3]);
+        }
+        cluster.sync();
+        const int rows = kShrinkRows / parts;
+        for (int i = tid; i < rows * tiles * 4; i += kThreads) {
+            const int r = part0 * rows + i / (tiles * 4), c = 2 * (i % (tiles * 4));
+            const AdapterTile &tile = tiles_of[c / 8];
+            if (slots[r] != tile.slot) continue;
+            float2 o[kCluster], v = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int q = 0; q < kCluster; ++q)
+                if (q < parts) o[q] = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(sums, q) + r * kSumLd + c);
+#pragma unroll
+            for (int q = 0; q < kCluster; ++q)
+                if (q < parts) v.x += o[q].x, v.y += o[q].y;
+            *reinterpret_cast<float2 *>(p.t + (long long)(base + r) * p.t_ld + tile.to + c % 8) = v;
+        }
+        cluster.sync();              // (the list of tiles and the sums have been read)
+    }
 }
 
 // y += scale B t: a block takes 64 rows and p.stream_chunks chunks of 32 outputs; four warps side by side in the rows, two in the outputs
@@ -942,8 +984,13 @@ template <bool F16, bool YF32> __global__ void __launch_bounds__(kThreads, 2) ad
             }
             __syncthreads();
             const int m = warp & 3;
-            add_chunks<F16, YF32, kStreamStep>(s, reinterpret_cast<const uint4 *>(s.b + slot * s.b_stride), frag + (size_t)m * rk * PT * 32, rk, s.scale[slot], row + m * 16, row_at + m * 16,
-                                               nc0 + (warp >> 2) * kStreamStep, nc1, 2 * kStreamStep, reinterpret_cast<float *>(smem) + warp * 16 * kTileLd, lane);
+            const uint4 *bs = reinterpret_cast<const uint4 *>(s.b + slot * s.b_stride), *tf = frag + (size_t)m * rk * PT * 32;
+            float *piece = reinterpret_cast<float *>(smem) + warp * 16 * kTileLd;
+            if (s.y_vec)
+                add_chunks<F16, YF32, kStreamStep>(s, bs, tf, rk, s.scale[slot], row + m * 16, row_at + m * 16, nc0 + (warp >> 2) * kStreamStep, nc1, 2 * kStreamStep, piece, lane);
+            else
+#pragma unroll 1
+                for (int c = nc0 + (warp >> 2); c < nc1; c += 2) add_column<F16, YF32>(s, bs, tf, rk, s.scale[slot], row_at + m * 16, c, piece, lane);
             __syncthreads();
         }
 }
@@ -1012,7 +1059,11 @@ template <bool F16, bool XF32, bool YF32> cudaError_t run(AdaptersParams p, int 
         int most = 0;
         cudaError_t e = resident_clusters(reinterpret_cast<const void *>(adapters_few_kernel<F16, XF32, YF32>), smem, sm_count, &most);
         if (e != cudaSuccess) return e;
-        return launch(adapters_few_kernel<F16, XF32, YF32>, p, dim3((unsigned)(std::min(p.m * p.sets, most) * kCluster)), dim3(kCluster), smem, st);
+        int chunks = 0;
+        for (int i = 0; i < p.sets; ++i) chunks = std::max(chunks, p.set[i].nchunks);
+        p.most_copies = std::max(1, chunks / (2 * kCluster * kWarps));
+        const int clusters = (int)std::min<long long>((long long)p.m * p.sets * p.most_copies, most);
+        return launch(adapters_few_kernel<F16, XF32, YF32>, p, dim3((unsigned)(clusters * kCluster)), dim3(kCluster), smem, st);
     }
     // blocks that split K: as many as run at a time, of eight chunks each at least
     int parts = kCluster;
@@ -1020,8 +1071,12 @@ template <bool F16, bool XF32, bool YF32> cudaError_t run(AdaptersParams p, int 
     // A block reads t before its outputs: the more chunks of them, the better, while the SMs have some ten blocks each to share out
     int widest = 0;
     for (int i = 0; i < p.sets; ++i) widest = std::max(widest, p.set[i].nchunks);
+    // (a warp takes four at a time, of unaligned outputs one)
+    bool aligned = true;
+    for (int i = 0; i < p.sets; ++i) aligned = aligned && p.set[i].y_vec;
     p.stream_chunks = 64;
-    while (p.stream_chunks > 8 && (long long)((p.m + kStreamRows - 1) / kStreamRows) * p.sets * ((widest + p.stream_chunks - 1) / p.stream_chunks) < 20ll * sm_count)
+    while (p.stream_chunks > (aligned ? 8 : 2) &&
+           (long long)((p.m + kStreamRows - 1) / kStreamRows) * p.sets * ((widest + p.stream_chunks - 1) / p.stream_chunks) < 20ll * sm_count)
         p.stream_chunks /= 2;
     // t of as many rows at a time as there is room for
     const int room = (int)std::min<size_t>(t_floats / (size_t)p.t_ld / kStreamRows * kStreamRows, size_t(32767) * kStreamRows);

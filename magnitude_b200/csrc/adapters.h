@@ -37,6 +37,7 @@ struct AdaptersParams {
     const int *rows;                 // [m]: every row's slot
     int m;
     int *status;
+    int most_copies;                 // few rows: clusters that may share the outputs of an item
     int rank_pad;                    // largest rank of the sets, in multiples of 16
     // more rows: t = A x on its way from one launch to the next, [row][t_ld]
     float *t;
