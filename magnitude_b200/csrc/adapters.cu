@@ -147,19 +147,27 @@ template <bool YF32> __device__ __forceinline__ void store_y(uint8_t *y, float v
     else *reinterpret_cast<__nv_bfloat16 *>(y) = __float2bfloat16_rn(v);
 }
 
-// acc += sixteen rows (planes of eight elements of rows g, g + 8) times a fragment of A: 32 of K, eight ranks
-template <bool F16, int PX> __device__ __forceinline__ void multiply_tile(const uint32_t (&f0)[PX][4], const uint32_t (&f1)[PX][4], const uint4 &w, float (&acc)[4]) {
+// acc += sixteen rows (planes of eight elements of rows g, g + 8) times a fragment of A: 32 of K, eight ranks.  EXACT: the products are added up
+// apart, lower planes first, and join acc in one rounded addition: the tensor cores cut off what they add to a large sum.
+template <bool F16, int PX, bool EXACT> __device__ __forceinline__ void multiply_tile(const uint32_t (&f0)[PX][4], const uint32_t (&f1)[PX][4], const uint4 &w, float (&acc)[4]) {
     constexpr int PA = F16 ? 2 : 1;
+    float apart[4] = {0.f, 0.f, 0.f, 0.f};
+    float(&c)[4] = EXACT ? apart : acc;
+    uint32_t b0[2][PA], b1[2][PA];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        uint32_t b0[PA], b1[PA];
-        adapter_planes<F16, PA>(h ? w.z : w.x, b0);
-        adapter_planes<F16, PA>(h ? w.w : w.y, b1);
-#pragma unroll
-        for (int px = 0; px < PX; ++px)
-#pragma unroll
-            for (int pa = 0; pa < PA; ++pa) mma_bf16(acc, f0[px][2 * h], f1[px][2 * h], f0[px][2 * h + 1], f1[px][2 * h + 1], b0[pa], b1[pa]);
+        adapter_planes<F16, PA>(h ? w.z : w.x, b0[h]);
+        adapter_planes<F16, PA>(h ? w.w : w.y, b1[h]);
     }
+#pragma unroll
+    for (int px = PX - 1; px >= 0; --px)
+#pragma unroll
+        for (int pa = PA - 1; pa >= 0; --pa)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) mma_bf16(c, f0[px][2 * h], f1[px][2 * h], f0[px][2 * h + 1], f1[px][2 * h + 1], b0[h][pa], b1[h][pa]);
+    if (EXACT)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] += apart[j];
 }
 
 // B t of sixteen rows and a chunk of 32 outputs: acc of column tile i: rows g, g + 8, outputs 8 t + 2 i, + 1.  fragments(k, w): the lane's two
@@ -182,10 +190,15 @@ template <bool F16, int PT, int UNROLL, typename Fragments> __device__ __forcein
             uint32_t b0[PA], b1[PA];
             adapter_planes<F16, PA>(i & 1 ? w[i >> 1].z : w[i >> 1].x, b0);
             adapter_planes<F16, PA>(i & 1 ? w[i >> 1].w : w[i >> 1].y, b1);
+            float apart[4] = {0.f, 0.f, 0.f, 0.f};       // (as in multiply_tile)
+            float(&c)[4] = PT == 3 ? apart : acc[i];
 #pragma unroll
-            for (int q = 0; q < PT; ++q)
+            for (int q = PT - 1; q >= 0; --q)
 #pragma unroll
-                for (int pa = 0; pa < PA; ++pa) mma_bf16(acc[i], f[q].x, f[q].y, f[q].z, f[q].w, b0[pa], b1[pa]);
+                for (int pa = PA - 1; pa >= 0; --pa) mma_bf16(c, f[q].x, f[q].y, f[q].z, f[q].w, b0[pa], b1[pa]);
+            if (PT == 3)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] += apart[j];
         }
     }
 }
@@ -580,7 +593,7 @@ __device__ __forceinline__ void few_pass(const AdaptersParams &p, const AdapterS
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
                 if (i >= tiles) break;
-                multiply_tile<F16, PX>(f[0], f[1], lds128(w + i * 512), acc[i]);
+                multiply_tile<F16, PX, YF32>(f[0], f[1], lds128(w + i * 512), acc[i]);
             }
             w += tiles * 512;
             if (--left == 0) {
@@ -774,7 +787,7 @@ struct AdapterTile {
     int step, to;                        // 16-byte words from chunk to chunk; its place in a row of t
     int slot;
 };
-template <bool F16, bool XF32> __global__ void __launch_bounds__(kThreads, 2) adapters_shrink_kernel(const __grid_constant__ AdaptersParams p) {
+template <bool F16, bool XF32, bool YF32> __global__ void __launch_bounds__(kThreads, 2) adapters_shrink_kernel(const __grid_constant__ AdaptersParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int slots[kShrinkRows];
     __shared__ int kind[kShrinkRows], kind_end[kShrinkRows];      // the slots that occur, and the rank tiles up to the end of each one's
@@ -897,7 +910,7 @@ template <bool F16, bool XF32> __global__ void __launch_bounds__(kThreads, 2) ad
 #pragma unroll
                     for (int i = 0; i < kSumTiles; ++i) {
                         if (!(wanted >> i & 1)) continue;
-                        multiply_tile<F16, PX>(f[0], f[1], *reinterpret_cast<const uint4 *>(stage + kShrinkX + ((c * kSumTiles + i) * 32 + lane) * 16), acc[i]);
+                        multiply_tile<F16, PX, YF32>(f[0], f[1], *reinterpret_cast<const uint4 *>(stage + kShrinkX + ((c * kSumTiles + i) * 32 + lane) * 16), acc[i]);
                     }
                 }
             __syncthreads();         // this stage has been read
@@ -1082,7 +1095,7 @@ template <bool F16, bool XF32, bool YF32> cudaError_t run(AdaptersParams p, int 
     const int room = (int)std::min<size_t>(t_floats / (size_t)p.t_ld / kStreamRows * kStreamRows, size_t(32767) * kStreamRows);
     for (int done = 0, all = p.m; done < all; done += room) {
         p.m = std::min(room, all - done);
-        cudaError_t e = launch(adapters_shrink_kernel<F16, XF32>, p, dim3((unsigned)((p.m + kShrinkRows - 1) / kShrinkRows), (unsigned)parts), dim3(1, (unsigned)parts),
+        cudaError_t e = launch(adapters_shrink_kernel<F16, XF32, YF32>, p, dim3((unsigned)((p.m + kShrinkRows - 1) / kShrinkRows), (unsigned)parts), dim3(1, (unsigned)parts),
                                kShrinkSmem, st);
         if (e != cudaSuccess) return e;
         e = launch(adapters_stream_kernel<F16, YF32>, p,

@@ -414,3 +414,21 @@ def test_refusals(backend, layer):
     no("contiguous int32", lambda: backend.apply_adapters([s], xa, torch.zeros(6, dtype=torch.int32, device="cuda")[::2], [y]))
     other.close()
     backend.sync()
+
+
+@pytest.mark.parametrize("m", [3, 600])
+@pytest.mark.parametrize("x_dtype,dtype", [(BF16, BF16), (F32, torch.float16)])
+def test_adapters_long_sums_keep_their_bits(backend, m, x_dtype, dtype):
+    """Sums of 16 thousand terms, fp32 results, relative root mean square error.  The tensor cores cut off what they add: on average a third
+    of 2^-23 of the sum so far.  A chunk of 32 terms is at most twelve such additions to sums that grow, half their number in effect: 6 * 0.3 * 2^-23 =
+    2.1e-7 of the chunk, and as much of the whole, chunks being independent; adding some 20 partial sums up in fp32 costs sqrt(10) 2^-24 / sqrt(3) =
+    1.1e-7, B t as much as a chunk again, 2.1e-7, the result's rounding 3e-8: 3.2e-7 together, and twice that is taken.  (All terms added on the
+    tensor cores to one sum: above 1e-6.)"""
+    g = torch.Generator().manual_seed(m)
+    s = Set(backend, 256, 16000, [16], dtype, 16, 61)
+    x = torch.randn((m, 16000), generator=g).to(x_dtype).cuda()
+    slots = torch.zeros(m, dtype=torch.int32, device="cuda")
+    y = torch.zeros(m, 256, device="cuda")
+    backend.apply_adapters([s.handle], x, slots, [y])
+    want, _ = s.want(x, slots, torch.zeros(m, 256))
+    assert float((y.cpu().double() - want).norm() / want.norm()) <= 6.4e-7
