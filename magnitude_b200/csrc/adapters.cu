@@ -802,6 +802,11 @@ template <bool F16, bool XF32, bool YF32> __global__ void __launch_bounds__(kThr
     constexpr int PX = XF32 ? 3 : 1, XB = XF32 ? 4 : 2, BATCH = batch_chunks(XF32);
     pdl_launch_dependents();
     pdl_wait();
+    // the thread's share of every piece of x: 16 bytes at x_at of rows x_row, x_row + 16, .., x_rows of which exist
+    const int x_at = tid & 15, x_row = tid >> 4, x_rows = min(max((p.m - base - x_row + 15) / 16, 0), kShrinkRows / 16);
+    const long long x_step = 16 * p.ldx * XB;
+    const uint8_t *x_from = reinterpret_cast<const uint8_t *>(p.x) + (long long)(base + x_row) * p.ldx * XB;
+    static_assert(kXBytes == 16 * 16 && kThreads == 16 * 16, "a thread's rows");
     auto tiles_in = [&](int set, int slot) { return active(p.set[set], slot) ? (p.set[set].rank[slot] + 7) / 8 : 0; };
     // the slots that occur, in the order of their first rows, and the tiles of each: all sets'
     int slot = -1;
@@ -836,7 +841,7 @@ template <bool F16, bool XF32, bool YF32> __global__ void __launch_bounds__(kThr
     if (first_row) kind[run.x - 1] = slot, kind_end[run.x - 1] = run.y;
     __syncthreads();
     // eight tiles at a time, of whichever adapters: x is read once for all of them
-    for (int first = 0; first < all_tiles; first += kSumTiles) {
+    for (int first = blockIdx.z * kSumTiles; first < all_tiles; first += gridDim.z * kSumTiles) {
         const int tiles = min(all_tiles - first, kSumTiles);
         if (tid < tiles) {
             int k = 0;
@@ -860,28 +865,27 @@ template <bool F16, bool XF32, bool YF32> __global__ void __launch_bounds__(kThr
             for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
         auto fetch = [&](int kc, uint8_t *stage) {
             const int chunks = min(BATCH, kc1 - kc);
-            for (int i = tid; i < kShrinkRows * (kXBytes / 16); i += kThreads) {      // 16 bytes of a row; zeros beyond the rows and K
-                const int r = i / (kXBytes / 16), unit = i % (kXBytes / 16), k = kc * 32 + unit * 16 / XB;
-                const long long row = base + r;
-                const uint8_t *from = reinterpret_cast<const uint8_t *>(p.x) + (row * p.ldx + k) * XB;
-                uint8_t *to = stage + r * kXBytes + 16 * x_unit<XF32>(r, unit);
-                const int left = row < p.m && unit * 16 < chunks * 32 * XB ? min(max((p.K - k) * XB, 0), 16) : 0;
-                if (p.x_vec) {
-                    if (left == 0) from = reinterpret_cast<const uint8_t *>(p.x);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(left) : "memory");
-                } else {
-                    const uint4 w = load_words<XF32>(from, left / XB);
-                    *reinterpret_cast<uint4 *>(to) = w;
-                }
+            // 16 bytes of every sixteenth row; zeros beyond the rows and K
+            const int k = kc * 32 + x_at * 16 / XB, left = x_at * 16 < chunks * 32 * XB ? min(max((p.K - k) * XB, 0), 16) : 0;
+            const uint8_t *from = x_from + (long long)k * XB;
+            uint8_t *to = stage + x_row * kXBytes + 16 * x_unit<XF32>(x_row, x_at);
+#pragma unroll
+            for (int j = 0; j < kShrinkRows / 16; ++j) {
+                const int bytes = j < x_rows ? left : 0;
+                if (p.x_vec)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to) + j * 16 * kXBytes), "l"(bytes ? from : reinterpret_cast<const uint8_t *>(p.x)), "r"(bytes) : "memory");
+                else
+                    *reinterpret_cast<uint4 *>(to + j * 16 * kXBytes) = load_words<XF32>(from, bytes / XB);
+                from += x_step;
             }
             for (int i = warp; i < tiles; i += kWarps) {
                 const AdapterTile tile = tiles_of[i];
-                for (int c = 0; c < chunks; ++c)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(stage + kShrinkX + ((c * kSumTiles + i) * 32 + lane) * 16)),
-                                 "l"(tile.from + (size_t)(kc + c) * tile.step + lane)
-                                 : "memory");
+                const uint4 *src = tile.from + (size_t)kc * tile.step + lane;
+                uint32_t dst = smem_u32(stage + kShrinkX + (i * 32 + lane) * 16);
+                for (int c = 0; c < chunks; ++c, src += tile.step, dst += kSumTiles * 512)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
         };
         int turn = 0;
         if (kc0 < kc1) fetch(kc0, smem);
@@ -1095,7 +1099,9 @@ template <bool F16, bool XF32, bool YF32> cudaError_t run(AdaptersParams p, int 
     const int room = (int)std::min<size_t>(t_floats / (size_t)p.t_ld / kStreamRows * kStreamRows, size_t(32767) * kStreamRows);
     for (int done = 0, all = p.m; done < all; done += room) {
         p.m = std::min(room, all - done);
-        cudaError_t e = launch(adapters_shrink_kernel<F16, XF32, YF32>, p, dim3((unsigned)((p.m + kShrinkRows - 1) / kShrinkRows), (unsigned)parts), dim3(1, (unsigned)parts),
+        // blocks that take other rank tiles of the same rows (of two adapters, mostly): while there are SMs for them
+        const int row_tiles = (p.m + kShrinkRows - 1) / kShrinkRows, apart = std::max(1, std::min((2 * p.t_ld / 8 + kSumTiles - 1) / kSumTiles, 2 * sm_count / (row_tiles * parts)));
+        cudaError_t e = launch(adapters_shrink_kernel<F16, XF32, YF32>, p, dim3((unsigned)row_tiles, (unsigned)parts, (unsigned)apart), dim3(1, (unsigned)parts),
                                kShrinkSmem, st);
         if (e != cudaSuccess) return e;
         e = launch(adapters_stream_kernel<F16, YF32>, p,
