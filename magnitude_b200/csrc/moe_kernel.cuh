@@ -462,12 +462,13 @@ __device__ __forceinline__ void moe_multiply(MoeRing<D> &ring, MoeHead &head, co
                                              int n, bool active, int warp, int lane, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
     constexpr int REC = moe_rec_bytes(QT);
     auto work = [&](auto mode, auto more) {
+        uint32_t full = smem_u32(head.full) + 8 * ring.stage, at = ring.stage * stage_bytes;
+        asm volatile("" : "+r"(lane));       // (kept in a register: read again every step, it would be a wait every step)
         for (int s = 0; s < steps; ++s) {
             // after a failure the products are left out, but shared sums are still counted
-            ring.ok = ring.ok && __all_sync(0xFFFFFFFFu, ring_wait(smem_u32(&head.full[ring.stage]), ring.phase, &head.fail, status));
+            ring.ok = ring.ok && __all_sync(0xFFFFFFFFu, ring_wait(full, ring.phase, &head.fail, status));
             if (!ring.ok) break;
             if (active) {
-                uint32_t at = ring.stage * stage_bytes;
                 MoeRecord<QT, P>::template run<decltype(mode)>(smem + at + warp * REC, lane, smem + at + kMoeWarps * REC, zero, col, acc);
                 if constexpr (decltype(more)::NL > 0) {
                     asm volatile("" : "+r"(at)::"memory");       // the weights are unpacked again, not kept
@@ -475,8 +476,10 @@ __device__ __forceinline__ void moe_multiply(MoeRing<D> &ring, MoeHead &head, co
                 }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&head.empty[ring.stage]));
+            if (lane == 0) mbar_arrive(full + (uint32_t)sizeof(head.full));      // (empty lies behind full)
+            full += 8, at += stage_bytes;
             ring.next();
+            if (ring.stage == 0) full -= 8 * D, at = 0;
         }
     };
     using None = MoeMode<0, 1>;
@@ -537,7 +540,6 @@ __device__ __forceinline__ void moe_produce(MoeRing<D> &ring, bool &full_ring, M
         const uint32_t bar = smem_u32(&head.full[ring.stage]);
         if (what & kMoeWeightsAlone) {
             if (lane < kMoeGroupLanes) reinterpret_cast<int2 *>(&head.group[ring.stage])[lane] = words;
-            fence_proxy_async();             // the readers' last accesses precede the copies
             __syncwarp();
             if (lane == 0) mbar_expect_tx(bar, tiles * REC + n * IMG);
         }
