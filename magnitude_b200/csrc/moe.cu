@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(256) moe_repack_kernel(const MoeRepack p, long
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int rec = (int)(id % p.nrec), tile = (int)(id / p.nrec % p.tiles);
     const long long expert = id / p.nrec / p.tiles;
-    uint8_t *out = p.dst + expert * p.dst_expert + ((long long)tile * p.nrec + rec) * moe_rec_bytes(p.qt);
+    uint8_t *out = p.dst + expert * p.dst_expert + moe_record_at(tile, rec, p.tiles, p.nrec) * moe_rec_bytes(p.qt);
     // row i of the tile, or null beyond the matrix
     auto row_of = [&](int i) -> const uint8_t * {
         const int r = p.paired ? tile * 8 + (i & 7) : tile * 16 + i;

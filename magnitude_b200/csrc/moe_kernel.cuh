@@ -527,11 +527,11 @@ __device__ __forceinline__ void moe_produce(MoeRing<D> &ring, bool &full_ring, M
     const int even = __shfl_sync(0xFFFFFFFFu, words.x, 1 + lane % kMoeGroupRows / 2), odd = __shfl_sync(0xFFFFFFFFu, words.y, 1 + lane % kMoeGroupRows / 2);
     const int row = ((lane & 1 ? odd : even) >> p.shift) & 0xFFFF;      // of the images
     const int tiles = min(kMoeWarps, w.tiles - tile0);
-    // lanes 0 .. 7: the record of a tile; lanes 16 .. 31: the image of a row
-    const bool copies = lane < 16 ? (what & kMoeWeightsAlone) && lane < tiles : (what & kMoeImagesAlone) && lane - 16 < n;
-    const uint8_t *src = lane < 16 ? w.w + expert * w.expert_bytes + ((long long)(tile0 + lane) * w.nrec + r0) * REC
+    // lane 0: the tiles' records; lanes 16 .. 31: the image of a row
+    const bool copies = lane < 16 ? (what & kMoeWeightsAlone) && lane == 0 : (what & kMoeImagesAlone) && lane - 16 < n;
+    const uint8_t *src = lane < 16 ? w.w + expert * w.expert_bytes + moe_record_at(tile0, r0, w.tiles, w.nrec) * REC
                                    : p.img + (size_t)(lane - 16 < n ? row : 0) * p.img_stride + (size_t)r0 * IMG;
-    const uint32_t at = lane < 16 ? lane * REC : kMoeWarps * REC + (lane - 16) * IMG, size = lane < 16 ? REC : IMG;
+    const uint32_t at = lane < 16 ? 0 : kMoeWarps * REC + (lane - 16) * IMG, size = lane < 16 ? tiles * REC : IMG;
     for (int s = 0; s < steps; ++s) {
         if (full_ring) {
             ring.ok = __all_sync(0xFFFFFFFFu, ring_wait(smem_u32(&head.empty[ring.stage]), ring.phase ^ 1, &head.fail, p.status));

@@ -83,18 +83,21 @@ template <int QT, int P> __global__ void __launch_bounds__(kOneThreads, 2) moe_o
     // the record that is fetched next: unit fu, record fr
     int fu = blockIdx.x, fr = warp;
     const uint8_t *from = nullptr;
+    int step = 0;                        // bytes from record to record of the tile
     auto seek = [&]() {                  // from fu on, the first unit that has an expert
         for (; fu < units; fu += gridDim.x) {
             const int e = expert_of(fu);
             if ((unsigned)e < (unsigned)p.choice.experts) {
-                from = w.w + e * w.expert_bytes + (long long)(fu % w.tiles) * w.nrec * REC;
+                const int tile = fu % w.tiles;
+                from = w.w + e * w.expert_bytes + moe_record_at(tile, 0, w.tiles, w.nrec) * REC;
+                step = min(kMoeWarps, w.tiles - tile / kMoeWarps * kMoeWarps) * REC;
                 break;
             }
         }
     };
     auto fetch = [&]() {
         if (fr >= w.nrec || fu >= units) return;
-        ring.fill(from + (long long)fr * REC, REC, lane);
+        ring.fill(from + (long long)fr * step, REC, lane);
         fr += kMoeWarps;
         if (fr >= w.nrec && warp < w.nrec) fr = warp, fu += gridDim.x, seek();
     };
@@ -165,7 +168,7 @@ template <int QT, int P> __global__ void __launch_bounds__(kOneThreads, 2) moe_o
             const int c = fj / w.nrec, r = fj - c * w.nrec, t = ft, e = __shfl_sync(0xFFFFFFFFu, id, c);
             if (++fj == j1) fj = j0, ft += gridDim.x;
             if ((unsigned)e < (unsigned)p.choice.experts) {
-                ring.fill(w.w + e * w.expert_bytes + ((long long)t * w.nrec + r) * REC, REC, lane);
+                ring.fill(w.w + e * w.expert_bytes + moe_record_at(t, r, w.tiles, w.nrec) * REC, REC, lane);
                 return;
             }
         }

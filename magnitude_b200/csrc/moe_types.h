@@ -8,9 +8,9 @@ namespace b200q {
 // ---------------------------------------------------------------------------------------------
 // Weights of experts
 //
-// An expert's matrix is cut into tiles of 16 rows x 256 weights ("records"); the records of a tile of rows follow each
-// other, then the next tile's, then the next expert's.  A warp multiplies one record at a time, so a record is one
-// contiguous piece of memory, and inside it the weights lie in the order in which the lanes of a warp take them as the A
+// An expert's matrix is cut into tiles of 16 rows x 256 weights ("records"); A block
+// multiplies eight tiles side by side (a "run"), one record of each at a time, and those eight lie next to each other: one copy brings them.  Run
+// after run, inside a run 256 weights after 256 weights.  Inside a record the weights lie in the order in which the lanes of a warp take them as the A
 // operand of mma.m16n8k32: lane 4 g + t owns, of rows g and g + 8 and of every block of 32 weights, weights 4 t .. 4 t + 3 and
 // 16 + 4 t .. 16 + 4 t + 3.  The 16-byte vectors of the 32 lanes lie side by side, so both the copy into shared memory and the
 // reads from it are whole 512-byte lines.  Gate and up of the gated product share tiles: rows 0 .. 7 of a tile are
@@ -59,6 +59,12 @@ __host__ __device__ constexpr int moe_depth(int qt, int planes, int column_tiles
 }
 
 constexpr int kMoeMaxRows = 512, kMoeMaxTopK = 16, kMoeMaxSlots = kMoeMaxRows * kMoeMaxTopK, kMoeMaxExperts = 1024;
+
+// where a record lies in an expert's matrix, in records (the last run may have fewer tiles)
+__host__ __device__ __forceinline__ long long moe_record_at(int tile, int rec, int tiles, int nrec) {
+    const int run = tile / kMoeWarps * kMoeWarps, wide = tiles - run < kMoeWarps ? tiles - run : kMoeWarps;
+    return (long long)run * nrec + (long long)rec * wide + (tile - run);
+}
 
 // rows of one expert that are multiplied together
 constexpr int kMoeGroupRows = 16;
