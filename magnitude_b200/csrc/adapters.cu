@@ -1,19 +1,20 @@
 // Low-rank adapters of many requests beside a shared projection: y[m] += scale * B (A x[m]) with the adapter that row m picks.
 //
 //   * up to kFewRows rows (sequences decoding together, in any order, or the pieces of a few prompts): one launch of clusters of eight blocks.
-//     A cluster takes up to sixteen rows of one adapter and one projection at a time; its blocks split K for t = A x, add their parts
-//     up through distributed shared memory in the order of the blocks, and split N for y += scale * B t, so t never leaves the SMs.
-//     Every block finds the rows of each adapter for itself.
-//   * more rows (long runs of one adapter): two launches, t = A x for tiles of 32 rows (K cut into a few ranges to fill the chip), then
-//     y += scale * B t as one stream over y.  A tile takes the adapters that occur among its rows one after the other.
+//     An item is up to sixteen rows of one adapter and one projection; one, two, four or eight blocks of a cluster take it, by its bytes: they
+//     split K for t = A x, add their parts up through distributed shared memory in the order of the blocks, and split N for y += scale * B t,
+//     so t never leaves the SMs.  Every block finds the rows of each adapter for itself.
+//   * more rows (long runs of one adapter): two launches, t = A x for tiles of 128 rows (K cut into up to eight ranges, joined the same way),
+//     then y += scale * B t as one stream over y.
 // Both products run on mma.sync.m16n8k16 with bf16 operands and fp32 sums, the rows as M.  Operands of more bits are cut into
 // bf16 planes: fp32 activations three (exact), fp16 adapters two (exact), t three where y is fp32 (exact) and two where y
 // is rounded to bf16 anyway (an error of at most 2^-15 of t).  The adapters are kept in fragment order, so a load is 512 bytes a warp.
+// Measured (us on the device): one row, 4096 x 4096, rank 16: 6.7; 48 rows of 33 adapters, ranks 8 to 64, q, k and v of K 4096: 22.5 (39 MB, 1.7 TB/s; the
+// bytes alone 6.1); 333 rows of fp32 x 11003 outputs: 28; 4096 rows of K 5120, gate and up of 25600 outputs: 210 (of which y, read and
+// written once, 130).
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <mutex>
-#include <vector>
 
 #include "adapters.h"
 #include "launch.h"
@@ -520,9 +521,9 @@ static_assert(few_sums(true) >= size_t(kWarps) * 16 * kTileLd * 4, "a piece of o
 size_t few_smem(int rank_pad, int planes, bool x_f32) { return kFewRing + few_sums(x_f32) + size_t(16) * rank_pad * 4 + size_t(rank_pad / 16) * planes * 512; }
 
 // One adapter against up to sixteen rows.  A warp takes neighbouring chunks of K, then of N; the fragments of A and then of B come through its ring in
-// pieces of 4 KB (of a small rank, those of several chunks), so that B is on its way while t is joined; rows of x are asked for two chunks ahead,
-// rows of y one.  What a step costs is the instructions of one warp after the other, more than their number: hence few and large pieces, and
-// buffers that take turns (a copy from one to the other would wait for the load).
+// pieces of 4 KB (of a small rank, those of several chunks), so that B is on its way while t is joined; x is asked for a chunk ahead.  What
+// bounds a warp is its instructions one after the other, at some four cycles each, not their number or the bytes: hence few and large pieces, one copy of
+// the loop for all chunks (two that took turns: no faster, the code no longer fitted its cache) and no register that is put by (a third slower).
 template <bool F16, bool XF32, bool YF32>
 __device__ __forceinline__ void few_pass(const AdaptersParams &p, const AdapterSet &s, int slot, const int *row, const long long *row_at, int log_parts, int copy, int copies, uint8_t *memory, WarpRing<kFewDepth> &ring,
                                          volatile int *fail) {
@@ -1032,19 +1033,18 @@ template <typename Kernel> cudaError_t launch(Kernel kern, const AdaptersParams 
     return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
-// Clusters of eight blocks of a kernel that run at a time; asked for once per kernel, shared memory and device
+// Clusters of eight blocks of a kernel that run at a time; a thread remembers what it asked for last
 cudaError_t resident_clusters(const void *kern, size_t smem, int sm_count, int *out) {
     struct Known {
         const void *kern;
         size_t smem;
         int device, clusters;
     };
-    static std::mutex mutex;
-    static std::vector<Known> known;
+    static thread_local Known known[16];
+    static thread_local unsigned next = 0;
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return e;
-    std::lock_guard<std::mutex> lock(mutex);
     for (const Known &k : known)
         if (k.kern == kern && k.smem == smem && k.device == device) {
             *out = k.clusters;
@@ -1064,7 +1064,7 @@ cudaError_t resident_clusters(const void *kern, size_t smem, int sm_count, int *
     int n = 0;
     if ((e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg)) != cudaSuccess) return e;
     *out = std::max(n, 1);
-    known.push_back(Known{kern, smem, device, *out});
+    known[next++ % 16] = Known{kern, smem, device, *out};
     return cudaSuccess;
 }
 
