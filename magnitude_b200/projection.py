@@ -159,6 +159,13 @@ class Backend:
         return ProjectionWeight(self, out.value)
 
     # -- device-pointer path (torch tensors hold the memory) ---------------------------------
+    def _row_stream(self, stream) -> c_void_p:
+        """The stream a call on this GPU's tensors belongs to: the current one of this GPU, whichever is the current GPU."""
+        raw = getattr(_torch()._C, "_cuda_getCurrentRawStream", None)
+        if stream is not None or raw is None:
+            return self._stream_ptr(_torch().cuda.current_stream(self.device) if stream is None else stream)
+        return c_void_p(raw(self.device))
+
     @staticmethod
     def _stream_ptr(stream) -> c_void_p:
         if stream is None:
@@ -310,7 +317,7 @@ class Backend:
             out = torch.empty((m, layer.n_embd), dtype=out_dtype or torch.float32, device=x.device)
         yp, yd, ldy = matrix(out, "out", self.device, layer.n_embd, _TORCH_DTYPE, m)
         self._check(B.lib().b200q_moe_run(self._h, layer._h, xp, xd, m, ldx, ip, ldi, wp, ldw, yp, yd, ldy,
-                                          B.MOE_ACCUMULATE if accumulate else 0, self._stream_ptr(stream)))
+                                          B.MOE_ACCUMULATE if accumulate else 0, self._row_stream(stream)))
         return out
 
     def router(self, weight, top_k: int, *, scoring: int = B.SCORING_SOFTMAX, normalise: bool = True, scale: float = 1.0, logit_bias=None,
@@ -330,7 +337,7 @@ class Backend:
             weights = torch.empty((m, router.top_k), dtype=torch.float32, device=x.device)
         ip, _, ldi = matrix(ids, "ids", self.device, router.top_k, {torch.int32: 0}, m)
         wp, _, ldw = matrix(weights, "weights", self.device, router.top_k, {torch.float32: 0}, m)
-        self._check(B.lib().b200q_router_run(self._h, router._h, xp, xd, m, ldx, ip, ldi, wp, ldw, self._stream_ptr(stream)))
+        self._check(B.lib().b200q_router_run(self._h, router._h, xp, xd, m, ldx, ip, ldi, wp, ldw, self._row_stream(stream)))
         return ids, weights
 
     def adapters(self, n: int, k: int, dtype, max_adapters: int, max_rank: int) -> AdapterSet:
@@ -345,8 +352,7 @@ class Backend:
             raise invalid("apply_adapters takes 1..4 sets and as many outputs")
         xp, xd, ldx = matrix(x, "x", self.device, sets[0].k, _TORCH_DTYPE)
         m = x.shape[0]
-        if slots.dim() != 1 or slots.dtype != torch.int32 or slots.shape[0] != m or not slots.is_cuda or slots.device.index != self.device or (
-                m > 1 and slots.stride(0) != 1):
+        if slots.dtype != torch.int32 or slots.shape != (m,) or slots.get_device() != self.device or (m > 1 and slots.stride(0) != 1):
             raise invalid(f"slots is {slots.dtype} {tuple(slots.shape)} on {slots.device}, not contiguous int32 ({m},) on cuda:{self.device}")
         n = len(sets)
         parts = [matrix(o, "an output", self.device, s.n, _TORCH_DTYPE, m) for s, o in zip(sets, outs)]
@@ -354,7 +360,7 @@ class Backend:
             raise invalid("the outputs of one call are of one dtype")
         self._check(B.lib().b200q_adapters_apply(
             self._h, (c_void_p * n)(*[s._h for s in sets]), n, xp, xd, m, ldx, slots.data_ptr(), (c_void_p * n)(*[p[0] for p in parts]),
-            parts[0][1], (c_int64 * n)(*[p[2] for p in parts]), self._stream_ptr(stream)))
+            parts[0][1], (c_int64 * n)(*[p[2] for p in parts]), self._row_stream(stream)))
         return outs
 
     # -- host-buffer path (the reference's own boundary: host in, host out) ------------------
