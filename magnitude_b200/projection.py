@@ -18,14 +18,20 @@ from . import _binding as B
 from .rows import AdapterSet, MoeLayer, Router, invalid, matrix
 
 _TORCH_DTYPE = {}
+_INT32, _FLOAT32 = {}, {}                # what choices and their weights may be, filled likewise
+_POINTERS, _INTS = [c_void_p * n for n in range(5)], [c_int64 * n for n in range(5)]
+_torch_module = None
 
 
 def _torch():
-    import torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
 
-    if not _TORCH_DTYPE:
         _TORCH_DTYPE.update({torch.float32: B.TYPE_F32, torch.bfloat16: B.TYPE_BF16})
-    return torch
+        _INT32[torch.int32], _FLOAT32[torch.float32] = 0, 0
+        _torch_module = torch
+    return _torch_module
 
 
 def tensor_storage_bytes(qtype: int, n_elements: int) -> int:
@@ -311,8 +317,8 @@ class Backend:
             raise invalid("accumulate needs an output to add to")
         xp, xd, ldx = matrix(x, "x", self.device, layer.n_embd, _TORCH_DTYPE)
         m = x.shape[0]
-        ip, _, ldi = matrix(ids, "ids", self.device, layer.top_k, {torch.int32: 0}, m)
-        wp, _, ldw = matrix(weights, "weights", self.device, layer.top_k, {torch.float32: 0}, m)
+        ip, _, ldi = matrix(ids, "ids", self.device, layer.top_k, _INT32, m)
+        wp, _, ldw = matrix(weights, "weights", self.device, layer.top_k, _FLOAT32, m)
         if out is None:
             out = torch.empty((m, layer.n_embd), dtype=out_dtype or torch.float32, device=x.device)
         yp, yd, ldy = matrix(out, "out", self.device, layer.n_embd, _TORCH_DTYPE, m)
@@ -335,8 +341,8 @@ class Backend:
             ids = torch.empty((m, router.top_k), dtype=torch.int32, device=x.device)
         if weights is None:
             weights = torch.empty((m, router.top_k), dtype=torch.float32, device=x.device)
-        ip, _, ldi = matrix(ids, "ids", self.device, router.top_k, {torch.int32: 0}, m)
-        wp, _, ldw = matrix(weights, "weights", self.device, router.top_k, {torch.float32: 0}, m)
+        ip, _, ldi = matrix(ids, "ids", self.device, router.top_k, _INT32, m)
+        wp, _, ldw = matrix(weights, "weights", self.device, router.top_k, _FLOAT32, m)
         self._check(B.lib().b200q_router_run(self._h, router._h, xp, xd, m, ldx, ip, ldi, wp, ldw, self._row_stream(stream)))
         return ids, weights
 
@@ -355,12 +361,14 @@ class Backend:
         if slots.dtype != torch.int32 or slots.shape != (m,) or slots.get_device() != self.device or (m > 1 and slots.stride(0) != 1):
             raise invalid(f"slots is {slots.dtype} {tuple(slots.shape)} on {slots.device}, not contiguous int32 ({m},) on cuda:{self.device}")
         n = len(sets)
-        parts = [matrix(o, "an output", self.device, s.n, _TORCH_DTYPE, m) for s, o in zip(sets, outs)]
-        if any(p[1] != parts[0][1] for p in parts):
-            raise invalid("the outputs of one call are of one dtype")
-        self._check(B.lib().b200q_adapters_apply(
-            self._h, (c_void_p * n)(*[s._h for s in sets]), n, xp, xd, m, ldx, slots.data_ptr(), (c_void_p * n)(*[p[0] for p in parts]),
-            parts[0][1], (c_int64 * n)(*[p[2] for p in parts]), self._row_stream(stream)))
+        handles, ptrs, lds, dtype = _POINTERS[n](), _POINTERS[n](), _INTS[n](), None
+        for i in range(n):
+            handles[i] = sets[i]._h.value
+            ptrs[i], d, lds[i] = matrix(outs[i], "an output", self.device, sets[i].n, _TORCH_DTYPE, m)
+            if dtype is not None and d != dtype:
+                raise invalid("the outputs of one call are of one dtype")
+            dtype = d
+        self._check(B.lib().b200q_adapters_apply(self._h, handles, n, xp, xd, m, ldx, slots.data_ptr(), ptrs, dtype, lds, self._row_stream(stream)))
         return outs
 
     # -- host-buffer path (the reference's own boundary: host in, host out) ------------------
