@@ -310,7 +310,7 @@ long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
     }
 cudaError_t few_down(int qt, const MoeFewDown &p, int planes, int tiles, int grid, cudaStream_t st) { MOE_BY_TYPE(moe_few_down, p, planes, tiles, grid, st) }
 cudaError_t gate_up_launch(int qt, const MoeGateUp &p, int planes, int tiles, int grid, cudaStream_t st) { MOE_BY_TYPE(moe_gate_up, p, planes, tiles, grid, st) }
-cudaError_t many_down(int qt, const MoeDown &p, int planes, int grid, cudaStream_t st) { MOE_BY_TYPE(moe_down, p, planes, grid, st) }
+cudaError_t many_down(int qt, const MoeDown &p, int planes, int tiles, int grid, cudaStream_t st) { MOE_BY_TYPE(moe_down, p, planes, tiles, grid, st) }
 size_t one_smem(int qt, int planes, int records) { MOE_BY_TYPE(moe_one_smem, planes, records) }
 cudaError_t one_gate_up(int qt, const MoeOneGateUp &p, int planes, int grid, cudaStream_t st) { MOE_BY_TYPE(moe_one_gate_up, p, planes, grid, st) }
 cudaError_t one_down(int qt, const MoeOneDown &p, int planes, int grid, cudaStream_t st) { MOE_BY_TYPE(moe_one_down, p, planes, grid, st) }
@@ -367,6 +367,19 @@ size_t moe_workspace(const MoeShapeInfo &s, MoeBuffers *out, uint8_t *base) {
     return at;
 }
 
+// Column tiles of a group, by how many rows an expert has on average.  Fewer tiles are fewer registers and instructions; more of them share a group's
+// weights.  One or two, us: 128 experts of 2048 x 768, Q4_K and Q6_K, 1 row an expert 52.8 : 56.4, 2: 75.0 : 77.1, 4: 104 : 98 (a tile holds four
+// rows; with 31-bit activations two, and 2 rows an expert are 99 : 84); Q8_0, 2.3 rows: 144 : 129.  Two or four: the K types, whose scales are
+// integers, lose by four tiles' double unpacking at 4 to 40 rows an expert (98 : 134, 217 : 258, 90 : 96; 31 bits: 6 rows 60 : 72) and gain later (31 bits,
+// 24 rows: 572 : 558); Q4_0 and MXFP4 gain from about two tiles' rows on (9 rows 186 : 175; 31 bits 3.8 rows 101 : 110, 9 rows 183 : 172), Q8_0, which
+// needs no unpacking, later (9 rows 137 : 142, 48 rows 489 : 402).
+static int group_tiles(int qt, int planes, bool few, double rows_per_expert) {
+    const double tile_rows = 8.0 / planes;
+    if (few) return rows_per_expert * 2 <= tile_rows ? 1 : 2;
+    const double most = qt == QT_Q4_K || qt == QT_Q5_K || qt == QT_Q6_K ? 5.5 : qt == QT_Q8_0 ? 2.0 : 1.0;
+    return rows_per_expert > most * 2 * tile_rows ? kMoeManyTiles : 2;
+}
+
 cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches) {
     const MoeShapeInfo &s = r.shape;
     const int slots = r.choice.m * (int)s.top_k, grid = 2 * s.sm_count;
@@ -394,7 +407,7 @@ cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches) {
     h.img = r.buf.h_img;
     h.img_stride = (unsigned)(h_rec * moe_image_bytes(planes));
     const bool few = r.choice.m <= kMoeFewRows;
-    const int tiles = !few ? kMoeManyTiles : r.choice.m * planes <= 8 ? 1 : 2;
+    const int tiles = group_tiles(r.gate_up_type, planes, few, (double)slots / s.n_experts);
     const int warps = kPrepThreads / 32, spread = s.sm_count;
     const MoePrep pr{x, r.choice, moe_group_rows(planes, tiles), r.buf.lists};
     const unsigned x_grid = 1 + (unsigned)std::min<long long>(ceil_div((long long)r.choice.m * x_rec, warps), spread);
@@ -413,7 +426,7 @@ cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches) {
         return few_down(r.down_type, d, planes, tiles, grid, st);
     }
     const MoeDown d{product(down, h, 0), r.buf.z, ceil_div(s.n_embd, 16) * 16};
-    if ((e = many_down(r.down_type, d, planes, grid, st)) != cudaSuccess) return e;
+    if ((e = many_down(r.down_type, d, planes, tiles, grid, st)) != cudaSuccess) return e;
     const MoeCombine cb{r.choice, r.out, r.buf.z, d.ld_z};
     *launches = 5;
     return launch(moe_combine_kernel, cb, dim3((unsigned)ceil_div(s.n_embd, 256), (unsigned)r.choice.m), 256, st);

@@ -839,6 +839,9 @@ template <typename Kernel, typename Params> cudaError_t moe_launch(Kernel kern, 
         return tiles <= 2 ? few(p, planes, tiles, grid, st) : many(p, planes, grid, st);                                              \
     }                                                                                                                             \
     cudaError_t moe_few_down_##NAME(const MoeFewDown &p, int planes, int tiles, int grid, cudaStream_t st) { return few(p, planes, tiles, grid, st); } \
-    cudaError_t moe_down_##NAME(const MoeDown &p, int planes, int grid, cudaStream_t st) { return many(p, planes, grid, st); }       \
+    cudaError_t moe_down_##NAME(const MoeDown &p, int planes, int tiles, int grid, cudaStream_t st) {                               \
+        if (tiles > 2) return many(p, planes, grid, st);                                                                              \
+        return planes == 2 ? MoeKernels<2, 2>::run(p, grid, st) : MoeKernels<4, 2>::run(p, grid, st);                                 \
+    }                                                                                                                             \
     cudaError_t moe_wait_limit_##NAME(unsigned long long ns) { return cudaMemcpyToSymbol(s_wait_limit_ns, &ns, sizeof(ns)); }        \
     }

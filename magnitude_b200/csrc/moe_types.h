@@ -41,14 +41,14 @@ __host__ __device__ constexpr int moe_rec_bytes(int qt) { return 16 * (qt == QT_
 __host__ __device__ constexpr int moe_image_bytes(int planes) { return planes * (256 + 16) + 16; }
 
 constexpr int kMoeThreads = 32 * (kMoeWarps + 1);      // with the producer
-constexpr int kMoeFewRows = 16;          // up to so many rows their outputs are added up inside the down product
+constexpr int kMoeFewRows = 32;          // up to so many rows their outputs are added up inside the down product
 constexpr int kMoeManyTiles = 4;         // column tiles of a group of more rows
 
 // A block's ring: a stage holds eight records and the images of a group's rows.  As many stages (2 to 4) as leave room for two blocks an
-// SM: half of 228 KB each, less 1 KB that a block costs by itself and what it has beside the ring (few rows: 8 KB of outputs).
-constexpr int kMoeSmem = 113664, kMoeFewSmem = 105472, kMoeMaxDepth = 4;
+// SM: half of 228 KB each, less 1 KB that a block costs by itself and what it has beside the ring (few rows: 16 KB of outputs).
+constexpr int kMoeSmem = 113664, kMoeFewSmem = 97280, kMoeMaxDepth = 4;
 constexpr int kMoeOneSmem = 112640;      // (the same for one row, less what is beside)
-constexpr int kMoePart = 256;            // floats of a warp's share of a cut unit: two per lane and column tile, or 16 outputs of 16 rows
+constexpr int kMoePart = 16 * kMoeFewRows;            // floats of a warp's share of a cut unit: two per lane and column tile, or 16 outputs of the rows
 __host__ __device__ constexpr int moe_group_rows(int planes, int column_tiles) { return column_tiles * 8 / planes; }
 __host__ __device__ constexpr int moe_stage_bytes(int qt, int planes, int column_tiles) {
     return kMoeWarps * moe_rec_bytes(qt) + moe_group_rows(planes, column_tiles) * moe_image_bytes(planes);
@@ -201,7 +201,7 @@ cudaError_t moe_run(const MoeRun &r, cudaStream_t st, int *launches);
 #define MOE_DECLARE(NAME)                                                                                               \
     cudaError_t moe_gate_up_##NAME(const MoeGateUp &p, int planes, int tiles, int grid, cudaStream_t st);                 \
     cudaError_t moe_few_down_##NAME(const MoeFewDown &p, int planes, int tiles, int grid, cudaStream_t st);               \
-    cudaError_t moe_down_##NAME(const MoeDown &p, int planes, int grid, cudaStream_t st);                                 \
+    cudaError_t moe_down_##NAME(const MoeDown &p, int planes, int tiles, int grid, cudaStream_t st);                      \
     size_t moe_one_smem_##NAME(int planes, int records);                                                                  \
     cudaError_t moe_one_gate_up_##NAME(const MoeOneGateUp &p, int planes, int grid, cudaStream_t st);                     \
     cudaError_t moe_one_down_##NAME(const MoeOneDown &p, int planes, int grid, cudaStream_t st);                          \

@@ -20,7 +20,7 @@ from test_gpu_moe import Case  # noqa: E402
 from test_gpu_moe import _check as check_moe  # noqa: E402
 
 BF16, F32 = torch.bfloat16, torch.float32
-ROWS = [1, 2, 7, 16, 17, 40]          # every launch plan of an expert layer: one row, a few, more
+ROWS = [1, 2, 7, 16, 32, 33, 40]      # every launch plan of an expert layer: one row, a few, more
 
 
 @pytest.fixture(scope="module")
