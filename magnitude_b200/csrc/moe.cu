@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(256) moe_repack_kernel(const MoeRepack p, long
         }
     }
     if (p.qt == QT_Q5_K) at = 2560;
-    if (p.qt == QT_Q6_K) at = 3072;
+    if (p.qt == QT_Q6_K) at = 6 * 512;
     if (p.qt == QT_Q8_0) at = 4096;
     if (p.qt == QT_MXFP4) bytes = 8;
     for (int i = 0; i < bytes; ++i) out[at + bytes * lane + i] = head[i];

@@ -195,7 +195,7 @@ template <int P> struct MoeRecord<QT_Q6_K, P> {
     static __device__ __forceinline__ void run(const uint8_t *rec, int lane, const uint8_t *img, const uint8_t *zero, const MoeColumns<NT> &col, float (&acc)[NT][2]) {
         constexpr int NL = Mode::NL, F = Mode::F, O = Mode::O;
         const int g = lane >> 2;
-        const uint4 s0 = moe_lds(rec + 3072 + 16 * g), s1 = moe_lds(rec + 3072 + 16 * g + 128);
+        const uint4 s0 = moe_lds(rec + 6 * 512 + 16 * g), s1 = moe_lds(rec + 6 * 512 + 16 * g + 128);
         const float d[2] = {half_bits_to_float(*reinterpret_cast<const uint16_t *>(rec + 3328 + 2 * g)) * 0.25f,
                             half_bits_to_float(*reinterpret_cast<const uint16_t *>(rec + 3328 + 2 * g + 16)) * 0.25f};
         const uint8_t *bp[F];

@@ -8,9 +8,9 @@ namespace b200q {
 // ---------------------------------------------------------------------------------------------
 // Weights of experts
 //
-// An expert's matrix is cut into tiles of 16 rows x 256 weights ("records"); A block
+// An expert's matrix is cut into tiles of 16 rows x 256 weights ("records").  A block
 // multiplies eight tiles side by side (a "run"), one record of each at a time, and those eight lie next to each other: one copy brings them.  Run
-// after run, inside a run 256 weights after 256 weights.  Inside a record the weights lie in the order in which the lanes of a warp take them as the A
+// follows run, inside a run 256 weights follow 256 weights.  Inside a record the weights lie in the order in which the lanes of a warp take them as the A
 // operand of mma.m16n8k32: lane 4 g + t owns, of rows g and g + 8 and of every block of 32 weights, weights 4 t .. 4 t + 3 and
 // 16 + 4 t .. 16 + 4 t + 3.  The 16-byte vectors of the 32 lanes lie side by side, so both the copy into shared memory and the
 // reads from it are whole 512-byte lines.  Gate and up of the gated product share tiles: rows 0 .. 7 of a tile are

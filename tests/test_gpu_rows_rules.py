@@ -231,6 +231,43 @@ def test_adapters_a_bad_row_spoils_no_other(backend, m, dtype):
         assert _same(got[keep], clean[keep])
 
 
+# ---- far apart -----
+
+@pytest.fixture(scope="module")
+def far():
+    """Room for rows whose offsets pass 2^31 elements (5.4 GB of bf16; only the rows themselves are ever touched)."""
+    free = torch.cuda.mem_get_info()[0]
+    if free < 16 << 30:
+        pytest.skip("too little device memory free")
+    x, y = torch.empty(2 ** 31 + 2 ** 28, dtype=BF16, device="cuda"), torch.empty(2 ** 31 + 2 ** 28, dtype=BF16, device="cuda")
+    return lambda m, n, second: (y if second else x).as_strided((m, n), (2 ** 31 // (m - 1) // 8 * 8 + 8, 1))
+
+
+@pytest.mark.parametrize("m", [3, 12, 40])
+def test_moe_and_router_rows_far_apart(backend, layer, far, m):
+    x, ids, w = layer.inputs(m, BF16, 71)
+    r = backend.router(torch.randn((8, 512), generator=torch.Generator().manual_seed(72)), 3, max_rows=m)
+    ids, w = backend.route(r, x)
+    fx, fy = far(m, 512, False), far(m, 512, True)
+    fx.copy_(x)
+    ids2, w2 = backend.route(r, fx)
+    assert torch.equal(ids, ids2) and torch.equal(w, w2)
+    assert _same(backend.run_moe(layer.layer, fx, ids, w, out=fy).contiguous(), backend.run_moe(layer.layer, x, ids, w, out_dtype=BF16))
+
+
+@pytest.mark.parametrize("m", [3, 100, 600])
+def test_adapters_rows_far_apart(backend, far, m):
+    s = Set(backend, 200, 320, [8, 16], BF16, 16, 73)
+    g = torch.Generator().manual_seed(74)
+    x, y0 = torch.randn((m, 320), generator=g).to(BF16).cuda(), torch.randn((m, 200), generator=g).to(BF16).cuda()
+    slots = torch.tensor([i % 3 - 1 for i in range(m)], dtype=torch.int32, device="cuda")
+    fx, fy = far(m, 320, False), far(m, 200, True)
+    fx.copy_(x)
+    fy.copy_(y0)
+    backend.apply_adapters([s.handle], fx, slots, [fy])
+    assert _same(fy.contiguous(), backend.apply_adapters([s.handle], x, slots, [y0])[0])
+
+
 # ---- together ----------------------------------------------------------------------------------------
 
 class Block:
