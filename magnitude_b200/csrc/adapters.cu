@@ -792,6 +792,7 @@ template <bool F16, bool XF32, bool YF32> __global__ void __launch_bounds__(kThr
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int slots[kShrinkRows];
     __shared__ int kind[kShrinkRows], kind_end[kShrinkRows];      // the slots that occur, and the rank tiles up to the end of each one's
+    __shared__ short kind_tiles[kAdapterMaxSets][kShrinkRows];    // each set's of them
     __shared__ int2 sums_of[kShrinkRows / 32];
     __shared__ AdapterTile tiles_of[kSumTiles];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -810,7 +811,7 @@ template <bool F16, bool XF32, bool YF32> __global__ void __launch_bounds__(kThr
     static_assert(kXBytes == 16 * 16 && kThreads == 16 * 16, "a thread's rows");
     auto tiles_in = [&](int set, int slot) { return active(p.set[set], slot) ? (p.set[set].rank[slot] + 7) / 8 : 0; };
     // the slots that occur, in the order of their first rows, and the tiles of each: all sets'
-    int slot = -1;
+    int slot = -1, tiles_of_set[kAdapterMaxSets];
     bool first_row = false;
     if (tid < kShrinkRows) {
         slot = base + tid < p.m ? p.rows[base + tid] : -1;
@@ -824,7 +825,11 @@ template <bool F16, bool XF32, bool YF32> __global__ void __launch_bounds__(kThr
             for (int q = 0; q < warp * 32; ++q) first_row = first_row && slots[q] != slot;
         if (first_row) {
             run.x = 1;
-            for (int set = 0; set < p.sets; ++set) run.y += tiles_in(set, slot);
+#pragma unroll
+            for (int set = 0; set < kAdapterMaxSets; ++set) {
+                tiles_of_set[set] = set < p.sets ? tiles_in(set, slot) : 0;
+                run.y += tiles_of_set[set];
+            }
         }
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
@@ -839,7 +844,11 @@ template <bool F16, bool XF32, bool YF32> __global__ void __launch_bounds__(kThr
         if (w < warp) run.x += sums_of[w].x, run.y += sums_of[w].y;
         all_tiles += sums_of[w].y;
     }
-    if (first_row) kind[run.x - 1] = slot, kind_end[run.x - 1] = run.y;
+    if (first_row) {
+        kind[run.x - 1] = slot, kind_end[run.x - 1] = run.y;
+#pragma unroll
+        for (int set = 0; set < kAdapterMaxSets; ++set) kind_tiles[set][run.x - 1] = (short)tiles_of_set[set];
+    }
     __syncthreads();
     // eight tiles at a time, of whichever adapters: x is read once for all of them
     for (int first = blockIdx.z * kSumTiles; first < all_tiles; first += gridDim.z * kSumTiles) {
@@ -848,9 +857,9 @@ template <bool F16, bool XF32, bool YF32> __global__ void __launch_bounds__(kThr
             int k = 0;
             while (kind_end[k] <= first + tid) ++k;
             int set = 0, tile = first + tid - (k ? kind_end[k - 1] : 0);
-            while (tile >= tiles_in(set, kind[k])) tile -= tiles_in(set++, kind[k]);
+            while (tile >= kind_tiles[set][k]) tile -= kind_tiles[set++][k];
             const AdapterSet &s = p.set[set];
-            const int rt = tiles_in(set, kind[k]);
+            const int rt = kind_tiles[set][k];
             tiles_of[tid] = AdapterTile{reinterpret_cast<const uint4 *>(s.a + kind[k] * s.a_stride) + tile * 32, rt * 32, s.t_at + 8 * tile, kind[k]};
         }
         __syncthreads();
